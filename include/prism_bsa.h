@@ -43,6 +43,9 @@ typedef enum {
   PRISM_ERR_UNSUPPORTED = 3,
 } prism_status_t;
 
+/* Element types of the norm, rotary and clipping entry points. */
+typedef enum { PRISM_BF16 = 0, PRISM_FP16 = 1, PRISM_FP32 = 2 } prism_dtype_t;
+
 /* Thread-local text of the last error raised on this host thread. */
 const char* prism_last_error(void);
 /* ABI version (incremented on any signature change). */
@@ -489,6 +492,72 @@ prism_status_t prism_bsa_bwd_noalloc(const void* q, const void* k, const void* v
                                      const uint32_t* bits_q, const uint32_t* bits_k,
                                      const uint64_t* tile_bits, void* dq, void* dk, void* dv,
                                      cudaStream_t stream);
+
+/* ---- Operators of a transformer block around the attention.  No counterpart in the
+ * reference's attention package: its blocks use torch.nn.RMSNorm, a stored rotary table and
+ * torch's gradient clipping.
+ *
+ * Residual addition + RMS norm of rows (dtype: prism_dtype_t; row strides ld* in elements,
+ * outputs contiguous [rows, cols]):
+ *   h = x + r rounded to the rows' type (r NULL: h = x, and the h argument is NULL),
+ *   y_j = w_j h_j (mean h^2 + eps)^(-1/2),  weight [cols] fp32 or NULL (w = 1).
+ * rstd [rows] fp32 (or NULL) receives (mean h^2 + eps)^(-1/2) for the backward.  Sums fp32.
+ *
+ * prism_add_rms_norm_fp8: y as e4m3 rows y8 [rows, cols] with scale [rows] fp32,
+ * y ~ y8 * scale: scale = max(max_j |y_j| / 448, 2^-100), rounded to nearest even.  A row with a
+ * NaN or an infinity has scale NaN.  normalize = 0: the rows are not normalised (y = w h).
+ *
+ * prism_add_rms_norm_bwd: gy = dL/dy and gh = dL/dh (NULL: zero) -> dx = dL/dh in total
+ * (= dL/dx = dL/dr), contiguous, and dweight [cols] fp32 (NULL: not wanted; fixed summation
+ * order).  workspace: prism_add_rms_norm_bwd_workspace_bytes(rows, cols), used with dweight. */
+prism_status_t prism_add_rms_norm(const void* x, int64_t ldx, const void* r, int64_t ldr,
+                                  const float* weight, float eps, int64_t rows, int cols, int dtype,
+                                  void* y, void* h, float* rstd, cudaStream_t stream);
+prism_status_t prism_add_rms_norm_fp8(const void* x, int64_t ldx, const void* r, int64_t ldr,
+                                      const float* weight, float eps, int normalize, int64_t rows,
+                                      int cols, int dtype, void* y8, float* scale, void* h,
+                                      cudaStream_t stream);
+size_t prism_add_rms_norm_bwd_workspace_bytes(int64_t rows, int cols);
+prism_status_t prism_add_rms_norm_bwd(const void* gy, int64_t ldgy, const void* h, int64_t ldh,
+                                      const void* gh, int64_t ldgh, const float* weight,
+                                      const float* rstd, int64_t rows, int cols, int dtype, void* dx,
+                                      void* workspace, float* dweight, cudaStream_t stream);
+
+/* Rotary positions of q [batch, seq, q_heads, dim] and k [batch, seq, k_heads, dim] in one
+ * launch (either may have 0 heads): the first rot columns of each head form rot / 2 pairs,
+ * (2j, 2j + 1) if interleaved, else (j, j + rot / 2); pair j, as a complex number, is multiplied
+ * by scale * exp(i p f_j) (conjugate != 0: by the conjugate, the gradient); columns from rot on
+ * are copied.  freqs [rot / 2] fp64, radians per position.  positions: int32 or int64
+ * (positions_64) at b * position_strides[0] + s * position_strides[1] + axis, with axis 0 for
+ * pairs below section_ends[0], 1 below section_ends[1], 2 from there on (one axis: both ends
+ * rot / 2).  Strides {batch, seq, head} in elements; columns contiguous.  Output may not
+ * overlap the input.  The pointer arguments marked const int64_t* / const int* are host arrays. */
+prism_status_t prism_rotary(const void* q, const int64_t* q_strides, int q_heads, const void* k,
+                            const int64_t* k_strides, int k_heads, int64_t batch, int64_t seq, int dim,
+                            int rot, int interleaved, const void* positions, int positions_64,
+                            const int64_t* position_strides, const int* section_ends,
+                            const double* freqs, float scale, int conjugate, int dtype, void* q_out,
+                            const int64_t* q_out_strides, void* k_out, const int64_t* k_out_strides,
+                            cudaStream_t stream);
+
+/* Global gradient norm and clipping over count tensors (host arrays of device pointers, element
+ * counts and prism_dtype_t): norm [1] fp32 = sqrt(sum of all squares), outs[i] = grads[i] *
+ * min(1, max_norm / (norm + 1e-6)).  outs[i] is grads[i] itself (in place; nothing is written
+ * when the factor is 1) or a buffer that overlaps no gradient.  Squares and sums fp64, fixed
+ * order.  A NaN norm makes every output NaN.  workspace:
+ * prism_clip_grad_norm_workspace_bytes(sizes, count), 16-byte aligned. */
+size_t prism_clip_grad_norm_workspace_bytes(const int64_t* sizes, int64_t count);
+prism_status_t prism_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* sizes,
+                                    const int* dtypes, int64_t count, float max_norm, void* workspace,
+                                    float* norm, cudaStream_t stream);
+
+/* 8-bit projection: C[m, n] (bf16, row stride ldc) = x_scale[m] w_scale[n] sum_k x8(m, k) w8(n, k)
+ * (+ bias[n] fp32), x8 [M, K] and w8 [N, K] e4m3 rows (strides ldx, ldw in bytes), scales fp32 as
+ * prism_add_rms_norm_fp8 makes them; fp32 accumulation, one rounding.  K, ldx, ldw multiples of
+ * 16; x8 and w8 16-byte aligned.  Bounded waits report through prism_device_status (411-413). */
+prism_status_t prism_linear_fp8(const void* x8, int64_t ldx, const float* x_scale, const void* w8,
+                                int64_t ldw, const float* w_scale, const float* bias, int M, int N,
+                                int K, void* c, int64_t ldc, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

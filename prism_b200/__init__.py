@@ -16,6 +16,12 @@ Public entry points mirror the reference names:
                               block_sparse_attention/bias_rectification.py:380, 261 (inference)
   select_zone_shapes          block_sparse_attention/dynamic_block_shape.py:358
   all_to_all_4D / all_gather  hymm/utils/communications.py:277, 401
+Operators of a transformer block around the attention (no counterpart in the reference's
+attention package):
+  add_rms_norm, add_rms_norm_fp8, quantize_rows_fp8   residual + RMS norm, 8-bit rows (norm.py)
+  linear_fp8                  projection of 8-bit rows (linear.py)
+  apply_rotary, rotary_frequencies   rotary positions (rotary.py)
+  clip_grad_norm              global gradient norm and clipping (grad_clip.py)
 The kernels live in libprism_bsa.so (C ABI: include/prism_bsa.h).
 """
 from .bias_rectification import bsa_rectified_sparse_attn, bsa_taylor_sparse_attn  # noqa: F401
@@ -33,6 +39,10 @@ from .dynamic_block_shape import (  # noqa: F401
     ALL_CANDIDATE_SHAPES, CANDIDATE_SHAPES_64, CANDIDATE_SHAPES_128, NUM_CANDIDATES,
     NUM_CANDIDATES_64, ZONE_SIZE, compute_effective_gradient, select_zone_shapes,
 )
+from .grad_clip import clip_grad_norm  # noqa: F401
+from .linear import linear_fp8  # noqa: F401
+from .norm import add_rms_norm, add_rms_norm_fp8, quantize_rows_fp8  # noqa: F401
 from .ops import token_norms  # noqa: F401
+from .rotary import apply_rotary, rotary_frequencies  # noqa: F401
 
 __version__ = "0.1.0"

@@ -58,6 +58,15 @@ SIGNATURES = {
     "prism_norm_rope_pack_bwd_workspace_bytes": (_SZ, [_I64, _I, _I]),
     "prism_norm_rope_pack_bwd": (_I, [_P, _P, _I64, _I64, _I64, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I64,
                                       _P, _P, _P]),
+    "prism_add_rms_norm": (_I, [_P, _I64, _P, _I64, _P, _F, _I64, _I, _I, _P, _P, _P, _P]),
+    "prism_add_rms_norm_fp8": (_I, [_P, _I64, _P, _I64, _P, _F, _I, _I64, _I, _I, _P, _P, _P, _P]),
+    "prism_add_rms_norm_bwd_workspace_bytes": (_SZ, [_I64, _I]),
+    "prism_add_rms_norm_bwd": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I, _I, _P, _P, _P, _P]),
+    "prism_rotary": (_I, [_P, _P, _I, _P, _P, _I, _I64, _I64, _I, _I, _I, _P, _I, _P, _P, _P, _F, _I, _I, _P, _P, _P,
+                          _P, _P]),
+    "prism_clip_grad_norm_workspace_bytes": (_SZ, [_P, _I64]),
+    "prism_clip_grad_norm": (_I, [_P, _P, _P, _P, _I64, _F, _P, _P, _P]),
+    "prism_linear_fp8": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _I, _I, _I, _P, _I64, _P]),
     "prism_bsa_fwd_qk": (_I, [_P, _P, _P, _I, _I64, _I64, _I, _F, _P, _P, _P, _P, _P, _P]),
     "prism_bsa_bwd_qk": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I, _F, _P, _P, _P, _P, _P, _P, _P, _P]),
     "prism_bsa_fwd": (_I, [_P, _P, _P, _I, _I64, _I, _F, _P, _P, _P, _P, _P, _P]),
@@ -82,7 +91,9 @@ KERNELS = {
     "prism_bsa_fwd_keybias": 1, "prism_correction_stats": 1, "prism_taylor_prep": 1,
     "prism_key_log_bias": 1, "prism_rows_to_bf16": 1, "prism_taylor_merge": 1,
     "prism_rectified_apply": 1, "prism_rectified_contract": 1, "prism_norm_rope_pack": 1,
-    "prism_gemm_bf16": 1, "prism_norm_rope_pack_bwd": 4,
+    "prism_gemm_bf16": 1, "prism_norm_rope_pack_bwd": 4, "prism_add_rms_norm": 1,
+    "prism_add_rms_norm_fp8": 1, "prism_add_rms_norm_bwd": 3, "prism_rotary": 1,
+    "prism_clip_grad_norm": 3, "prism_linear_fp8": 1,
 }
 launch_count = 0
 

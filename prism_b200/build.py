@@ -28,6 +28,10 @@ SOURCES = {
     "producer_kernels.cu": ["-fmad=false"],
     "bsa_tc.cu": [],
     "gemm_tc.cu": [],
+    "gemm_fp8.cu": [],
+    "norm_kernels.cu": [],
+    "rotary_kernels.cu": [],
+    "clip_kernels.cu": [],
 }
 
 

@@ -1691,6 +1691,7 @@ prism_status_t launch_dq(const void* q, const void* k, const void* v, const void
 using namespace prism;
 
 int prism_gemm_device_status_internal(void);
+int prism_gemm8_device_status_internal(void);
 
 extern "C" {
 
@@ -1702,8 +1703,9 @@ int prism_device_status(void) {
     cudaMemcpyToSymbol(tc::g_tc_error, &zero, sizeof(int));
   }
   const int g = prism_gemm_device_status_internal();  // the GEMM kernels' word (gemm_tc.cu)
-  if (g < 0) return -1;
-  return v != 0 ? v : g;
+  const int g8 = prism_gemm8_device_status_internal();  // and gemm_fp8.cu's
+  if (g < 0 || g8 < 0) return -1;
+  return v != 0 ? v : g != 0 ? g : g8;
 }
 
 // Row indices of the [heads * S, D] views are 32-bit TMA coordinates.

@@ -1,0 +1,301 @@
+// 8-bit projection on the sm_100a tensor cores:
+//
+//   C[m, n] (bf16) = xs[m] ws[n] sum_k X8(m, k) W8(n, k)  (+ bias[n])
+//
+// X8 [M, K] rows with a scale each (prism_add_rms_norm_fp8), W8 [N, K] rows with a scale per
+// output feature, both e4m3, K contiguous; products are exact and sums fp32 in the tensor core,
+// the scales and the bias are applied in fp32, and the result is rounded once.
+//
+// The weight is the tensor core's M side (128 output features to a tile) and the tokens its N
+// side, 16 to 256 of them to a tile: a call with one token then streams the weight through
+// 16-column products instead of multiplying 127 rows of padding.
+//
+// Persistent kernel, one CTA per SM.  Warp 4 streams weight and token tiles (128 bytes of K)
+// with TMA into a ring, warp 5 issues tcgen05.mma kind::f8f6f4 (K = 32 an instruction) into one
+// of two TMEM accumulators, warps 0-3 (thread = output feature) drain the other.  At 256 tokens
+// one instruction reads 4 KB + 8 KB of shared memory in 128 clocks (of 128 B/clk).  Every wait
+// is bounded (sm100.cuh); one that gives up sets this file's device error word.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+#include <stdint.h>
+
+#include <mutex>
+
+#include "prism_common.cuh"
+#include "sm100.cuh"
+
+namespace prism {
+namespace gemm8 {
+
+using namespace sm100;
+
+__device__ int g_gemm8_error = 0;
+enum : int { kErrProducer = 411, kErrMma = 412, kErrEpilogue = 413 };
+
+constexpr int kThreads = 192;
+constexpr int kFeatures = 128, kStepK = 128;  // a tile's features; bytes of K in a stage
+constexpr int kABytes = kFeatures * kStepK;
+
+template <int kTokens>
+struct Shape {
+  static constexpr int kBBytes = kTokens * kStepK;
+  static constexpr int kStageBytes = kABytes + kBBytes;
+  static constexpr int kStages = kTokens == 256 ? 4 : kTokens == 128 ? 6 : 8;
+  static constexpr int kColumns = kTokens <= 16 ? 32 : 2 * kTokens;  // TMEM: two accumulators
+  static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = kAccFull + 2,
+                       kDrain = kAccEmpty + 2, kBars = kDrain + 1;
+  static constexpr int kBarAt = kStages * kStageBytes;
+  static constexpr int kTmemAt = kBarAt + kBars * 8;
+  static constexpr int kAbortAt = kTmemAt + 4;
+  static constexpr size_t kSmem = 1024 + kAbortAt + 4;
+};
+
+// Four K = 32 products of one 128-byte stage; descriptor steps of 32 bytes, in 16-byte units.
+__device__ __forceinline__ void mma_stage(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p0, p1;\n .reg .b64 a1, a2, a3, b1, b2, b3;\n"
+      " setp.ne.b32 p0, %4, 0;\n setp.eq.b32 p1, %4, %4;\n"
+      " add.s64 a1, %1, 2;\n add.s64 a2, %1, 4;\n add.s64 a3, %1, 6;\n"
+      " add.s64 b1, %2, 2;\n add.s64 b2, %2, 4;\n add.s64 b3, %2, 6;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p0;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a1, b1, %3, p1;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a2, b2, %3, p1;\n"
+      " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a3, b3, %3, p1;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// kind::f8f6f4 instruction descriptor: fp32 accumulation ([4,6) = 1), e4m3 operands (formats 0),
+// both K-major, N >> 3 in [17,23), M >> 4 in [24,29).
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+template <int kTokens>
+__global__ void __launch_bounds__(kThreads, 1)
+    linear_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, int M, int N,
+                  int K, const float* __restrict__ xs, const float* __restrict__ ws, const float* __restrict__ bias,
+                  __nv_bfloat16* __restrict__ c, int64_t ldc) {
+  using S = Shape<kTokens>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const uint32_t sb = smem_u32(sm);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto bar = [&](int i) { return sb + S::kBarAt + 8 * i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + S::kAbortAt);
+  const int tf = (N + kFeatures - 1) / kFeatures, tt = (M + kTokens - 1) / kTokens;
+  const int tiles = tf * tt;
+  const int nk = (K + kStepK - 1) / kStepK;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(bar(S::kFull + i), 1);
+      mbar_init(bar(S::kEmpty + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(S::kAccFull + i), 1);
+      mbar_init(bar(S::kAccEmpty + i), 4);
+    }
+    mbar_init(bar(S::kDrain), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 5) {
+    tmem_alloc(sb + S::kTmemAt, S::kColumns);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + S::kTmemAt);
+
+  if (warp == 4) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+        const int n0 = (t % tf) * kFeatures, m0 = (t / tf) * kTokens;
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const int s = it % S::kStages;
+          if (it >= S::kStages && !mbar_wait(bar(S::kEmpty + s), ((it / S::kStages) - 1) & 1, abort_flag,
+                                             &g_gemm8_error, kErrProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t a = sb + s * S::kStageBytes, fb = bar(S::kFull + s);
+          mbar_expect_tx(fb, S::kStageBytes);
+          tma_load_2d(a, &tm_w, kb * kStepK, n0, fb);
+          tma_load_2d(a + kABytes, &tm_x, kb * kStepK, m0, fb);
+        }
+      }
+      // every issued copy has landed before the CTA may leave
+      for (int i = it > S::kStages ? it - S::kStages : 0; i < it; ++i)
+        mbar_wait(bar(S::kFull + i % S::kStages), (i / S::kStages) & 1, abort_flag, &g_gemm8_error, kErrProducer);
+    }
+  } else if (warp == 5) {
+    if (lane == 0) {
+      constexpr uint32_t kIdesc = idesc_e4m3(kFeatures, kTokens);
+      int it = 0, tl = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++tl) {
+        const int ab = tl & 1;
+        if (tl >= 2 && !mbar_wait(bar(S::kAccEmpty + ab), ((tl >> 1) - 1) & 1, abort_flag, &g_gemm8_error, kErrMma))
+          break;
+        tc_fence_after();
+        for (int kb = 0; kb < nk; ++kb, ++it) {
+          const int s = it % S::kStages;
+          if (!mbar_wait(bar(S::kFull + s), (it / S::kStages) & 1, abort_flag, &g_gemm8_error, kErrMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t a = sb + s * S::kStageBytes;
+          mma_stage(tmem + ab * kTokens, desc_k_sw128(a), desc_k_sw128(a + kABytes), kIdesc, kb > 0 ? 1u : 0u);
+          mma_commit(bar(S::kEmpty + s));
+        }
+        if (ok) mma_commit(bar(S::kAccFull + ab));
+      }
+      mma_commit(bar(S::kDrain));
+      mbar_wait(bar(S::kDrain), 0, abort_flag, &g_gemm8_error, kErrMma);
+    }
+  } else {
+    const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    int tl = 0;
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++tl) {
+      const int ab = tl & 1;
+      const int n = (t % tf) * kFeatures + warp * 32 + lane, m0 = (t / tf) * kTokens;
+      const float scale = n < N ? __ldg(ws + n) : 0.0f, b = bias && n < N ? __ldg(bias + n) : 0.0f;
+      const bool ok = mbar_wait(bar(S::kAccFull + ab), (tl >> 1) & 1, abort_flag, &g_gemm8_error, kErrEpilogue);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int cc = 0; cc < kTokens; cc += 16) {
+        if (m0 + cc >= M) break;
+        uint32_t raw[16];
+        tmem_ld16(t_lane + ab * kTokens + cc, raw);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int m = m0 + cc + i;
+          if (m < M && n < N)
+            c[(int64_t)m * ldc + n] = __float2bfloat16_rn(fmaf(__uint_as_float(raw[i]) * __ldg(xs + m), scale, b));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(S::kAccEmpty + ab));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, S::kColumns);
+  }
+}
+
+// ------------------------------------------------------------------ host
+using EncodeFn = PFN_cuTensorMapEncodeTiled_v12000;
+
+static EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+  });
+  return fn;
+}
+
+// 2D map of e4m3 rows, boxes of 128 bytes x box_rows, 128-byte swizzle; zeros outside.
+static prism_status_t make_map(CUtensorMap* map, const void* ptr, int64_t rows, int64_t cols, int64_t ld,
+                               int box_rows) {
+  EncodeFn enc = encode_fn();
+  if (enc == nullptr) {
+    set_error("prism_linear_fp8: cuTensorMapEncodeTiled is unavailable from the driver");
+    return PRISM_ERR_CUDA;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t box[2] = {kStepK, (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("prism_linear_fp8: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return PRISM_ERR_CUDA;
+  }
+  return PRISM_OK;
+}
+
+template <int kTokens>
+static prism_status_t launch(const void* x8, int64_t ldx, const float* xs, const void* w8, int64_t ldw,
+                             const float* ws, const float* bias, int M, int N, int K, void* c, int64_t ldc,
+                             cudaStream_t stream) {
+  using S = Shape<kTokens>;
+  CUtensorMap mw, mx;
+  prism_status_t st = make_map(&mw, w8, N, K, ldw, kFeatures);
+  if (st != PRISM_OK) return st;
+  st = make_map(&mx, x8, M, K, ldx, kTokens);
+  if (st != PRISM_OK) return st;
+  int dev = 0, sms = 0;
+  PRISM_CHECK_CUDA(cudaGetDevice(&dev), "prism_linear_fp8: cudaGetDevice");
+  PRISM_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "prism_linear_fp8: SM count");
+  PRISM_CHECK_CUDA(cudaFuncSetAttribute(linear_kernel<kTokens>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)S::kSmem),
+                   "prism_linear_fp8: smem attribute");
+  const int64_t tiles = (int64_t)((N + kFeatures - 1) / kFeatures) * ((M + kTokens - 1) / kTokens);
+  PRISM_CHECK_ARG(tiles < ((int64_t)1 << 30), "prism_linear_fp8: the output has too many tiles");
+  linear_kernel<kTokens><<<(unsigned)(tiles < sms ? tiles : sms), kThreads, S::kSmem, stream>>>(
+      mw, mx, M, N, K, xs, ws, bias, (__nv_bfloat16*)c, ldc);
+  PRISM_CHECK_LAUNCH("prism_linear_fp8");
+  return PRISM_OK;
+}
+
+}  // namespace gemm8
+}  // namespace prism
+
+using namespace prism;
+
+int prism_gemm8_device_status_internal(void) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, gemm8::g_gemm8_error, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(gemm8::g_gemm8_error, &zero, sizeof(int));
+  }
+  return v;
+}
+
+extern "C" prism_status_t prism_linear_fp8(const void* x8, int64_t ldx, const float* x_scale, const void* w8,
+                                           int64_t ldw, const float* w_scale, const float* bias, int M, int N,
+                                           int K, void* c, int64_t ldc, cudaStream_t stream) {
+  PRISM_CHECK_ARG(M >= 0 && M < (1 << 30) && N >= 1 && N < (1 << 30) && K >= 1 && K < (1 << 30) && K % 16 == 0,
+                  "prism_linear_fp8: bad sizes (N >= 1, K a positive multiple of 16)");
+  if (M == 0) return PRISM_OK;
+  PRISM_CHECK_ARG(x8 && x_scale && w8 && w_scale && c, "prism_linear_fp8: null pointer");
+  PRISM_CHECK_ARG(ldx >= K && ldw >= K && ldx % 16 == 0 && ldw % 16 == 0 && ldc >= N,
+                  "prism_linear_fp8: 8-bit row strides must be multiples of 16 and cover K, ldc must cover N");
+  PRISM_CHECK_ARG(aligned16(x8) && aligned16(w8), "prism_linear_fp8: 8-bit tensors must be 16-byte aligned");
+  // the smallest tile that holds every token, 256 at most: fewer columns, fewer wasted products
+  if (M <= 16) return gemm8::launch<16>(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
+  if (M <= 32) return gemm8::launch<32>(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
+  if (M <= 64) return gemm8::launch<64>(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
+  if (M <= 128) return gemm8::launch<128>(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
+  return gemm8::launch<256>(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
+}

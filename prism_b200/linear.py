@@ -10,6 +10,9 @@
   rank into the same output, the first with the bias, the others accumulating,
   so the heads -> sequence unpack never materialises.  Backward: per source rank
   the slice of d(recv) and the matching columns of dW.
+* ``linear_fp8(x8, x_scale, w8, w_scale, bias)``: a projection of 8-bit rows
+  (``prism_linear_fp8``), for inference: x8 and its scales from
+  ``prism_b200.norm.add_rms_norm_fp8``, the weight's from ``quantize_rows_fp8(weight)``.
 """
 from __future__ import annotations
 
@@ -97,4 +100,27 @@ def o_proj_packed(recv: torch.Tensor, weight: torch.Tensor, bias: Optional[torch
     return _PackedOProj.apply(recv.contiguous(), weight, bias, heads, S_local)
 
 
-__all__ = ["linear", "o_proj_packed"]
+def linear_fp8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_scale: torch.Tensor,
+               bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x8 [..., K], w8 [N, K] float8_e4m3fn, x_scale [...] and w_scale [N] fp32 (the value of an
+    element is its 8-bit value times its row's scale) -> [..., N] bf16 = x W^T + bias.  K a
+    multiple of 16."""
+    if x8.dtype != torch.float8_e4m3fn or w8.dtype != torch.float8_e4m3fn:
+        raise TypeError(f"linear_fp8 expects float8_e4m3fn operands, got {x8.dtype} and {w8.dtype}")
+    if x8.dim() < 1 or w8.dim() != 2 or x8.shape[-1] != w8.shape[1]:
+        raise ValueError(f"linear_fp8: x {tuple(x8.shape)} and W {tuple(w8.shape)} do not match")
+    if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
+        raise TypeError("linear_fp8 expects fp32 scales")
+    if x_scale.shape != x8.shape[:-1] or w_scale.shape != w8.shape[:1]:
+        raise ValueError("linear_fp8: one scale a row of x and of W")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x_scale, w_scale, bias)):
+        raise NotImplementedError("linear_fp8 is inference only")
+    K = x8.shape[-1]
+    x2 = x8.reshape(-1, K)
+    x2, w2 = (t if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= K and t.data_ptr() % 16 == 0
+              else t.clone(memory_format=torch.contiguous_format) for t in (x2, w8))
+    out = ops.linear_fp8(x2, x_scale.reshape(-1).contiguous(), w2, w_scale.contiguous(), bias)
+    return out.view(*x8.shape[:-1], w8.shape[0])
+
+
+__all__ = ["linear", "linear_fp8", "o_proj_packed"]

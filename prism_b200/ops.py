@@ -425,6 +425,148 @@ def norm_rope_pack_bwd(g: torch.Tensor, x, heads: int, S: int, gamma=None, rstd=
     return dx, dgamma
 
 
+# ----------------------------------------------- operators around the attention
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # prism_dtype_t
+
+
+def _dtype_code(t: torch.Tensor, what: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{what} expects bf16, fp16 or fp32, got {t.dtype}")
+    return code
+
+
+def _same_device(*ts):
+    """Every tensor on one CUDA device, which is made the current one for the launch (the
+    kernels launch on that device's current stream)."""
+    _check_cuda(*ts)
+    dev = None
+    for t in ts:
+        if t is not None:
+            if dev is None:
+                dev = t.device
+            elif t.device != dev:
+                raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    return torch.cuda.device(dev)
+
+
+def _fp32_vector(w: Optional[torch.Tensor], n: int, what: str):
+    if w is None:
+        return None
+    if w.dim() != 1 or w.shape[0] != n:
+        raise ValueError(f"{what} must have shape [{n}], got {tuple(w.shape)}")
+    return w.to(torch.float32).contiguous()
+
+
+def _rows2d(t: Optional[torch.Tensor], cols: int):
+    """[..., cols] -> a [rows, cols] view with unit column stride (a copy where there is none)."""
+    if t is None:
+        return None
+    t = t.reshape(-1, cols)
+    return t if cols == 1 or t.stride(1) == 1 else t.contiguous()
+
+
+def _ld(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.stride(0)
+
+
+def _rows_input(x, residual, weight, what):
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"{what} needs at least one column")
+    code = _dtype_code(x, what)
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+        raise ValueError(f"{what}: the residual must have the shape and type of x")
+    cols = x.shape[-1]
+    return code, cols, _rows2d(x, cols), _rows2d(residual, cols), _fp32_vector(weight, cols, "weight")
+
+
+def add_rms_norm(x, residual=None, weight=None, eps: float = 1e-6, want_rstd: bool = False):
+    """prism_add_rms_norm: (y, h, rstd), y and h shaped as x, rstd [rows] fp32 or None; h is
+    None without a residual."""
+    with _same_device(x, residual, weight):
+        code, cols, x2, r2, w = _rows_input(x, residual, weight, "add_rms_norm")
+        rows = x2.shape[0]
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
+        _lib.call("prism_add_rms_norm", _p(x2), _ld(x2), _p(r2), _ld(r2), _p(w), float(eps), rows, cols, code,
+                  _p(y), _p(h), _p(rstd), _stream(x))
+    return y, h, rstd
+
+
+def add_rms_norm_fp8(x, residual=None, weight=None, eps: float = 1e-6, normalize: bool = True):
+    """prism_add_rms_norm_fp8: (y8 e4m3 shaped as x, scale [x.shape[:-1]] fp32, h or None)."""
+    with _same_device(x, residual, weight):
+        code, cols, x2, r2, w = _rows_input(x, residual, weight, "add_rms_norm_fp8")
+        y8 = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        _lib.call("prism_add_rms_norm_fp8", _p(x2), _ld(x2), _p(r2), _ld(r2), _p(w), float(eps), int(normalize),
+                  x2.shape[0], cols, code, _p(y8), _p(scale), _p(h), _stream(x))
+    return y8, scale, h
+
+
+def add_rms_norm_bwd(gy, h, rstd, gh=None, weight=None, want_dweight: bool = True):
+    """prism_add_rms_norm_bwd: (dx shaped as h, dweight [cols] fp32 or None)."""
+    with _same_device(gy, h, rstd, gh, weight):
+        code, cols = _dtype_code(h, "add_rms_norm_bwd"), h.shape[-1]
+        g2, h2, gh2 = _rows2d(gy, cols), _rows2d(h, cols), _rows2d(gh, cols)
+        w = _fp32_vector(weight, cols, "weight")
+        rows = h2.shape[0]
+        dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
+        dw = torch.empty(cols, dtype=torch.float32, device=h.device) if want_dweight else None
+        ws = (_ws(_lib.query("prism_add_rms_norm_bwd_workspace_bytes", rows, cols), h.device)
+              if want_dweight else None)
+        _lib.call("prism_add_rms_norm_bwd", _p(g2), _ld(g2), _p(h2), _ld(h2), _p(gh2), _ld(gh2), _p(w), _p(rstd),
+                  rows, cols, code, _p(dx), _p(ws), _p(dw), _stream(h))
+    return dx, dw
+
+
+def rotary(q, k, positions, freqs, section_ends, interleaved: bool, scale: float, conjugate: bool = False):
+    """prism_rotary on q [B, S, Hq, D] and k [B, S, Hk, D] or None (unit column stride);
+    positions [B, S, axes] integers with unit axis stride, freqs [rot / 2] fp64 -> new (q, k)."""
+    with _same_device(q, k, positions, freqs):
+        B, S, hq, D = q.shape
+        hk = 0 if k is None else k.shape[2]
+        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        s3 = lambda t: None if t is None else (ctypes.c_int64 * 3)(*t.stride()[:3])
+        _lib.call("prism_rotary", _p(q), s3(q), hq, _p(k), s3(k), hk, B, S, D, 2 * freqs.shape[0], int(interleaved),
+                  _p(positions), int(positions.dtype == torch.int64), (ctypes.c_int64 * 2)(*positions.stride()[:2]),
+                  (ctypes.c_int * 2)(*section_ends), _p(freqs), float(scale), int(conjugate),
+                  _dtype_code(q, "rotary"), _p(qo), s3(qo), _p(ko), s3(ko), _stream(q))
+    return qo, ko
+
+
+def clip_grad_norm(grads, outs, max_norm: float) -> torch.Tensor:
+    """prism_clip_grad_norm over dense tensors (outs[i] may be grads[i]) -> norm, 0-dim fp32."""
+    dev = grads[0].device
+    with torch.cuda.device(dev):
+        n = len(grads)
+        ptrs = (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads])
+        optrs = (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
+        sizes = (ctypes.c_int64 * n)(*[g.numel() for g in grads])
+        codes = (ctypes.c_int * n)(*[_dtype_code(g, "clip_grad_norm") for g in grads])
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        ws = _ws(_lib.query("prism_clip_grad_norm_workspace_bytes", sizes, n), dev)
+        _lib.call("prism_clip_grad_norm", ptrs, optrs, sizes, codes, n, float(max_norm), _p(ws), _p(norm),
+                  _stream(norm))
+    return norm
+
+
+def linear_fp8(x8, x_scale, w8, w_scale, bias=None) -> torch.Tensor:
+    """prism_linear_fp8: x8 [M, K], w8 [N, K] e4m3 (unit column stride), x_scale [M], w_scale [N]
+    fp32 -> [M, N] bf16."""
+    with _same_device(x8, x_scale, w8, w_scale, bias):
+        M, K = x8.shape
+        N = w8.shape[0]
+        out = torch.empty(M, N, dtype=torch.bfloat16, device=x8.device)
+        b = _fp32_vector(bias, N, "bias")
+        _lib.call("prism_linear_fp8", _p(x8), x8.stride(0), _p(x_scale), _p(w8), w8.stride(0), _p(w_scale), _p(b),
+                  M, N, K, _p(out), N, _stream(x8))
+    return out
+
+
 # --------------------------------------------------------- guided selection
 def gather_values(x: torch.Tensor, grid, grid_padded, src_idx: torch.Tensor) -> torch.Tensor:
     """Per-token values [T*H*W] on grid -> fp32 [len(src_idx)] in the chunk order, 0 at padding."""
