@@ -545,8 +545,8 @@ prism_status_t prism_rotary(const void* q, const int64_t* q_strides, int q_heads
  * min(1, max_norm / (norm + 1e-6)).  outs[i] is grads[i] itself (in place; nothing is written
  * when the factor is 1) or a buffer that overlaps no gradient.  Squares and sums fp64, fixed
  * order.  A NaN norm makes every output NaN.  workspace:
- * prism_clip_grad_norm_workspace_bytes(sizes, count), 16-byte aligned. */
-size_t prism_clip_grad_norm_workspace_bytes(const int64_t* sizes, int64_t count);
+ * prism_clip_grad_norm_workspace_bytes(count), 8-byte aligned. */
+size_t prism_clip_grad_norm_workspace_bytes(int64_t count);
 prism_status_t prism_clip_grad_norm(const void* const* grads, void* const* outs, const int64_t* sizes,
                                     const int* dtypes, int64_t count, float max_norm, void* workspace,
                                     float* norm, cudaStream_t stream);

@@ -64,7 +64,7 @@ SIGNATURES = {
     "prism_add_rms_norm_bwd": (_I, [_P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I, _I, _P, _P, _P, _P]),
     "prism_rotary": (_I, [_P, _P, _I, _P, _P, _I, _I64, _I64, _I, _I, _I, _P, _I, _P, _P, _P, _F, _I, _I, _P, _P, _P,
                           _P, _P]),
-    "prism_clip_grad_norm_workspace_bytes": (_SZ, [_P, _I64]),
+    "prism_clip_grad_norm_workspace_bytes": (_SZ, [_I64]),
     "prism_clip_grad_norm": (_I, [_P, _P, _P, _P, _I64, _F, _P, _P, _P]),
     "prism_linear_fp8": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _I, _I, _I, _P, _I64, _P]),
     "prism_bsa_fwd_qk": (_I, [_P, _P, _P, _I, _I64, _I64, _I, _F, _P, _P, _P, _P, _P, _P]),
@@ -93,7 +93,7 @@ KERNELS = {
     "prism_rectified_apply": 1, "prism_rectified_contract": 1, "prism_norm_rope_pack": 1,
     "prism_gemm_bf16": 1, "prism_norm_rope_pack_bwd": 4, "prism_add_rms_norm": 1,
     "prism_add_rms_norm_fp8": 1, "prism_add_rms_norm_bwd": 3, "prism_rotary": 1,
-    "prism_clip_grad_norm": 3, "prism_linear_fp8": 1,
+    "prism_clip_grad_norm": 2, "prism_linear_fp8": 1,
 }
 launch_count = 0
 
@@ -129,14 +129,19 @@ def load(build_if_missing: bool = True):
         return L
 
 
+_entries = {}  # name -> (bound entry point, kernels that it launches)
+
+
 def call(name: str, *args):
     """Invoke an entry point; raise PrismError with the library's message on failure."""
     global launch_count
-    L = load()
-    rc = getattr(L, name)(*args)
-    launch_count += KERNELS.get(name, 0)
+    entry = _entries.get(name)
+    if entry is None:
+        entry = _entries[name] = (getattr(load(), name), KERNELS.get(name, 0))
+    rc = entry[0](*args)
+    launch_count += entry[1]
     if rc != 0:
-        msg = L.prism_last_error().decode(errors="replace")
+        msg = _lib.prism_last_error().decode(errors="replace")
         if "Either sparsity or cdf_threshold" in msg or "unknown dynamic-block method" in msg:
             raise ValueError(msg)
         raise PrismError(f"{name} failed ({rc}): {msg}")

@@ -4,6 +4,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "prism_common.cuh"
 
 namespace prism {
@@ -21,6 +23,41 @@ template <> struct Elem<float> {
   static __device__ __forceinline__ float to_f(float v) { return v; }
   static __device__ __forceinline__ float from_f(float v) { return v; }
 };
+
+// A 16-byte vector of elements as fp32 values, and back (round to nearest even).
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& v, float (&f)[16 / sizeof(T)]) {
+  const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      f[i] = __uint_as_float(u[i]);
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const float2 p = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
+      f[2 * i] = p.x, f[2 * i + 1] = p.y;
+    } else {
+      f[2 * i] = __uint_as_float(u[i] << 16), f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float (&f)[16 / sizeof(T)]) {
+  uint32_t u[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      u[i] = __float_as_uint(f[i]);
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const __half2 p = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t*>(&p);
+    } else {
+      const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+      u[i] = *reinterpret_cast<const uint32_t*>(&p);
+    }
+  }
+  return make_uint4(u[0], u[1], u[2], u[3]);
+}
+__device__ __forceinline__ bool is_aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // Calls fn with a null pointer of the element type that `dtype` names; false if none does.
 template <typename F>

@@ -7,50 +7,62 @@ import torch
 
 from . import ops
 
-
 def _flat_order(g: torch.Tensor, o: torch.Tensor):
     """(g, o) with their dimensions permuted so that both are contiguous, or None: elements of
-    dense tensors with the same strides match one to one in memory order."""
+    dense tensors with the same shape and strides match one to one in memory order."""
     if g.is_contiguous() and o.is_contiguous():
         return g, o
+    if g.shape != o.shape:
+        return None
     order = sorted(range(g.dim()), key=lambda d: (-g.stride(d), d))
     gp, op = g.permute(order), o.permute(order)
     return (gp, op) if gp.is_contiguous() and op.is_contiguous() else None
 
 
-@torch.no_grad()
+def _one_device(tensors) -> None:
+    devices = set(map(torch.Tensor.get_device, tensors))
+    if min(devices) < 0:
+        ops._check_cuda(*tensors)
+    if len(devices) > 1:
+        raise ValueError("gradients and outputs must be on one device")
+
+
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *,
                    out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """norm = sqrt(sum of the squares of every element of every gradient) -> 0-dim fp32 tensor on
     the gradients' device; the gradients become g * min(1, max_norm / (norm + 1e-6)), in place or
-    in ``out`` (a tensor of the same shape and type for each gradient, overlapping none of them).  bf16, fp16 and fp32 gradients may be mixed.  A norm that is not a
-    number makes every gradient NaN; max_norm = inf only measures the norm."""
+    in ``out``: for each gradient a tensor of its type and number of elements (its own shape, or
+    its slice of a flat buffer, filled in row-major order) that overlaps none of them.  bf16,
+    fp16 and fp32 gradients may be mixed.  A norm that is not a number makes every gradient NaN;
+    max_norm = inf only measures the norm."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    outs = grads if out is None else ([out] if isinstance(out, torch.Tensor) else list(out))
     if not max_norm >= 0:
         raise ValueError(f"max_norm must be a number that is not negative, got {max_norm}")
-    if len(outs) != len(grads):
-        raise ValueError(f"{len(grads)} gradients, {len(outs)} outputs")
+    outs = grads
+    if out is not None:
+        outs = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(outs) != len(grads):
+            raise ValueError(f"{len(grads)} gradients, {len(outs)} outputs")
     if not grads:
         return torch.zeros(())
-    dev = grads[0].device
-    ops._check_cuda(*grads)
-    ops._check_cuda(*outs)
+    _one_device(grads if outs is grads else grads + outs)
+    contiguous = torch.Tensor.is_contiguous
+    if all(map(contiguous, grads)) and (outs is grads or all(map(contiguous, outs))):
+        return ops.clip_grad_norm(grads, outs, max_norm)
     src, dst, copies = [], [], []
-    for g, o in zip(grads, outs):
-        if g.device != dev or o.device != dev:
-            raise ValueError("gradients and outputs must be on one device")
-        if o.shape != g.shape or o.dtype != g.dtype:
-            raise ValueError("an output must have the shape and type of its gradient")
-        pair = _flat_order(g, o)
-        if pair is None:  # gaps in memory, or two orders: through a contiguous copy
-            pair = (g.clone(memory_format=torch.contiguous_format),) * 2
-            copies.append((o, pair[1]))
-        src.append(pair[0])
-        dst.append(pair[1])
-    norm = ops.clip_grad_norm(src, dst, max_norm)
-    for o, c in copies:
-        o.copy_(c)
+    with torch.no_grad():
+        for g, o in zip(grads, outs):
+            pair = _flat_order(g, o)
+            if pair is None:  # gaps in memory, or two orders: through a contiguous copy
+                if o.numel() != g.numel():
+                    raise ValueError("an output must have as many elements as its gradient")
+                pair = (g.clone(memory_format=torch.contiguous_format),) * 2
+                copies.append((o, pair[1]))
+            src.append(pair[0])
+            dst.append(pair[1])
+        norm = ops.clip_grad_norm(src, dst, max_norm)
+        for o, c in copies:
+            o.copy_(c.view(o.shape))
     return norm
 
 

@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import ctypes
 import math
+from array import array
+from operator import attrgetter
 from typing import Optional, Tuple
 
 import torch
@@ -426,7 +428,11 @@ def norm_rope_pack_bwd(g: torch.Tensor, x, heads: int, S: int, gamma=None, rstd=
 
 
 # ----------------------------------------------- operators around the attention
+# The wrappers below pass addresses as plain integers and touch each tensor as little as they
+# can: at one token the host's share of a call is longer than the kernel's.
+_dtype_of = attrgetter("dtype")
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # prism_dtype_t
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _dtype_code(t: torch.Tensor, what: str) -> int:
@@ -436,18 +442,32 @@ def _dtype_code(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _same_device(*ts):
-    """Every tensor on one CUDA device, which is made the current one for the launch (the
-    kernels launch on that device's current stream)."""
-    _check_cuda(*ts)
-    dev = None
+def _device_of(*ts) -> int:
+    """The one CUDA device that every tensor is on."""
+    index = None
     for t in ts:
         if t is not None:
-            if dev is None:
-                dev = t.device
-            elif t.device != dev:
-                raise ValueError(f"tensors on different devices: {dev} and {t.device}")
-    return torch.cuda.device(dev)
+            if not t.is_cuda:
+                _check_cuda(t)
+            i = t.get_device()
+            if index is None:
+                index = i
+            elif i != index:
+                raise ValueError(f"tensors on different devices: cuda:{index} and cuda:{i}")
+    return index
+
+
+def _launch(name: str, index: int, *args) -> None:
+    """_lib.call on the device's current stream, with the device made current if it is not."""
+    if index == _current_device():
+        _lib.call(name, *args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, _raw_stream(index))
+
+
+def _at(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
 
 
 def _fp32_vector(w: Optional[torch.Tensor], n: int, what: str):
@@ -455,19 +475,24 @@ def _fp32_vector(w: Optional[torch.Tensor], n: int, what: str):
         return None
     if w.dim() != 1 or w.shape[0] != n:
         raise ValueError(f"{what} must have shape [{n}], got {tuple(w.shape)}")
-    return w.to(torch.float32).contiguous()
+    return w if w.dtype == torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous()
 
 
 def _rows2d(t: Optional[torch.Tensor], cols: int):
     """[..., cols] -> a [rows, cols] view with unit column stride (a copy where there is none)."""
     if t is None:
         return None
-    t = t.reshape(-1, cols)
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
     return t if cols == 1 or t.stride(1) == 1 else t.contiguous()
 
 
 def _ld(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.stride(0)
+
+
+def _new_like(x: torch.Tensor, dtype=None) -> torch.Tensor:
+    return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 def _rows_input(x, residual, weight, what):
@@ -483,87 +508,99 @@ def _rows_input(x, residual, weight, what):
 def add_rms_norm(x, residual=None, weight=None, eps: float = 1e-6, want_rstd: bool = False):
     """prism_add_rms_norm: (y, h, rstd), y and h shaped as x, rstd [rows] fp32 or None; h is
     None without a residual."""
-    with _same_device(x, residual, weight):
-        code, cols, x2, r2, w = _rows_input(x, residual, weight, "add_rms_norm")
-        rows = x2.shape[0]
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
-        _lib.call("prism_add_rms_norm", _p(x2), _ld(x2), _p(r2), _ld(r2), _p(w), float(eps), rows, cols, code,
-                  _p(y), _p(h), _p(rstd), _stream(x))
+    dev = _device_of(x, residual, weight)
+    code, cols, x2, r2, w = _rows_input(x, residual, weight, "add_rms_norm")
+    rows = x2.shape[0]
+    y = _new_like(x)
+    h = None if residual is None else _new_like(x)
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
+    _launch("prism_add_rms_norm", dev, x2.data_ptr(), x2.stride(0), _at(r2), _ld(r2), _at(w), eps, rows, cols, code,
+            y.data_ptr(), _at(h), _at(rstd))
     return y, h, rstd
 
 
 def add_rms_norm_fp8(x, residual=None, weight=None, eps: float = 1e-6, normalize: bool = True):
     """prism_add_rms_norm_fp8: (y8 e4m3 shaped as x, scale [x.shape[:-1]] fp32, h or None)."""
-    with _same_device(x, residual, weight):
-        code, cols, x2, r2, w = _rows_input(x, residual, weight, "add_rms_norm_fp8")
-        y8 = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        h = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _lib.call("prism_add_rms_norm_fp8", _p(x2), _ld(x2), _p(r2), _ld(r2), _p(w), float(eps), int(normalize),
-                  x2.shape[0], cols, code, _p(y8), _p(scale), _p(h), _stream(x))
+    dev = _device_of(x, residual, weight)
+    code, cols, x2, r2, w = _rows_input(x, residual, weight, "add_rms_norm_fp8")
+    y8 = _new_like(x, torch.float8_e4m3fn)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    h = None if residual is None else _new_like(x)
+    _launch("prism_add_rms_norm_fp8", dev, x2.data_ptr(), x2.stride(0), _at(r2), _ld(r2), _at(w), eps, int(normalize),
+            x2.shape[0], cols, code, y8.data_ptr(), scale.data_ptr(), _at(h))
     return y8, scale, h
 
 
 def add_rms_norm_bwd(gy, h, rstd, gh=None, weight=None, want_dweight: bool = True):
     """prism_add_rms_norm_bwd: (dx shaped as h, dweight [cols] fp32 or None)."""
-    with _same_device(gy, h, rstd, gh, weight):
-        code, cols = _dtype_code(h, "add_rms_norm_bwd"), h.shape[-1]
-        g2, h2, gh2 = _rows2d(gy, cols), _rows2d(h, cols), _rows2d(gh, cols)
-        w = _fp32_vector(weight, cols, "weight")
-        rows = h2.shape[0]
-        dx = torch.empty(h.shape, dtype=h.dtype, device=h.device)
-        dw = torch.empty(cols, dtype=torch.float32, device=h.device) if want_dweight else None
-        ws = (_ws(_lib.query("prism_add_rms_norm_bwd_workspace_bytes", rows, cols), h.device)
-              if want_dweight else None)
-        _lib.call("prism_add_rms_norm_bwd", _p(g2), _ld(g2), _p(h2), _ld(h2), _p(gh2), _ld(gh2), _p(w), _p(rstd),
-                  rows, cols, code, _p(dx), _p(ws), _p(dw), _stream(h))
+    dev = _device_of(gy, h, rstd, gh, weight)
+    code, cols = _dtype_code(h, "add_rms_norm_bwd"), h.shape[-1]
+    g2, h2, gh2 = _rows2d(gy, cols), _rows2d(h, cols), _rows2d(gh, cols)
+    w = _fp32_vector(weight, cols, "weight")
+    rows = h2.shape[0]
+    dx = _new_like(h)
+    dw = ws = None
+    if want_dweight:
+        dw = torch.empty(cols, dtype=torch.float32, device=h.device)
+        ws = _ws(_lib.query("prism_add_rms_norm_bwd_workspace_bytes", rows, cols), h.device)
+    _launch("prism_add_rms_norm_bwd", dev, g2.data_ptr(), g2.stride(0), h2.data_ptr(), h2.stride(0), _at(gh2),
+            _ld(gh2), _at(w), rstd.data_ptr(), rows, cols, code, dx.data_ptr(), _at(ws), _at(dw))
     return dx, dw
+
+
+_Strides3, _Strides2, _Ends = ctypes.c_int64 * 3, ctypes.c_int64 * 2, ctypes.c_int * 2
 
 
 def rotary(q, k, positions, freqs, section_ends, interleaved: bool, scale: float, conjugate: bool = False):
     """prism_rotary on q [B, S, Hq, D] and k [B, S, Hk, D] or None (unit column stride);
     positions [B, S, axes] integers with unit axis stride, freqs [rot / 2] fp64 -> new (q, k)."""
-    with _same_device(q, k, positions, freqs):
-        B, S, hq, D = q.shape
-        hk = 0 if k is None else k.shape[2]
-        qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        s3 = lambda t: None if t is None else (ctypes.c_int64 * 3)(*t.stride()[:3])
-        _lib.call("prism_rotary", _p(q), s3(q), hq, _p(k), s3(k), hk, B, S, D, 2 * freqs.shape[0], int(interleaved),
-                  _p(positions), int(positions.dtype == torch.int64), (ctypes.c_int64 * 2)(*positions.stride()[:2]),
-                  (ctypes.c_int * 2)(*section_ends), _p(freqs), float(scale), int(conjugate),
-                  _dtype_code(q, "rotary"), _p(qo), s3(qo), _p(ko), s3(ko), _stream(q))
+    dev = _device_of(q, k, positions, freqs)
+    B, S, hq, D = q.shape
+    hk, ko, k_at, k_in, ko_at, k_out = 0, None, None, None, None, None
+    qo = _new_like(q)
+    if k is not None:
+        hk, ko = k.shape[2], _new_like(k)
+        k_at, k_in, ko_at, k_out = k.data_ptr(), _Strides3(*k.stride()[:3]), ko.data_ptr(), _Strides3(S * hk * D, hk * D, D)
+    _launch("prism_rotary", dev, q.data_ptr(), _Strides3(*q.stride()[:3]), hq, k_at, k_in, hk, B, S, D,
+            2 * freqs.shape[0], int(interleaved), positions.data_ptr(), int(positions.dtype == torch.int64),
+            _Strides2(*positions.stride()[:2]), _Ends(*section_ends), freqs.data_ptr(), scale, int(conjugate),
+            _dtype_code(q, "rotary"), qo.data_ptr(), _Strides3(S * hq * D, hq * D, D), ko_at, k_out)
     return qo, ko
 
 
 def clip_grad_norm(grads, outs, max_norm: float) -> torch.Tensor:
-    """prism_clip_grad_norm over dense tensors (outs[i] may be grads[i]) -> norm, 0-dim fp32."""
-    dev = grads[0].device
-    with torch.cuda.device(dev):
-        n = len(grads)
-        ptrs = (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads])
-        optrs = (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
-        sizes = (ctypes.c_int64 * n)(*[g.numel() for g in grads])
-        codes = (ctypes.c_int * n)(*[_dtype_code(g, "clip_grad_norm") for g in grads])
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        ws = _ws(_lib.query("prism_clip_grad_norm_workspace_bytes", sizes, n), dev)
-        _lib.call("prism_clip_grad_norm", ptrs, optrs, sizes, codes, n, float(max_norm), _p(ws), _p(norm),
-                  _stream(norm))
+    """prism_clip_grad_norm over contiguous tensors of one device (outs[i] may be grads[i]) ->
+    norm, 0-dim fp32."""
+    dev, n = grads[0].device, len(grads)
+    ptrs = array("q", map(torch.Tensor.data_ptr, grads))
+    sizes = array("q", map(torch.Tensor.numel, grads))
+    types = list(map(_dtype_of, grads))
+    try:
+        codes = array("i", map(_DTYPES.__getitem__, types))
+    except KeyError as e:
+        raise TypeError(f"clip_grad_norm expects bf16, fp16 or fp32, got {e.args[0]}") from None
+    optrs = ptrs
+    if outs is not grads:
+        optrs = array("q", map(torch.Tensor.data_ptr, outs))
+        if list(map(torch.Tensor.numel, outs)) != sizes.tolist() or list(map(_dtype_of, outs)) != types:
+            raise ValueError("an output must have the type and the number of elements of its gradient")
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = _ws(_lib.query("prism_clip_grad_norm_workspace_bytes", n), dev)
+    _launch("prism_clip_grad_norm", norm.get_device(), *(a.buffer_info()[0] for a in (ptrs, optrs, sizes, codes)), n,
+            max_norm, ws.data_ptr(), norm.data_ptr())
     return norm
 
 
 def linear_fp8(x8, x_scale, w8, w_scale, bias=None) -> torch.Tensor:
     """prism_linear_fp8: x8 [M, K], w8 [N, K] e4m3 (unit column stride), x_scale [M], w_scale [N]
     fp32 -> [M, N] bf16."""
-    with _same_device(x8, x_scale, w8, w_scale, bias):
-        M, K = x8.shape
-        N = w8.shape[0]
-        out = torch.empty(M, N, dtype=torch.bfloat16, device=x8.device)
-        b = _fp32_vector(bias, N, "bias")
-        _lib.call("prism_linear_fp8", _p(x8), x8.stride(0), _p(x_scale), _p(w8), w8.stride(0), _p(w_scale), _p(b),
-                  M, N, K, _p(out), N, _stream(x8))
+    dev = _device_of(x8, x_scale, w8, w_scale, bias)
+    M, K = x8.shape
+    N = w8.shape[0]
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=x8.device)
+    b = _fp32_vector(bias, N, "bias")
+    _launch("prism_linear_fp8", dev, x8.data_ptr(), x8.stride(0), x_scale.data_ptr(), w8.data_ptr(), w8.stride(0),
+            w_scale.data_ptr(), _at(b), M, N, K, out.data_ptr(), N)
     return out
 
 

@@ -162,3 +162,17 @@ def test_refusals(cuda):
         clip_grad_norm([g.double()], 1.0)
     with pytest.raises(_lib.PrismError):
         clip_grad_norm([g, torch.ones(3)], 1.0)
+
+
+def test_slices_of_a_flat_buffer_as_outputs(cuda):
+    """A 2D gradient into its slice of a flat buffer, row-major whatever the gradient's strides."""
+    g = torch.randn(30, 50, generator=torch.Generator().manual_seed(4)).to(cuda)
+    for grad in (g, g.t().contiguous().t(), torch.cat((g, g), 1)[:, :50]):
+        flat = torch.zeros(1600, device=cuda)
+        norm = clip_grad_norm([grad], 0.5, out=[flat[32:1532]])
+        _check([grad], [g], [flat[32:1532].view(30, 50)], norm, 0.5)
+        assert not bool(flat[:32].any()) and not bool(flat[1532:].any())
+    with pytest.raises(ValueError):
+        clip_grad_norm([g], 1.0, out=[flat[:1499]])
+    with pytest.raises(ValueError):
+        clip_grad_norm([g.t()], 1.0, out=[flat[:1499]])
