@@ -4,12 +4,20 @@
 //   u   = (mean_j h_j^2 + eps)^(-1/2)
 //   y_j = w_j h_j u
 // 8-bit rows: s = max(max_j |y_j| / 448, 2^-100), y8_j = e4m3(y_j / s).  u cancels in y_j / s,
-// so one reduction gives both sum h^2 and max |w h|.  A row that holds a NaN or an infinity
-// has scale NaN.
+// so one reduction gives both sum h^2 and max |w h|.  A row that holds a NaN or an infinity (or,
+// normalised, whose squares overflow fp32) has scale NaN.
 // Backward, with gy = dL/dy and gh = dL/dh:
 //   dL/dh_j = u (w_j gy_j) - h_j u^3 / C * sum_i w_i gy_i h_i + gh_j   (also dL/dx and dL/dr)
 //   dL/dw_j = sum over rows of gy_j h_j u
 // Sums, u and the gradient of w are held in fp32.
+//
+// Bound by memory: each tensor is read or written once.  A row stays with one group of threads --
+// a power of two of lanes for narrow rows, a CTA for wide ones -- which holds it in registers
+// between the row's reduction and its outputs, 8 or 16 elements a thread.  Groups are persistent
+// (they hold their columns of w, and sum their columns of dL/dw, in registers over all their
+// rows) and fetch the next rows with cp.async into slots of shared memory that only the fetching
+// thread reads: no barrier but the reduction's, and the loads of kStages rows are on their way
+// while one is reduced.
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -20,34 +28,396 @@ namespace norm {
 
 constexpr float kFp8Max = 448.0f;                      // largest finite e4m3 value
 constexpr float kScaleFloor = 7.8886090522101181e-31f;  // 2^-100: 1 / scale stays finite
-constexpr int kThreads = 256;
+constexpr float kFloatMax = 3.402823466e38f;
+constexpr int kThreads = 256;   // of the kernels whose groups are smaller than a CTA
+constexpr int kSms = 148;
 
 struct SumMax {
   float sum, max;
 };
 
-// Block reduction of a sum and a maximum, in a fixed order; every thread gets the result.
-__device__ __forceinline__ SumMax block_sum_max(SumMax v, SumMax* red) {
-  v.sum = warp_sum(v.sum);
-  v.max = warp_max(v.max);
-  const int w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  if ((threadIdx.x & 31) == 0) red[w] = v;
-  __syncthreads();
-  SumMax t = red[0];
-  for (int i = 1; i < nw; ++i) {
-    t.sum += red[i].sum;
-    t.max = fmaxf(t.max, red[i].max);
+// Sum and maximum over the `group` lanes of a sub-warp, or over the CTA; every thread gets them.
+// `red` alternates between two rows, so that one barrier a reduction is enough.
+template <bool kCta>
+__device__ __forceinline__ SumMax group_reduce(SumMax v, int group, SumMax (*red)[32], int turn) {
+  const int top = kCta ? 16 : group / 2;
+  for (int o = top; o >= 1; o >>= 1) {
+    v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
+    v.max = fmaxf(v.max, __shfl_xor_sync(0xffffffffu, v.max, o));
   }
-  return t;
+  if constexpr (kCta) {
+    SumMax* row = red[turn & 1];
+    const int nw = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) row[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = row[0];
+    for (int i = 1; i < nw; ++i) {
+      v.sum += row[i].sum;
+      v.max = fmaxf(v.max, row[i].max);
+    }
+  }
+  return v;
 }
 
-// One CTA per row; kQuant: 8-bit rows; normalize = 0: the rows themselves (u = 1).
+// scale of an 8-bit row and the factor that takes w h to its 8-bit values.
+struct Quant {
+  float scale, factor;
+};
+__device__ __forceinline__ Quant quantizer(const SumMax& t, float u) {
+  Quant q;
+  q.scale = fmaxf(t.max * u / kFp8Max, kScaleFloor);
+  if (!(t.sum <= kFloatMax)) q.scale = NAN;
+  q.factor = u / q.scale;
+  return q;
+}
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+
+// Where a thread works: its group's rows and its columns of a row.  With kShift the rows are not
+// 16-byte aligned, all tensors' in the same way: `lead` single elements, vectors, single elements;
+// a thread has at most one single element.  The rows of a group are all shifted alike (the groups'
+// row step is a multiple of the period of the shifts).
+template <typename T, int kPer, bool kCta, bool kShift>
+struct Place {
+  static constexpr int kWidth = 16 / sizeof(T), kVecs = kPer / kWidth;
+  int group, lane, lead, vecs, single;  // single: column of the single element, or -1
+  int64_t first, warp_first, step;      // the group's first row, that of the warp's first group
+
+  __device__ __forceinline__ Place(const T* base, int64_t ld, int cols, int group_) {
+    group = kCta ? (int)blockDim.x : group_;
+    lane = kCta ? (int)threadIdx.x : (int)(threadIdx.x & (group - 1));
+    const int per_cta = kCta ? 1 : (int)blockDim.x / group;
+    const int64_t at = (int64_t)blockIdx.x * per_cta;
+    first = kCta ? at : at + threadIdx.x / group;
+    warp_first = kCta ? at : at + (threadIdx.x & ~31u) / group;
+    step = (int64_t)gridDim.x * per_cta;
+    lead = 0, single = -1;
+    if (kShift) {
+      const unsigned off = (unsigned)(reinterpret_cast<uintptr_t>(base) + (uint64_t)(first * ld) * sizeof(T)) & 15u;
+      lead = min(cols, (int)((16u - off) & 15u) / (int)sizeof(T));
+    }
+    vecs = (cols - lead) / kWidth;
+    if (kShift) {
+      const int tail = cols - lead - vecs * kWidth;
+      if (lane < lead) single = lane;
+      else if (lane - lead < tail) single = cols - tail + lane - lead;
+    }
+  }
+  // column of the thread's v-th vector, or -1
+  __device__ __forceinline__ int column(int v) const {
+    const int i = lane + v * group;
+    return i < vecs ? lead + i * kWidth : -1;
+  }
+};
+
+// Thread-private slots: kStages rows of kTensors tensors.
+template <int kTensors, int kVecs, int kStages>
+struct Ring {
+  uint4* slots;
+  __device__ __forceinline__ explicit Ring(uint4* smem) : slots(smem + threadIdx.x) {}
+  __device__ __forceinline__ uint4* at(int stage, int tensor, int v) const {
+    return slots + ((stage * kTensors + tensor) * kVecs + v) * (int)blockDim.x;
+  }
+  static __device__ __forceinline__ void load(uint4* slot, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(slot)), "l"(src)
+                 : "memory");
+  }
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
+  static __device__ __forceinline__ void drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+};
+
+// A thread's columns of w (1 without a weight) as registers; one more for the single element.
+template <int kPer, typename P>
+__device__ __forceinline__ void load_weight(const P& p, const float* w, float (&wv)[kPer], float& ws) {
+#pragma unroll
+  for (int v = 0; v < P::kVecs; ++v) {
+    const int c = p.column(v);
+#pragma unroll
+    for (int e = 0; e < P::kWidth; ++e) wv[v * P::kWidth + e] = w && c >= 0 ? __ldg(w + c + e) : 1.0f;
+  }
+  ws = w && p.single >= 0 ? __ldg(w + p.single) : 1.0f;
+}
+
+// Rows on their way: what 220 KB hold of 1,024 threads' slots.  Only fp32 rows at 16 elements a
+// thread (64 bytes) have to do with one.
+constexpr int fwd_stages(int bytes) { return bytes <= 32 ? 3 : 1; }
+constexpr int bwd_stages(int bytes) { return bytes <= 32 ? 2 : 1; }
+
+// kQuant: 8-bit rows.  normalize = 0: the rows themselves (u = 1).
+template <typename T, int kPer, bool kCta, bool kShift, bool kQuant>
+__global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
+    fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ r, int64_t ldr,
+               const float* __restrict__ w, float eps, int normalize, int64_t rows, int cols, int group,
+               void* __restrict__ y, T* __restrict__ h, float* __restrict__ aux) {
+  using P = Place<T, kPer, kCta, kShift>;
+  constexpr int kWidth = P::kWidth, kVecs = P::kVecs;
+  extern __shared__ uint4 smem[];
+  __shared__ SumMax red[2][32];
+  const P p(x, ldx, cols, group);
+  constexpr int kStages = fwd_stages(kPer * sizeof(T));
+  const Ring<2, kVecs, kStages> ring(smem);
+  const auto fetch = [&](int64_t row, int stage) {
+    if (row < rows) {
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const int c = p.column(v);
+        if (c >= 0) {
+          ring.load(ring.at(stage, 0, v), x + row * ldx + c);
+          if (r) ring.load(ring.at(stage, 1, v), r + row * ldr + c);
+        }
+      }
+    }
+    ring.commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) fetch(p.first + s * p.step, s);
+  float wv[kPer], ws;
+  load_weight(p, w, wv, ws);
+  const bool has_single = kShift && p.single >= 0;
+  float xs = 0.0f, rs = 0.0f;
+  const auto fetch_single = [&](int64_t row) {
+    if (has_single && row < rows) {
+      xs = Elem<T>::to_f(x[row * ldx + p.single]);
+      if (r) rs = Elem<T>::to_f(r[row * ldr + p.single]);
+    }
+  };
+  if (kShift) fetch_single(p.first);
+
+  int stage = 0, turn = 0;
+  for (int64_t row = p.first, warp_row = p.warp_first; warp_row < rows; row += p.step, warp_row += p.step, ++turn) {
+    ring.wait();
+    const bool live = row < rows;
+    float hv[kPer], hs = xs;
+    SumMax t = {0.0f, 0.0f};
+    const auto take = [&](float f, float wf) {
+      t.sum += normalize ? f * f : f * 0.0f;  // without a norm, only a NaN or an infinity counts
+      if (kQuant) t.max = fmaxf(t.max, fabsf(f * wf));
+    };
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      const int c = p.column(v);
+      float f[kWidth] = {};
+      if (live && c >= 0) {
+        unpack<T>(*ring.at(stage, 0, v), f);
+        if (r) {
+          float g[kWidth];
+          unpack<T>(*ring.at(stage, 1, v), g);
+#pragma unroll
+          for (int e = 0; e < kWidth; ++e) f[e] += g[e];
+          const uint4 packed = pack<T>(f);
+          *reinterpret_cast<uint4*>(h + row * cols + c) = packed;
+          unpack<T>(packed, f);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kWidth; ++e) {
+        hv[v * kWidth + e] = f[e];
+        take(f[e], wv[v * kWidth + e]);
+      }
+    }
+    if (has_single && live) {
+      if (r) {
+        const T v = Elem<T>::from_f(xs + rs);
+        h[row * cols + p.single] = v;
+        hs = Elem<T>::to_f(v);
+      }
+      take(hs, ws);
+    }
+    fetch(row + kStages * p.step, stage);
+    if (kShift) fetch_single(row + p.step);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    t = group_reduce<kCta>(t, p.group, red, turn);
+    const float u = normalize ? rsqrtf(t.sum / (float)cols + eps) : 1.0f;
+    if (!live) continue;
+    if constexpr (kQuant) {
+      const Quant q = quantizer(t, u);
+      uint8_t* out = static_cast<uint8_t*>(y) + row * cols;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const int c = p.column(v);
+        if (c < 0) continue;
+        uint32_t b[kWidth / 4];
+#pragma unroll
+        for (int e = 0; e < kWidth; e += 4) {
+          const int i = v * kWidth + e;
+          b[e / 4] = e4m3x2(hv[i] * wv[i] * q.factor, hv[i + 1] * wv[i + 1] * q.factor) |
+                     e4m3x2(hv[i + 2] * wv[i + 2] * q.factor, hv[i + 3] * wv[i + 3] * q.factor) << 16;
+        }
+        if constexpr (kShift) {  // the bytes' alignment is not the elements'
+          if (reinterpret_cast<uintptr_t>(out + c) % 4 == 0) {
+#pragma unroll
+            for (int e = 0; e < kWidth; e += 4) *reinterpret_cast<uint32_t*>(out + c + e) = b[e / 4];
+          } else {
+#pragma unroll
+            for (int e = 0; e < kWidth; ++e) out[c + e] = (uint8_t)(b[e / 4] >> (8 * (e % 4)));
+          }
+        } else if constexpr (kWidth == 8) {
+          *reinterpret_cast<uint2*>(out + c) = make_uint2(b[0], b[1]);
+        } else {
+          *reinterpret_cast<uint32_t*>(out + c) = b[0];
+        }
+      }
+      if (has_single) out[p.single] = (uint8_t)e4m3x2(hs * ws * q.factor, 0.0f);
+      if (p.lane == 0) aux[row] = q.scale;
+    } else {
+      T* out = static_cast<T*>(y) + row * cols;
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const int c = p.column(v);
+        if (c < 0) continue;
+        float f[kWidth];
+#pragma unroll
+        for (int e = 0; e < kWidth; ++e) f[e] = hv[v * kWidth + e] * u * wv[v * kWidth + e];
+        *reinterpret_cast<uint4*>(out + c) = pack<T>(f);
+      }
+      if (has_single) out[p.single] = Elem<T>::from_f(hs * u * ws);
+      if (p.lane == 0 && aux) aux[row] = u;
+    }
+  }
+  ring.drain();
+}
+
+// dL/dh of the rows, and each CTA's sum of dL/dw -> part[CTA][cols] (part NULL: not wanted).
+template <typename T, int kPer, bool kCta, bool kShift>
+__global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
+    bwd_kernel(const T* __restrict__ gy, int64_t ldgy, const T* __restrict__ h, int64_t ldh,
+               const T* __restrict__ gh, int64_t ldgh, const float* __restrict__ w,
+               const float* __restrict__ rstd, int64_t rows, int cols, int group, T* __restrict__ dx,
+               float* __restrict__ part) {
+  using P = Place<T, kPer, kCta, kShift>;
+  constexpr int kWidth = P::kWidth, kVecs = P::kVecs;
+  extern __shared__ uint4 smem[];
+  __shared__ SumMax red[2][32];
+  const P p(gy, ldgy, cols, group);
+  constexpr int kStages = bwd_stages(kPer * sizeof(T));
+  const Ring<3, kVecs, kStages> ring(smem);
+  const auto fetch = [&](int64_t row, int stage) {
+    if (row < rows) {
+#pragma unroll
+      for (int v = 0; v < kVecs; ++v) {
+        const int c = p.column(v);
+        if (c >= 0) {
+          ring.load(ring.at(stage, 0, v), gy + row * ldgy + c);
+          ring.load(ring.at(stage, 1, v), h + row * ldh + c);
+          if (gh) ring.load(ring.at(stage, 2, v), gh + row * ldgh + c);
+        }
+      }
+    }
+    ring.commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kStages; ++s) fetch(p.first + s * p.step, s);
+  float wv[kPer], ws, dw[kPer] = {}, dws = 0.0f;
+  load_weight(p, w, wv, ws);
+  const bool has_single = kShift && p.single >= 0;
+  float gs = 0.0f, hs = 0.0f, ghs = 0.0f, u_next = 0.0f;
+  const auto fetch_single = [&](int64_t row) {
+    if (row < rows) {
+      u_next = __ldg(rstd + row);
+      if (has_single) {
+        gs = Elem<T>::to_f(gy[row * ldgy + p.single]);
+        hs = Elem<T>::to_f(h[row * ldh + p.single]);
+        if (gh) ghs = Elem<T>::to_f(gh[row * ldgh + p.single]);
+      }
+    }
+  };
+  fetch_single(p.first);
+
+  int stage = 0, turn = 0;
+  for (int64_t row = p.first, warp_row = p.warp_first; warp_row < rows; row += p.step, warp_row += p.step, ++turn) {
+    ring.wait();
+    const bool live = row < rows;
+    const float u = u_next, gs0 = gs, hs0 = hs, ghs0 = ghs;
+    SumMax t = {0.0f, 0.0f};
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      if (!live || p.column(v) < 0) continue;
+      float g[kWidth], hf[kWidth];
+      unpack<T>(*ring.at(stage, 0, v), g);
+      unpack<T>(*ring.at(stage, 1, v), hf);
+#pragma unroll
+      for (int e = 0; e < kWidth; ++e) {
+        const float gh_e = g[e] * hf[e];
+        t.sum += gh_e * wv[v * kWidth + e];
+        dw[v * kWidth + e] += gh_e * u;
+      }
+    }
+    if (has_single && live) {
+      t.sum += gs0 * hs0 * ws;
+      dws += gs0 * hs0 * u;
+    }
+    fetch_single(row + p.step);
+    t = group_reduce<kCta>(t, p.group, red, turn);
+    const float k = t.sum * u * u * u / (float)cols;
+    // the row is read a second time from its slots: held in registers it would spill
+#pragma unroll
+    for (int v = 0; v < kVecs; ++v) {
+      const int c = p.column(v);
+      if (!live || c < 0) continue;
+      float g[kWidth], hf[kWidth], add[kWidth] = {};
+      unpack<T>(*ring.at(stage, 0, v), g);
+      unpack<T>(*ring.at(stage, 1, v), hf);
+      if (gh) unpack<T>(*ring.at(stage, 2, v), add);
+#pragma unroll
+      for (int e = 0; e < kWidth; ++e) add[e] += g[e] * wv[v * kWidth + e] * u - hf[e] * k;
+      *reinterpret_cast<uint4*>(dx + row * cols + c) = pack<T>(add);
+    }
+    if (has_single && live) dx[row * cols + p.single] = Elem<T>::from_f(gs0 * ws * u - hs0 * k + ghs0);
+    fetch(row + kStages * p.step, stage);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  ring.drain();
+  if (part == nullptr) return;
+  float* out = part + (int64_t)blockIdx.x * cols;
+  float* mine = out;
+  float* sums = reinterpret_cast<float*>(smem);  // [groups of the CTA][cols], the ring is done
+  if (!kCta) {
+    __syncthreads();
+    mine = sums + (int)(threadIdx.x / p.group) * cols;
+  }
+#pragma unroll
+  for (int v = 0; v < kVecs; ++v) {
+    const int c = p.column(v);
+    if (c < 0) continue;
+#pragma unroll
+    for (int e = 0; e < kWidth; ++e) mine[c + e] = dw[v * kWidth + e];
+  }
+  if (has_single) mine[p.single] = dws;
+  if (!kCta) {
+    __syncthreads();
+    const int groups = blockDim.x / p.group;
+    for (int c = threadIdx.x; c < cols; c += blockDim.x) {
+      float s = 0.0f;
+      for (int i = 0; i < groups; ++i) s += sums[i * cols + c];
+      out[c] = s;
+    }
+  }
+}
+
+// dL/dw = sum of the partial sums: 32 columns a CTA, 32 threads a column, in a fixed order.
+__global__ void __launch_bounds__(1024)
+    weight_sum_kernel(const float* __restrict__ part, int parts, int cols, float* __restrict__ dw) {
+  __shared__ float red[32][33];
+  const int lane = threadIdx.x & 31, group = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (c < cols)
+    for (int i = group; i < parts; i += 32) s += part[(int64_t)i * cols + c];
+  red[group][lane] = s;
+  __syncthreads();
+  s = warp_sum(red[lane][group]);
+  if (lane == 0 && blockIdx.x * 32 + group < cols) dw[blockIdx.x * 32 + group] = s;
+}
+
+// ------------------------------------------- rows of any width, alignment and stride
+// One CTA per row, element by element.
 template <typename T, bool kQuant>
 __global__ void __launch_bounds__(kThreads)
-    fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ r, int64_t ldr,
-               const float* __restrict__ w, float eps, int normalize, int cols, void* __restrict__ y,
-               T* h, float* __restrict__ aux) {
-  __shared__ SumMax red[32];
+    fwd_any_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ r, int64_t ldr,
+                   const float* __restrict__ w, float eps, int normalize, int cols, void* __restrict__ y,
+                   T* h, float* __restrict__ aux) {
+  __shared__ SumMax red[2][32];
   const int64_t row = blockIdx.x;
   const T* xr = x + row * ldx;
   const T* rr = r ? r + row * ldr : nullptr;
@@ -60,22 +430,20 @@ __global__ void __launch_bounds__(kThreads)
       hr[c] = v;
     }
     const float f = Elem<T>::to_f(v);
-    t.sum += f * f;
+    t.sum += normalize ? f * f : f * 0.0f;
     if (kQuant) t.max = fmaxf(t.max, fabsf(w ? f * w[c] : f));
   }
-  t = block_sum_max(t, red);
+  t = group_reduce<true>(t, kThreads, red, 0);
   const float u = normalize ? rsqrtf(t.sum / (float)cols + eps) : 1.0f;
-  const T* src = rr ? hr : xr;
+  const T* src = rr ? hr : xr;  // each thread reads back what it wrote
   if constexpr (kQuant) {
-    float scale = fmaxf(t.max * u / kFp8Max, kScaleFloor);
-    if (!(t.sum <= 3.402823466e38f)) scale = NAN;
-    const float inv = u / scale;
-    auto* out = static_cast<__nv_fp8_storage_t*>(y) + row * cols;
+    const Quant q = quantizer(t, u);
+    uint8_t* out = static_cast<uint8_t*>(y) + row * cols;
     for (int c = threadIdx.x; c < cols; c += kThreads) {
       const float f = Elem<T>::to_f(src[c]);
-      out[c] = __nv_cvt_float_to_fp8((w ? f * w[c] : f) * inv, __NV_SATFINITE, __NV_E4M3);
+      out[c] = (uint8_t)e4m3x2((w ? f * w[c] : f) * q.factor, 0.0f);
     }
-    if (threadIdx.x == 0) aux[row] = scale;
+    if (threadIdx.x == 0) aux[row] = q.scale;
   } else {
     T* out = static_cast<T*>(y) + row * cols;
     for (int c = threadIdx.x; c < cols; c += kThreads) {
@@ -86,13 +454,12 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// dL/dh of one row per CTA.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    bwd_row_kernel(const T* __restrict__ gy, int64_t ldgy, const T* __restrict__ h, int64_t ldh,
+    bwd_any_kernel(const T* __restrict__ gy, int64_t ldgy, const T* __restrict__ h, int64_t ldh,
                    const T* __restrict__ gh, int64_t ldgh, const float* __restrict__ w,
                    const float* __restrict__ rstd, int cols, T* __restrict__ dx) {
-  __shared__ SumMax red[32];
+  __shared__ SumMax red[2][32];
   const int64_t row = blockIdx.x;
   const T* gr = gy + row * ldgy;
   const T* hr = h + row * ldh;
@@ -101,7 +468,7 @@ __global__ void __launch_bounds__(kThreads)
     const float g = Elem<T>::to_f(gr[c]);
     t.sum += (w ? g * w[c] : g) * Elem<T>::to_f(hr[c]);
   }
-  t = block_sum_max(t, red);
+  t = group_reduce<true>(t, kThreads, red, 0);
   const float u = rstd[row], k = t.sum * u * u * u / (float)cols;
   for (int c = threadIdx.x; c < cols; c += kThreads) {
     const float g = Elem<T>::to_f(gr[c]);
@@ -111,10 +478,10 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Partial sums of dL/dw over slabs of rows (blockIdx.y), one thread per column.
+// Partial sums of dL/dw over slabs of `per` rows (blockIdx.y), one thread per column.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    bwd_weight_kernel(const T* __restrict__ gy, int64_t ldgy, const T* __restrict__ h, int64_t ldh,
+    weight_any_kernel(const T* __restrict__ gy, int64_t ldgy, const T* __restrict__ h, int64_t ldh,
                       const float* __restrict__ rstd, int64_t rows, int cols, int64_t per,
                       float* __restrict__ part) {
   const int c = blockIdx.x * kThreads + threadIdx.x;
@@ -126,43 +493,166 @@ __global__ void __launch_bounds__(kThreads)
   part[(int64_t)blockIdx.y * cols + c] = s;
 }
 
-// dL/dw = sum of the slabs' partial sums in slab order.
-__global__ void __launch_bounds__(kThreads)
-    bwd_weight_sum_kernel(const float* __restrict__ part, int slabs, int cols, float* __restrict__ dw) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= cols) return;
-  float s = 0.0f;
-  for (int i = 0; i < slabs; ++i) s += part[(int64_t)i * cols + c];
-  dw[c] = s;
+// ------------------------------------------------------------------ host
+struct Operand {
+  const void* ptr;  // NULL: absent
+  int64_t ld;
+};
+
+// How a call runs: by whole vectors, by vectors between single elements, or element by element.
+struct Plan {
+  bool any = true, shift = false, cta = false;
+  int per = 8, group = 32, threads = kThreads, grid = 0;
+  size_t smem = 0;
+};
+
+constexpr int kMaxParts = 4 * kSms + 8;  // CTAs of a persistent launch, at most
+
+// `tensors`: the row tensors of one element size, `loaded` of them inputs.  Vectors need rows that start alike in 16 bytes:
+// all aligned (with whole vectors to a row), or all shifted alike.  A thread takes 16 elements
+// where 8 would need more than 512 threads to a row (fewer threads, more CTAs to an SM: 5,120
+// columns run as 3 CTAs of 320 threads), and a row of up to 32 threads' elements goes to a
+// power-of-two group of lanes.
+template <size_t kSize>
+Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int loaded, int (*stages)(int)) {
+  constexpr int kWidth = 16 / (int)kSize;
+  Plan p;
+  const auto off = [](const void* q) { return (unsigned)(reinterpret_cast<uintptr_t>(q) & 15); };
+  bool aligned = cols % kWidth == 0, alike = true;
+  for (int i = 0; i < count; ++i) {
+    if (tensors[i].ptr == nullptr) continue;
+    aligned = aligned && off(tensors[i].ptr) == 0 && (rows == 1 || tensors[i].ld % kWidth == 0);
+    alike = alike && off(tensors[i].ptr) == off(tensors[0].ptr) && off(tensors[i].ptr) % kSize == 0 &&
+            (rows == 1 || tensors[i].ld % kWidth == tensors[0].ld % kWidth);
+  }
+  if (!aligned && !alike) return p;
+  p.shift = !aligned;
+  const int need = (cols + 7) / 8;
+  p.per = need > 512 ? 16 : 8;
+  const int lanes = (cols + p.per - 1) / p.per;  // threads that a row keeps busy
+  if (lanes > 1024) return p;
+  p.any = false;
+  if (lanes <= 32) {
+    // the single elements (fewer than two vectors) need a lane each
+    p.group = p.shift ? 2 * kWidth : 1;
+    while (p.group < lanes) p.group *= 2;
+  } else {
+    p.cta = true;
+    p.threads = (lanes + 31) / 32 * 32;
+  }
+  const int per_cta = p.cta ? 1 : p.threads / p.group;
+  // the ring, and room for a sum of dL/dw from each group
+  const int bytes = p.per * (int)kSize;
+  p.smem = (size_t)loaded * stages(bytes) * bytes * p.threads;
+  const size_t sums = p.cta ? 0 : (size_t)per_cta * cols * sizeof(float);
+  if (p.smem < sums) p.smem = sums;
+  const int by_regs = 65536 / (64 * p.threads), by_smem = (int)((220 << 10) / (p.smem + 1024));
+  int per_sm = by_regs < by_smem ? by_regs : by_smem;
+  per_sm = per_sm > 4 ? 4 : per_sm;
+  if (per_sm < 1) per_sm = 1;
+  const int64_t want = (rows + per_cta - 1) / per_cta;
+  p.grid = (int)(want < per_sm * kSms ? want : per_sm * kSms);
+  // groups' rows shifted alike: the row step is a multiple of the shifts' period (up to kWidth)
+  if (p.shift && (p.grid * per_cta) % kWidth != 0) p.grid = (p.grid + kWidth - 1) / kWidth * kWidth;
+  return p;
 }
 
-constexpr int kSlabs = 296;
+template <typename K>
+cudaError_t allow_smem(K kernel, size_t bytes) {
+  return bytes > (40 << 10)  // 48 KB without asking, static arrays included
+             ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)
+             : cudaSuccess;
+}
+
+// Calls fn with the plan's compile-time choices: fn(elements a thread, CTA rows, shifted rows).
+template <typename F>
+cudaError_t with_plan(const Plan& p, F&& fn) {
+  using std::integral_constant;
+  const auto shift = [&](auto per, auto cta) {
+    return p.shift ? fn(per, cta, integral_constant<bool, true>{}) : fn(per, cta, integral_constant<bool, false>{});
+  };
+  const auto cta = [&](auto per) {
+    return p.cta ? shift(per, integral_constant<bool, true>{}) : shift(per, integral_constant<bool, false>{});
+  };
+  return p.per == 8 ? cta(integral_constant<int, 8>{}) : cta(integral_constant<int, 16>{});
+}
+
+template <typename T, bool kQuant>
+cudaError_t forward(const T* x, int64_t ldx, const T* r, int64_t ldr, const float* w, float eps, int normalize,
+                    int64_t rows, int cols, void* y, T* h, float* aux, cudaStream_t stream) {
+  const Operand tensors[4] = {{x, ldx}, {r, ldr}, {h, cols}, {kQuant ? nullptr : y, cols}};
+  Plan p = plan_rows<sizeof(T)>(tensors, 4, rows, cols, 2, fwd_stages);
+  // whole vectors of bytes: the 8-bit rows start on their own vectors' boundaries
+  if (kQuant && !p.any && !p.shift && reinterpret_cast<uintptr_t>(y) % (16 / sizeof(T)) != 0) p.any = true;
+  if (p.any) {
+    fwd_any_kernel<T, kQuant><<<(unsigned)rows, kThreads, 0, stream>>>(x, ldx, r, ldr, w, eps, normalize, cols, y, h,
+                                                                       aux);
+    return cudaGetLastError();
+  }
+  return with_plan(p, [&](auto per, auto cta, auto shift) {
+    const auto kernel = fwd_kernel<T, per(), cta(), shift(), kQuant>;
+    const cudaError_t e = allow_smem(kernel, p.smem);
+    if (e != cudaSuccess) return e;
+    kernel<<<p.grid, p.threads, p.smem, stream>>>(x, ldx, r, ldr, w, eps, normalize, rows, cols, p.group, y, h, aux);
+    return cudaGetLastError();
+  });
+}
+
+template <typename T>
+cudaError_t backward(const T* gy, int64_t ldgy, const T* h, int64_t ldh, const T* gh, int64_t ldgh, const float* w,
+                     const float* rstd, int64_t rows, int cols, T* dx, float* part, float* dw, cudaStream_t stream) {
+  const Operand tensors[4] = {{gy, ldgy}, {h, ldh}, {gh, ldgh}, {dx, cols}};
+  const Plan p = plan_rows<sizeof(T)>(tensors, 4, rows, cols, 3, bwd_stages);
+  int parts = p.grid;
+  if (p.any) {
+    bwd_any_kernel<T><<<(unsigned)rows, kThreads, 0, stream>>>(gy, ldgy, h, ldh, gh, ldgh, w, rstd, cols, dx);
+    if (dw) {
+      const int64_t slabs = rows < kMaxParts ? rows : kMaxParts, per = (rows + slabs - 1) / slabs;
+      parts = (int)slabs;
+      weight_any_kernel<T><<<dim3((unsigned)((cols + kThreads - 1) / kThreads), (unsigned)slabs), kThreads, 0, stream>>>(
+          gy, ldgy, h, ldh, rstd, rows, cols, per, part);
+    }
+  } else {
+    const cudaError_t e = with_plan(p, [&](auto per, auto cta, auto shift) {
+      const auto kernel = bwd_kernel<T, per(), cta(), shift()>;
+      const cudaError_t a = allow_smem(kernel, p.smem);
+      if (a != cudaSuccess) return a;
+      kernel<<<p.grid, p.threads, p.smem, stream>>>(gy, ldgy, h, ldh, gh, ldgh, w, rstd, rows, cols, p.group, dx,
+                                                    dw ? part : nullptr);
+      return cudaGetLastError();
+    });
+    if (e != cudaSuccess) return e;
+  }
+  if (dw) weight_sum_kernel<<<(unsigned)((cols + 31) / 32), 1024, 0, stream>>>(part, parts, cols, dw);
+  return cudaGetLastError();
+}
+
+bool rows_ok(int64_t rows, int cols) {
+  return rows >= 0 && rows < ((int64_t)1 << 31) && cols >= 1 && cols < (1 << 30);
+}
 
 }  // namespace norm
 }  // namespace prism
 
 using namespace prism;
 
-namespace {
-bool rows_ok(int64_t rows, int cols) { return rows >= 0 && rows < ((int64_t)1 << 31) && cols >= 1; }
-}  // namespace
-
 extern "C" {
 
 prism_status_t prism_add_rms_norm(const void* x, int64_t ldx, const void* r, int64_t ldr,
                                   const float* weight, float eps, int64_t rows, int cols, int dtype,
                                   void* y, void* h, float* rstd, cudaStream_t stream) {
-  PRISM_CHECK_ARG(rows_ok(rows, cols) && ldx >= 0 && ldr >= 0, "prism_add_rms_norm: bad sizes");
+  PRISM_CHECK_ARG(norm::rows_ok(rows, cols) && ldx >= 0 && ldr >= 0, "prism_add_rms_norm: bad sizes");
   if (rows == 0) return PRISM_OK;
   PRISM_CHECK_ARG(x && y && (r == nullptr) == (h == nullptr),
                   "prism_add_rms_norm: null pointer (h goes with r)");
+  cudaError_t err = cudaSuccess;
   const bool known = dispatch_dtype(dtype, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    norm::fwd_kernel<T, false><<<(unsigned)rows, norm::kThreads, 0, stream>>>(
-        (const T*)x, ldx, (const T*)r, ldr, weight, eps, 1, cols, y, (T*)h, rstd);
+    err = norm::forward<T, false>((const T*)x, ldx, (const T*)r, ldr, weight, eps, 1, rows, cols, y, (T*)h, rstd,
+                                  stream);
   });
   PRISM_CHECK_ARG(known, "prism_add_rms_norm: unknown element type %d", dtype);
-  PRISM_CHECK_LAUNCH("prism_add_rms_norm");
+  PRISM_CHECK_CUDA(err, "prism_add_rms_norm");
   return PRISM_OK;
 }
 
@@ -170,52 +660,48 @@ prism_status_t prism_add_rms_norm_fp8(const void* x, int64_t ldx, const void* r,
                                       const float* weight, float eps, int normalize, int64_t rows,
                                       int cols, int dtype, void* y8, float* scale, void* h,
                                       cudaStream_t stream) {
-  PRISM_CHECK_ARG(rows_ok(rows, cols) && ldx >= 0 && ldr >= 0, "prism_add_rms_norm_fp8: bad sizes");
+  PRISM_CHECK_ARG(norm::rows_ok(rows, cols) && ldx >= 0 && ldr >= 0, "prism_add_rms_norm_fp8: bad sizes");
   if (rows == 0) return PRISM_OK;
   PRISM_CHECK_ARG(x && y8 && scale && (r == nullptr) == (h == nullptr),
                   "prism_add_rms_norm_fp8: null pointer (h goes with r)");
+  cudaError_t err = cudaSuccess;
   const bool known = dispatch_dtype(dtype, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    norm::fwd_kernel<T, true><<<(unsigned)rows, norm::kThreads, 0, stream>>>(
-        (const T*)x, ldx, (const T*)r, ldr, weight, eps, normalize, cols, y8, (T*)h, scale);
+    err = norm::forward<T, true>((const T*)x, ldx, (const T*)r, ldr, weight, eps, normalize, rows, cols, y8, (T*)h,
+                                 scale, stream);
   });
   PRISM_CHECK_ARG(known, "prism_add_rms_norm_fp8: unknown element type %d", dtype);
-  PRISM_CHECK_LAUNCH("prism_add_rms_norm_fp8");
+  PRISM_CHECK_CUDA(err, "prism_add_rms_norm_fp8");
   return PRISM_OK;
 }
 
 size_t prism_add_rms_norm_bwd_workspace_bytes(int64_t rows, int cols) {
-  const int64_t slabs = rows < norm::kSlabs ? rows : norm::kSlabs;
-  return (size_t)slabs * (size_t)cols * sizeof(float);
+  // a partial sum of dL/dw for each CTA; rows shifted in 16 bytes round the CTAs up to 8
+  const int64_t parts = rows + 8 < norm::kMaxParts ? rows + 8 : norm::kMaxParts;
+  return rows <= 0 || cols <= 0 ? 0 : (size_t)parts * (size_t)cols * sizeof(float);
 }
 
 prism_status_t prism_add_rms_norm_bwd(const void* gy, int64_t ldgy, const void* h, int64_t ldh,
                                       const void* gh, int64_t ldgh, const float* weight,
                                       const float* rstd, int64_t rows, int cols, int dtype, void* dx,
                                       void* workspace, float* dweight, cudaStream_t stream) {
-  PRISM_CHECK_ARG(rows_ok(rows, cols) && ldgy >= 0 && ldh >= 0 && ldgh >= 0,
+  PRISM_CHECK_ARG(norm::rows_ok(rows, cols) && ldgy >= 0 && ldh >= 0 && ldgh >= 0,
                   "prism_add_rms_norm_bwd: bad sizes");
   PRISM_CHECK_ARG(rows == 0 || (gy && h && rstd && dx && (dweight == nullptr || workspace)),
                   "prism_add_rms_norm_bwd: null pointer");
   if (rows == 0) {
-    if (dweight) PRISM_CHECK_CUDA(cudaMemsetAsync(dweight, 0, sizeof(float) * cols, stream), "prism_add_rms_norm_bwd");
+    if (dweight)
+      PRISM_CHECK_CUDA(cudaMemsetAsync(dweight, 0, sizeof(float) * cols, stream), "prism_add_rms_norm_bwd");
     return PRISM_OK;
   }
-  const int64_t slabs = rows < norm::kSlabs ? rows : norm::kSlabs, per = (rows + slabs - 1) / slabs;
-  const unsigned groups = (unsigned)((cols + norm::kThreads - 1) / norm::kThreads);
+  cudaError_t err = cudaSuccess;
   const bool known = dispatch_dtype(dtype, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    norm::bwd_row_kernel<T><<<(unsigned)rows, norm::kThreads, 0, stream>>>(
-        (const T*)gy, ldgy, (const T*)h, ldh, (const T*)gh, ldgh, weight, rstd, cols, (T*)dx);
-    if (dweight) {
-      norm::bwd_weight_kernel<T><<<dim3(groups, (unsigned)slabs), norm::kThreads, 0, stream>>>(
-          (const T*)gy, ldgy, (const T*)h, ldh, rstd, rows, cols, per, (float*)workspace);
-      norm::bwd_weight_sum_kernel<<<groups, norm::kThreads, 0, stream>>>((const float*)workspace, (int)slabs,
-                                                                         cols, dweight);
-    }
+    err = norm::backward<T>((const T*)gy, ldgy, (const T*)h, ldh, (const T*)gh, ldgh, weight, rstd, rows, cols,
+                            (T*)dx, (float*)workspace, dweight, stream);
   });
   PRISM_CHECK_ARG(known, "prism_add_rms_norm_bwd: unknown element type %d", dtype);
-  PRISM_CHECK_LAUNCH("prism_add_rms_norm_bwd");
+  PRISM_CHECK_CUDA(err, "prism_add_rms_norm_bwd");
   return PRISM_OK;
 }
 

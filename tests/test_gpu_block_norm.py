@@ -66,6 +66,36 @@ def test_forward(rows, cols, dtype, residual, cuda):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [16, 24, 36, 256, 264, 512, 1000, 1024, 2048, 2056, 4096, 4100, 8192, 8200, 16384,
+                                  16392])
+def test_widths_at_the_limits_of_each_form(cols, dtype, cuda):
+    """Widths on both sides of the places where the work is split differently (lanes to a row,
+    elements to a thread, whole CTAs, shared memory), forward, 8-bit and backward, over more
+    rows than one CTA takes at a time and a group's share of one row more or less."""
+    rows = 1200 if cols <= 4100 else 450
+    x, r, w, gy, gh = _inputs(rows, cols, dtype, cuda, seed=cols)
+    x.requires_grad_(), w.requires_grad_()
+    y, h = add_rms_norm(x, r, w, EPS)
+    dx, dw = torch.autograd.grad((y, h), (x, w), (gy, gh))
+    with torch.no_grad():
+        h64, u, y64 = _forward64(x, r, w)
+        assert torch.equal(h.double(), h64)
+        _within(y, y64, _a(cols) * y64.abs(), dtype, "y")
+        y8, s, h8 = add_rms_norm_fp8(x, r, w, EPS)
+        s64 = (y64.abs().amax(-1) / 448)[:, None]
+        assert torch.equal(h8, h) and bool(((s.double()[:, None] - s64).abs() <= (_a(cols) + 2.0 ** -21) * s64).all())
+        v = y64 / s64
+        assert bool(((y8.float().double() - v).abs() <= 2.0 ** -4 * v.abs() + 2.0 ** -10 + 2 * _a(cols) * v.abs()).all())
+        g, k = gy.double(), u ** 3 / cols
+        terms = g * w.double() * h64
+        ref = g * w.double() * u - h64 * k * terms.sum(-1, keepdim=True) + gh.double()
+        size = (g * w.double() * u).abs() + h64.abs() * k * terms.abs().sum(-1, keepdim=True) + gh.double().abs()
+        _within(dx, ref, 4 * _a(cols) * size, dtype, "dx")
+        each = g * h64 * u
+        assert bool(((dw.double() - each.sum(0)).abs() <= ((rows + 64) * 2.0 ** -24 + _a(cols)) * each.abs().sum(0)).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("offset,width", [(0, 200), (1, 193), (8, 264)])
 def test_row_strides_and_offsets(dtype, offset, width, cuda):
     """Rows of wider tensors, starting at aligned and unaligned columns; 3D inputs; zero strides."""
@@ -160,7 +190,7 @@ def test_unused_outputs_and_partial_gradients(cuda):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (1, 5120), (65, 1536), (33, 1535), (2, 20011), (2, 40960),
-                                       (0, 64)])
+                                       (0, 64), (19, 1100)])
 def test_8bit_rows(rows, cols, dtype, cuda):
     """|y8 - y / scale| is half a unit of e4m3: 2^-4 of the value, or 2^-10 below its normals."""
     x, r, w, _, _ = _inputs(rows, cols, dtype, cuda, seed=3)
