@@ -140,10 +140,9 @@ __device__ __forceinline__ void load_weight(const P& p, const float* w, float (&
   ws = w && p.single >= 0 ? __ldg(w + p.single) : 1.0f;
 }
 
-// Rows on their way: what 220 KB hold of 1,024 threads' slots.  Only fp32 rows at 16 elements a
-// thread (64 bytes) have to do with one.
-constexpr int fwd_stages(int bytes) { return bytes <= 32 ? 3 : 1; }
-constexpr int bwd_stages(int bytes) { return bytes <= 32 ? 2 : 1; }
+// Rows of a group on their way.  fp32 rows at 16 elements a thread (64 bytes) have to do with one:
+// 220 KB hold no more of 1,024 threads' slots.
+constexpr int stages(int bytes) { return bytes <= 32 ? 2 : 1; }
 
 // kQuant: 8-bit rows.  normalize = 0: the rows themselves (u = 1).
 template <typename T, int kPer, bool kCta, bool kShift, bool kQuant>
@@ -156,7 +155,7 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
   extern __shared__ uint4 smem[];
   __shared__ SumMax red[2][32];
   const P p(x, ldx, cols, group);
-  constexpr int kStages = fwd_stages(kPer * sizeof(T));
+  constexpr int kStages = stages(kPer * sizeof(T));
   const Ring<2, kVecs, kStages> ring(smem);
   const auto fetch = [&](int64_t row, int stage) {
     if (row < rows) {
@@ -291,7 +290,7 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
   extern __shared__ uint4 smem[];
   __shared__ SumMax red[2][32];
   const P p(gy, ldgy, cols, group);
-  constexpr int kStages = bwd_stages(kPer * sizeof(T));
+  constexpr int kStages = stages(kPer * sizeof(T));
   const Ring<3, kVecs, kStages> ring(smem);
   const auto fetch = [&](int64_t row, int stage) {
     if (row < rows) {
@@ -502,19 +501,23 @@ struct Operand {
 // How a call runs: by whole vectors, by vectors between single elements, or element by element.
 struct Plan {
   bool any = true, shift = false, cta = false;
-  int per = 8, group = 32, threads = kThreads, grid = 0;
-  size_t smem = 0;
+  int per = 8, group = 32, threads = kThreads, per_cta = 1, align = 1, grid = 0;
+  size_t ring = 0, smem = 0;
 };
 
-constexpr int kMaxParts = 4 * kSms + 8;  // CTAs of a persistent launch, at most
+constexpr int kMaxPerSm = 16, kMaxParts = kMaxPerSm * kSms + 8;  // CTAs of a persistent launch, at most
 
-// `tensors`: the row tensors of one element size, `loaded` of them inputs.  Vectors need rows that start alike in 16 bytes:
-// all aligned (with whole vectors to a row), or all shifted alike.  A thread takes 16 elements
-// where 8 would need more than 512 threads to a row (fewer threads, more CTAs to an SM: 5,120
-// columns run as 3 CTAs of 320 threads), and a row of up to 32 threads' elements goes to a
-// power-of-two group of lanes.
+// `tensors`: the row tensors of one element size, `loaded` of them inputs.  Vectors need rows that
+// start alike in 16 bytes: all aligned (with whole vectors to a row), or all shifted alike.
+//
+// A thread takes 8 elements of a row, or 16 where 8 would need more than `wide` threads: fewer
+// warps to a barrier and more CTAs to an SM, against fewer registers for other rows.  Measured at
+// 1,024 / 2,048 / 4,096 bf16 columns (120 M elements; 8 against 16 a thread, us):
+//   forward 155 / 174 / 155 against 168 / 170 / 178,  8-bit 177 / 167 / 171 against 188 / 151 / 149,
+//   backward 184 / 155 / 170 against 287 / 200 / 142
+// hence 512, 128 and 256.  A row of up to 32 threads' elements goes to a power-of-two group of lanes.
 template <size_t kSize>
-Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int loaded, int (*stages)(int)) {
+Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int loaded, int wide) {
   constexpr int kWidth = 16 / (int)kSize;
   Plan p;
   const auto off = [](const void* q) { return (unsigned)(reinterpret_cast<uintptr_t>(q) & 15); };
@@ -528,7 +531,10 @@ Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int lo
   if (!aligned && !alike) return p;
   p.shift = !aligned;
   const int need = (cols + 7) / 8;
-  p.per = need > 512 ? 16 : 8;
+  // Shifted rows: 16 a thread sooner (1,535 bf16 columns forward 253 -> 156 us, backward 313 -> 183),
+  // but for the fp32 backward, which then has one row on its way (18 -> 22 us at 4,095 x 1,535).
+  if (p.shift && wide > 128 && (kSize == 2 || loaded == 2)) wide = 128;
+  p.per = need > wide ? 16 : 8;
   const int lanes = (cols + p.per - 1) / p.per;  // threads that a row keeps busy
   if (lanes > 1024) return p;
   p.any = false;
@@ -545,16 +551,36 @@ Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int lo
   const int bytes = p.per * (int)kSize;
   p.smem = (size_t)loaded * stages(bytes) * bytes * p.threads;
   const size_t sums = p.cta ? 0 : (size_t)per_cta * cols * sizeof(float);
+  p.ring = p.smem;
   if (p.smem < sums) p.smem = sums;
-  const int by_regs = 65536 / (64 * p.threads), by_smem = (int)((220 << 10) / (p.smem + 1024));
-  int per_sm = by_regs < by_smem ? by_regs : by_smem;
-  per_sm = per_sm > 4 ? 4 : per_sm;
-  if (per_sm < 1) per_sm = 1;
-  const int64_t want = (rows + per_cta - 1) / per_cta;
-  p.grid = (int)(want < per_sm * kSms ? want : per_sm * kSms);
-  // groups' rows shifted alike: the row step is a multiple of the shifts' period (up to kWidth)
-  if (p.shift && (p.grid * per_cta) % kWidth != 0) p.grid = (p.grid + kWidth - 1) / kWidth * kWidth;
+  p.per_cta = per_cta;
+  p.align = p.shift ? kWidth : 1;
   return p;
+}
+
+// The persistent grid: as many CTAs an SM as keep `budget` bytes of rows on their way, and two
+// (one computes while the other waits at its barrier) if that is at most 80 KB.  More bytes are
+// worse where the kernel also writes much: 120 M bf16 elements in 2,048 columns forward (half of
+// the traffic writes) took 150 us with 48 KB an SM and 177 us with 96 KB; 8-bit rows 131 us with
+// 64 KB and 145 us with 80 KB; the backward (a quarter writes) wants all that fit.
+void size_grid(Plan& p, int64_t rows, int budget, int regs) {
+  const int fit[] = {65536 / (((regs + 7) / 8 * 8) * p.threads), 2048 / p.threads, (int)((220 << 10) / (p.smem + 1024)),
+                     kMaxPerSm};
+  if (p.shift) budget = 180 << 10;  // their single elements are loaded a row ahead only
+  int per_sm = budget / (int)p.ring;
+  if (per_sm < 2) per_sm = p.ring <= 40 << 10 ? 2 : 1;
+  for (int f : fit) per_sm = per_sm < f ? per_sm : f;
+  if (per_sm < 1) per_sm = 1;
+  const int64_t want = (rows + p.per_cta - 1) / p.per_cta;
+  p.grid = (int)(want < per_sm * kSms ? want : per_sm * kSms);
+  // groups' rows shifted alike: the row step is a multiple of the shifts' period
+  if (p.grid * p.per_cta % p.align != 0) p.grid = (p.grid + p.align - 1) / p.align * p.align;
+}
+
+template <typename K>
+int registers_of(K kernel) {
+  cudaFuncAttributes a;
+  return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 64;
 }
 
 template <typename K>
@@ -581,7 +607,7 @@ template <typename T, bool kQuant>
 cudaError_t forward(const T* x, int64_t ldx, const T* r, int64_t ldr, const float* w, float eps, int normalize,
                     int64_t rows, int cols, void* y, T* h, float* aux, cudaStream_t stream) {
   const Operand tensors[4] = {{x, ldx}, {r, ldr}, {h, cols}, {kQuant ? nullptr : y, cols}};
-  Plan p = plan_rows<sizeof(T)>(tensors, 4, rows, cols, 2, fwd_stages);
+  Plan p = plan_rows<sizeof(T)>(tensors, 4, rows, cols, 2, kQuant ? 128 : 512);
   // whole vectors of bytes: the 8-bit rows start on their own vectors' boundaries
   if (kQuant && !p.any && !p.shift && reinterpret_cast<uintptr_t>(y) % (16 / sizeof(T)) != 0) p.any = true;
   if (p.any) {
@@ -591,6 +617,8 @@ cudaError_t forward(const T* x, int64_t ldx, const T* r, int64_t ldr, const floa
   }
   return with_plan(p, [&](auto per, auto cta, auto shift) {
     const auto kernel = fwd_kernel<T, per(), cta(), shift(), kQuant>;
+    static const int regs = registers_of(kernel);
+    size_grid(p, rows, kQuant ? 64 << 10 : 48 << 10, regs);
     const cudaError_t e = allow_smem(kernel, p.smem);
     if (e != cudaSuccess) return e;
     kernel<<<p.grid, p.threads, p.smem, stream>>>(x, ldx, r, ldr, w, eps, normalize, rows, cols, p.group, y, h, aux);
@@ -602,8 +630,8 @@ template <typename T>
 cudaError_t backward(const T* gy, int64_t ldgy, const T* h, int64_t ldh, const T* gh, int64_t ldgh, const float* w,
                      const float* rstd, int64_t rows, int cols, T* dx, float* part, float* dw, cudaStream_t stream) {
   const Operand tensors[4] = {{gy, ldgy}, {h, ldh}, {gh, ldgh}, {dx, cols}};
-  const Plan p = plan_rows<sizeof(T)>(tensors, 4, rows, cols, 3, bwd_stages);
-  int parts = p.grid;
+  Plan p = plan_rows<sizeof(T)>(tensors, 4, rows, cols, 3, 256);
+  int parts = 0;
   if (p.any) {
     bwd_any_kernel<T><<<(unsigned)rows, kThreads, 0, stream>>>(gy, ldgy, h, ldh, gh, ldgh, w, rstd, cols, dx);
     if (dw) {
@@ -615,6 +643,9 @@ cudaError_t backward(const T* gy, int64_t ldgy, const T* h, int64_t ldh, const T
   } else {
     const cudaError_t e = with_plan(p, [&](auto per, auto cta, auto shift) {
       const auto kernel = bwd_kernel<T, per(), cta(), shift()>;
+      static const int regs = registers_of(kernel);
+      size_grid(p, rows, 180 << 10, regs);
+      parts = p.grid;
       const cudaError_t a = allow_smem(kernel, p.smem);
       if (a != cudaSuccess) return a;
       kernel<<<p.grid, p.threads, p.smem, stream>>>(gy, ldgy, h, ldh, gh, ldgh, w, rstd, rows, cols, p.group, dx,
