@@ -35,21 +35,30 @@ __device__ int g_gemm8_error = 0;
 enum : int { kErrProducer = 411, kErrMma = 412, kErrEpilogue = 413 };
 
 constexpr int kThreads = 192;
+constexpr int kMaxSplits = 8;  // CTAs of a portable cluster
 constexpr int kFeatures = 128, kStepK = 128;  // a tile's features; bytes of K in a stage
 constexpr int kABytes = kFeatures * kStepK;
+
+// The epilogue turns 16 tokens of a warp's 32 features at a time; rows of 36 words keep its 16-byte
+// reads off each other's banks.
+constexpr int kTurnRow = 36, kTurnBytes = 16 * kTurnRow * 4;
 
 template <int kTokens>
 struct Shape {
   static constexpr int kBBytes = kTokens * kStepK;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStages = kTokens == 256 ? 4 : kTokens == 128 ? 6 : 8;
+  // 256 tokens fill an SM; smaller tiles leave room for a second CTA (at most 100 KB each)
+  static constexpr int kCtas = kTokens == 256 ? 1 : 2;
+  static constexpr int kStages = kTokens == 256 ? 4 : (96 << 10) / kStageBytes;
   static constexpr int kColumns = kTokens <= 16 ? 32 : 2 * kTokens;  // TMEM: two accumulators
   static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = kAccFull + 2,
                        kDrain = kAccEmpty + 2, kBars = kDrain + 1;
-  static constexpr int kBarAt = kStages * kStageBytes;
+  static constexpr int kTurnAt = kStages * kStageBytes;  // the epilogue warps' transposition buffers
+  static constexpr int kBarAt = kTurnAt + 4 * kTurnBytes;
   static constexpr int kTmemAt = kBarAt + kBars * 8;
   static constexpr int kAbortAt = kTmemAt + 4;
   static constexpr size_t kSmem = 1024 + kAbortAt + 4;
+  static_assert(kFeatures * kTokens * 4 <= kTurnAt, "a split's partial sums reuse the ring");
 };
 
 // Four K = 32 products of one 128-byte stage; descriptor steps of 32 bytes, in 16-byte units.
@@ -83,11 +92,35 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+// Every thread of the cluster's CTAs: shared memory written before is seen after.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Four words of CTA `rank`'s shared memory, at this CTA's address.
+__device__ __forceinline__ float4 peer_load(uint32_t addr, uint32_t rank) {
+  float4 v;
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(there)
+               : "memory");
+  return v;
+}
+
+// splits = 1: persistent CTAs over the tiles.  splits > 1: a cluster of that many CTAs to a tile,
+// each over its part of K; their partial sums are added over distributed shared memory in rank
+// order, each CTA adding up its share of the tile's tokens.
 template <int kTokens>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, Shape<kTokens>::kCtas)
     linear_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, int M, int N,
                   int K, const float* __restrict__ xs, const float* __restrict__ ws, const float* __restrict__ bias,
-                  __nv_bfloat16* __restrict__ c, int64_t ldc) {
+                  __nv_bfloat16* __restrict__ c, int64_t ldc, int splits) {
   using S = Shape<kTokens>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -97,7 +130,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + S::kAbortAt);
   const int tf = (N + kFeatures - 1) / kFeatures, tt = (M + kTokens - 1) / kTokens;
   const int tiles = tf * tt;
-  const int nk = (K + kStepK - 1) / kStepK;
+  const int steps = (K + kStepK - 1) / kStepK;
+  const int rank = splits > 1 ? (int)cluster_rank() : 0;
+  const int k_begin = (int)((int64_t)steps * rank / splits), k_end = (int)((int64_t)steps * (rank + 1) / splits);
+  const int first = (int)blockIdx.x / splits, next = (int)gridDim.x / splits;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kStages; ++i) {
@@ -125,9 +161,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       int it = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x) {
+      for (int t = first; ok && t < tiles; t += next) {
         const int n0 = (t % tf) * kFeatures, m0 = (t / tf) * kTokens;
-        for (int kb = 0; kb < nk; ++kb, ++it) {
+        for (int kb = k_begin; kb < k_end; ++kb, ++it) {
           const int s = it % S::kStages;
           if (it >= S::kStages && !mbar_wait(bar(S::kEmpty + s), ((it / S::kStages) - 1) & 1, abort_flag,
                                              &g_gemm8_error, kErrProducer)) {
@@ -149,12 +185,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kIdesc = idesc_e4m3(kFeatures, kTokens);
       int it = 0, tl = 0;
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < tiles; t += gridDim.x, ++tl) {
+      for (int t = first; ok && t < tiles; t += next, ++tl) {
         const int ab = tl & 1;
         if (tl >= 2 && !mbar_wait(bar(S::kAccEmpty + ab), ((tl >> 1) - 1) & 1, abort_flag, &g_gemm8_error, kErrMma))
           break;
         tc_fence_after();
-        for (int kb = 0; kb < nk; ++kb, ++it) {
+        for (int kb = k_begin; kb < k_end; ++kb, ++it) {
           const int s = it % S::kStages;
           if (!mbar_wait(bar(S::kFull + s), (it / S::kStages) & 1, abort_flag, &g_gemm8_error, kErrMma)) {
             ok = false;
@@ -162,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           tc_fence_after();
           const uint32_t a = sb + s * S::kStageBytes;
-          mma_stage(tmem + ab * kTokens, desc_k_sw128(a), desc_k_sw128(a + kABytes), kIdesc, kb > 0 ? 1u : 0u);
+          mma_stage(tmem + ab * kTokens, desc_k_sw128(a), desc_k_sw128(a + kABytes), kIdesc, kb > k_begin ? 1u : 0u);
           mma_commit(bar(S::kEmpty + s));
         }
         if (ok) mma_commit(bar(S::kAccFull + ab));
@@ -172,25 +208,65 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    float* turn = reinterpret_cast<float*>(sm + S::kTurnAt + warp * kTurnBytes);
+    // after the turn a lane has 8 features of tokens row and row + 8 of the 16
+    const int row = lane / 4, column = (lane % 4) * 8;
+    const bool wide = N % 8 == 0 && ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(c) & 15) == 0;
     int tl = 0;
-    for (int t = blockIdx.x; t < tiles; t += gridDim.x, ++tl) {
+    for (int t = first; t < tiles; t += next, ++tl) {
       const int ab = tl & 1;
-      const int n = (t % tf) * kFeatures + warp * 32 + lane, m0 = (t / tf) * kTokens;
-      const float scale = n < N ? __ldg(ws + n) : 0.0f, b = bias && n < N ? __ldg(bias + n) : 0.0f;
+      const int n = (t % tf) * kFeatures + warp * 32 + column, m0 = (t / tf) * kTokens;
+      float scale[8], b[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        scale[e] = n + e < N ? __ldg(ws + n + e) : 0.0f;
+        b[e] = bias && n + e < N ? __ldg(bias + n + e) : 0.0f;
+      }
       const bool ok = mbar_wait(bar(S::kAccFull + ab), (tl >> 1) & 1, abort_flag, &g_gemm8_error, kErrEpilogue);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
 #pragma unroll 1
       for (int cc = 0; cc < kTokens; cc += 16) {
         if (m0 + cc >= M) break;
+        float xs_of[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int m = m0 + cc + row + 8 * i;
+          xs_of[i] = m < M ? __ldg(xs + m) : 0.0f;
+        }
         uint32_t raw[16];
         tmem_ld16(t_lane + ab * kTokens + cc, raw);
+        if (splits > 1) {  // into the ring, which the products are done with
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int m = m0 + cc + i;
-          if (m < M && n < N)
-            c[(int64_t)m * ldc + n] = __float2bfloat16_rn(fmaf(__uint_as_float(raw[i]) * __ldg(xs + m), scale, b));
+          for (int i = 0; i < 16; ++i)
+            reinterpret_cast<uint32_t*>(sm)[(cc + i) * kFeatures + warp * 32 + lane] = raw[i];
+          continue;
         }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) turn[i * kTurnRow + lane] = __uint_as_float(raw[i]);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int m = m0 + cc + row + 8 * i;
+          const float4* from = reinterpret_cast<const float4*>(turn + (row + 8 * i) * kTurnRow + column);
+          const float4 lo = from[0], hi = from[1];
+          const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+          float y[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = fmaf(v[e] * xs_of[i], scale[e], b[e]);
+          if (m >= M) continue;
+          __nv_bfloat16* to = c + (int64_t)m * ldc + n;
+          if (wide) {
+            if (n < N)
+              *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]),
+                                                         pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n + e < N) to[e] = __float2bfloat16_rn(y[e]);
+          }
+        }
+        __syncwarp();
       }
       tc_fence_before();
       __syncwarp();
@@ -202,6 +278,51 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, S::kColumns);
+  }
+  if (splits > 1) {
+    cluster_sync();
+    // a warp to a token, a lane to 4 features; two tokens' loads of all parts on their way
+    const int n = (first % tf) * kFeatures + 4 * lane, m0 = (first / tf) * kTokens, count = min(kTokens, M - m0);
+    float scale[4], b[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      scale[e] = n + e < N ? __ldg(ws + n + e) : 0.0f;
+      b[e] = bias && n + e < N ? __ldg(bias + n + e) : 0.0f;
+    }
+    const bool wide = N % 4 == 0 && ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(c) & 7) == 0;
+    const int end = count * (rank + 1) / splits;
+    for (int i = count * rank / splits + warp; i < end; i += 2 * (kThreads / 32)) {
+      float sum[2][4] = {};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int at = i + u * (kThreads / 32);
+        if (at >= end) break;
+#pragma unroll
+        for (int r = 0; r < kMaxSplits; ++r) {
+          if (r >= splits) break;
+          const float4 v = peer_load(sb + (at * kFeatures + 4 * lane) * 4, r);
+          sum[u][0] += v.x, sum[u][1] += v.y, sum[u][2] += v.z, sum[u][3] += v.w;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int at = i + u * (kThreads / 32);
+        if (at >= end) break;
+        const float x = __ldg(xs + m0 + at);
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = fmaf(sum[u][e] * x, scale[e], b[e]);
+        __nv_bfloat16* to = c + (int64_t)(m0 + at) * ldc + n;
+        if (wide) {
+          if (n < N) *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < N) to[e] = __float2bfloat16_rn(y[e]);
+        }
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its sums
   }
 }
 
@@ -243,27 +364,39 @@ static prism_status_t make_map(CUtensorMap* map, const void* ptr, int64_t rows, 
   return PRISM_OK;
 }
 
+constexpr int kSms = 148;
+static int64_t tiles_of(int M, int N, int tokens) {
+  return (int64_t)((N + kFeatures - 1) / kFeatures) * ((M + tokens - 1) / tokens);
+}
+
 template <int kTokens>
 static prism_status_t launch(const void* x8, int64_t ldx, const float* xs, const void* w8, int64_t ldw,
                              const float* ws, const float* bias, int M, int N, int K, void* c, int64_t ldc,
-                             cudaStream_t stream) {
+                             int splits, cudaStream_t stream) {
   using S = Shape<kTokens>;
   CUtensorMap mw, mx;
   prism_status_t st = make_map(&mw, w8, N, K, ldw, kFeatures);
   if (st != PRISM_OK) return st;
   st = make_map(&mx, x8, M, K, ldx, kTokens);
   if (st != PRISM_OK) return st;
-  int dev = 0, sms = 0;
-  PRISM_CHECK_CUDA(cudaGetDevice(&dev), "prism_linear_fp8: cudaGetDevice");
-  PRISM_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev), "prism_linear_fp8: SM count");
   PRISM_CHECK_CUDA(cudaFuncSetAttribute(linear_kernel<kTokens>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (int)S::kSmem),
                    "prism_linear_fp8: smem attribute");
-  const int64_t tiles = (int64_t)((N + kFeatures - 1) / kFeatures) * ((M + kTokens - 1) / kTokens);
-  PRISM_CHECK_ARG(tiles < ((int64_t)1 << 30), "prism_linear_fp8: the output has too many tiles");
-  linear_kernel<kTokens><<<(unsigned)(tiles < sms ? tiles : sms), kThreads, S::kSmem, stream>>>(
-      mw, mx, M, N, K, xs, ws, bias, (__nv_bfloat16*)c, ldc);
-  PRISM_CHECK_LAUNCH("prism_linear_fp8");
+  const int64_t tiles = tiles_of(M, N, kTokens);
+  cudaLaunchConfig_t config = {};
+  const int64_t slots = kSms * S::kCtas;
+  config.gridDim = dim3((unsigned)(splits > 1 ? tiles * splits : tiles < slots ? tiles : slots));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = S::kSmem;
+  config.stream = stream;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = splits, cluster.val.clusterDim.y = 1, cluster.val.clusterDim.z = 1;
+  config.attrs = &cluster;
+  config.numAttrs = splits > 1 ? 1 : 0;
+  PRISM_CHECK_CUDA(cudaLaunchKernelEx(&config, linear_kernel<kTokens>, mw, mx, M, N, K, xs, ws, bias,
+                                      (__nv_bfloat16*)c, ldc, splits),
+                   "prism_linear_fp8");
   return PRISM_OK;
 }
 
@@ -292,10 +425,24 @@ extern "C" prism_status_t prism_linear_fp8(const void* x8, int64_t ldx, const fl
   PRISM_CHECK_ARG(ldx >= K && ldw >= K && ldx % 16 == 0 && ldw % 16 == 0 && ldc >= N,
                   "prism_linear_fp8: 8-bit row strides must be multiples of 16 and cover K, ldc must cover N");
   PRISM_CHECK_ARG(aligned16(x8) && aligned16(w8), "prism_linear_fp8: 8-bit tensors must be 16-byte aligned");
-  // the smallest tile that holds every token, 256 at most: fewer columns, fewer wasted products
-  if (M <= 16) return gemm8::launch<16>(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
-  if (M <= 32) return gemm8::launch<32>(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
-  if (M <= 64) return gemm8::launch<64>(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
-  if (M <= 128) return gemm8::launch<128>(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
-  return gemm8::launch<256>(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
+  PRISM_CHECK_ARG(gemm8::tiles_of(M, N, 128) < ((int64_t)1 << 30), "prism_linear_fp8: the output has too many tiles");
+  // The smallest tile that holds every token.  Past 128 tokens: 128, of which an SM holds two, where
+  // that evens out few rounds of tiles (512 tokens of 5,120 x 5,120: 23.5 us against 25.3) or the
+  // epilogue counts (32,768 tokens of 512 x 1,536: 57 against 92); else 256, which reads less shared
+  // memory (4,096 tokens of 5,120 x 5,120: 89 against 96).
+  int tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  if (M > 128 && K > 1024 && gemm8::tiles_of(M, N, 256) > 2 * gemm8::kSms) tokens = 256;
+  // K in parts while the tiles leave SMs without work, if each part keeps five steps of a K long
+  // enough to pay the exchange of 2.6 us (one token of 5,120 x 5,120: 15.1 us whole, 11.0 / 9.2 in
+  // 2 / 4 parts; K = 1,536: 9.8 whole, 12.3 in two)
+  const int64_t tiles = gemm8::tiles_of(M, N, tokens), room = tokens == 256 ? gemm8::kSms : 2 * gemm8::kSms;
+  const int steps = (K + gemm8::kStepK - 1) / gemm8::kStepK;
+  int splits = 1;
+  while (splits < gemm8::kMaxSplits && tiles * splits * 2 <= room && steps >= 20 && steps >= 10 * splits) splits *= 2;
+  const auto launch = tokens == 16    ? gemm8::launch<16>
+                      : tokens == 32  ? gemm8::launch<32>
+                      : tokens == 64  ? gemm8::launch<64>
+                      : tokens == 128 ? gemm8::launch<128>
+                                      : gemm8::launch<256>;
+  return launch(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, splits, stream);
 }

@@ -113,14 +113,21 @@ def linear_fp8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_scal
         raise TypeError("linear_fp8 expects fp32 scales")
     if x_scale.shape != x8.shape[:-1] or w_scale.shape != w8.shape[:1]:
         raise ValueError("linear_fp8: one scale a row of x and of W")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x_scale, w_scale, bias)):
+    if torch.is_grad_enabled() and (x_scale.requires_grad or w_scale.requires_grad or
+                                    (bias is not None and bias.requires_grad)):
         raise NotImplementedError("linear_fp8 is inference only")
     K = x8.shape[-1]
-    x2 = x8.reshape(-1, K)
-    x2, w2 = (t if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.stride(0) >= K and t.data_ptr() % 16 == 0
-              else t.clone(memory_format=torch.contiguous_format) for t in (x2, w8))
-    out = ops.linear_fp8(x2, x_scale.reshape(-1).contiguous(), w2, w_scale.contiguous(), bias)
-    return out.view(*x8.shape[:-1], w8.shape[0])
+    x2 = x8 if x8.dim() == 2 else x8.reshape(-1, K)
+    out = ops.linear_fp8(_rows16(x2), x_scale.reshape(-1).contiguous(),
+                         _rows16(w8), w_scale.contiguous(), bias)
+    return out if x2 is x8 else out.view(*x8.shape[:-1], w8.shape[0])
+
+
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """t, or a contiguous copy where its 8-bit rows do not start on 16-byte boundaries."""
+    row, column = t.stride()
+    fits = column == 1 and row % 16 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0
+    return t if fits else t.clone(memory_format=torch.contiguous_format)
 
 
 __all__ = ["linear", "linear_fp8", "o_proj_packed"]

@@ -551,9 +551,11 @@ def add_rms_norm_bwd(gy, h, rstd, gh=None, weight=None, want_dweight: bool = Tru
 _Strides3, _Strides2, _Ends = ctypes.c_int64 * 3, ctypes.c_int64 * 2, ctypes.c_int * 2
 
 
-def rotary(q, k, positions, freqs, section_ends, interleaved: bool, scale: float, conjugate: bool = False):
-    """prism_rotary on q [B, S, Hq, D] and k [B, S, Hk, D] or None (unit column stride);
-    positions [B, S, axes] integers with unit axis stride, freqs [rot / 2] fp64 -> new (q, k)."""
+def rotary(q, k, positions, position_strides, freqs, section_ends, interleaved: bool, scale: float,
+           conjugate: bool = False):
+    """prism_rotary on q [B, S, Hq, D] and k [B, S, Hk, D] or None (unit column stride); integer
+    positions with the given batch and token strides (and unit axis stride), freqs [rot / 2] fp64
+    -> new (q, k)."""
     dev = _device_of(q, k, positions, freqs)
     B, S, hq, D = q.shape
     hk, ko, k_at, k_in, ko_at, k_out = 0, None, None, None, None, None
@@ -563,7 +565,7 @@ def rotary(q, k, positions, freqs, section_ends, interleaved: bool, scale: float
         k_at, k_in, ko_at, k_out = k.data_ptr(), _Strides3(*k.stride()[:3]), ko.data_ptr(), _Strides3(S * hk * D, hk * D, D)
     _launch("prism_rotary", dev, q.data_ptr(), _Strides3(*q.stride()[:3]), hq, k_at, k_in, hk, B, S, D,
             2 * freqs.shape[0], int(interleaved), positions.data_ptr(), int(positions.dtype == torch.int64),
-            _Strides2(*positions.stride()[:2]), _Ends(*section_ends), freqs.data_ptr(), scale, int(conjugate),
+            _Strides2(*position_strides), _Ends(*section_ends), freqs.data_ptr(), scale, int(conjugate),
             _dtype_code(q, "rotary"), qo.data_ptr(), _Strides3(S * hq * D, hq * D, D), ko_at, k_out)
     return qo, ko
 
