@@ -148,5 +148,21 @@ def call(name: str, *args):
     return rc
 
 
+_pairs = None
+
+
+def tensor_pairs():
+    """prism_tensor_pairs (csrc/tensor_list.cpp), built if it is absent, called with the GIL held."""
+    global _pairs
+    if _pairs is None:
+        path = _build.tensor_list_lib()
+        if not os.path.exists(path):
+            _build.build_tensor_list()
+        fn = ctypes.PyDLL(path).prism_tensor_pairs
+        fn.restype, fn.argtypes = _I, [ctypes.py_object, ctypes.py_object, _I64, _P, _P]
+        _pairs = fn
+    return _pairs
+
+
 def query(name: str, *args) -> int:
     return int(getattr(load(), name)(*args))

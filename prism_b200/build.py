@@ -9,9 +9,11 @@ default contraction.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -33,6 +35,31 @@ SOURCES = {
     "rotary_kernels.cu": [],
     "clip_kernels.cu": [],
 }
+
+
+def tensor_list_lib() -> str:
+    """The library of csrc/tensor_list.cpp, named after the torch and Python that it is built for."""
+    import torch
+    tag = f"{torch.__version__}_py{sys.version_info.major}{sys.version_info.minor}"
+    return os.path.join(HERE, f"libprism_tensor_list_{re.sub('[^0-9A-Za-z.]', '-', tag)}.so")
+
+
+def build_tensor_list(verbose: bool = False, force: bool = False) -> str:
+    import torch
+    src, target = os.path.join(CSRC, "tensor_list.cpp"), tensor_list_lib()
+    if force or _stale(target, [src, os.path.join(ROOT, "include", "prism_bsa.h")]):
+        base = os.path.dirname(torch.__file__)
+        includes = [os.path.join(ROOT, "include"), os.path.join(base, "include"),
+                    os.path.join(base, "include", "torch", "csrc", "api", "include"),
+                    sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
+        cmd = [os.environ.get("CXX") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+        cmd += [f"-I{d}" for d in includes] + [src, "-o", target, "-L" + os.path.join(base, "lib"), "-ltorch_python",
+                                               "-ltorch_cpu", "-lc10"]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+    return target
 
 
 def nvcc() -> str:
@@ -68,6 +95,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+    build_tensor_list(verbose=verbose, force=force)
     return LIB
 
 

@@ -19,12 +19,13 @@ def _flat_order(g: torch.Tensor, o: torch.Tensor):
     return (gp, op) if gp.is_contiguous() and op.is_contiguous() else None
 
 
-def _one_device(tensors) -> None:
-    devices = set(map(torch.Tensor.get_device, tensors))
-    if min(devices) < 0:
-        ops._check_cuda(*tensors)
-    if len(devices) > 1:
-        raise ValueError("gradients and outputs must be on one device")
+def _check(grads, outs) -> None:
+    """What the kernel asks of each tensor, with the error that says so."""
+    ops._device_of(*grads, *outs)
+    for g, o in zip(grads, outs):
+        ops._dtype_code(g, "clip_grad_norm")
+        if o.dtype != g.dtype or o.numel() != g.numel():
+            raise ValueError("an output must have the type and the number of elements of its gradient")
 
 
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *,
@@ -45,17 +46,15 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *,
             raise ValueError(f"{len(grads)} gradients, {len(outs)} outputs")
     if not grads:
         return torch.zeros(())
-    _one_device(grads if outs is grads else grads + outs)
-    contiguous = torch.Tensor.is_contiguous
-    if all(map(contiguous, grads)) and (outs is grads or all(map(contiguous, outs))):
-        return ops.clip_grad_norm(grads, outs, max_norm)
+    norm = ops.clip_grad_norm(grads, outs, max_norm)
+    if norm is not None:
+        return norm
+    _check(grads, outs)
     src, dst, copies = [], [], []
     with torch.no_grad():
         for g, o in zip(grads, outs):
             pair = _flat_order(g, o)
             if pair is None:  # gaps in memory, or two orders: through a contiguous copy
-                if o.numel() != g.numel():
-                    raise ValueError("an output must have as many elements as its gradient")
                 pair = (g.clone(memory_format=torch.contiguous_format),) * 2
                 copies.append((o, pair[1]))
             src.append(pair[0])

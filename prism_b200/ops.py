@@ -9,8 +9,6 @@ from __future__ import annotations
 
 import ctypes
 import math
-from array import array
-from operator import attrgetter
 from typing import Optional, Tuple
 
 import torch
@@ -430,7 +428,6 @@ def norm_rope_pack_bwd(g: torch.Tensor, x, heads: int, S: int, gamma=None, rstd=
 # ----------------------------------------------- operators around the attention
 # The wrappers below pass addresses as plain integers and touch each tensor as little as they
 # can: at one token the host's share of a call is longer than the kernel's.
-_dtype_of = attrgetter("dtype")
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # prism_dtype_t
 _current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
@@ -570,26 +567,21 @@ def rotary(q, k, positions, position_strides, freqs, section_ends, interleaved: 
     return qo, ko
 
 
-def clip_grad_norm(grads, outs, max_norm: float) -> torch.Tensor:
-    """prism_clip_grad_norm over contiguous tensors of one device (outs[i] may be grads[i]) ->
-    norm, 0-dim fp32."""
-    dev, n = grads[0].device, len(grads)
-    ptrs = array("q", map(torch.Tensor.data_ptr, grads))
-    sizes = array("q", map(torch.Tensor.numel, grads))
-    types = list(map(_dtype_of, grads))
-    try:
-        codes = array("i", map(_DTYPES.__getitem__, types))
-    except KeyError as e:
-        raise TypeError(f"clip_grad_norm expects bf16, fp16 or fp32, got {e.args[0]}") from None
-    optrs = ptrs
-    if outs is not grads:
-        optrs = array("q", map(torch.Tensor.data_ptr, outs))
-        if list(map(torch.Tensor.numel, outs)) != sizes.tolist() or list(map(_dtype_of, outs)) != types:
-            raise ValueError("an output must have the type and the number of elements of its gradient")
+def clip_grad_norm(grads: list, outs: list, max_norm: float) -> Optional[torch.Tensor]:
+    """prism_clip_grad_norm over lists of contiguous tensors (outs may be grads) -> norm, 0-dim
+    fp32; None where the lists are not of contiguous CUDA tensors on one device, alike in type and
+    number of elements (nothing has happened then)."""
+    n = len(grads)
+    table, codes = (ctypes.c_int64 * (3 * n))(), (ctypes.c_int * n)()
+    at, codes_at = ctypes.addressof(table), ctypes.addressof(codes)
+    index = _lib.tensor_pairs()(grads, outs, n, at, codes_at)
+    if index < 0:
+        return None
+    dev = grads[0].device
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws = _ws(_lib.query("prism_clip_grad_norm_workspace_bytes", n), dev)
-    _launch("prism_clip_grad_norm", norm.get_device(), *(a.buffer_info()[0] for a in (ptrs, optrs, sizes, codes)), n,
-            max_norm, ws.data_ptr(), norm.data_ptr())
+    _launch("prism_clip_grad_norm", index, at, at + 8 * n, at + 16 * n, codes_at, n, max_norm, ws.data_ptr(),
+            norm.data_ptr())
     return norm
 
 
