@@ -148,20 +148,27 @@ def call(name: str, *args):
     return rc
 
 
-_pairs = None
+_torch_ops = None
 
 
-def tensor_pairs():
-    """prism_tensor_pairs (csrc/tensor_list.cpp), built if it is absent, called with the GIL held."""
-    global _pairs
-    if _pairs is None:
-        path = _build.tensor_list_lib()
+def torch_ops():
+    """The extension module of csrc/torch_ops.cpp (built if it is absent)."""
+    global _torch_ops
+    if _torch_ops is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries are what the extension links to)
+        load()
+        path = _build.torch_ops_lib()
         if not os.path.exists(path):
-            _build.build_tensor_list()
-        fn = ctypes.PyDLL(path).prism_tensor_pairs
-        fn.restype, fn.argtypes = _I, [ctypes.py_object, ctypes.py_object, _I64, _P, _P]
-        _pairs = fn
-    return _pairs
+            _build.build_torch_ops()
+        loader = importlib.machinery.ExtensionFileLoader("prism_torch_ops", path)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("prism_torch_ops", loader))
+        loader.exec_module(module)
+        module.set_error(PrismError)
+        _torch_ops = module
+    return _torch_ops
 
 
 def query(name: str, *args) -> int:

@@ -37,25 +37,27 @@ SOURCES = {
 }
 
 
-def tensor_list_lib() -> str:
-    """The library of csrc/tensor_list.cpp, named after the torch and Python that it is built for."""
+def torch_ops_lib() -> str:
+    """The extension of csrc/torch_ops.cpp, named after the torch and Python that it is built for."""
     import torch
     tag = f"{torch.__version__}_py{sys.version_info.major}{sys.version_info.minor}"
-    return os.path.join(HERE, f"libprism_tensor_list_{re.sub('[^0-9A-Za-z.]', '-', tag)}.so")
+    return os.path.join(HERE, f"prism_torch_ops_{re.sub('[^0-9A-Za-z.]', '-', tag)}.so")
 
 
-def build_tensor_list(verbose: bool = False, force: bool = False) -> str:
+def build_torch_ops(verbose: bool = False, force: bool = False) -> str:
     import torch
-    src, target = os.path.join(CSRC, "tensor_list.cpp"), tensor_list_lib()
+    src, target = os.path.join(CSRC, "torch_ops.cpp"), torch_ops_lib()
     if force or _stale(target, [src, os.path.join(ROOT, "include", "prism_bsa.h")]):
         base = os.path.dirname(torch.__file__)
+        cuda = os.path.dirname(os.path.dirname(os.path.realpath(nvcc())))
         includes = [os.path.join(ROOT, "include"), os.path.join(base, "include"),
                     os.path.join(base, "include", "torch", "csrc", "api", "include"),
-                    sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
-        cmd = [os.environ.get("CXX") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared",
+                    sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+        cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared",
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-        cmd += [f"-I{d}" for d in includes] + [src, "-o", target, "-L" + os.path.join(base, "lib"), "-ltorch_python",
-                                               "-ltorch_cpu", "-lc10"]
+        cmd += [f"-I{d}" for d in includes] + [src, "-o", target, "-L" + os.path.join(base, "lib"), "-L" + HERE]
+        # libprism_bsa.so is the one next to the extension; torch's libraries are loaded already
+        cmd += ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-lprism_bsa", "-Wl,-rpath,$ORIGIN"]
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
@@ -95,7 +97,7 @@ def build(verbose: bool = False, force: bool = False) -> str:
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
-    build_tensor_list(verbose=verbose, force=force)
+    build_torch_ops(verbose=verbose, force=force)
     return LIB
 
 

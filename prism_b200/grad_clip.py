@@ -5,7 +5,7 @@ from typing import Optional, Sequence
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 def _flat_order(g: torch.Tensor, o: torch.Tensor):
     """(g, o) with their dimensions permuted so that both are contiguous, or None: elements of
@@ -21,9 +21,12 @@ def _flat_order(g: torch.Tensor, o: torch.Tensor):
 
 def _check(grads, outs) -> None:
     """What the kernel asks of each tensor, with the error that says so."""
-    ops._device_of(*grads, *outs)
+    ops._check_cuda(*grads, *outs)
     for g, o in zip(grads, outs):
-        ops._dtype_code(g, "clip_grad_norm")
+        if g.device != grads[0].device or o.device != g.device:
+            raise ValueError("gradients and outputs must be on one device")
+        if g.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise TypeError(f"clip_grad_norm expects bf16, fp16 or fp32, got {g.dtype}")
         if o.dtype != g.dtype or o.numel() != g.numel():
             raise ValueError("an output must have the type and the number of elements of its gradient")
 
@@ -46,7 +49,7 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *,
             raise ValueError(f"{len(grads)} gradients, {len(outs)} outputs")
     if not grads:
         return torch.zeros(())
-    norm = ops.clip_grad_norm(grads, outs, max_norm)
+    norm = _lib.torch_ops().clip_grad_norm(grads, outs, max_norm)
     if norm is not None:
         return norm
     _check(grads, outs)
@@ -59,7 +62,7 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *,
                 copies.append((o, pair[1]))
             src.append(pair[0])
             dst.append(pair[1])
-        norm = ops.clip_grad_norm(src, dst, max_norm)
+        norm = _lib.torch_ops().clip_grad_norm(src, dst, max_norm)
         for o, c in copies:
             o.copy_(c.view(o.shape))
     return norm

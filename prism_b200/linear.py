@@ -20,7 +20,7 @@ from typing import Optional
 
 import torch
 
-from . import ops
+from . import _lib, ops
 
 
 class _Linear(torch.autograd.Function):
@@ -105,29 +105,7 @@ def linear_fp8(x8: torch.Tensor, x_scale: torch.Tensor, w8: torch.Tensor, w_scal
     """x8 [..., K], w8 [N, K] float8_e4m3fn, x_scale [...] and w_scale [N] fp32 (the value of an
     element is its 8-bit value times its row's scale) -> [..., N] bf16 = x W^T + bias.  K a
     multiple of 16."""
-    if x8.dtype != torch.float8_e4m3fn or w8.dtype != torch.float8_e4m3fn:
-        raise TypeError(f"linear_fp8 expects float8_e4m3fn operands, got {x8.dtype} and {w8.dtype}")
-    if x8.dim() < 1 or w8.dim() != 2 or x8.shape[-1] != w8.shape[1]:
-        raise ValueError(f"linear_fp8: x {tuple(x8.shape)} and W {tuple(w8.shape)} do not match")
-    if x_scale.dtype != torch.float32 or w_scale.dtype != torch.float32:
-        raise TypeError("linear_fp8 expects fp32 scales")
-    if x_scale.shape != x8.shape[:-1] or w_scale.shape != w8.shape[:1]:
-        raise ValueError("linear_fp8: one scale a row of x and of W")
-    if torch.is_grad_enabled() and (x_scale.requires_grad or w_scale.requires_grad or
-                                    (bias is not None and bias.requires_grad)):
-        raise NotImplementedError("linear_fp8 is inference only")
-    K = x8.shape[-1]
-    x2 = x8 if x8.dim() == 2 else x8.reshape(-1, K)
-    out = ops.linear_fp8(_rows16(x2), x_scale.reshape(-1).contiguous(),
-                         _rows16(w8), w_scale.contiguous(), bias)
-    return out if x2 is x8 else out.view(*x8.shape[:-1], w8.shape[0])
-
-
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """t, or a contiguous copy where its 8-bit rows do not start on 16-byte boundaries."""
-    row, column = t.stride()
-    fits = column == 1 and row % 16 == 0 and row >= t.shape[1] and t.data_ptr() % 16 == 0
-    return t if fits else t.clone(memory_format=torch.contiguous_format)
+    return _lib.torch_ops().linear_fp8(x8, x_scale, w8, w_scale, bias)
 
 
 __all__ = ["linear", "linear_fp8", "o_proj_packed"]

@@ -425,179 +425,6 @@ def norm_rope_pack_bwd(g: torch.Tensor, x, heads: int, S: int, gamma=None, rstd=
     return dx, dgamma
 
 
-# ----------------------------------------------- operators around the attention
-# The wrappers below pass addresses as plain integers and touch each tensor as little as they
-# can: at one token the host's share of a call is longer than the kernel's.
-_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}  # prism_dtype_t
-_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
-
-
-def _dtype_code(t: torch.Tensor, what: str) -> int:
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{what} expects bf16, fp16 or fp32, got {t.dtype}")
-    return code
-
-
-def _device_of(*ts) -> int:
-    """The one CUDA device that every tensor is on."""
-    index = None
-    for t in ts:
-        if t is not None:
-            if not t.is_cuda:
-                _check_cuda(t)
-            i = t.get_device()
-            if index is None:
-                index = i
-            elif i != index:
-                raise ValueError(f"tensors on different devices: cuda:{index} and cuda:{i}")
-    return index
-
-
-def _launch(name: str, index: int, *args) -> None:
-    """_lib.call on the device's current stream, with the device made current if it is not."""
-    if index == _current_device():
-        _lib.call(name, *args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            _lib.call(name, *args, _raw_stream(index))
-
-
-def _at(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
-
-
-def _fp32_vector(w: Optional[torch.Tensor], n: int, what: str):
-    if w is None:
-        return None
-    if w.dim() != 1 or w.shape[0] != n:
-        raise ValueError(f"{what} must have shape [{n}], got {tuple(w.shape)}")
-    return w if w.dtype == torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous()
-
-
-def _rows2d(t: Optional[torch.Tensor], cols: int):
-    """[..., cols] -> a [rows, cols] view with unit column stride (a copy where there is none)."""
-    if t is None:
-        return None
-    if t.dim() != 2:
-        t = t.reshape(-1, cols)
-    return t if cols == 1 or t.stride(1) == 1 else t.contiguous()
-
-
-def _ld(t: Optional[torch.Tensor]) -> int:
-    return 0 if t is None else t.stride(0)
-
-
-def _new_like(x: torch.Tensor, dtype=None) -> torch.Tensor:
-    return torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format)
-
-
-def _rows_input(x, residual, weight, what):
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"{what} needs at least one column")
-    code = _dtype_code(x, what)
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError(f"{what}: the residual must have the shape and type of x")
-    cols = x.shape[-1]
-    return code, cols, _rows2d(x, cols), _rows2d(residual, cols), _fp32_vector(weight, cols, "weight")
-
-
-def add_rms_norm(x, residual=None, weight=None, eps: float = 1e-6, want_rstd: bool = False):
-    """prism_add_rms_norm: (y, h, rstd), y and h shaped as x, rstd [rows] fp32 or None; h is
-    None without a residual."""
-    dev = _device_of(x, residual, weight)
-    code, cols, x2, r2, w = _rows_input(x, residual, weight, "add_rms_norm")
-    rows = x2.shape[0]
-    y = _new_like(x)
-    h = None if residual is None else _new_like(x)
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_rstd else None
-    _launch("prism_add_rms_norm", dev, x2.data_ptr(), x2.stride(0), _at(r2), _ld(r2), _at(w), eps, rows, cols, code,
-            y.data_ptr(), _at(h), _at(rstd))
-    return y, h, rstd
-
-
-def add_rms_norm_fp8(x, residual=None, weight=None, eps: float = 1e-6, normalize: bool = True):
-    """prism_add_rms_norm_fp8: (y8 e4m3 shaped as x, scale [x.shape[:-1]] fp32, h or None)."""
-    dev = _device_of(x, residual, weight)
-    code, cols, x2, r2, w = _rows_input(x, residual, weight, "add_rms_norm_fp8")
-    y8 = _new_like(x, torch.float8_e4m3fn)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    h = None if residual is None else _new_like(x)
-    _launch("prism_add_rms_norm_fp8", dev, x2.data_ptr(), x2.stride(0), _at(r2), _ld(r2), _at(w), eps, int(normalize),
-            x2.shape[0], cols, code, y8.data_ptr(), scale.data_ptr(), _at(h))
-    return y8, scale, h
-
-
-def add_rms_norm_bwd(gy, h, rstd, gh=None, weight=None, want_dweight: bool = True):
-    """prism_add_rms_norm_bwd: (dx shaped as h, dweight [cols] fp32 or None)."""
-    dev = _device_of(gy, h, rstd, gh, weight)
-    code, cols = _dtype_code(h, "add_rms_norm_bwd"), h.shape[-1]
-    g2, h2, gh2 = _rows2d(gy, cols), _rows2d(h, cols), _rows2d(gh, cols)
-    w = _fp32_vector(weight, cols, "weight")
-    rows = h2.shape[0]
-    dx = _new_like(h)
-    dw = ws = None
-    if want_dweight:
-        dw = torch.empty(cols, dtype=torch.float32, device=h.device)
-        ws = _ws(_lib.query("prism_add_rms_norm_bwd_workspace_bytes", rows, cols), h.device)
-    _launch("prism_add_rms_norm_bwd", dev, g2.data_ptr(), g2.stride(0), h2.data_ptr(), h2.stride(0), _at(gh2),
-            _ld(gh2), _at(w), rstd.data_ptr(), rows, cols, code, dx.data_ptr(), _at(ws), _at(dw))
-    return dx, dw
-
-
-_Strides3, _Strides2, _Ends = ctypes.c_int64 * 3, ctypes.c_int64 * 2, ctypes.c_int * 2
-
-
-def rotary(q, k, positions, position_strides, freqs, section_ends, interleaved: bool, scale: float,
-           conjugate: bool = False):
-    """prism_rotary on q [B, S, Hq, D] and k [B, S, Hk, D] or None (unit column stride); integer
-    positions with the given batch and token strides (and unit axis stride), freqs [rot / 2] fp64
-    -> new (q, k)."""
-    dev = _device_of(q, k, positions, freqs)
-    B, S, hq, D = q.shape
-    hk, ko, k_at, k_in, ko_at, k_out = 0, None, None, None, None, None
-    qo = _new_like(q)
-    if k is not None:
-        hk, ko = k.shape[2], _new_like(k)
-        k_at, k_in, ko_at, k_out = k.data_ptr(), _Strides3(*k.stride()[:3]), ko.data_ptr(), _Strides3(S * hk * D, hk * D, D)
-    _launch("prism_rotary", dev, q.data_ptr(), _Strides3(*q.stride()[:3]), hq, k_at, k_in, hk, B, S, D,
-            2 * freqs.shape[0], int(interleaved), positions.data_ptr(), int(positions.dtype == torch.int64),
-            _Strides2(*position_strides), _Ends(*section_ends), freqs.data_ptr(), scale, int(conjugate),
-            _dtype_code(q, "rotary"), qo.data_ptr(), _Strides3(S * hq * D, hq * D, D), ko_at, k_out)
-    return qo, ko
-
-
-def clip_grad_norm(grads: list, outs: list, max_norm: float) -> Optional[torch.Tensor]:
-    """prism_clip_grad_norm over lists of contiguous tensors (outs may be grads) -> norm, 0-dim
-    fp32; None where the lists are not of contiguous CUDA tensors on one device, alike in type and
-    number of elements (nothing has happened then)."""
-    n = len(grads)
-    table, codes = (ctypes.c_int64 * (3 * n))(), (ctypes.c_int * n)()
-    at, codes_at = ctypes.addressof(table), ctypes.addressof(codes)
-    index = _lib.tensor_pairs()(grads, outs, n, at, codes_at)
-    if index < 0:
-        return None
-    dev = grads[0].device
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    ws = _ws(_lib.query("prism_clip_grad_norm_workspace_bytes", n), dev)
-    _launch("prism_clip_grad_norm", index, at, at + 8 * n, at + 16 * n, codes_at, n, max_norm, ws.data_ptr(),
-            norm.data_ptr())
-    return norm
-
-
-def linear_fp8(x8, x_scale, w8, w_scale, bias=None) -> torch.Tensor:
-    """prism_linear_fp8: x8 [M, K], w8 [N, K] e4m3 (unit column stride), x_scale [M], w_scale [N]
-    fp32 -> [M, N] bf16."""
-    dev = _device_of(x8, x_scale, w8, w_scale, bias)
-    M, K = x8.shape
-    N = w8.shape[0]
-    out = torch.empty((M, N), dtype=torch.bfloat16, device=x8.device)
-    b = _fp32_vector(bias, N, "bias")
-    _launch("prism_linear_fp8", dev, x8.data_ptr(), x8.stride(0), x_scale.data_ptr(), w8.data_ptr(), w8.stride(0),
-            w_scale.data_ptr(), _at(b), M, N, K, out.data_ptr(), N)
-    return out
-
-
 # --------------------------------------------------------- guided selection
 def gather_values(x: torch.Tensor, grid, grid_padded, src_idx: torch.Tensor) -> torch.Tensor:
     """Per-token values [T*H*W] on grid -> fp32 [len(src_idx)] in the chunk order, 0 at padding."""

@@ -28,6 +28,24 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_refusals_say_what_they_got():
+    """Shapes and types in the messages, raised before any device is looked at."""
+    x, pos = torch.zeros(2, 1, 16), torch.arange(2)
+    freqs, _ = rotary_frequencies(16)
+    f8 = lambda *s: torch.zeros(*s).to(torch.float8_e4m3fn)
+    for error, text, call in [
+            (ValueError, "8 columns", lambda: prism_b200.apply_rotary(x[..., :8], None, pos, freqs)),
+            (ValueError, "[3]", lambda: prism_b200.apply_rotary(x, None, torch.arange(3), freqs)),
+            (ValueError, "add up to 8", lambda: prism_b200.apply_rotary(x, None, pos, freqs, sections=(3, 3))),
+            (ValueError, "'x'", lambda: prism_b200.apply_rotary(x, None, pos, freqs, layout="x")),
+            (TypeError, "Float", lambda: prism_b200.apply_rotary(x, None, pos.float(), freqs)),
+            (ValueError, "[2, 32]", lambda: prism_b200.linear_fp8(f8(2, 32), torch.ones(2), f8(2, 16), torch.ones(2))),
+            (ValueError, "1 outputs", lambda: prism_b200.clip_grad_norm([x, x], 1.0, out=[x]))]:
+        with pytest.raises(error) as e:
+            call()
+        assert text in str(e.value)
+
+
 def test_c_entries_refuse_bad_arguments():
     """Every refusal below comes from the host checks, before any CUDA call."""
     L = _lib.load()
