@@ -4,8 +4,8 @@
 //   u   = (mean_j h_j^2 + eps)^(-1/2)
 //   y_j = w_j h_j u
 // 8-bit rows: s = max(max_j |y_j| / 448, 2^-100), y8_j = e4m3(y_j / s).  u cancels in y_j / s,
-// so one reduction gives both sum h^2 and max |w h|.  A row that holds a NaN or an infinity (or,
-// normalised, whose squares overflow fp32) has scale NaN.
+// so one reduction gives both sum h^2 and max |w h|.  A row that holds a NaN or an infinity has
+// scale NaN.
 // Backward, with gy = dL/dy and gh = dL/dh:
 //   dL/dh_j = u (w_j gy_j) - h_j u^3 / C * sum_i w_i gy_i h_i + gh_j   (also dL/dx and dL/dr)
 //   dL/dw_j = sum over rows of gy_j h_j u
@@ -36,6 +36,13 @@ struct SumMax {
   float sum, max;
 };
 
+// The larger one, a NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
 // Sum and maximum over the `group` lanes of a sub-warp, or over the CTA; every thread gets them.
 // `red` alternates between two rows, so that one barrier a reduction is enough.
 template <bool kCta>
@@ -43,7 +50,7 @@ __device__ __forceinline__ SumMax group_reduce(SumMax v, int group, SumMax (*red
   const int top = kCta ? 16 : group / 2;
   for (int o = top; o >= 1; o >>= 1) {
     v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
-    v.max = fmaxf(v.max, __shfl_xor_sync(0xffffffffu, v.max, o));
+    v.max = max_nan(v.max, __shfl_xor_sync(0xffffffffu, v.max, o));
   }
   if constexpr (kCta) {
     SumMax* row = red[turn & 1];
@@ -53,7 +60,7 @@ __device__ __forceinline__ SumMax group_reduce(SumMax v, int group, SumMax (*red
     v = row[0];
     for (int i = 1; i < nw; ++i) {
       v.sum += row[i].sum;
-      v.max = fmaxf(v.max, row[i].max);
+      v.max = max_nan(v.max, row[i].max);
     }
   }
   return v;
@@ -66,7 +73,7 @@ struct Quant {
 __device__ __forceinline__ Quant quantizer(const SumMax& t, float u) {
   Quant q;
   q.scale = fmaxf(t.max * u / kFp8Max, kScaleFloor);
-  if (!(t.sum <= kFloatMax)) q.scale = NAN;
+  if (!(t.max <= kFloatMax)) q.scale = NAN;
   q.factor = u / q.scale;
   return q;
 }
@@ -188,11 +195,14 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
   for (int64_t row = p.first, warp_row = p.warp_first; warp_row < rows; row += p.step, warp_row += p.step, ++turn) {
     ring.wait();
     const bool live = row < rows;
-    float hv[kPer], hs = xs;
+    float hv[kPer], hs = xs;  // w h for 8-bit rows
     SumMax t = {0.0f, 0.0f};
-    const auto take = [&](float f, float wf) {
-      t.sum += normalize ? f * f : f * 0.0f;  // without a norm, only a NaN or an infinity counts
-      if (kQuant) t.max = fmaxf(t.max, fabsf(f * wf));
+    const auto take = [&](float& f, float wf) {
+      if (!kQuant || normalize) t.sum += f * f;
+      if (kQuant) {
+        f *= wf;
+        t.max = max_nan(t.max, fabsf(f));
+      }
     };
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
@@ -212,8 +222,8 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
       }
 #pragma unroll
       for (int e = 0; e < kWidth; ++e) {
-        hv[v * kWidth + e] = f[e];
         take(f[e], wv[v * kWidth + e]);
+        hv[v * kWidth + e] = f[e];
       }
     }
     if (has_single && live) {
@@ -241,8 +251,8 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
 #pragma unroll
         for (int e = 0; e < kWidth; e += 4) {
           const int i = v * kWidth + e;
-          b[e / 4] = e4m3x2(hv[i] * wv[i] * q.factor, hv[i + 1] * wv[i + 1] * q.factor) |
-                     e4m3x2(hv[i + 2] * wv[i + 2] * q.factor, hv[i + 3] * wv[i + 3] * q.factor) << 16;
+          b[e / 4] = e4m3x2(hv[i] * q.factor, hv[i + 1] * q.factor) |
+                     e4m3x2(hv[i + 2] * q.factor, hv[i + 3] * q.factor) << 16;
         }
         if constexpr (kShift) {  // the bytes' alignment is not the elements'
           if (reinterpret_cast<uintptr_t>(out + c) % 4 == 0) {
@@ -258,7 +268,7 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
           *reinterpret_cast<uint32_t*>(out + c) = b[0];
         }
       }
-      if (has_single) out[p.single] = (uint8_t)e4m3x2(hs * ws * q.factor, 0.0f);
+      if (has_single) out[p.single] = (uint8_t)e4m3x2(hs * q.factor, 0.0f);
       if (p.lane == 0) aux[row] = q.scale;
     } else {
       T* out = static_cast<T*>(y) + row * cols;
@@ -429,8 +439,8 @@ __global__ void __launch_bounds__(kThreads)
       hr[c] = v;
     }
     const float f = Elem<T>::to_f(v);
-    t.sum += normalize ? f * f : f * 0.0f;
-    if (kQuant) t.max = fmaxf(t.max, fabsf(w ? f * w[c] : f));
+    t.sum += f * f;
+    if (kQuant) t.max = max_nan(t.max, fabsf(w ? f * w[c] : f));
   }
   t = group_reduce<true>(t, kThreads, red, 0);
   const float u = normalize ? rsqrtf(t.sum / (float)cols + eps) : 1.0f;
@@ -507,7 +517,7 @@ struct Plan {
 
 constexpr int kMaxPerSm = 16, kMaxParts = kMaxPerSm * kSms + 8;  // CTAs of a persistent launch, at most
 
-// `tensors`: the row tensors of one element size, `loaded` of them inputs.  Vectors need rows that
+// `tensors`: the row tensors of one element size, the first `loaded` of them inputs.  Vectors need rows that
 // start alike in 16 bytes: all aligned (with whole vectors to a row), or all shifted alike.
 //
 // A thread takes 8 elements of a row, or 16 where 8 would need more than `wide` threads: fewer
@@ -551,7 +561,9 @@ Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int lo
   const int bytes = p.per * (int)kSize;
   p.smem = (size_t)loaded * stages(bytes) * bytes * p.threads;
   const size_t sums = p.cta ? 0 : (size_t)per_cta * cols * sizeof(float);
-  p.ring = p.smem;
+  int present = 0;
+  for (int i = 0; i < loaded; ++i) present += tensors[i].ptr != nullptr;
+  p.ring = p.smem / loaded * present;
   if (p.smem < sums) p.smem = sums;
   p.per_cta = per_cta;
   p.align = p.shift ? kWidth : 1;

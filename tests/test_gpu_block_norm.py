@@ -237,6 +237,17 @@ def test_rows_of_zeros_and_of_non_finite_values(cols, cuda):
     assert bool(s0[[1, 3, 5]].isfinite().all())
 
 
+def test_8bit_rows_of_large_and_tiny_values(cuda):
+    """Rows whose squares leave fp32 quantise as they stand: the scale is the maximum over 448."""
+    for size in (1e25, 1e-25):
+        x = (torch.randn(5, 700, generator=torch.Generator().manual_seed(6)) * size).to(cuda)
+        x8, s = quantize_rows_fp8(x)
+        ref = (x.double().abs().amax(-1) / 448)
+        assert bool(((s.double() - ref).abs() <= 2.0 ** -22 * ref).all())
+        v = x.double() / s.double()[:, None]
+        assert bool(((x8.float().double() - v).abs() <= 2.0 ** -4 * v.abs() * (1 + 2.0 ** -18) + 2.0 ** -10).all())
+
+
 def test_offsets_past_32_bits(cuda):
     rows, cols = 420_001, 5120          # 2.15e9 elements
     x = torch.empty(rows, cols, dtype=torch.bfloat16, device=cuda)
