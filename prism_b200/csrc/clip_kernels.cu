@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
   const float v = (float)sqrt(block_sum(s));
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm = v;
   float f = max_norm / (v + 1e-6f);
-  f = f > 1.0f ? 1.0f : f;  // a NaN norm stays a NaN factor
+  f = f > 1.0f || isinf(max_norm) ? 1.0f : f;  // a NaN norm stays a NaN factor
   for_runs(t, chunks, [&](int k, int64_t at, int n) {
     if (f == 1.0f && t.in[k] == t.out[k]) return;  // in place, nothing to clip
     if (t.dtype[k] == PRISM_BF16) scale_run((const __nv_bfloat16*)t.in[k] + at, (__nv_bfloat16*)t.out[k] + at, n, f);

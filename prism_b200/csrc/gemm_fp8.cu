@@ -7,14 +7,18 @@
 // the scales and the bias are applied in fp32, and the result is rounded once.
 //
 // The weight is the tensor core's M side (128 output features to a tile) and the tokens its N
-// side, 16 to 256 of them to a tile: a call with one token then streams the weight through
-// 16-column products instead of multiplying 127 rows of padding.
+// side, 16 to 128 of them to a tile: a call with one token then streams the weight through
+// 16-column products instead of multiplying 127 rows of padding.  Large products run on pairs of
+// CTAs (below) with tiles of 256 x 256.
 //
-// Persistent kernel, one CTA per SM.  Warp 4 streams weight and token tiles (128 bytes of K)
-// with TMA into a ring, warp 5 issues tcgen05.mma kind::f8f6f4 (K = 32 an instruction) into one
-// of two TMEM accumulators, warps 0-3 (thread = output feature) drain the other.  At 256 tokens
-// one instruction reads 4 KB + 8 KB of shared memory in 128 clocks (of 128 B/clk).  Every wait
-// is bounded (sm100.cuh); one that gives up sets this file's device error word.
+// Persistent kernels.  Warp 4 streams weight and token tiles (128 bytes of K) with TMA into a ring,
+// warp 5 issues tcgen05.mma kind::f8f6f4 (K = 32 an instruction) into one of two TMEM accumulators,
+// warps 0-3 (thread = output feature) drain the other.  Every wait is bounded (sm100.cuh); one
+// that gives up sets this file's device error word.
+//
+// Measured: one token of 5,120 x 5,120 9.1 us; 75,600 tokens 1.37 ms, 2.90 PFLOP/s in a short run
+// (0.88 of twice the measured bf16 rate; tensor pipe 84 % busy) and 2.4 in a long one under the
+// power cap.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -47,9 +51,7 @@ template <int kTokens>
 struct Shape {
   static constexpr int kBBytes = kTokens * kStepK;
   static constexpr int kStageBytes = kABytes + kBBytes;
-  // 256 tokens fill an SM; smaller tiles leave room for a second CTA (at most 100 KB each)
-  static constexpr int kCtas = kTokens == 256 ? 1 : 2;
-  static constexpr int kStages = kTokens == 256 ? 4 : (96 << 10) / kStageBytes;
+  static constexpr int kStages = (96 << 10) / kStageBytes;  // an SM holds two CTAs
   static constexpr int kColumns = kTokens <= 16 ? 32 : 2 * kTokens;  // TMEM: two accumulators
   static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = kAccFull + 2,
                        kDrain = kAccEmpty + 2, kBars = kDrain + 1;
@@ -92,6 +94,73 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "memory");
 }
 
+// What a warp of the epilogue does with its 32 features (lanes of TMEM) of a tile: 16 tokens at a
+// time through its buffer, after which a lane has 8 features of the tokens `row` and `row` + 8 and
+// writes them as 16 bytes.
+struct Epilogue {
+  float* turn;
+  const float *xs, *ws, *bias;
+  __nv_bfloat16* c;
+  int64_t ldc;
+  int M, N, row, column;
+  bool wide;
+
+  __device__ __forceinline__ Epilogue(uint8_t* buffer, int M_, int N_, const float* xs_, const float* ws_,
+                                      const float* bias_, __nv_bfloat16* c_, int64_t ldc_)
+      : turn(reinterpret_cast<float*>(buffer)), xs(xs_), ws(ws_), bias(bias_), c(c_), ldc(ldc_), M(M_), N(N_) {
+    const int lane = threadIdx.x & 31;
+    row = lane / 4, column = (lane % 4) * 8;
+    wide = N % 8 == 0 && ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(c) & 15) == 0;
+  }
+
+  // tokens [m0, m0 + tokens) of features [n0, n0 + 32), accumulated at TMEM address `acc`
+  __device__ __forceinline__ void store(uint32_t acc, int n0, int m0, int tokens) const {
+    const int lane = threadIdx.x & 31, n = n0 + column;
+    float scale[8], b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      scale[e] = n + e < N ? __ldg(ws + n + e) : 0.0f;
+      b[e] = bias && n + e < N ? __ldg(bias + n + e) : 0.0f;
+    }
+#pragma unroll 1
+    for (int cc = 0; cc < tokens && m0 + cc < M; cc += 16) {
+      float xs_of[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int m = m0 + cc + row + 8 * i;
+        xs_of[i] = m < M ? __ldg(xs + m) : 0.0f;
+      }
+      uint32_t raw[16];
+      tmem_ld16(acc + cc, raw);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) turn[i * kTurnRow + lane] = __uint_as_float(raw[i]);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int m = m0 + cc + row + 8 * i;
+        const float4* from = reinterpret_cast<const float4*>(turn + (row + 8 * i) * kTurnRow + column);
+        const float4 lo = from[0], hi = from[1];
+        const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = fmaf(v[e] * xs_of[i], scale[e], b[e]);
+        if (m >= M) continue;
+        __nv_bfloat16* to = c + (int64_t)m * ldc + n;
+        if (wide) {
+          if (n < N)
+            *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]),
+                                                       pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e < N) to[e] = __float2bfloat16_rn(y[e]);
+        }
+      }
+      __syncwarp();
+    }
+  }
+};
+
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -117,7 +186,7 @@ __device__ __forceinline__ float4 peer_load(uint32_t addr, uint32_t rank) {
 // each over its part of K; their partial sums are added over distributed shared memory in rank
 // order, each CTA adding up its share of the tile's tokens.
 template <int kTokens>
-__global__ void __launch_bounds__(kThreads, Shape<kTokens>::kCtas)
+__global__ void __launch_bounds__(kThreads, 2)
     linear_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, int M, int N,
                   int K, const float* __restrict__ xs, const float* __restrict__ ws, const float* __restrict__ bias,
                   __nv_bfloat16* __restrict__ c, int64_t ldc, int splits) {
@@ -207,66 +276,26 @@ __global__ void __launch_bounds__(kThreads, Shape<kTokens>::kCtas)
       mbar_wait(bar(S::kDrain), 0, abort_flag, &g_gemm8_error, kErrMma);
     }
   } else {
+    const Epilogue out(sm + S::kTurnAt + warp * kTurnBytes, M, N, xs, ws, bias, c, ldc);
     const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
-    float* turn = reinterpret_cast<float*>(sm + S::kTurnAt + warp * kTurnBytes);
-    // after the turn a lane has 8 features of tokens row and row + 8 of the 16
-    const int row = lane / 4, column = (lane % 4) * 8;
-    const bool wide = N % 8 == 0 && ldc % 8 == 0 && (reinterpret_cast<uintptr_t>(c) & 15) == 0;
     int tl = 0;
     for (int t = first; t < tiles; t += next, ++tl) {
       const int ab = tl & 1;
-      const int n = (t % tf) * kFeatures + warp * 32 + column, m0 = (t / tf) * kTokens;
-      float scale[8], b[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        scale[e] = n + e < N ? __ldg(ws + n + e) : 0.0f;
-        b[e] = bias && n + e < N ? __ldg(bias + n + e) : 0.0f;
-      }
+      const int n0 = (t % tf) * kFeatures + warp * 32, m0 = (t / tf) * kTokens;
       const bool ok = mbar_wait(bar(S::kAccFull + ab), (tl >> 1) & 1, abort_flag, &g_gemm8_error, kErrEpilogue);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
+      if (splits > 1) {  // into the ring, which the products are done with
 #pragma unroll 1
-      for (int cc = 0; cc < kTokens; cc += 16) {
-        if (m0 + cc >= M) break;
-        float xs_of[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int m = m0 + cc + row + 8 * i;
-          xs_of[i] = m < M ? __ldg(xs + m) : 0.0f;
-        }
-        uint32_t raw[16];
-        tmem_ld16(t_lane + ab * kTokens + cc, raw);
-        if (splits > 1) {  // into the ring, which the products are done with
+        for (int cc = 0; cc < kTokens && m0 + cc < M; cc += 16) {
+          uint32_t raw[16];
+          tmem_ld16(t_lane + ab * kTokens + cc, raw);
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             reinterpret_cast<uint32_t*>(sm)[(cc + i) * kFeatures + warp * 32 + lane] = raw[i];
-          continue;
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) turn[i * kTurnRow + lane] = __uint_as_float(raw[i]);
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int m = m0 + cc + row + 8 * i;
-          const float4* from = reinterpret_cast<const float4*>(turn + (row + 8 * i) * kTurnRow + column);
-          const float4 lo = from[0], hi = from[1];
-          const float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-          float y[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = fmaf(v[e] * xs_of[i], scale[e], b[e]);
-          if (m >= M) continue;
-          __nv_bfloat16* to = c + (int64_t)m * ldc + n;
-          if (wide) {
-            if (n < N)
-              *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]),
-                                                         pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (n + e < N) to[e] = __float2bfloat16_rn(y[e]);
-          }
-        }
-        __syncwarp();
+      } else {
+        out.store(t_lane + ab * kTokens, n0, m0, kTokens);
       }
       tc_fence_before();
       __syncwarp();
@@ -326,6 +355,220 @@ __global__ void __launch_bounds__(kThreads, Shape<kTokens>::kCtas)
   }
 }
 
+// ------------------------------------------------------------ CTA pairs
+// Two CTAs of a cluster share a tile of 256 features x 256 tokens: cta_group::2 products with
+// M = 256, whose features 0-127 are in the even CTA's TMEM and shared memory and 128-255 in the
+// odd one's, while each CTA holds 128 of the tokens.  An instruction then reads 4 KB + 4 KB of each
+// CTA's shared memory in 128 clocks instead of 4 KB + 8 KB, and a token tile is fetched once for
+// 256 features.  Both CTAs' copies complete on the even CTA's barriers (a relay by the odd CTA would
+// cost a release at cluster scope, 0.9 us, for each stage); the even CTA's warp 5 issues every
+// product and commits its completions to both CTAs.  Every wait is bounded.
+struct Pair {
+  static constexpr int kTokens = 256, kHalf = 128, kStages = 6;
+  static constexpr int kStageBytes = kABytes + kHalf * kStepK;
+  // Full (even CTA): both CTAs' copies; Empty, AccFull: products done; AccEmpty (even CTA): the
+  // epilogue warps of both
+  static constexpr int kFull = 0, kEmpty = kStages, kAccFull = 2 * kStages, kAccEmpty = kAccFull + 2,
+                       kDrain = kAccEmpty + 2, kBars = kDrain + 1;
+  static constexpr int kTurnAt = kStages * kStageBytes, kBarAt = kTurnAt + 4 * kTurnBytes;
+  static constexpr int kTmemAt = kBarAt + kBars * 8, kAbortAt = kTmemAt + 4;
+  static constexpr size_t kSmem = 1024 + kAbortAt + 4;
+};
+
+__device__ __forceinline__ void mma_pair_stage(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p0, p1;\n .reg .b64 a1, a2, a3, b1, b2, b3;\n"
+      " setp.ne.b32 p0, %4, 0;\n setp.eq.b32 p1, %4, %4;\n"
+      " add.s64 a1, %1, 2;\n add.s64 a2, %1, 4;\n add.s64 a3, %1, 6;\n"
+      " add.s64 b1, %2, 2;\n add.s64 b2, %2, 4;\n add.s64 b3, %2, 6;\n"
+      " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p0;\n"
+      " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a1, b1, %3, p1;\n"
+      " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a2, b2, %3, p1;\n"
+      " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a3, b3, %3, p1;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives once on the barrier at this offset in both CTAs when this thread's products so far are done.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile(
+      "{\n .reg .b16 m;\n mov.b16 m, 3;\n"
+      " tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n}\n" ::"r"(
+          bar)
+      : "memory");
+}
+// The even CTA's barrier at this offset.
+__device__ __forceinline__ uint32_t in_even(uint32_t bar) {
+  uint32_t there;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(there) : "r"(bar));
+  return there;
+}
+__device__ __forceinline__ void arrive_even(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_even(bar)) : "memory");
+}
+// A tile into this CTA's shared memory that completes on a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ bool try_pair(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n"
+      " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+      " selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// A bounded wait on a barrier that the other CTA arrives on (sm100.cuh's mbar_wait, acquiring at
+// cluster scope).
+__device__ __forceinline__ bool wait_pair(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+  if (try_pair(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 16; ++i)
+      if (try_pair(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (*reinterpret_cast<volatile int*>(&g_gemm8_error) != 0) {
+      *abort_flag = 1;
+      return false;
+    }
+    if (globaltimer() - t0 > *reinterpret_cast<volatile unsigned long long*>(&g_wait_limit_ns)) {
+      *abort_flag = 1;
+      atomicCAS(&g_gemm8_error, 0, code);
+      return false;
+    }
+  }
+}
+
+// A wait at the end of the kernel that also holds after another wait gave up: up to 50 ms for what is
+// in flight towards this CTA.
+__device__ __forceinline__ void settle(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try(bar, parity) && globaltimer() - t0 < 50000000ull) {
+  }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    linear_pair_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x, int M, int N,
+                       int K, const float* __restrict__ xs, const float* __restrict__ ws,
+                       const float* __restrict__ bias, __nv_bfloat16* __restrict__ c, int64_t ldc) {
+  using S = Pair;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const uint32_t sb = smem_u32(sm);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
+  auto bar = [&](int i) { return sb + S::kBarAt + 8 * i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + S::kAbortAt);
+  const int tf = (N + 2 * kFeatures - 1) / (2 * kFeatures), tt = (M + S::kTokens - 1) / S::kTokens;
+  const int tiles = tf * tt, steps = (K + kStepK - 1) / kStepK;
+  const int first = (int)blockIdx.x / 2, next = (int)gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(bar(S::kFull + i), 1);
+      mbar_init(bar(S::kEmpty + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(S::kAccFull + i), 1);
+      mbar_init(bar(S::kAccEmpty + i), 8);
+    }
+    mbar_init(bar(S::kDrain), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sb + S::kTmemAt), "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers are set up before an arrival crosses
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + S::kTmemAt);
+
+  if (warp == 4) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += next) {
+        const int n0 = (t % tf) * 2 * kFeatures + rank * kFeatures, m0 = (t / tf) * S::kTokens + rank * S::kHalf;
+        for (int kb = 0; kb < steps; ++kb, ++it) {
+          const int s = it % S::kStages;
+          if (it >= S::kStages &&
+              !wait_pair(bar(S::kEmpty + s), ((it / S::kStages) - 1) & 1, abort_flag, kErrProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t a = sb + s * S::kStageBytes, fb = in_even(bar(S::kFull + s));
+          // the stage's one arrival; the odd CTA's bytes may come before it, the phase ends after it
+          if (rank == 0) mbar_expect_tx(bar(S::kFull + s), 2 * S::kStageBytes);
+          tma_load_pair(a, &tm_w, kb * kStepK, n0, fb);
+          tma_load_pair(a + kABytes, &tm_x, kb * kStepK, m0, fb);
+        }
+      }
+      // before either CTA may leave (both end in cluster_sync): every copy of both has landed, and
+      // the last completions have arrived at this CTA's barriers
+      for (int i = it > S::kStages ? it - S::kStages : 0; i < it; ++i) {
+        if (rank == 0) settle(bar(S::kFull + i % S::kStages), (i / S::kStages) & 1);
+        settle(bar(S::kEmpty + i % S::kStages), (i / S::kStages) & 1);
+      }
+    }
+  } else if (warp == 5) {
+    if (lane == 0 && rank == 0) {
+      constexpr uint32_t kIdesc = idesc_e4m3(2 * kFeatures, S::kTokens);
+      int it = 0, tl = 0;
+      bool ok = true;
+      for (int t = first; ok && t < tiles; t += next, ++tl) {
+        const int ab = tl & 1;
+        if (tl >= 2 && !wait_pair(bar(S::kAccEmpty + ab), ((tl >> 1) - 1) & 1, abort_flag, kErrMma)) break;
+        tc_fence_after();
+        for (int kb = 0; kb < steps; ++kb, ++it) {
+          const int s = it % S::kStages;
+          ok = wait_pair(bar(S::kFull + s), (it / S::kStages) & 1, abort_flag, kErrMma);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a = sb + s * S::kStageBytes;
+          mma_pair_stage(tmem + ab * S::kTokens, desc_k_sw128(a), desc_k_sw128(a + kABytes), kIdesc, kb > 0 ? 1u : 0u);
+          commit_pair(bar(S::kEmpty + s));
+        }
+        if (ok) commit_pair(bar(S::kAccFull + ab));
+      }
+      commit_pair(bar(S::kDrain));
+    }
+    if (lane == 0) settle(bar(S::kDrain), 0);  // both CTAs: the even one's commits are done, here too
+  } else {
+    const Epilogue out(sm + S::kTurnAt + warp * kTurnBytes, M, N, xs, ws, bias, c, ldc);
+    const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    int tl = 0;
+    for (int t = first; t < tiles; t += next, ++tl) {
+      const int ab = tl & 1;
+      const int n0 = (t % tf) * 2 * kFeatures + rank * kFeatures + warp * 32, m0 = (t / tf) * S::kTokens;
+      const bool ok = wait_pair(bar(S::kAccFull + ab), (tl >> 1) & 1, abort_flag, kErrEpilogue);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      out.store(t_lane + ab * S::kTokens, n0, m0, S::kTokens);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_even(bar(S::kAccEmpty + ab));
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // neither CTA frees its TMEM or leaves while the other may still reach it
+  if (warp == 5) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
 // ------------------------------------------------------------------ host
 using EncodeFn = PFN_cuTensorMapEncodeTiled_v12000;
 
@@ -369,6 +612,10 @@ static int64_t tiles_of(int M, int N, int tokens) {
   return (int64_t)((N + kFeatures - 1) / kFeatures) * ((M + tokens - 1) / tokens);
 }
 
+static int64_t pair_tiles_of(int M, int N) {
+  return (int64_t)((N + 2 * kFeatures - 1) / (2 * kFeatures)) * ((M + Pair::kTokens - 1) / Pair::kTokens);
+}
+
 template <int kTokens>
 static prism_status_t launch(const void* x8, int64_t ldx, const float* xs, const void* w8, int64_t ldw,
                              const float* ws, const float* bias, int M, int N, int K, void* c, int64_t ldc,
@@ -384,8 +631,7 @@ static prism_status_t launch(const void* x8, int64_t ldx, const float* xs, const
                    "prism_linear_fp8: smem attribute");
   const int64_t tiles = tiles_of(M, N, kTokens);
   cudaLaunchConfig_t config = {};
-  const int64_t slots = kSms * S::kCtas;
-  config.gridDim = dim3((unsigned)(splits > 1 ? tiles * splits : tiles < slots ? tiles : slots));
+  config.gridDim = dim3((unsigned)(splits > 1 ? tiles * splits : tiles < 2 * kSms ? tiles : 2 * kSms));
   config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = S::kSmem;
   config.stream = stream;
@@ -397,6 +643,24 @@ static prism_status_t launch(const void* x8, int64_t ldx, const float* xs, const
   PRISM_CHECK_CUDA(cudaLaunchKernelEx(&config, linear_kernel<kTokens>, mw, mx, M, N, K, xs, ws, bias,
                                       (__nv_bfloat16*)c, ldc, splits),
                    "prism_linear_fp8");
+  return PRISM_OK;
+}
+
+static prism_status_t launch_pair(const void* x8, int64_t ldx, const float* xs, const void* w8, int64_t ldw,
+                                  const float* ws, const float* bias, int M, int N, int K, void* c, int64_t ldc,
+                                  cudaStream_t stream) {
+  CUtensorMap mw, mx;
+  prism_status_t st = make_map(&mw, w8, N, K, ldw, kFeatures);
+  if (st != PRISM_OK) return st;
+  st = make_map(&mx, x8, M, K, ldx, Pair::kHalf);
+  if (st != PRISM_OK) return st;
+  PRISM_CHECK_CUDA(cudaFuncSetAttribute(linear_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)Pair::kSmem),
+                   "prism_linear_fp8: smem attribute");
+  const int64_t tiles = pair_tiles_of(M, N), pairs = tiles < kSms / 2 ? tiles : kSms / 2;
+  linear_pair_kernel<<<(unsigned)(2 * pairs), kThreads, Pair::kSmem, stream>>>(mw, mx, M, N, K, xs, ws, bias,
+                                                                              (__nv_bfloat16*)c, ldc);
+  PRISM_CHECK_LAUNCH("prism_linear_fp8");
   return PRISM_OK;
 }
 
@@ -426,23 +690,24 @@ extern "C" prism_status_t prism_linear_fp8(const void* x8, int64_t ldx, const fl
                   "prism_linear_fp8: 8-bit row strides must be multiples of 16 and cover K, ldc must cover N");
   PRISM_CHECK_ARG(aligned16(x8) && aligned16(w8), "prism_linear_fp8: 8-bit tensors must be 16-byte aligned");
   PRISM_CHECK_ARG(gemm8::tiles_of(M, N, 128) < ((int64_t)1 << 30), "prism_linear_fp8: the output has too many tiles");
-  // The smallest tile that holds every token.  Past 128 tokens: 128, of which an SM holds two, where
-  // that evens out few rounds of tiles (512 tokens of 5,120 x 5,120: 23.5 us against 25.3) or the
-  // epilogue counts (32,768 tokens of 512 x 1,536: 57 against 92); else 256, which reads less shared
-  // memory (4,096 tokens of 5,120 x 5,120: 89 against 96).
-  int tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  if (M > 128 && K > 1024 && gemm8::tiles_of(M, N, 256) > 2 * gemm8::kSms) tokens = 256;
+  // Pairs of CTAs on 256 x 256 where there are more than two rounds of such halves and K is long
+  // enough to hide the epilogue (2,048 tokens of 5,120 x 5,120: 52 us against 56 with 128-token
+  // tiles; 1,024 tokens, one round and a bit: 36 with those; 32,768 tokens of 512 x 1,536: 57, of
+  // which two CTAs an SM hide each other's epilogues).
+  if (M > 128 && K > 1024 && gemm8::tiles_of(M, N, 256) > 2 * gemm8::kSms)
+    return gemm8::launch_pair(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
+  // else the smallest tile that holds every token, 128 at most
+  const int tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
   // K in parts while the tiles leave SMs without work, if each part keeps five steps of a K long
   // enough to pay the exchange of 2.6 us (one token of 5,120 x 5,120: 15.1 us whole, 11.0 / 9.2 in
   // 2 / 4 parts; K = 1,536: 9.8 whole, 12.3 in two)
-  const int64_t tiles = gemm8::tiles_of(M, N, tokens), room = tokens == 256 ? gemm8::kSms : 2 * gemm8::kSms;
+  const int64_t tiles = gemm8::tiles_of(M, N, tokens), room = 2 * gemm8::kSms;
   const int steps = (K + gemm8::kStepK - 1) / gemm8::kStepK;
   int splits = 1;
   while (splits < gemm8::kMaxSplits && tiles * splits * 2 <= room && steps >= 20 && steps >= 10 * splits) splits *= 2;
   const auto launch = tokens == 16    ? gemm8::launch<16>
                       : tokens == 32  ? gemm8::launch<32>
                       : tokens == 64  ? gemm8::launch<64>
-                      : tokens == 128 ? gemm8::launch<128>
-                                      : gemm8::launch<256>;
+                                      : gemm8::launch<128>;
   return launch(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, splits, stream);
 }

@@ -122,6 +122,9 @@ def test_zero_gradients_and_measuring_only(cuda):
     norm = clip_grad_norm(grads, float("inf"))
     _check(grads, [before], grads, norm, float("inf"))
     assert float(clip_grad_norm([], 1.0)) == 0.0
+    grads[0][5] = float("inf")
+    before = grads[0].clone()
+    assert float(clip_grad_norm(grads, float("inf"))) == float("inf") and torch.equal(grads[0], before)
 
 
 def test_offsets_past_32_bits(cuda):

@@ -51,6 +51,17 @@ def test_layer_sizes(M, N, K, cuda):
     assert _lib.load().prism_device_status() == 0
 
 
+@pytest.mark.parametrize("M,N,K", [(9450, 5120, 1152), (20_001, 1000, 1168), (3001, 13_832, 2064), (76_000, 264, 1040),
+                                   (5000, 5001, 1040), (10_000, 4224, 5120)])
+def test_many_tiles(M, N, K, cuda):
+    """More tiles than SMs at a long K: odd numbers of 128-feature halves, ragged tokens, output rows
+    that allow no wide stores."""
+    x8, xs, w8, ws, b = _inputs(M, N, K, cuda)
+    y = linear_fp8(x8, xs, w8, ws, b)
+    _check(y, x8, xs, w8, ws, b)
+    assert torch.equal(y, linear_fp8(x8, xs, w8, ws, b)) and _lib.load().prism_device_status() == 0
+
+
 def test_shapes_strides_and_alignment(cuda):
     x8, xs, w8, ws, b = _inputs(60, 200, 256, cuda)
     ref = linear_fp8(x8, xs, w8, ws, b)
