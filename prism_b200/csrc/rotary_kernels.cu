@@ -22,6 +22,7 @@ namespace prism {
 namespace rotary {
 
 constexpr int kThreads = 128;   // a CTA's, where a head is not wider (256: 470 -> 510 us at 80 heads of 128)
+constexpr int kSms = 148;
 constexpr int kMaxDim = 1024, kMaxThreads = 1024;  // one element a thread, at worst
 
 struct Tensors {
@@ -314,8 +315,10 @@ cudaError_t launch(const Tensors& t, const Positions& p, const double* freqs, in
   const int heads = t.heads[0] + t.heads[1];
   Split s;
   s.units = kAdjacent ? dim / kVec : rot / 2 / kVec + (dim - rot) / kVec;
-  // equal rounds of heads in up to kThreads threads (a head wider than that has them all)
-  const int groups = s.units < kThreads ? kThreads / s.units : 1, rounds = (heads + groups - 1) / groups;
+  // equal rounds of heads in up to kThreads threads, or, for few tokens, in 512 for the shortest way
+  // through (a head wider than that has them all)
+  const int limit = tokens <= kSms ? 512 : kThreads;
+  const int groups = s.units < limit ? limit / s.units : 1, rounds = (heads + groups - 1) / groups;
   s.heads_at_once = (heads + rounds - 1) / rounds;
   s.tokens_at_once = groups / s.heads_at_once;
   const int threads = (s.units * s.heads_at_once * s.tokens_at_once + 31) / 32 * 32;
@@ -323,9 +326,12 @@ cudaError_t launch(const Tensors& t, const Positions& p, const double* freqs, in
   // eight tokens a thread (along the heads: eight items), within 16 KB of factors; few tokens are
   // spread over the SMs
   int per = (along_heads ? (7 + rounds) / rounds : 8) * s.tokens_at_once;
-  const int room = rot > 0 ? (16 << 10) / (rot / 2 * (int)sizeof(float2)) : per, spread = (tokens + 147) / 148;
+  const int room = rot > 0 ? (16 << 10) / (rot / 2 * (int)sizeof(float2)) : per, spread = (tokens + kSms - 1) / kSms;
   per = per < room ? per : room;
   per = per < spread ? per : spread;
+  // whole waves of CTAs (64 registers a thread), where there are few
+  const int slots = kSms * (1024 / threads > 0 ? 1024 / threads : 1), waves = (tokens / per + slots - 1) / slots;
+  if (waves > 0 && waves < 8) per = (tokens + waves * slots - 1) / (waves * slots);
   s.cta_tokens = per;
   const auto kernel = along_heads ? rotary_kernel<T, kVec, kAdjacent, true> : rotary_kernel<T, kVec, kAdjacent, false>;
   kernel<<<(tokens + per - 1) / per, threads, per * (rot / 2) * sizeof(float2), stream>>>(
