@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kMaxThreads)
                   const double* __restrict__ freqs, int tokens, int seq, Split split, int rot, int interleaved,
                   float scale, float sign) {
   using U = Unit<T, kVec, kAdjacent>;
-  constexpr int kBatch = kAdjacent ? 4 : 2;  // 16-byte loads of a thread on their way: 4
+  constexpr int kBatch = kAdjacent ? 4 : kAlongHeads ? 2 : 3;  // units of a thread on their way
   constexpr int kPairs = U::kPairs;
   extern __shared__ float2 factors[];        // [token of the CTA][pair]
   const int half = rot / 2, heads = t.heads[0] + t.heads[1];
