@@ -43,27 +43,42 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return m;
 }
 
-// Sum and maximum over the `group` lanes of a sub-warp, or over the CTA; every thread gets them.
-// `red` alternates between two rows, so that one barrier a reduction is enough.
-template <bool kCta>
-__device__ __forceinline__ SumMax group_reduce(SumMax v, int group, SumMax (*red)[32], int turn) {
-  const int top = kCta ? 16 : group / 2;
-  for (int o = top; o >= 1; o >>= 1) {
+// Sum, and maximum where kMax, over aligned runs of `lanes` lanes, a power of two; every lane
+// gets them.
+template <bool kMax>
+__device__ __forceinline__ SumMax lane_reduce(SumMax v, int lanes) {
+  for (int o = lanes / 2; o >= 1; o >>= 1) {
     v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
-    v.max = max_nan(v.max, __shfl_xor_sync(0xffffffffu, v.max, o));
-  }
-  if constexpr (kCta) {
-    SumMax* row = red[turn & 1];
-    const int nw = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) row[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = row[0];
-    for (int i = 1; i < nw; ++i) {
-      v.sum += row[i].sum;
-      v.max = max_nan(v.max, row[i].max);
-    }
+    if constexpr (kMax) v.max = max_nan(v.max, __shfl_xor_sync(0xffffffffu, v.max, o));
   }
   return v;
+}
+
+// The same over a whole warp: the maximum in one instruction.
+template <bool kMax>
+__device__ __forceinline__ SumMax warp_reduce(SumMax v) {
+  if constexpr (kMax) asm volatile("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(v.max));
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
+  return v;
+}
+
+// The same over the group of lanes, or over the CTA.  `red` alternates between two rows, so that
+// one barrier a reduction is enough.
+template <bool kCta, bool kMax>
+__device__ __forceinline__ SumMax group_reduce(SumMax v, int group, SumMax (*red)[32], int turn) {
+  if constexpr (kCta) {
+    v = warp_reduce<kMax>(v);
+    SumMax* row = red[turn & 1];
+    const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) row[threadIdx.x >> 5] = v;
+    __syncthreads();
+    // every warp adds up the warps' values in the same tree
+    v = lane < warps ? row[lane] : SumMax{0.0f, 0.0f};
+    return warp_reduce<kMax>(v);
+  } else {
+    return lane_reduce<kMax>(v, group);
+  }
 }
 
 // scale of an 8-bit row and the factor that takes w h to its 8-bit values.
@@ -72,9 +87,9 @@ struct Quant {
 };
 __device__ __forceinline__ Quant quantizer(const SumMax& t, float u) {
   Quant q;
-  q.scale = fmaxf(t.max * u / kFp8Max, kScaleFloor);
+  q.scale = fmaxf(t.max * u * (1.0f / kFp8Max), kScaleFloor);
   if (!(t.max <= kFloatMax)) q.scale = NAN;
-  q.factor = u / q.scale;
+  q.factor = __fdividef(u, q.scale);  // two units off at most; the scale is below 2^120
   return q;
 }
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
@@ -191,10 +206,11 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
   };
   if (kShift) fetch_single(p.first);
 
+  const float inv_cols = 1.0f / (float)cols;
   int stage = 0, turn = 0;
   for (int64_t row = p.first, warp_row = p.warp_first; warp_row < rows; row += p.step, warp_row += p.step, ++turn) {
     ring.wait();
-    const bool live = row < rows;
+    const bool live = kCta || row < rows;
     float hv[kPer], hs = xs;  // w h for 8-bit rows
     SumMax t = {0.0f, 0.0f};
     const auto take = [&](float& f, float wf) {
@@ -237,8 +253,8 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
     fetch(row + kStages * p.step, stage);
     if (kShift) fetch_single(row + p.step);
     stage = stage + 1 == kStages ? 0 : stage + 1;
-    t = group_reduce<kCta>(t, p.group, red, turn);
-    const float u = normalize ? rsqrtf(t.sum / (float)cols + eps) : 1.0f;
+    t = group_reduce<kCta, kQuant>(t, p.group, red, turn);
+    const float u = normalize ? rsqrtf(t.sum * inv_cols + eps) : 1.0f;
     if (!live) continue;
     if constexpr (kQuant) {
       const Quant q = quantizer(t, u);
@@ -334,10 +350,11 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
   };
   fetch_single(p.first);
 
+  const float inv_cols = 1.0f / (float)cols;
   int stage = 0, turn = 0;
   for (int64_t row = p.first, warp_row = p.warp_first; warp_row < rows; row += p.step, warp_row += p.step, ++turn) {
     ring.wait();
-    const bool live = row < rows;
+    const bool live = kCta || row < rows;
     const float u = u_next, gs0 = gs, hs0 = hs, ghs0 = ghs;
     SumMax t = {0.0f, 0.0f};
 #pragma unroll
@@ -358,8 +375,8 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
       dws += gs0 * hs0 * u;
     }
     fetch_single(row + p.step);
-    t = group_reduce<kCta>(t, p.group, red, turn);
-    const float k = t.sum * u * u * u / (float)cols;
+    t = group_reduce<kCta, false>(t, p.group, red, turn);
+    const float k = t.sum * u * u * u * inv_cols;
     // the row is read a second time from its slots: held in registers it would spill
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
@@ -442,7 +459,7 @@ __global__ void __launch_bounds__(kThreads)
     t.sum += f * f;
     if (kQuant) t.max = max_nan(t.max, fabsf(w ? f * w[c] : f));
   }
-  t = group_reduce<true>(t, kThreads, red, 0);
+  t = group_reduce<true, kQuant>(t, kThreads, red, 0);
   const float u = normalize ? rsqrtf(t.sum / (float)cols + eps) : 1.0f;
   const T* src = rr ? hr : xr;  // each thread reads back what it wrote
   if constexpr (kQuant) {
@@ -477,7 +494,7 @@ __global__ void __launch_bounds__(kThreads)
     const float g = Elem<T>::to_f(gr[c]);
     t.sum += (w ? g * w[c] : g) * Elem<T>::to_f(hr[c]);
   }
-  t = group_reduce<true>(t, kThreads, red, 0);
+  t = group_reduce<true, false>(t, kThreads, red, 0);
   const float u = rstd[row], k = t.sum * u * u * u / (float)cols;
   for (int c = threadIdx.x; c < cols; c += kThreads) {
     const float g = Elem<T>::to_f(gr[c]);
