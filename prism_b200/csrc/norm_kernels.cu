@@ -538,11 +538,15 @@ constexpr int kMaxPerSm = 16, kMaxParts = kMaxPerSm * kSms + 8;  // CTAs of a pe
 // start alike in 16 bytes: all aligned (with whole vectors to a row), or all shifted alike.
 //
 // A thread takes 8 elements of a row, or 16 where 8 would need more than `wide` threads: fewer
-// warps to a barrier and more CTAs to an SM, against fewer registers for other rows.  Measured at
-// 1,024 / 2,048 / 4,096 bf16 columns (120 M elements; 8 against 16 a thread, us):
-//   forward 155 / 174 / 155 against 168 / 170 / 178,  8-bit 177 / 167 / 171 against 188 / 151 / 149,
-//   backward 184 / 155 / 170 against 287 / 200 / 142
-// hence 512, 128 and 256.  A row of up to 32 threads' elements goes to a power-of-two group of lanes.
+// warps to a barrier and more CTAs to an SM, against more rows on their way and fewer idle lanes in
+// narrow rows.  Measured at 1,024 / 2,048 / 4,096 columns (us, 8 against 16 a thread):
+//   bf16, 120 M elements: forward 164 / 161 / 167 against 156 / 145 / 164,
+//     8-bit 151 / 147 / 140 against 145 / 140 / 127, backward 146 / 147 / 148 against 148 / 147 / 153
+//   fp32, 60 M elements: forward 156 / 160 / 161 against 149 / 150 / 159,
+//     8-bit 128 / 127 / 122 against 119 / 120 / 120, backward 155 / 155 / 143 against 141 / 140 / 144
+// and at 768 columns (8 M bf16 elements) forward 10.0 against 12.5, 8-bit 11.0 against 12.9; bf16
+// backward at 5,120: 173 against 149.  Hence 96, for the bf16 backward 512.  A row of up to 32
+// threads' elements goes to a power-of-two group of lanes.
 template <size_t kSize>
 Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int loaded, int wide) {
   constexpr int kWidth = 16 / (int)kSize;
@@ -558,9 +562,9 @@ Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int lo
   if (!aligned && !alike) return p;
   p.shift = !aligned;
   const int need = (cols + 7) / 8;
-  // Shifted rows: 16 a thread sooner (1,535 bf16 columns forward 253 -> 156 us, backward 313 -> 183),
-  // but for the fp32 backward, which then has one row on its way (18 -> 22 us at 4,095 x 1,535).
-  if (p.shift && wide > 128 && (kSize == 2 || loaded == 2)) wide = 128;
+  // Shifted rows: 16 a thread helps the bf16 backward too (1,535 columns 313 -> 183 us), but not the
+  // fp32 one, which then has one row on its way (18 -> 22 us at 4,095 x 1,535).
+  if (p.shift) wide = kSize == 4 && loaded == 3 ? 256 : 128;
   p.per = need > wide ? 16 : 8;
   const int lanes = (cols + p.per - 1) / p.per;  // threads that a row keeps busy
   if (lanes > 1024) return p;
@@ -636,7 +640,7 @@ template <typename T, bool kQuant>
 cudaError_t forward(const T* x, int64_t ldx, const T* r, int64_t ldr, const float* w, float eps, int normalize,
                     int64_t rows, int cols, void* y, T* h, float* aux, cudaStream_t stream) {
   const Operand tensors[4] = {{x, ldx}, {r, ldr}, {h, cols}, {kQuant ? nullptr : y, cols}};
-  Plan p = plan_rows<sizeof(T)>(tensors, 4, rows, cols, 2, kQuant ? 128 : 512);
+  Plan p = plan_rows<sizeof(T)>(tensors, 4, rows, cols, 2, 96);
   // whole vectors of bytes: the 8-bit rows start on their own vectors' boundaries
   if (kQuant && !p.any && !p.shift && reinterpret_cast<uintptr_t>(y) % (16 / sizeof(T)) != 0) p.any = true;
   if (p.any) {
@@ -659,7 +663,7 @@ template <typename T>
 cudaError_t backward(const T* gy, int64_t ldgy, const T* h, int64_t ldh, const T* gh, int64_t ldgh, const float* w,
                      const float* rstd, int64_t rows, int cols, T* dx, float* part, float* dw, cudaStream_t stream) {
   const Operand tensors[4] = {{gy, ldgy}, {h, ldh}, {gh, ldgh}, {dx, cols}};
-  Plan p = plan_rows<sizeof(T)>(tensors, 4, rows, cols, 3, 256);
+  Plan p = plan_rows<sizeof(T)>(tensors, 4, rows, cols, 3, sizeof(T) == 2 ? 512 : 96);
   int parts = 0;
   if (p.any) {
     bwd_any_kernel<T><<<(unsigned)rows, kThreads, 0, stream>>>(gy, ldgy, h, ldh, gh, ldgh, w, rstd, cols, dx);
