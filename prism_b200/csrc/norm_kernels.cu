@@ -146,7 +146,13 @@ struct Ring {
                  : "memory");
   }
   static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-  static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
+  // The oldest of the `depth` rows on their way has arrived.
+  static __device__ __forceinline__ void wait(int depth = kStages) {
+    if (depth == kStages)
+      asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+    else
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
   static __device__ __forceinline__ void drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 };
 
@@ -162,15 +168,16 @@ __device__ __forceinline__ void load_weight(const P& p, const float* w, float (&
   ws = w && p.single >= 0 ? __ldg(w + p.single) : 1.0f;
 }
 
-// Rows of a group on their way.  fp32 rows at 16 elements a thread (64 bytes) have to do with one:
+// Rows of a group on their way, at most.  fp32 rows at 16 elements a thread (64 bytes) have to do with one:
 // 220 KB hold no more of 1,024 threads' slots.
 constexpr int stages(int bytes) { return bytes <= 32 ? 2 : 1; }
 
-// kQuant: 8-bit rows.  normalize = 0: the rows themselves (u = 1).
+// kQuant: 8-bit rows.  normalize = 0: the rows themselves (u = 1).  depth: rows of a group on their
+// way, one or kStages.
 template <typename T, int kPer, bool kCta, bool kShift, bool kQuant>
 __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
     fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ r, int64_t ldr,
-               const float* __restrict__ w, float eps, int normalize, int64_t rows, int cols, int group,
+               const float* __restrict__ w, float eps, int normalize, int64_t rows, int cols, int group, int depth,
                void* __restrict__ y, T* __restrict__ h, float* __restrict__ aux) {
   using P = Place<T, kPer, kCta, kShift>;
   constexpr int kWidth = P::kWidth, kVecs = P::kVecs;
@@ -193,7 +200,8 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
     ring.commit();
   };
 #pragma unroll
-  for (int s = 0; s < kStages; ++s) fetch(p.first + s * p.step, s);
+  for (int s = 0; s < kStages; ++s)
+    if (s < depth) fetch(p.first + s * p.step, s);
   float wv[kPer], ws;
   load_weight(p, w, wv, ws);
   const bool has_single = kShift && p.single >= 0;
@@ -209,7 +217,7 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
   const float inv_cols = 1.0f / (float)cols;
   int stage = 0, turn = 0;
   for (int64_t row = p.first, warp_row = p.warp_first; warp_row < rows; row += p.step, warp_row += p.step, ++turn) {
-    ring.wait();
+    ring.wait(depth);
     const bool live = kCta || row < rows;
     float hv[kPer], hs = xs;  // w h for 8-bit rows
     SumMax t = {0.0f, 0.0f};
@@ -250,9 +258,9 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
       }
       take(hs, ws);
     }
-    fetch(row + kStages * p.step, stage);
+    fetch(row + depth * p.step, stage);
     if (kShift) fetch_single(row + p.step);
-    stage = stage + 1 == kStages ? 0 : stage + 1;
+    stage = stage + 1 == depth ? 0 : stage + 1;
     t = group_reduce<kCta, kQuant>(t, p.group, red, turn);
     const float u = normalize ? rsqrtf(t.sum * inv_cols + eps) : 1.0f;
     if (!live) continue;
@@ -528,7 +536,7 @@ struct Operand {
 // How a call runs: by whole vectors, by vectors between single elements, or element by element.
 struct Plan {
   bool any = true, shift = false, cta = false;
-  int per = 8, group = 32, threads = kThreads, per_cta = 1, align = 1, grid = 0;
+  int per = 8, group = 32, threads = kThreads, per_cta = 1, align = 1, depth = 1, grid = 0;
   size_t ring = 0, smem = 0;
 };
 
@@ -580,7 +588,8 @@ Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int lo
   const int per_cta = p.cta ? 1 : p.threads / p.group;
   // the ring, and room for a sum of dL/dw from each group
   const int bytes = p.per * (int)kSize;
-  p.smem = (size_t)loaded * stages(bytes) * bytes * p.threads;
+  p.depth = stages(bytes);
+  p.smem = (size_t)loaded * p.depth * bytes * p.threads;
   const size_t sums = p.cta ? 0 : (size_t)per_cta * cols * sizeof(float);
   int present = 0;
   for (int i = 0; i < loaded; ++i) present += tensors[i].ptr != nullptr;
@@ -594,12 +603,19 @@ Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int lo
 // The persistent grid: as many CTAs an SM as keep `budget` bytes of rows on their way, and two
 // (one computes while the other waits at its barrier) if that is at most 80 KB.  More bytes are
 // worse where the kernel also writes much: 120 M bf16 elements in 2,048 columns forward (half of
-// the traffic writes) took 150 us with 48 KB an SM and 177 us with 96 KB; 8-bit rows 131 us with
-// 64 KB and 145 us with 80 KB; the backward (a quarter writes) wants all that fit.
-void size_grid(Plan& p, int64_t rows, int budget, int regs) {
+// the traffic writes) took 145 us with 48 KB an SM and 168 us with 96 KB; 8-bit rows in 4,096
+// columns 127 us with 64 KB and 149 us with 96 KB; the backward (a quarter writes) wants all that
+// fit.  So the forward has one row of a group on its way where a second one would leave the budget
+// to a single CTA: 5,120 columns 152 against 168 us, 8-bit rows 128 against 145 us.
+void size_grid(Plan& p, int64_t rows, int budget, int regs, bool forward) {
+  if (p.shift) budget = 180 << 10;  // their single elements are loaded a row ahead only
+  if (forward && p.cta && p.depth == 2 && (int)p.ring < budget && 2 * (int)p.ring > budget) {
+    p.depth = 1;
+    p.ring /= 2;
+    p.smem /= 2;
+  }
   const int fit[] = {65536 / (((regs + 7) / 8 * 8) * p.threads), 2048 / p.threads, (int)((220 << 10) / (p.smem + 1024)),
                      kMaxPerSm};
-  if (p.shift) budget = 180 << 10;  // their single elements are loaded a row ahead only
   int per_sm = budget / (int)p.ring;
   if (per_sm < 2) per_sm = p.ring <= 40 << 10 ? 2 : 1;
   for (int f : fit) per_sm = per_sm < f ? per_sm : f;
@@ -651,10 +667,11 @@ cudaError_t forward(const T* x, int64_t ldx, const T* r, int64_t ldr, const floa
   return with_plan(p, [&](auto per, auto cta, auto shift) {
     const auto kernel = fwd_kernel<T, per(), cta(), shift(), kQuant>;
     static const int regs = registers_of(kernel);
-    size_grid(p, rows, kQuant ? 64 << 10 : 48 << 10, regs);
+    size_grid(p, rows, kQuant ? 64 << 10 : 48 << 10, regs, true);
     const cudaError_t e = allow_smem(kernel, p.smem);
     if (e != cudaSuccess) return e;
-    kernel<<<p.grid, p.threads, p.smem, stream>>>(x, ldx, r, ldr, w, eps, normalize, rows, cols, p.group, y, h, aux);
+    kernel<<<p.grid, p.threads, p.smem, stream>>>(x, ldx, r, ldr, w, eps, normalize, rows, cols, p.group, p.depth, y, h,
+                                                 aux);
     return cudaGetLastError();
   });
 }
@@ -677,7 +694,7 @@ cudaError_t backward(const T* gy, int64_t ldgy, const T* h, int64_t ldh, const T
     const cudaError_t e = with_plan(p, [&](auto per, auto cta, auto shift) {
       const auto kernel = bwd_kernel<T, per(), cta(), shift()>;
       static const int regs = registers_of(kernel);
-      size_grid(p, rows, 180 << 10, regs);
+      size_grid(p, rows, 180 << 10, regs, false);
       parts = p.grid;
       const cudaError_t a = allow_smem(kernel, p.smem);
       if (a != cudaSuccess) return a;
