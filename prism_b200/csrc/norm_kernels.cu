@@ -43,41 +43,43 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return m;
 }
 
-// Sum, and maximum where kMax, over aligned runs of `lanes` lanes, a power of two; every lane
-// gets them.
-template <bool kMax>
+// Sum where kSum, maximum where kMax, over aligned runs of `lanes` lanes, a power of two; every
+// lane gets them.
+template <bool kSum, bool kMax>
 __device__ __forceinline__ SumMax lane_reduce(SumMax v, int lanes) {
   for (int o = lanes / 2; o >= 1; o >>= 1) {
-    v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
+    if constexpr (kSum) v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
     if constexpr (kMax) v.max = max_nan(v.max, __shfl_xor_sync(0xffffffffu, v.max, o));
   }
   return v;
 }
 
 // The same over a whole warp: the maximum in one instruction.
-template <bool kMax>
+template <bool kSum, bool kMax>
 __device__ __forceinline__ SumMax warp_reduce(SumMax v) {
   if constexpr (kMax) asm volatile("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(v.max));
+  if constexpr (kSum) {
 #pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
+    for (int o = 16; o >= 1; o >>= 1) v.sum += __shfl_xor_sync(0xffffffffu, v.sum, o);
+  }
   return v;
 }
 
 // The same over the group of lanes, or over the CTA.  `red` alternates between two rows, so that
 // one barrier a reduction is enough.
-template <bool kCta, bool kMax>
+template <bool kCta, bool kSum, bool kMax>
 __device__ __forceinline__ SumMax group_reduce(SumMax v, int group, SumMax (*red)[32], int turn) {
   if constexpr (kCta) {
-    v = warp_reduce<kMax>(v);
+    v = warp_reduce<kSum, kMax>(v);
     SumMax* row = red[turn & 1];
     const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
     if (lane == 0) row[threadIdx.x >> 5] = v;
     __syncthreads();
     // every warp adds up the warps' values in the same tree
     v = lane < warps ? row[lane] : SumMax{0.0f, 0.0f};
-    return warp_reduce<kMax>(v);
+    return warp_reduce<kSum, kMax>(v);
   } else {
-    return lane_reduce<kMax>(v, group);
+    return lane_reduce<kSum, kMax>(v, group);
   }
 }
 
@@ -172,12 +174,13 @@ __device__ __forceinline__ void load_weight(const P& p, const float* w, float (&
 // 220 KB hold no more of 1,024 threads' slots.
 constexpr int stages(int bytes) { return bytes <= 32 ? 2 : 1; }
 
-// kQuant: 8-bit rows.  normalize = 0: the rows themselves (u = 1).  depth: rows of a group on their
-// way, one or kStages.
-template <typename T, int kPer, bool kCta, bool kShift, bool kQuant>
+// kQuant: 8-bit rows.  Without kNorm the rows themselves (u = 1, no sum: 60,000 x 5,120 bf16 to 8
+// bits 162 us, with a sum that nothing reads 191).  depth: rows of a group on their way, one or
+// kStages.
+template <typename T, int kPer, bool kCta, bool kShift, bool kQuant, bool kNorm>
 __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
     fwd_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ r, int64_t ldr,
-               const float* __restrict__ w, float eps, int normalize, int64_t rows, int cols, int group, int depth,
+               const float* __restrict__ w, float eps, int64_t rows, int cols, int group, int depth,
                void* __restrict__ y, T* __restrict__ h, float* __restrict__ aux) {
   using P = Place<T, kPer, kCta, kShift>;
   constexpr int kWidth = P::kWidth, kVecs = P::kVecs;
@@ -222,9 +225,9 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
     float hv[kPer], hs = xs;  // w h for 8-bit rows
     SumMax t = {0.0f, 0.0f};
     const auto take = [&](float& f, float wf) {
-      if (!kQuant || normalize) t.sum += f * f;
+      if (kNorm) t.sum += f * f;
       if (kQuant) {
-        f *= wf;
+        if (kNorm || w) f *= wf;
         t.max = max_nan(t.max, fabsf(f));
       }
     };
@@ -261,8 +264,8 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
     fetch(row + depth * p.step, stage);
     if (kShift) fetch_single(row + p.step);
     stage = stage + 1 == depth ? 0 : stage + 1;
-    t = group_reduce<kCta, kQuant>(t, p.group, red, turn);
-    const float u = normalize ? rsqrtf(t.sum * inv_cols + eps) : 1.0f;
+    t = group_reduce<kCta, kNorm, kQuant>(t, p.group, red, turn);
+    const float u = kNorm ? rsqrtf(t.sum * inv_cols + eps) : 1.0f;
     if (!live) continue;
     if constexpr (kQuant) {
       const Quant q = quantizer(t, u);
@@ -383,7 +386,7 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
       dws += gs0 * hs0 * u;
     }
     fetch_single(row + p.step);
-    t = group_reduce<kCta, false>(t, p.group, red, turn);
+    t = group_reduce<kCta, true, false>(t, p.group, red, turn);
     const float k = t.sum * u * u * u * inv_cols;
     // the row is read a second time from its slots: held in registers it would spill
 #pragma unroll
@@ -467,7 +470,7 @@ __global__ void __launch_bounds__(kThreads)
     t.sum += f * f;
     if (kQuant) t.max = max_nan(t.max, fabsf(w ? f * w[c] : f));
   }
-  t = group_reduce<true, kQuant>(t, kThreads, red, 0);
+  t = group_reduce<true, true, kQuant>(t, kThreads, red, 0);
   const float u = normalize ? rsqrtf(t.sum / (float)cols + eps) : 1.0f;
   const T* src = rr ? hr : xr;  // each thread reads back what it wrote
   if constexpr (kQuant) {
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(kThreads)
     const float g = Elem<T>::to_f(gr[c]);
     t.sum += (w ? g * w[c] : g) * Elem<T>::to_f(hr[c]);
   }
-  t = group_reduce<true, false>(t, kThreads, red, 0);
+  t = group_reduce<true, true, false>(t, kThreads, red, 0);
   const float u = rstd[row], k = t.sum * u * u * u / (float)cols;
   for (int c = threadIdx.x; c < cols; c += kThreads) {
     const float g = Elem<T>::to_f(gr[c]);
@@ -664,16 +667,20 @@ cudaError_t forward(const T* x, int64_t ldx, const T* r, int64_t ldr, const floa
                                                                        aux);
     return cudaGetLastError();
   }
-  return with_plan(p, [&](auto per, auto cta, auto shift) {
-    const auto kernel = fwd_kernel<T, per(), cta(), shift(), kQuant>;
-    static const int regs = registers_of(kernel);
-    size_grid(p, rows, kQuant ? 64 << 10 : 48 << 10, regs, true);
-    const cudaError_t e = allow_smem(kernel, p.smem);
-    if (e != cudaSuccess) return e;
-    kernel<<<p.grid, p.threads, p.smem, stream>>>(x, ldx, r, ldr, w, eps, normalize, rows, cols, p.group, p.depth, y, h,
-                                                 aux);
-    return cudaGetLastError();
-  });
+  const auto run = [&](auto norm) {
+    return with_plan(p, [&](auto per, auto cta, auto shift) {
+      const auto kernel = fwd_kernel<T, per(), cta(), shift(), kQuant, norm()>;
+      static const int regs = registers_of(kernel);
+      size_grid(p, rows, kQuant ? 64 << 10 : 48 << 10, regs, true);
+      const cudaError_t e = allow_smem(kernel, p.smem);
+      if (e != cudaSuccess) return e;
+      kernel<<<p.grid, p.threads, p.smem, stream>>>(x, ldx, r, ldr, w, eps, rows, cols, p.group, p.depth, y, h, aux);
+      return cudaGetLastError();
+    });
+  };
+  if constexpr (kQuant)
+    if (!normalize) return run(std::false_type{});
+  return run(std::true_type{});
 }
 
 template <typename T>
