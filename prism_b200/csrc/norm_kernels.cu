@@ -557,7 +557,7 @@ constexpr int kMaxPerSm = 16, kMaxParts = kMaxPerSm * kSms + 8;  // CTAs of a pe
 //     8-bit 128 / 127 / 122 against 119 / 120 / 120, backward 155 / 155 / 143 against 141 / 140 / 144
 // and at 768 columns (8 M bf16 elements) forward 10.0 against 12.5, 8-bit 11.0 against 12.9; bf16
 // backward at 5,120: 173 against 149.  Hence 96, for the bf16 backward 512.  A row of up to 32
-// threads' elements goes to a power-of-two group of lanes.
+// threads' elements, 8 each, goes to a power-of-two group of lanes.
 template <size_t kSize>
 Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int loaded, int wide) {
   constexpr int kWidth = 16 / (int)kSize;
@@ -649,10 +649,9 @@ cudaError_t with_plan(const Plan& p, F&& fn) {
   const auto shift = [&](auto per, auto cta) {
     return p.shift ? fn(per, cta, integral_constant<bool, true>{}) : fn(per, cta, integral_constant<bool, false>{});
   };
-  const auto cta = [&](auto per) {
-    return p.cta ? shift(per, integral_constant<bool, true>{}) : shift(per, integral_constant<bool, false>{});
-  };
-  return p.per == 8 ? cta(integral_constant<int, 8>{}) : cta(integral_constant<int, 16>{});
+  using std::true_type;
+  if (p.per == 16) return shift(integral_constant<int, 16>{}, true_type{});  // wide rows
+  return p.cta ? shift(integral_constant<int, 8>{}, true_type{}) : shift(integral_constant<int, 8>{}, std::false_type{});
 }
 
 template <typename T, bool kQuant>
