@@ -697,14 +697,22 @@ extern "C" prism_status_t prism_linear_fp8(const void* x8, int64_t ldx, const fl
   if (M > 128 && K > 1024 && gemm8::tiles_of(M, N, 256) > 2 * gemm8::kSms)
     return gemm8::launch_pair(x8, ldx, x_scale, w8, ldw, w_scale, bias, M, N, K, c, ldc, stream);
   // else the smallest tile that holds every token, 128 at most
-  const int tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
-  // K in parts while the tiles leave SMs without work, if each part keeps five steps of a K long
-  // enough to pay the exchange of 2.6 us (one token of 5,120 x 5,120: 15.1 us whole, 11.0 / 9.2 in
-  // 2 / 4 parts; K = 1,536: 9.8 whole, 12.3 in two)
-  const int64_t tiles = gemm8::tiles_of(M, N, tokens), room = 2 * gemm8::kSms;
   const int steps = (K + gemm8::kStepK - 1) / gemm8::kStepK;
+  int tokens = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  // A short K: smaller tiles while they leave SMs without work (125 tokens of 5,120 x 1,536 in tiles
+  // of 128 / 64 / 32 tokens, 40 / 80 / 160 tiles: 9.8 / 8.5 / 8.7 us; 706 of 160 x 368 down to 16
+  // tokens: 7.2 / 5.8 / 5.0 / 4.7), from 128 to 64 also for a little more than one round (133 of
+  // 7,312 x 464, 174 tiles: 8.1 / 6.8 us; in 290 of 32 tokens 7.6)
+  constexpr int kSplitSteps = 20;
+  while (steps < kSplitSteps && tokens > 16 &&
+         gemm8::tiles_of(M, N, tokens / 2) <= (tokens == 128 ? gemm8::kSms * 4 / 3 : gemm8::kSms))
+    tokens /= 2;
+  // A long one in parts, if each keeps five steps: enough to pay the exchange of 2.6 us (one token
+  // of 5,120 x 5,120: 15.1 us whole, 11.0 / 9.2 in 2 / 4 parts; 125 tokens of K = 1,536: 8.5 whole, 9.9 in two)
+  const int64_t tiles = gemm8::tiles_of(M, N, tokens), room = 2 * gemm8::kSms;
   int splits = 1;
-  while (splits < gemm8::kMaxSplits && tiles * splits * 2 <= room && steps >= 20 && steps >= 10 * splits) splits *= 2;
+  while (splits < gemm8::kMaxSplits && tiles * splits * 2 <= room && steps >= kSplitSteps && steps >= 10 * splits)
+    splits *= 2;
   const auto launch = tokens == 16    ? gemm8::launch<16>
                       : tokens == 32  ? gemm8::launch<32>
                       : tokens == 64  ? gemm8::launch<64>
