@@ -16,9 +16,9 @@
 // warps 0-3 (thread = output feature) drain the other.  Every wait is bounded (sm100.cuh); one
 // that gives up sets this file's device error word.
 //
-// Measured: one token of 5,120 x 5,120 9.1 us; 125 of 5,120 x 1,536 8.4; 75,600 tokens 1.37 ms, 2.90 PFLOP/s in a short run
-// (0.88 of twice the measured bf16 rate; tensor pipe 80 to 84 % busy) and 2.4 in a long one under the
-// power cap.
+// Measured: one token of 5,120 x 5,120 9.1 us; 125 of 5,120 x 1,536 8.4; 75,600 tokens of
+// 5,120 x 5,120 1.37 ms, 2.90 PFLOP/s in a short run (0.88 of twice the measured bf16 rate; tensor
+// pipe 80 to 84 % busy) and 2.4 in a long one under the power cap.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
