@@ -212,6 +212,30 @@ def test_8bit_rows(rows, cols, dtype, cuda):
         assert bool(((x8.float().double() - v).abs() <= 2.0 ** -4 * v.abs() * (1 + 2.0 ** -18) + 2.0 ** -10).all())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cols", [128, 760, 768, 776, 1531, 3000, 5120, 5112, 6144, 10000])
+def test_many_rows_of_each_form(cols, dtype, cuda):
+    """More rows than a launch's groups hold at once, several times over, at widths where a group
+    keeps one row or two on their way: forward and 8-bit rows, with a norm and without."""
+    rows = max(1500, 3000000 // cols)
+    x, r, w, _, _ = _inputs(rows, cols, dtype, cuda, seed=cols + 1)
+    for residual in (r, None):
+        h64, _, y64 = _forward64(x, residual, w)
+        y, h = add_rms_norm(x, residual, w, EPS)
+        assert torch.equal(h.double(), h64)
+        _within(y, y64, _a(cols) * y64.abs(), dtype, "y")
+        y8, s, h8 = add_rms_norm_fp8(x, residual, w, EPS)
+        s64 = y64.abs().amax(-1, keepdim=True) / 448
+        assert torch.equal(h8, h) and bool(((s.double()[:, None] - s64).abs() <= (_a(cols) + 2.0 ** -21) * s64).all())
+        v = y64 / s64
+        assert bool(((y8.float().double() - v).abs() <= 2.0 ** -4 * v.abs() + 2.0 ** -10 + 2 * _a(cols) * v.abs()).all())
+    x8, s = quantize_rows_fp8(x)
+    ref = x.float().abs().amax(-1) / 448
+    assert bool(((s - ref).abs() <= 2.0 ** -22 * ref).all())
+    v = x.double() / s.double()[:, None]
+    assert bool(((x8.float().double() - v).abs() <= 2.0 ** -4 * v.abs() * (1 + 2.0 ** -18) + 2.0 ** -10).all())
+
+
 @pytest.mark.parametrize("cols", [96, 1535, 5120])
 def test_rows_of_zeros_and_of_non_finite_values(cols, cuda):
     """A zero row stays zero with the least scale; a row with a NaN or an infinity has scale NaN
