@@ -44,6 +44,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return m;
 }
 
+// The largest magnitude, a NaN if any is.
+__device__ __forceinline__ float max_abs_nan(float a, float b, float c) {
+  float m;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+  return m;
+}
+
 // Sum where kSum, maximum where kMax, over aligned runs of `lanes` lanes, a power of two; every
 // lane gets them.
 template <bool kSum, bool kMax>
@@ -176,7 +183,7 @@ __device__ __forceinline__ void load_weight(const P& p, const float* w, float (&
 constexpr int stages(int bytes) { return bytes <= 32 ? 2 : 1; }
 
 // kQuant: 8-bit rows.  Without kNorm the rows themselves (u = 1, no sum: 60,000 x 5,120 bf16 to 8
-// bits 162 us, with a sum that nothing reads 191).  depth: rows of a group on their way, one or
+// bits 160 us, with a sum that nothing reads 191).  depth: rows of a group on their way, one or
 // kStages.
 template <typename T, int kPer, bool kCta, bool kShift, bool kQuant, bool kNorm>
 __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
@@ -227,10 +234,7 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
     SumMax t = {0.0f, 0.0f};
     const auto take = [&](float& f, float wf) {
       if (kNorm) t.sum += f * f;
-      if (kQuant) {
-        if (kNorm || w) f *= wf;
-        t.max = max_nan(t.max, fabsf(f));
-      }
+      if (kQuant && (kNorm || w)) f *= wf;
     };
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
@@ -253,6 +257,10 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
         take(f[e], wv[v * kWidth + e]);
         hv[v * kWidth + e] = f[e];
       }
+      if (kQuant) {
+#pragma unroll
+        for (int e = 0; e < kWidth; e += 2) t.max = max_abs_nan(t.max, f[e], f[e + 1]);
+      }
     }
     if (has_single && live) {
       if (r) {
@@ -261,6 +269,7 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
         hs = Elem<T>::to_f(v);
       }
       take(hs, ws);
+      if (kQuant) t.max = max_abs_nan(t.max, hs, hs);
     }
     fetch(row + depth * p.step, stage);
     if (kShift) fetch_single(row + p.step);
