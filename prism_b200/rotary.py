@@ -48,7 +48,8 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, *, scaling: Opti
         pair = lambda beta: (rotary_dim * math.log(original_length / (beta * 2 * math.pi))) / (2 * math.log(theta))
         # the ramp may end behind the last pair: where that one still turns more than beta_slow times
         low, high = max(math.floor(pair(beta_fast)), 0), min(math.ceil(pair(beta_slow)), rotary_dim - 1)
-        ramp = ((j2 / 2 - low) / max(high - low, 1e-3)).clamp(0, 1)
+        # high <= 0: even the fastest pair turns no more than beta_slow times
+        ramp = ((j2 / 2 - low) / max(high - low, 1e-3)).clamp(0, 1) if high > 0 else torch.ones_like(j2)
         freqs = freqs * (1 - ramp) + freqs / factor * ramp
         gain = 0.1 * math.log(factor) + 1.0
     elif scaling not in (None, "ntk"):

@@ -36,3 +36,11 @@ def test_ramp_is_the_definitions(rotary_dim, theta, length, factor):
 def test_a_slowest_pair_that_turns_is_not_divided_by_the_whole_factor(rotary_dim, length, factor):
     turns, ratio = _ratio(rotary_dim, 1e4, factor, length)
     assert float(turns[-1]) > 1.2 and 1 / factor * 1.01 < ratio[-1] < 1
+
+
+@pytest.mark.parametrize("length,slow", [(1, 1.0), (4, 1.0), (6, 1.0), (20, 4.0)])
+def test_where_even_the_fastest_pair_turns_less_than_beta_slow(length, slow):
+    """Every pair is divided by the factor, the first one too."""
+    turns, ratio = _ratio(64, 1e4, 4.0, length, slow=slow)
+    assert float(turns[0]) < slow
+    assert all(math.isclose(r, 0.25, rel_tol=1e-12) for r in ratio)
