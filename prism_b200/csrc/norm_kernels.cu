@@ -9,7 +9,9 @@
 // Backward, with gy = dL/dy and gh = dL/dh:
 //   dL/dh_j = u (w_j gy_j) - h_j u^3 / C * sum_i w_i gy_i h_i + gh_j   (also dL/dx and dL/dr)
 //   dL/dw_j = sum over rows of gy_j h_j u
-// Sums, u and the gradient of w are held in fp32.
+// Sums, u and the gradient of w are held in fp32.  Where the squares of finite values leave it
+// (rows above some 1e19), the row is summed again times 2^-80: a branch that ordinary rows do not
+// take.  The backward forms h u, of order one, before any product with h.
 //
 // Bound by memory: each tensor is read or written once.  A row stays with one group of threads --
 // a power of two of lanes for narrow rows, a CTA for wide ones -- which holds it in registers
@@ -17,8 +19,8 @@
 // (they hold their columns of w, and sum their columns of dL/dw, in registers over all their
 // rows) and fetch the next rows with cp.async into slots of shared memory that only the fetching
 // thread reads: no barrier but the reduction's, and the loads of the next row or two are on their
-// way while one is reduced.  Measured at 75,600 x 5,120 bf16 with a residual: forward 475 us
-// (6.5 TB/s, half of it writes), backward 456 us (6.8); 9,450 rows to 8 bits 54 us (6.3).
+// way while one is reduced.  Measured at 75,600 x 5,120 bf16 with a residual: forward 484 us
+// (6.4 TB/s, half of it writes), backward 456 us (6.8); 9,450 rows to 8 bits 54 us (6.3).
 #include <cuda_fp8.h>
 #include <math.h>
 
@@ -30,6 +32,9 @@ namespace norm {
 constexpr float kFp8Max = 448.0f;                      // largest finite e4m3 value
 constexpr float kScaleFloor = 7.8886090522101181e-31f;  // 2^-100: 1 / scale stays finite
 constexpr float kFloatMax = 3.402823466e38f;
+// Takes every finite row's squares into fp32, 16,384 of up to 2^96, and leaves those that make up a sum of
+// 2^128 and more above 2^-32.
+constexpr float kDown = 8.2718061255302767e-25f;  // 2^-80
 constexpr int kThreads = 256;   // of the kernels whose groups are smaller than a CTA
 constexpr int kSms = 148;
 
@@ -182,6 +187,40 @@ __device__ __forceinline__ void load_weight(const P& p, const float* w, float (&
 // 220 KB hold no more of 1,024 threads' slots.
 constexpr int stages(int bytes) { return bytes <= 32 ? 2 : 1; }
 
+// A row of a group that met one whose squares leave fp32: from h as it is kept, summed and, if it is such a
+// row, normalised times kDown, element by element.  count: its columns, or 0 for a group that only takes
+// part in its warp's shuffles.  After the rows' loop, which it would take registers from; looking for such
+// rows costs the loop 2 % (forward of 75,600 x 5,120 bf16 474 -> 484 us).
+template <typename T, bool kCta, bool kQuant>
+__device__ __forceinline__ void large_row(const T* h, const float* w, float eps, int count, int64_t row, int cols, int lane,
+                                       int group, SumMax (*red)[32], int turn, void* y, float* aux) {
+  if constexpr (!kCta) __syncwarp();  // the group's other threads wrote h
+  SumMax t = {0.0f, 0.0f};
+#pragma unroll 1
+  for (int c = lane; c < count; c += group) {
+    const float f = Elem<T>::to_f(h[c]) * kDown;
+    t.sum += f * f;
+    if (kQuant) t.max = max_nan(t.max, fabsf(w ? f * w[c] : f));
+  }
+  t = group_reduce<kCta, true, kQuant>(t, group, red, turn);
+  // half of fp32's range, whose sums both ways have: the loop added them up in another order
+  if (!(t.sum > 0.5f * kFloatMax * kDown * kDown)) return;
+  const float u = rsqrtf(t.sum / (float)cols + eps * kDown * kDown);
+  Quant q = {};
+  if constexpr (kQuant) q = quantizer(t, u);
+#pragma unroll 1
+  for (int c = lane; c < count; c += group) {
+    float f = Elem<T>::to_f(h[c]) * kDown;
+    if (w) f *= w[c];
+    if constexpr (kQuant) static_cast<uint8_t*>(y)[row * cols + c] = (uint8_t)e4m3x2(f * q.factor, 0.0f);
+    else static_cast<T*>(y)[row * cols + c] = Elem<T>::from_f(f * u);
+  }
+  if (lane == 0 && count > 0) {
+    if constexpr (kQuant) aux[row] = q.scale;
+    else if (aux) aux[row] = u * kDown;
+  }
+}
+
 // kQuant: 8-bit rows.  Without kNorm the rows themselves (u = 1, no sum: 60,000 x 5,120 bf16 to 8
 // bits 160 us, with a sum that nothing reads 191).  depth: rows of a group on their way, one or
 // kStages.
@@ -196,6 +235,7 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
   __shared__ SumMax red[2][32];
   const P p(x, ldx, cols, group);
   constexpr int kStages = stages(kPer * sizeof(T));
+  constexpr bool kResum = kNorm && !std::is_same_v<T, __half>;  // fp16 squares always fit
   const Ring<2, kVecs, kStages> ring(smem);
   const auto fetch = [&](int64_t row, int stage) {
     if (row < rows) {
@@ -227,6 +267,7 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
 
   const float inv_cols = 1.0f / (float)cols;
   int stage = 0, turn = 0;
+  bool large = false;  // one of the group's rows is to be summed again
   for (int64_t row = p.first, warp_row = p.warp_first; warp_row < rows; row += p.step, warp_row += p.step, ++turn) {
     ring.wait(depth);
     const bool live = kCta || row < rows;
@@ -275,6 +316,7 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
     if (kShift) fetch_single(row + p.step);
     stage = stage + 1 == depth ? 0 : stage + 1;
     t = group_reduce<kCta, kNorm, kQuant>(t, p.group, red, turn);
+    if (kResum) large = large || t.sum > kFloatMax;
     const float u = kNorm ? rsqrtf(t.sum * inv_cols + eps) : 1.0f;
     if (!live) continue;
     if constexpr (kQuant) {
@@ -323,6 +365,13 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
     }
   }
   ring.drain();
+  if constexpr (kResum) {
+    if (kCta ? large : __any_sync(0xffffffffu, large)) {
+      for (int64_t row = p.first, warp_row = p.warp_first; warp_row < rows; row += p.step, warp_row += p.step, ++turn)
+        large_row<T, kCta, kQuant>(r ? h + row * cols : x + row * ldx, w, eps, large && row < rows ? cols : 0, row, cols,
+                                   p.lane, p.group, red, turn, y, aux);
+    }
+  }
 }
 
 // dL/dh of the rows, and each CTA's sum of dL/dw -> part[CTA][cols] (part NULL: not wanted).
@@ -386,18 +435,19 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
       unpack<T>(*ring.at(stage, 1, v), hf);
 #pragma unroll
       for (int e = 0; e < kWidth; ++e) {
-        const float gh_e = g[e] * hf[e];
-        t.sum += gh_e * wv[v * kWidth + e];
-        dw[v * kWidth + e] += gh_e * u;
+        const float d = g[e] * (hf[e] * u);
+        t.sum += d * wv[v * kWidth + e];
+        dw[v * kWidth + e] += d;
       }
     }
     if (has_single && live) {
-      t.sum += gs0 * hs0 * ws;
-      dws += gs0 * hs0 * u;
+      const float d = gs0 * (hs0 * u);
+      t.sum += d * ws;
+      dws += d;
     }
     fetch_single(row + p.step);
     t = group_reduce<kCta, true, false>(t, p.group, red, turn);
-    const float k = t.sum * u * u * u * inv_cols;
+    const float k = t.sum * inv_cols * u;
     // the row is read a second time from its slots: held in registers it would spill
 #pragma unroll
     for (int v = 0; v < kVecs; ++v) {
@@ -408,10 +458,10 @@ __global__ void __launch_bounds__(kCta ? 1024 : kThreads, kCta ? 1 : 4)
       unpack<T>(*ring.at(stage, 1, v), hf);
       if (gh) unpack<T>(*ring.at(stage, 2, v), add);
 #pragma unroll
-      for (int e = 0; e < kWidth; ++e) add[e] += g[e] * wv[v * kWidth + e] * u - hf[e] * k;
+      for (int e = 0; e < kWidth; ++e) add[e] += (g[e] * wv[v * kWidth + e] - hf[e] * k) * u;
       *reinterpret_cast<uint4*>(dx + row * cols + c) = pack<T>(add);
     }
-    if (has_single && live) dx[row * cols + p.single] = Elem<T>::from_f(gs0 * ws * u - hs0 * k + ghs0);
+    if (has_single && live) dx[row * cols + p.single] = Elem<T>::from_f((gs0 * ws - hs0 * k) * u + ghs0);
     fetch(row + kStages * p.step, stage);
     stage = stage + 1 == kStages ? 0 : stage + 1;
   }
@@ -481,23 +531,34 @@ __global__ void __launch_bounds__(kThreads)
     if (kQuant) t.max = max_nan(t.max, fabsf(w ? f * w[c] : f));
   }
   t = group_reduce<true, true, kQuant>(t, kThreads, red, 0);
-  const float u = normalize ? rsqrtf(t.sum / (float)cols + eps) : 1.0f;
   const T* src = rr ? hr : xr;  // each thread reads back what it wrote
+  float down = 1.0f;
+  if (normalize && t.sum > kFloatMax) {
+    down = kDown;
+    t = {0.0f, 0.0f};
+    for (int c = threadIdx.x; c < cols; c += kThreads) {
+      const float f = Elem<T>::to_f(src[c]) * down;
+      t.sum += f * f;
+      if (kQuant) t.max = max_nan(t.max, fabsf(w ? f * w[c] : f));
+    }
+    t = group_reduce<true, true, kQuant>(t, kThreads, red, 1);
+  }
+  const float u = normalize ? rsqrtf(t.sum / (float)cols + eps * down * down) : 1.0f;  // of the row times `down`
   if constexpr (kQuant) {
     const Quant q = quantizer(t, u);
     uint8_t* out = static_cast<uint8_t*>(y) + row * cols;
     for (int c = threadIdx.x; c < cols; c += kThreads) {
-      const float f = Elem<T>::to_f(src[c]);
+      const float f = Elem<T>::to_f(src[c]) * down;
       out[c] = (uint8_t)e4m3x2((w ? f * w[c] : f) * q.factor, 0.0f);
     }
     if (threadIdx.x == 0) aux[row] = q.scale;
   } else {
     T* out = static_cast<T*>(y) + row * cols;
     for (int c = threadIdx.x; c < cols; c += kThreads) {
-      const float f = Elem<T>::to_f(src[c]) * u;
+      const float f = Elem<T>::to_f(src[c]) * down * u;
       out[c] = Elem<T>::from_f(w ? f * w[c] : f);
     }
-    if (threadIdx.x == 0 && aux) aux[row] = u;
+    if (threadIdx.x == 0 && aux) aux[row] = u * down;
   }
 }
 
@@ -511,15 +572,16 @@ __global__ void __launch_bounds__(kThreads)
   const T* gr = gy + row * ldgy;
   const T* hr = h + row * ldh;
   SumMax t = {0.0f, 0.0f};
+  const float u = rstd[row];
   for (int c = threadIdx.x; c < cols; c += kThreads) {
     const float g = Elem<T>::to_f(gr[c]);
-    t.sum += (w ? g * w[c] : g) * Elem<T>::to_f(hr[c]);
+    t.sum += (w ? g * w[c] : g) * (Elem<T>::to_f(hr[c]) * u);
   }
   t = group_reduce<true, true, false>(t, kThreads, red, 0);
-  const float u = rstd[row], k = t.sum * u * u * u / (float)cols;
+  const float k = t.sum / (float)cols * u;
   for (int c = threadIdx.x; c < cols; c += kThreads) {
     const float g = Elem<T>::to_f(gr[c]);
-    float d = (w ? g * w[c] : g) * u - Elem<T>::to_f(hr[c]) * k;
+    float d = ((w ? g * w[c] : g) - Elem<T>::to_f(hr[c]) * k) * u;
     if (gh) d += Elem<T>::to_f(gh[row * ldgh + c]);
     dx[row * cols + c] = Elem<T>::from_f(d);
   }
@@ -536,7 +598,7 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
   float s = 0.0f;
   for (int64_t i = r0; i < r1; ++i)
-    s += Elem<T>::to_f(gy[i * ldgy + c]) * Elem<T>::to_f(h[i * ldh + c]) * rstd[i];
+    s += Elem<T>::to_f(gy[i * ldgy + c]) * (Elem<T>::to_f(h[i * ldh + c]) * rstd[i]);
   part[(int64_t)blockIdx.y * cols + c] = s;
 }
 
@@ -635,8 +697,12 @@ void size_grid(Plan& p, int64_t rows, int budget, int regs, bool forward) {
   if (per_sm < 1) per_sm = 1;
   const int64_t want = (rows + p.per_cta - 1) / p.per_cta;
   p.grid = (int)(want < per_sm * kSms ? want : per_sm * kSms);
-  // groups' rows shifted alike: the row step is a multiple of the shifts' period
-  if (p.grid * p.per_cta % p.align != 0) p.grid = (p.grid + p.align - 1) / p.align * p.align;
+  // groups' rows shifted alike: the row step is a multiple of the shifts' period (rounded down where the
+  // CTAs that this adds would wait for the others' SMs)
+  if (p.grid * p.per_cta % p.align != 0) {
+    const int up = (p.grid + p.align - 1) / p.align * p.align;
+    p.grid = up <= per_sm * kSms ? up : up - p.align;
+  }
 }
 
 template <typename K>
