@@ -711,12 +711,18 @@ int registers_of(K kernel) {
   return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 64;
 }
 
+// The limit is the kernel's, not the launch's, and calls from other threads set it too: always to `most`,
+// what any plan of this kernel asks for at most.
 template <typename K>
-cudaError_t allow_smem(K kernel, size_t bytes) {
+cudaError_t allow_smem(K kernel, size_t bytes, size_t most) {
   return bytes > (40 << 10)  // 48 KB without asking, static arrays included
-             ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes)
+             ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most)
              : cudaSuccess;
 }
+constexpr size_t most_smem(int tensors, int per, int size, bool cta) {
+  return (size_t)tensors * stages(per * size) * per * size * (cta ? 1024 : kThreads);
+}
+static_assert(most_smem(3, 16, 4, true) <= 220 << 10, "a CTA's shared memory");
 
 // Calls fn with the plan's compile-time choices: fn(elements a thread, CTA rows, shifted rows).
 template <typename F>
@@ -747,7 +753,7 @@ cudaError_t forward(const T* x, int64_t ldx, const T* r, int64_t ldr, const floa
       const auto kernel = fwd_kernel<T, per(), cta(), shift(), kQuant, norm()>;
       static const int regs = registers_of(kernel);
       size_grid(p, rows, kQuant ? 64 << 10 : 48 << 10, regs, true);
-      const cudaError_t e = allow_smem(kernel, p.smem);
+      const cudaError_t e = allow_smem(kernel, p.smem, most_smem(2, per(), sizeof(T), cta()));
       if (e != cudaSuccess) return e;
       kernel<<<p.grid, p.threads, p.smem, stream>>>(x, ldx, r, ldr, w, eps, rows, cols, p.group, p.depth, y, h, aux);
       return cudaGetLastError();
@@ -778,7 +784,7 @@ cudaError_t backward(const T* gy, int64_t ldgy, const T* h, int64_t ldh, const T
       static const int regs = registers_of(kernel);
       size_grid(p, rows, 180 << 10, regs, false);
       parts = p.grid;
-      const cudaError_t a = allow_smem(kernel, p.smem);
+      const cudaError_t a = allow_smem(kernel, p.smem, most_smem(3, per(), sizeof(T), cta()));
       if (a != cudaSuccess) return a;
       kernel<<<p.grid, p.threads, p.smem, stream>>>(gy, ldgy, h, ldh, gh, ldgh, w, rstd, rows, cols, p.group, dx,
                                                     dw ? part : nullptr);
