@@ -204,10 +204,11 @@ struct Turn {
   int ends[2];
   bool interleaved;
   double scale;
+  bool conjugate = false;  // the gradient's turn
 };
 
 // q [B, S, Hq, D], k [B, S, Hk, D] or undefined, unit column strides -> new (q, k).
-std::pair<Tensor, Tensor> turn_heads(const Tensor& q, const Tensor& k, const Turn& t, bool conjugate) {
+std::pair<Tensor, Tensor> turn_heads(const Tensor& q, const Tensor& k, const Turn& t) {
   const Launch launch(device_of({q, k, t.positions, t.freqs}));
   const Tensor qo = new_like(q), ko = k.defined() ? new_like(k) : Tensor();
   const auto strides = [](const Tensor& x) { return x.defined() ? x.strides().data() : nullptr; };
@@ -216,7 +217,7 @@ std::pair<Tensor, Tensor> turn_heads(const Tensor& q, const Tensor& k, const Tur
   check(prism_rotary(at(q), strides(q), (int)q.size(2), at(k), strides(k), k.defined() ? (int)k.size(2) : 0, q.size(0),
                      q.size(1), (int)q.size(3), 2 * (int)t.freqs.size(0), t.interleaved, at(t.positions),
                      t.positions.scalar_type() == at::kLong, t.strides, t.ends, (const double*)at(t.freqs),
-                     (float)t.scale, conjugate, dtype_code(q, "apply_rotary"), at(qo), strides(qo), at(ko), strides(ko),
+                     (float)t.scale, t.conjugate, dtype_code(q, "apply_rotary"), at(qo), strides(qo), at(ko), strides(ko),
                      launch.stream),
         "prism_rotary");
   return {qo, ko};
@@ -226,11 +227,11 @@ struct Rotary : torch::autograd::Function<Rotary> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Optional& k_in, const Turn& t) {
     const Tensor k = or_undefined(k_in);
     ctx->save_for_backward({t.positions, t.freqs});
-    ctx->saved_data["meta"] =
-        std::vector<int64_t>{t.strides[0], t.strides[1], t.ends[0], t.ends[1], (int64_t)t.interleaved};
+    ctx->saved_data["meta"] = std::vector<int64_t>{t.strides[0], t.strides[1],           t.ends[0],
+                                                   t.ends[1],    (int64_t)t.interleaved, (int64_t)t.conjugate};
     ctx->saved_data["scale"] = t.scale;
     ctx->set_materialize_grads(false);
-    auto [qo, ko] = turn_heads(q, k, t, false);
+    auto [qo, ko] = turn_heads(q, k, t);
     return k.defined() ? variable_list{qo, ko} : variable_list{qo};
   }
 
@@ -238,12 +239,18 @@ struct Rotary : torch::autograd::Function<Rotary> {
     const auto saved = ctx->get_saved_variables();
     const auto meta = ctx->saved_data["meta"].toIntVector();
     const Turn t = {saved[0], saved[1], {meta[0], meta[1]}, {(int)meta[2], (int)meta[3]}, meta[4] != 0,
-                    ctx->saved_data["scale"].toDouble()};
+                    ctx->saved_data["scale"].toDouble(), meta[5] == 0};
     const auto unit = [](const Tensor& g) { return !g.defined() || g.stride(-1) == 1 ? g : g.contiguous(); };
     const Tensor gq = unit(grads[0]), gk = grads.size() > 1 ? unit(grads[1]) : Tensor();
     if (!gq.defined() && !gk.defined()) return {Tensor(), Tensor(), Tensor()};
-    if (!gq.defined()) return {Tensor(), turn_heads(gk, Tensor(), t, true).first, Tensor()};  // k's alone
-    auto [dq, dk] = turn_heads(gq, gk, t, true);
+    // linear, so its own gradient: a node of the graph where one is made of the gradients
+    const auto turn = [&](const Tensor& a, const Tensor& b) {
+      if (!at::GradMode::is_enabled()) return turn_heads(a, b, t);
+      const variable_list out = apply(a, b.defined() ? Optional(b) : std::nullopt, t);
+      return std::make_pair(out[0], b.defined() ? out[1] : Tensor());
+    };
+    if (!gq.defined()) return {Tensor(), turn(gk, Tensor()).first, Tensor()};  // k's alone
+    auto [dq, dk] = turn(gq, gk);
     return {dq, dk, Tensor()};
   }
 };
@@ -303,7 +310,7 @@ std::tuple<Tensor, Optional> apply_rotary(const Tensor& q_in, const Optional& k_
     qo = out[0];
     if (k.defined()) ko = out[1];
   } else {
-    std::tie(qo, ko) = turn_heads(q, k, t, false);
+    std::tie(qo, ko) = turn_heads(q, k, t);
   }
   if (dims == 3) {
     qo = qo.squeeze(0);
