@@ -6,6 +6,7 @@
 // Built against the installed torch and linked to libprism_bsa.so (prism_b200/build.py).
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -128,6 +129,18 @@ std::tuple<Tensor, Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& r
   return {y, h, rstd};
 }
 
+// The gradients as parts of a graph that raises where it is differentiated.  `from`: what they depend on; the
+// node leads there, or a derivative with respect to these alone would go past it.
+std::pair<Tensor, Tensor> without_derivative(Tensor dx, Tensor dw, std::initializer_list<Tensor> from) {
+  const at::AutoGradMode grad(true);
+  variable_list in = {dx.requires_grad_(), dw.defined() ? dw.requires_grad_() : Tensor()};
+  in.insert(in.end(), from);
+  const auto node = std::make_shared<torch::autograd::DelayedError>("add_rms_norm: its gradient has no gradient",
+                                                                   (int64_t)in.size());
+  const variable_list out = (*node)(std::move(in));
+  return {out[0], out[1]};
+}
+
 struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
   // absent tensors are empty optionals: they have no edge in the graph
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Optional& residual, const Optional& weight,
@@ -148,6 +161,8 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
     const bool want_w = w.defined() && ctx->needs_input_grad(has_r ? 2 : 1);
     Tensor dx = gh, dw;
     if (gy.defined()) {  // else h = x + r alone passes its gradient on
+      const bool graph = at::GradMode::is_enabled();
+      const at::NoGradGuard no_grad;
       const int64_t cols = h.size(-1);
       const Tensor g2 = rows2d(gy, cols), h2 = rows2d(h, cols), gh2 = rows2d(gh, cols);
       const Tensor w2 = fp32_vector(w, cols, "weight");
@@ -165,6 +180,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
                                    at(workspace), (float*)at(dw), launch.stream),
             "prism_add_rms_norm_bwd");
       if (want_w) dw = dw.to(w.scalar_type());
+      if (graph) std::tie(dx, dw) = without_derivative(dx, dw, {gy, gh, h, w});
     }
     const bool want_r = has_r && ctx->needs_input_grad(1);
     return {ctx->needs_input_grad(0) ? dx : Tensor(), want_r ? dx : Tensor(), dw, Tensor()};

@@ -2,7 +2,8 @@
 
 * ``add_rms_norm(x, residual, weight, eps)`` -> (y, h): h = x + residual, rounded to the
   tensors' type, is the residual stream that the next layer adds to, and y its RMS norm times
-  weight; one pass, differentiable in x, residual and weight.
+  weight; one pass, differentiable in x, residual and weight, once: a gradient of y's gradient is an
+  error.
 * ``add_rms_norm_fp8`` -> (y8, scale, h): the same with y in 8 bits (e4m3) and one fp32 scale a
   row, y ~ y8 * scale, as ``prism_b200.linear.linear_fp8`` reads it.  For inference.
 * ``quantize_rows_fp8(x)`` -> (x8, scale): rows (a weight's output features, a layer's input)
