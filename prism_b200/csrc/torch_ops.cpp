@@ -96,6 +96,12 @@ bool wants_grad(std::initializer_list<Tensor> tensors) {
   return false;
 }
 
+// Forward-mode derivatives are not implemented: refused, since the kernels would drop the tangent.
+void refuse_tangents(std::initializer_list<Tensor> tensors, const char* what) {
+  for (const Tensor& t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 // ------------------------------------------------------------------ RMS norm
 struct Rows {
   int device, code;
@@ -189,6 +195,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
 
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& x, const Optional& residual, const Optional& weight, double eps) {
   const Tensor r = or_undefined(residual), w = or_undefined(weight);
+  refuse_tangents({x, r, w}, "add_rms_norm");
   if (wants_grad({x, r, w})) {
     const variable_list out = AddRmsNorm::apply(x, residual, weight, eps);
     return {out[0], r.defined() ? out[1] : x};
@@ -201,6 +208,7 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& x, const Optio
                                                     double eps, bool normalize) {
   const char* what = normalize ? "add_rms_norm_fp8" : "quantize_rows_fp8";
   const Tensor r = or_undefined(residual), w = or_undefined(weight);
+  refuse_tangents({x, r, w}, what);
   TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({x, r, w}), what, " is inference only: its 8-bit rounding has no gradient");
   const Rows in = rows_input(x, r, w, what);
   const Launch launch(in.device);
@@ -320,6 +328,7 @@ std::tuple<Tensor, Optional> apply_rotary(const Tensor& q_in, const Optional& k_
     if (k.defined()) k = k.unsqueeze(0);
   }
   device_of({q, k, t.positions, t.freqs});
+  refuse_tangents({q, k, t.freqs}, "apply_rotary");
   Tensor qo, ko;
   if (wants_grad({q, k})) {
     const variable_list out = Rotary::apply(q, k.defined() ? Optional(k) : std::nullopt, t);
@@ -354,6 +363,7 @@ Tensor linear_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, con
                    "linear_fp8 expects fp32 scales");
   TORCH_CHECK_VALUE(x_scale.sizes() == x8.sizes().slice(0, x8.dim() - 1) && w_scale.sizes() == w8.sizes().slice(0, 1),
                     "linear_fp8: one scale a row of x and of W");
+  refuse_tangents({x8, x_scale, w8, w_scale, bias}, "linear_fp8");
   TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({x_scale, w_scale, bias}), "linear_fp8 is inference only");
   const Launch launch(device_of({x8, x_scale, w8, w_scale, bias}));
   const int64_t K = w8.size(1), N = w8.size(0);
