@@ -329,6 +329,7 @@ std::tuple<Tensor, Optional> apply_rotary(const Tensor& q_in, const Optional& k_
   }
   device_of({q, k, t.positions, t.freqs});
   refuse_tangents({q, k, t.freqs}, "apply_rotary");
+  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({freqs}), "apply_rotary has no gradient with respect to freqs");
   Tensor qo, ko;
   if (wants_grad({q, k})) {
     const variable_list out = Rotary::apply(q, k.defined() ? Optional(k) : std::nullopt, t);
@@ -364,7 +365,7 @@ Tensor linear_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, con
   TORCH_CHECK_VALUE(x_scale.sizes() == x8.sizes().slice(0, x8.dim() - 1) && w_scale.sizes() == w8.sizes().slice(0, 1),
                     "linear_fp8: one scale a row of x and of W");
   refuse_tangents({x8, x_scale, w8, w_scale, bias}, "linear_fp8");
-  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({x_scale, w_scale, bias}), "linear_fp8 is inference only");
+  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({x8, x_scale, w8, w_scale, bias}), "linear_fp8 is inference only");
   const Launch launch(device_of({x8, x_scale, w8, w_scale, bias}));
   const int64_t K = w8.size(1), N = w8.size(0);
   const Tensor x2 = x8.dim() == 2 ? x8 : x8.reshape({-1, K});

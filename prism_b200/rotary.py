@@ -67,7 +67,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     positions: int32 or int64 [S] or [B, S]; with sections (a, b[, c]), the numbers of pairs
     that follow each axis, [.., S, 2 or 3].  freqs: fp64, radians per position
     (``rotary_frequencies``).  scale multiplies the rotated columns.  Any strides of batch,
-    token and head; differentiable in q and k."""
+    token and head; differentiable in q and k, any number of times."""
     return _lib.torch_ops().apply_rotary(q, k, positions, freqs, layout, sections, scale)
 
 
