@@ -543,7 +543,8 @@ prism_status_t prism_rotary(const void* q, const int64_t* q_strides, int q_heads
 /* Global gradient norm and clipping over count tensors (host arrays of device pointers, element
  * counts and prism_dtype_t): norm [1] fp32 = sqrt(sum of all squares), outs[i] = grads[i] *
  * min(1, max_norm / (norm + 1e-6)).  outs[i] is grads[i] itself (in place; nothing is written
- * when the factor is 1) or a buffer that overlaps no gradient.  Squares and sums fp64, fixed
+ * when the factor is 1) or a buffer that overlaps no gradient and no other output; else the call is
+ * refused.  A gradient that is given again in place counts each time and is scaled once.  Squares and sums fp64, fixed
  * order.  A NaN norm makes every output NaN, an infinite max_norm has factor 1.  workspace:
  * prism_clip_grad_norm_workspace_bytes(count), 8-byte aligned. */
 size_t prism_clip_grad_norm_workspace_bytes(int64_t count);

@@ -13,6 +13,10 @@
 // passes is not worth an order: reading backwards took 152 us instead of 154).
 #include <math.h>
 
+#include <algorithm>
+#include <new>
+#include <vector>
+
 #include "block_ops.cuh"
 
 namespace prism {
@@ -176,15 +180,128 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 
 inline int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
 
-// Calls fn(table, chunks) for each group of at most kMax non-empty tensors.
+// What a call reads and writes.  A CTA scales what another may still read, so that memory that is written may
+// belong to one entry only.
+struct Run {
+  uintptr_t begin, end;
+};
+struct Start {
+  uintptr_t begin;
+  int64_t tensor;
+};
+inline int64_t bytes_of(int dtype) { return dtype == PRISM_FP32 ? 4 : 2; }
+
+// By address.  Longer lists as packed words, by 11 of the bits in which addresses differ at a time.
+inline void sort_starts(std::vector<Start>& v) {
+  const auto before = [](const Start& a, const Start& b) { return a.begin < b.begin; };
+  if (std::is_sorted(v.begin(), v.end(), before)) return;
+  uintptr_t low = v[0].begin, high = low, differ = 0;
+  for (const Start& s : v) low = std::min(low, s.begin), high = std::max(high, s.begin), differ |= s.begin ^ v[0].begin;
+  int skip = 0, bits = 0, index_bits = 0;
+  while (!(differ >> skip & 1)) ++skip;
+  while ((high - low) >> skip >> bits) ++bits;
+  while (v.size() >> index_bits) ++index_bits;
+  if (v.size() < 48 || bits + index_bits > 64) {
+    std::sort(v.begin(), v.end(), before);
+    return;
+  }
+  std::vector<uint64_t> keys(v.size()), other(v.size());
+  for (size_t i = 0; i < v.size(); ++i) keys[i] = (uint64_t)((v[i].begin - low) >> skip) << index_bits | i;
+  constexpr int kDigit = 11;
+  for (int shift = index_bits; shift < index_bits + bits; shift += kDigit) {
+    uint32_t at[(1 << kDigit) + 1] = {};
+    for (uint64_t k : keys) ++at[(k >> shift & ((1 << kDigit) - 1)) + 1];
+    for (int i = 0; i + 1 < 1 << kDigit; ++i) at[i + 1] += at[i];
+    for (uint64_t k : keys) other[at[k >> shift & ((1 << kDigit) - 1)]++] = k;
+    keys.swap(other);
+  }
+  std::vector<Start> sorted(v.size());
+  for (size_t i = 0; i < v.size(); ++i) sorted[i] = v[keys[i] & ((1ull << index_bits) - 1)];
+  v.swap(sorted);
+}
+
+// The lists of a call, as its checks see them.
+struct Lists {
+  const void* const* in;
+  void* const* out;
+  const int64_t* n;
+  const int* dtype;
+  int64_t count;
+  bool measure;  // an infinite max_norm writes nothing in place
+
+  bool written(int64_t i) const { return n[i] > 0 && !(measure && in[i] == out[i]); }
+  bool read_only(int64_t i) const { return n[i] > 0 && (measure || in[i] != out[i]); }
+  Run span(const void* p, int64_t i) const {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(p);
+    return {begin, begin + n[i] * bytes_of(dtype[i])};
+  }
+};
+
+// What is written, as a few disjoint runs in order of address: outputs that are slices of flat buffers, or
+// short lists.  False where that does not work out.
+inline bool few_runs(const Lists& l, std::vector<Run>& runs) {
+  constexpr size_t kFew = 8;
+  for (int64_t i = 0; i < l.count; ++i) {
+    if (!l.written(i)) continue;
+    const Run s = l.span(l.out[i], i);
+    size_t r = 0;
+    while (r < runs.size() && runs[r].end != s.begin) ++r;
+    if (r < runs.size()) runs[r].end = s.end;
+    else if (r < kFew) runs.push_back(s);
+    else return false;
+  }
+  std::sort(runs.begin(), runs.end(), [](const Run& a, const Run& b) { return a.begin < b.begin; });
+  for (size_t r = 1; r < runs.size(); ++r)
+    if (runs[r].begin < runs[r - 1].end) return false;
+  return true;
+}
+
+// Marks the entries that are scaled in place by another entry (repeated; empty where there are none).  Returns the
+// index of an entry that shares memory otherwise, or -1.
+inline int64_t check_overlap(const Lists& l, std::vector<uint8_t>& repeated) {
+  std::vector<Run> runs;
+  if (!few_runs(l, runs)) {
+    runs.clear();
+    std::vector<Start> writes;
+    writes.reserve(l.count);
+    for (int64_t i = 0; i < l.count; ++i)
+      if (l.written(i)) writes.push_back({reinterpret_cast<uintptr_t>(l.out[i]), i});
+    sort_starts(writes);
+    runs.reserve(writes.size());
+    int64_t last = -1;
+    for (const Start& s : writes) {
+      const int64_t i = s.tensor;
+      if (last >= 0 && s.begin < runs.back().end) {
+        const bool same = l.out[i] == l.out[last] && l.n[i] == l.n[last] && l.dtype[i] == l.dtype[last];
+        if (!same || l.in[i] != l.out[i] || l.in[last] != l.out[last]) return i;
+        if (repeated.empty()) repeated.assign(l.count, 0);
+        repeated[i] = 1;
+        continue;
+      }
+      last = i;
+      runs.push_back(l.span(l.out[i], i));
+    }
+  }
+  for (int64_t i = 0; i < l.count; ++i) {
+    if (!l.read_only(i)) continue;
+    // the last run that begins before the gradient ends
+    const Run g = l.span(l.in[i], i);
+    const auto after =
+        std::lower_bound(runs.begin(), runs.end(), g.end, [](const Run& r, uintptr_t end) { return r.begin < end; });
+    if (after != runs.begin() && (after - 1)->end > g.begin) return i;
+  }
+  return -1;
+}
+
+// Calls fn(table, chunks) for each group of at most kMax non-empty tensors that `skip` (or NULL) does not name.
 template <int kMax, typename F>
 inline void for_tables(const void* const* in, void* const* out, const int64_t* n, const int* dtype, int64_t count,
-                       F&& fn) {
+                       const uint8_t* skip, F&& fn) {
   Table<kMax> t;
   t.count = 0;
   int64_t chunks = 0;
   for (int64_t i = 0; i <= count; ++i) {
-    const int64_t c = i < count ? chunks_of(n[i]) : 0;
+    const int64_t c = i < count && !(skip && skip[i]) ? chunks_of(n[i]) : 0;
     if (t.count > 0 && (i == count || t.count == kMax)) {
       t.first[t.count] = (int)chunks;
       fn(t, (int)chunks);
@@ -200,14 +317,14 @@ inline void for_tables(const void* const* in, void* const* out, const int64_t* n
 
 template <int kMax>
 inline void launch(const void* const* grads, void* const* outs, const int64_t* sizes, const int* dtypes, int64_t count,
-                   float max_norm, double* part, float* norm, cudaStream_t stream) {
+                   const uint8_t* repeated, float max_norm, double* part, float* norm, cudaStream_t stream) {
   int parts = 0;
-  for_tables<kMax>(grads, outs, sizes, dtypes, count, [&](const Table<kMax>& t, int chunks) {
+  for_tables<kMax>(grads, outs, sizes, dtypes, count, nullptr, [&](const Table<kMax>& t, int chunks) {
     const int grid = chunks < kBlocks ? chunks : kBlocks;
     square_kernel<kMax><<<grid, kThreads, 0, stream>>>(t, chunks, part + parts);
     parts += grid;
   });
-  for_tables<kMax>(grads, outs, sizes, dtypes, count, [&](const Table<kMax>& t, int chunks) {
+  for_tables<kMax>(grads, outs, sizes, dtypes, count, repeated, [&](const Table<kMax>& t, int chunks) {
     const int grid = chunks < kBlocks ? chunks : kBlocks;
     scale_kernel<kMax><<<grid, kThreads, 0, stream>>>(t, chunks, part, parts, max_norm, norm);
   });
@@ -244,8 +361,21 @@ prism_status_t prism_clip_grad_norm(const void* const* grads, void* const* outs,
     PRISM_CHECK_CUDA(cudaMemsetAsync(norm, 0, sizeof(float), stream), "prism_clip_grad_norm");
     return PRISM_OK;
   }
+  std::vector<uint8_t> repeated;
+  int64_t shared = -1;
+  try {
+    shared = clip::check_overlap({grads, outs, sizes, dtypes, count, isinf(max_norm) != 0}, repeated);
+  } catch (const std::bad_alloc&) {
+    set_error("prism_clip_grad_norm: out of host memory");
+    return PRISM_ERR_UNSUPPORTED;
+  }
+  PRISM_CHECK_ARG(shared < 0,
+                  "prism_clip_grad_norm: tensor %lld overlaps memory that the call writes (only a whole gradient may "
+                  "be its own output, and be given again)",
+                  (long long)shared);
   const auto launch = count <= clip::kSmallTable ? clip::launch<clip::kSmallTable> : clip::launch<clip::kTable>;
-  launch(grads, outs, sizes, dtypes, count, max_norm, (double*)workspace, norm, stream);
+  launch(grads, outs, sizes, dtypes, count, repeated.empty() ? nullptr : repeated.data(), max_norm, (double*)workspace,
+         norm, stream);
   PRISM_CHECK_LAUNCH("prism_clip_grad_norm");
   return PRISM_OK;
 }

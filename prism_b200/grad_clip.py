@@ -36,7 +36,9 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *,
     """norm = sqrt(sum of the squares of every element of every gradient) -> 0-dim fp32 tensor on
     the gradients' device; the gradients become g * min(1, max_norm / (norm + 1e-6)), in place or
     in ``out``: for each gradient a tensor of its type and number of elements (its own shape, or
-    its slice of a flat buffer, filled in row-major order) that overlaps none of them.  bf16,
+    its slice of a flat buffer, filled in row-major order) that overlaps none of them and no other
+    output.  A gradient that is given again in place (one tensor as the gradient of two inputs)
+    counts each time and is scaled once; other overlaps of what is written are refused.  bf16,
     fp16 and fp32 gradients may be mixed.  A norm that is not a number makes every gradient NaN;
     max_norm = inf only measures the norm."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
