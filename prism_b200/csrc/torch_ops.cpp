@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <optional>
 #include <string>
 #include <vector>
@@ -411,6 +412,10 @@ Optional clip_grad_norm(const std::vector<Tensor>& grads, const std::vector<Tens
   check(prism_clip_grad_norm(from.data(), to.data(), sizes.data(), codes.data(), (int64_t)n, (float)max_norm,
                              at(workspace), (float*)at(norm), launch.stream),
         "prism_clip_grad_norm");
+  // autograd sees that its saved tensors changed; an infinite max_norm writes nothing in place
+  const bool measure = std::isinf((float)max_norm);
+  for (size_t i = 0; i < n; ++i)
+    if (!outs[i].is_inference() && !(measure && from[i] == to[i])) outs[i].unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 

@@ -1,6 +1,7 @@
 """Global gradient norm over many tensors, and clipping, without a host synchronisation."""
 from __future__ import annotations
 
+import math
 from typing import Optional, Sequence
 
 import torch
@@ -61,7 +62,8 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, *,
             pair = _flat_order(g, o)
             if pair is None:  # gaps in memory, or two orders: through a contiguous copy
                 pair = (g.clone(memory_format=torch.contiguous_format),) * 2
-                copies.append((o, pair[1]))
+                if out is not None or max_norm != math.inf:
+                    copies.append((o, pair[1]))
             src.append(pair[0])
             dst.append(pair[1])
         norm = _lib.torch_ops().clip_grad_norm(src, dst, max_norm)
