@@ -543,7 +543,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
       commit_pair(bar(S::kDrain));
     }
-    if (lane == 0) settle(bar(S::kDrain), 0);  // both CTAs: the even one's commits are done, here too
   } else {
     const Epilogue out(sm + S::kTurnAt + warp * kTurnBytes, M, N, xs, ws, bias, c, ldc);
     const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
@@ -562,6 +561,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  // both CTAs: the even one's commits are done, here too.  Not before the CTA's own work is: the wait's
+  // 50 ms would start with the kernel, and a long call would leave with an arrival on its way.
+  if (warp == 5 && lane == 0) settle(bar(S::kDrain), 0);
+  __syncwarp();
   cluster_sync();  // neither CTA frees its TMEM or leaves while the other may still reach it
   if (warp == 5) {
     tc_fence_after();
