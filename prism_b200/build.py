@@ -8,6 +8,8 @@ default contraction.
 """
 from __future__ import annotations
 
+import contextlib
+import fcntl
 import os
 import re
 import shutil
@@ -44,7 +46,35 @@ def torch_ops_lib() -> str:
     return os.path.join(HERE, f"prism_torch_ops_{re.sub('[^0-9A-Za-z.]', '-', tag)}.so")
 
 
+@contextlib.contextmanager
+def _one_builder():
+    """One process (and thread) of this machine builds at a time; the others find its files."""
+    os.makedirs(BUILD, exist_ok=True)
+    with open(os.path.join(BUILD, ".lock"), "w") as f:
+        fcntl.flock(f, fcntl.LOCK_EX)
+        yield
+
+
+def _run(cmd, target: str, verbose: bool) -> None:
+    """Runs a compiler whose output goes to ``target``, which appears there whole or not at all."""
+    tmp = f"{target}.{os.getpid()}.tmp"
+    cmd = cmd + ["-o", tmp]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    try:
+        subprocess.run(cmd, check=True)
+        os.replace(tmp, target)
+    finally:
+        if os.path.exists(tmp):
+            os.remove(tmp)
+
+
 def build_torch_ops(verbose: bool = False, force: bool = False) -> str:
+    with _one_builder():
+        return _build_torch_ops(verbose, force)
+
+
+def _build_torch_ops(verbose: bool, force: bool) -> str:
     import torch
     src, target = os.path.join(CSRC, "torch_ops.cpp"), torch_ops_lib()
     if force or _stale(target, [src, os.path.join(ROOT, "include", "prism_bsa.h")]):
@@ -55,12 +85,10 @@ def build_torch_ops(verbose: bool = False, force: bool = False) -> str:
                     sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
         cmd = [shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-shared",
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
-        cmd += [f"-I{d}" for d in includes] + [src, "-o", target, "-L" + os.path.join(base, "lib"), "-L" + HERE]
+        cmd += [f"-I{d}" for d in includes] + [src, "-L" + os.path.join(base, "lib"), "-L" + HERE]
         # libprism_bsa.so is the one next to the extension; torch's libraries are loaded already
         cmd += ["-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-lprism_bsa", "-Wl,-rpath,$ORIGIN"]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+        _run(cmd, target, verbose)
     return target
 
 
@@ -79,7 +107,11 @@ def _stale(target: str, deps) -> bool:
 
 
 def build(verbose: bool = False, force: bool = False) -> str:
-    os.makedirs(BUILD, exist_ok=True)
+    with _one_builder():
+        return _build(verbose, force)
+
+
+def _build(verbose: bool, force: bool) -> str:
     headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
     headers.append(os.path.join(ROOT, "include", "prism_bsa.h"))
     objs = []
@@ -88,16 +120,10 @@ def build(verbose: bool = False, force: bool = False) -> str:
         o = os.path.join(BUILD, src.replace(".cu", ".o"))
         objs.append(o)
         if force or _stale(o, [s] + headers):
-            cmd = [nvcc()] + ARCH + COMMON + flags + ["-c", s, "-o", o]
-            if verbose:
-                print(" ".join(cmd), flush=True)
-            subprocess.run(cmd, check=True)
+            _run([nvcc()] + ARCH + COMMON + flags + ["-c", s], o, verbose)
     if force or _stale(LIB, objs):
-        cmd = [nvcc()] + ARCH + ["-shared", "-o", LIB] + objs
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
-    build_torch_ops(verbose=verbose, force=force)
+        _run([nvcc()] + ARCH + ["-shared"] + objs, LIB, verbose)
+    _build_torch_ops(verbose, force)
     return LIB
 
 
