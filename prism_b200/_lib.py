@@ -154,12 +154,16 @@ _torch_ops = None
 def torch_ops():
     """The extension module of csrc/torch_ops.cpp (built if it is absent)."""
     global _torch_ops
-    if _torch_ops is None:
-        import importlib.machinery
-        import importlib.util
+    if _torch_ops is not None:
+        return _torch_ops
+    import importlib.machinery
+    import importlib.util
 
-        import torch  # noqa: F401  (its libraries are what the extension links to)
-        load()
+    import torch  # noqa: F401  (its libraries are what the extension links to)
+    load()
+    with _lock:
+        if _torch_ops is not None:
+            return _torch_ops
         path = _build.torch_ops_lib()
         if not os.path.exists(path):
             _build.build_torch_ops()
@@ -168,7 +172,7 @@ def torch_ops():
         loader.exec_module(module)
         module.set_error(PrismError)
         _torch_ops = module
-    return _torch_ops
+        return module
 
 
 def query(name: str, *args) -> int:
