@@ -48,7 +48,8 @@ typedef enum { PRISM_BF16 = 0, PRISM_FP16 = 1, PRISM_FP32 = 2 } prism_dtype_t;
 
 /* Thread-local text of the last error raised on this host thread. */
 const char* prism_last_error(void);
-/* ABI version (incremented on any signature change). */
+/* ABI version (incremented on any signature change): of the header, and of the library. */
+#define PRISM_ABI_VERSION 5
 int prism_abi_version(void);
 /* Device-side status of the attention kernels: 0 when every bounded wait
  * inside them completed, otherwise the code of the first wait that gave up

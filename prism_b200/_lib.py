@@ -160,7 +160,7 @@ def torch_ops():
     import importlib.util
 
     import torch  # noqa: F401  (its libraries are what the extension links to)
-    load()
+    L = load()
     with _lock:
         if _torch_ops is not None:
             return _torch_ops
@@ -170,6 +170,10 @@ def torch_ops():
         loader = importlib.machinery.ExtensionFileLoader("prism_torch_ops", path)
         module = importlib.util.module_from_spec(importlib.util.spec_from_loader("prism_torch_ops", loader))
         loader.exec_module(module)
+        built, found = getattr(module, "abi_version", None), L.prism_abi_version()
+        if built != found:
+            raise PrismError(f"{path} was built for ABI version {built}, {lib_path()} has {found}; "
+                             "run `python -m prism_b200.build`")
         module.set_error(PrismError)
         _torch_ops = module
         return module

@@ -423,6 +423,7 @@ Optional clip_grad_norm(const std::vector<Tensor>& grads, const std::vector<Tens
 
 PYBIND11_MODULE(prism_torch_ops, m) {
   static PyObject* prism_error = nullptr;  // prism_b200._lib.PrismError
+  m.attr("abi_version") = PRISM_ABI_VERSION;
   m.def("set_error", [](py::object type) { prism_error = type.inc_ref().ptr(); });
   py::register_exception_translator([](std::exception_ptr p) {
     try {
