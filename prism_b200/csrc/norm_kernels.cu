@@ -508,7 +508,10 @@ __global__ void __launch_bounds__(1024)
 }
 
 // ------------------------------------------- rows of any width, alignment and stride
-// One CTA per row, element by element.
+// One CTA per row, element by element: rows of more than 16,384 columns, and rows whose tensors start
+// differently in 16 bytes.  The row is read again for its outputs, by the backward's weight gradient a third time.  4,000
+// rows of 16,392 bf16 columns: forward 131 us, 8-bit rows 125, backward 382 in three kernels; of
+// 16,384 columns in the kernels above 86, 79 and 99.
 template <typename T, bool kQuant>
 __global__ void __launch_bounds__(kThreads)
     fwd_any_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ r, int64_t ldr,
@@ -623,13 +626,14 @@ constexpr int kMaxPerSm = 16, kMaxParts = kMaxPerSm * kSms + 8;  // CTAs of a pe
 // A thread takes 8 elements of a row, or 16 where 8 would need more than `wide` threads: fewer
 // warps to a barrier and more CTAs to an SM, against more rows on their way and fewer idle lanes in
 // narrow rows.  Measured at 1,024 / 2,048 / 4,096 columns (us, 8 against 16 a thread):
-//   bf16, 120 M elements: forward 164 / 161 / 167 against 156 / 145 / 164,
-//     8-bit 151 / 147 / 140 against 145 / 140 / 127, backward 146 / 147 / 148 against 148 / 147 / 153
-//   fp32, 60 M elements: forward 156 / 160 / 161 against 149 / 150 / 159,
-//     8-bit 128 / 127 / 122 against 119 / 120 / 120, backward 155 / 155 / 143 against 141 / 140 / 144
-// and at 768 columns (8 M bf16 elements) forward 10.0 against 12.5, 8-bit 11.0 against 12.9; bf16
-// backward at 5,120: 173 against 149.  Hence 96, for the bf16 backward 512.  A row of up to 32
-// threads' elements, 8 each, goes to a power-of-two group of lanes.
+//   bf16, 120 M elements: forward 165 / 157 / 165 against 147 / 148 / 146,
+//     8-bit 141 / 135 / 130 against 132 / 129 / 128, backward 145 / 146 / 149 against 150 / 147 / 153
+//   fp32, 60 M elements: forward 156 / 158 / 163 against 150 / 151 / 158,
+//     8-bit 130 / 127 / 118 against 117 / 118 / 117, backward 155 / 153 / 143 against 141 / 139 / 144
+// and at 768 columns (8 M bf16 elements) forward 11.6 against 13.7, 8-bit 12.4 against 13.6; bf16
+// backward at 5,120: 173 against 149.  Hence 96, for the bf16 backward 512.  It is not best everywhere: at
+// 5,120 columns 8 a thread takes 146 us against 153 in the bf16 forward, 142 against 154 in the fp32 backward.
+// A row of up to 32 threads' elements, 8 each, goes to a power-of-two group of lanes.
 template <size_t kSize>
 Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int loaded, int wide) {
   constexpr int kWidth = 16 / (int)kSize;
@@ -678,10 +682,10 @@ Plan plan_rows(const Operand* tensors, int count, int64_t rows, int cols, int lo
 // The persistent grid: as many CTAs an SM as keep `budget` bytes of rows on their way, and two
 // (one computes while the other waits at its barrier) if that is at most 80 KB.  More bytes are
 // worse where the kernel also writes much: 120 M bf16 elements in 2,048 columns forward (half of
-// the traffic writes) took 145 us with 48 KB an SM and 168 us with 96 KB; 8-bit rows in 4,096
-// columns 127 us with 64 KB and 149 us with 96 KB; the backward (a quarter writes) wants all that
+// the traffic writes) took 148 us with 48 KB an SM and 174 us with 96 KB; 8-bit rows in 4,096
+// columns 128 us with 64 KB and 148 us with 96 KB; the backward (a quarter writes) wants all that
 // fit.  So the forward has one row of a group on its way where a second one would leave the budget
-// to a single CTA: 5,120 columns 152 against 168 us, 8-bit rows 128 against 145 us.
+// to a single CTA: 5,120 columns 153 against 173 us, 8-bit rows 130 against 135 us.
 void size_grid(Plan& p, int64_t rows, int budget, int regs, bool forward) {
   if (p.shift) budget = 180 << 10;  // their single elements are loaded a row ahead only
   if (forward && p.cta && p.depth == 2 && (int)p.ring < budget && 2 * (int)p.ring > budget) {
