@@ -49,7 +49,7 @@ typedef enum { PRISM_BF16 = 0, PRISM_FP16 = 1, PRISM_FP32 = 2 } prism_dtype_t;
 /* Thread-local text of the last error raised on this host thread. */
 const char* prism_last_error(void);
 /* ABI version (incremented on any signature change): of the header, and of the library. */
-#define PRISM_ABI_VERSION 5
+#define PRISM_ABI_VERSION 6
 int prism_abi_version(void);
 /* Device-side status of the attention kernels: 0 when every bounded wait
  * inside them completed, otherwise the code of the first wait that gave up
@@ -560,6 +560,36 @@ prism_status_t prism_clip_grad_norm(const void* const* grads, void* const* outs,
 prism_status_t prism_linear_fp8(const void* x8, int64_t ldx, const float* x_scale, const void* w8,
                                 int64_t ldw, const float* w_scale, const float* bias, int M, int N,
                                 int K, void* c, int64_t ldc, cudaStream_t stream);
+
+/* Dense attention over packed sequences: q [q_rows, q_heads, D], k and v [k_rows, k_heads, D] (D = 64 or
+ * 128; bf16 or fp16; q_heads / k_heads <= 128 query heads share a key head); sequence b < count is the rows
+ * [q_offsets[b], q_offsets[b + 1]) and [k_offsets[b], k_offsets[b + 1]) (device arrays of count + 1 int32, or
+ * int64 with offsets_64; non-decreasing, within the rows: else every output is NaN).  Of a sequence's n
+ * queries and m keys, query i attends all keys, or with causal != 0 the keys j <= i + m - n:
+ *   o_i = sum_j p_ij v_j,  p_ij = softmax_j(scale q_i . k_j), scale > 0;  o_i = 0 without a key.
+ * o [q_rows, q_heads, D] contiguous, 0 in rows that no sequence holds.  Strides {row, head} in elements, whole
+ * 16 bytes; columns contiguous.  A NaN or an infinity in one sequence reaches no other.  lse (NULL: not
+ * wanted): what the backward reads, of prism_packed_attention_stats_bytes.  Sums and statistics fp32.
+ *
+ * prism_packed_attention_bwd (bf16): dout = dL/do -> dq, dk, dv in the layouts of o and of contiguous k, v, each
+ * sum in a fixed order; dq or the pair dk, dv may be NULL (not wanted).  o and lse are the forward's;
+ * workspace: prism_packed_attention_stats_bytes.  No rows on either side is refused: the gradients are zero.
+ * Bounded waits report through prism_device_status (501-523). */
+size_t prism_packed_attention_stats_bytes(int64_t q_rows, int64_t count, int q_heads, int k_heads);
+prism_status_t prism_packed_attention(const void* q, const int64_t* q_strides, const void* k,
+                                      const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                      const void* q_offsets, const void* k_offsets, int offsets_64,
+                                      int64_t count, int64_t q_rows, int64_t k_rows, int q_heads,
+                                      int k_heads, int D, int causal, float scale, int dtype, void* o,
+                                      float* lse, cudaStream_t stream);
+prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
+                                          const int64_t* k_strides, const void* v,
+                                          const int64_t* v_strides, const void* o, const void* dout,
+                                          const int64_t* dout_strides, const float* lse,
+                                          const void* q_offsets, const void* k_offsets, int offsets_64,
+                                          int64_t count, int64_t q_rows, int64_t k_rows, int q_heads,
+                                          int k_heads, int D, int causal, float scale, void* workspace,
+                                          void* dq, void* dk, void* dv, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -43,6 +43,7 @@ from .grad_clip import clip_grad_norm  # noqa: F401
 from .linear import linear_fp8  # noqa: F401
 from .norm import add_rms_norm, add_rms_norm_fp8, quantize_rows_fp8  # noqa: F401
 from .ops import token_norms  # noqa: F401
+from .packed import packed_attention  # noqa: F401
 from .rotary import apply_rotary, rotary_frequencies  # noqa: F401
 
 __version__ = "0.1.0"

@@ -36,6 +36,7 @@ SOURCES = {
     "norm_kernels.cu": [],
     "rotary_kernels.cu": [],
     "clip_kernels.cu": [],
+    "packed_attention.cu": [],
 }
 
 

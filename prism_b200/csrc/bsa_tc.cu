@@ -45,6 +45,7 @@
 #include <mutex>
 
 #include "prism_common.cuh"
+#include "attention_tc.cuh"
 #include "sm100.cuh"
 
 namespace prism {
@@ -110,10 +111,6 @@ __device__ __forceinline__ int union_count(const uint32_t* ra, const uint32_t* r
   return c;
 }
 
-__device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
-  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
-}
-
 // Warp-uniform bounded wait (every lane must agree before a .sync.aligned op).
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
                                           int code) {
@@ -121,22 +118,6 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   ok = __all_sync(0xffffffffu, ok);
   if (!ok) *abort_flag = 1;
   return ok;
-}
-
-__device__ __forceinline__ float u2f(uint32_t x) { return __uint_as_float(x); }
-
-// 32 * N consecutive TMEM columns of this warp's 32 lanes -> registers (waited).
-template <int N>
-__device__ __forceinline__ void tmem_load(uint32_t taddr, float (&out)[32 * N]) {
-  uint32_t raw[N][32];
-#pragma unroll
-  for (int c = 0; c < N; ++c) tmem_ld32(taddr + c * 32, raw[c]);
-#pragma unroll
-  for (int c = 0; c < N; ++c) tmem_wait_ld_dep(raw[c]);
-#pragma unroll
-  for (int c = 0; c < N; ++c)
-#pragma unroll
-    for (int i = 0; i < 32; ++i) out[c * 32 + i] = u2f(raw[c][i]);
 }
 
 // Request at least this much dynamic shared memory so that a second CTA never
@@ -371,18 +352,6 @@ __device__ __forceinline__ void mask_keys(float (&s)[64], uint64_t vb) {
     if (!((vb >> c) & 1ull)) s[c] = -INFINITY;
 }
 
-__device__ __forceinline__ float tile_max(const float (&s)[64]) {
-  float m0 = s[0], m1 = s[1], m2 = s[2], m3 = s[3];
-#pragma unroll
-  for (int c = 4; c < 64; c += 4) {
-    m0 = fmaxf(m0, s[c]);
-    m1 = fmaxf(m1, s[c + 1]);
-    m2 = fmaxf(m2, s[c + 2]);
-    m3 = fmaxf(m3, s[c + 3]);
-  }
-  return fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-}
-
 // p = exp2(s * scale - m) for 64 scores as 32 bf16 pairs; returns the sum of the
 // fp32 p (even and odd columns summed separately, then added).  The exponent
 // arguments are packed f32x2 FFMAs (each lane rounds as fmaf does); the sums
@@ -409,20 +378,6 @@ __device__ __forceinline__ void exp_rows(float (&s)[64], float scale, float bias
     const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), sc, b);
     s[c] = ex2(x.x);
     s[c + 1] = ex2(x.y);
-  }
-}
-
-// Rows of this warp's TMEM lanes, columns [0, 32 * NC) of taddr, times alpha.
-template <int NC>
-__device__ __forceinline__ void scale_tmem_rows(uint32_t taddr, float alpha) {
-#pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    uint32_t raw[32];
-    tmem_ld32(taddr + c * 32, raw);
-    tmem_wait_ld_dep(raw);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) raw[i] = __float_as_uint(u2f(raw[i]) * alpha);
-    tmem_st32(taddr + c * 32, raw);
   }
 }
 
@@ -841,27 +796,6 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
 // and TMA fills need.  The bf16 pairs go back with 16x128b stores, whose
 // layout puts packed column 4 j + lane % 4 of lanes a, a + 8 in the registers
 // that hold them.
-__device__ __forceinline__ void tmem_ld_16x256b_x8(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,"
-      "%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-        "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-        "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st_16x128b_x8(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-      "r"(r[15])
-      : "memory");
-}
-
 // Key validity of this thread's four lanes: bit 2 hl + kk <=> key lane
 // 32 q + 16 hl + 8 kk + lane / 4 of the CTA is valid (q = lane quarter of the warp).
 __device__ __forceinline__ uint32_t dkdv_lane_valid(uint64_t tile_valid_bits, int quarter, int lane) {
@@ -1692,6 +1626,7 @@ using namespace prism;
 
 int prism_gemm_device_status_internal(void);
 int prism_gemm8_device_status_internal(void);
+int prism_packed_device_status_internal(void);
 
 extern "C" {
 
@@ -1704,8 +1639,9 @@ int prism_device_status(void) {
   }
   const int g = prism_gemm_device_status_internal();  // the GEMM kernels' word (gemm_tc.cu)
   const int g8 = prism_gemm8_device_status_internal();  // and gemm_fp8.cu's
-  if (g < 0 || g8 < 0) return -1;
-  return v != 0 ? v : g != 0 ? g : g8;
+  const int p = prism_packed_device_status_internal();  // and packed_attention.cu's
+  if (g < 0 || g8 < 0 || p < 0) return -1;
+  return v != 0 ? v : g != 0 ? g : g8 != 0 ? g8 : p;
 }
 
 // Row indices of the [heads * S, D] views are 32-bit TMA coordinates.

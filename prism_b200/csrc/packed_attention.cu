@@ -1,0 +1,1493 @@
+// Dense attention over packed sequences, forward and backward, on the sm_100a tensor cores.
+//
+// q [T, Hq, D], k and v [Tk, Hk, D]: sequence b is the rows [offsets[b], offsets[b + 1]) of its
+// tensors; G = Hq / Hk query heads share a key head.  With n queries and m keys of a sequence, query i
+// attends keys j < m, or, causal, j <= i + m - n (the last query is at the last key):
+//
+//   s_ij = scale q_i . k_j,   p_ij = exp(s_ij - max_j s_ij) / sum_j exp(..),   o_i = sum_j p_ij v_j
+//   delta_i = do_i . o_i,   ds_ij = p_ij (do_i . v_j - delta_i),
+//   dq_i = scale sum_j ds_ij k_j,   dk_j = scale sum_i ds_ij q_i,   dv_j = sum_i p_ij do_i,
+//
+// dk and dv over the queries of all G heads.  A row without keys has o = 0 and no gradients.
+//
+// Bound by the tensor cores (4 D operations a score forward, 10 D backward).  What the kernels share:
+//   * A tile of 128 rows holds all G heads of n = 128 / G tokens, row (token, head): one TMA box
+//     {64 columns, G heads, n tokens}.  Heads that share keys share their loads, a sequence of few
+//     tokens fills more of a tile than one head's rows would, and the diagonal of a causal tile is n
+//     keys wide instead of 128.  A G that does not divide 128 leaves 128 - n G rows zero.
+//   * A step is 128 keys (queries in dK / dV): an M = 128 product costs at least 45 clocks, so
+//     N = 128 is needed for the math rate.
+//   * Tiles end inside sequences, so a tile's last rows are the next sequence's (or lie behind the
+//     tensor: TMA reads zeros there).  Scores of such keys are replaced, not multiplied, and rows that
+//     a product sums over (V; K in dQ; Q and dO in dK / dV) are set to zero in shared memory first:
+//     a NaN in one sequence stays there, 0 * NaN being NaN.
+//   * Scores in log2 units; fp32 statistics and accumulators; P and dS rounded to the inputs' 16 bits
+//     for the second products, as the matrix instruction takes them.
+//   * A CTA finds its sequence by itself, with a scan of the offsets (no host copy of the lengths, no
+//     plan kernel); a grid has the upper bound of tiles that the row counts allow, and its spare CTAs
+//     clear the rows that no sequence holds.  Offsets that decrease or leave the tensors give NaN.
+//
+// Warp roles (320 threads): warps 0-7 softmax and epilogue (thread i of a warpgroup owns TMEM lane i),
+// warp 8 TMA producer, warp 9 MMA issuer (lane 0 issues; all lanes clear tail rows) and TMEM owner.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <cudaTypedefs.h>
+#include <stdint.h>
+
+#include <mutex>
+#include <type_traits>
+
+#include "attention_tc.cuh"
+#include "prism_common.cuh"
+#include "sm100.cuh"
+
+namespace prism {
+namespace packed {
+
+using namespace tc;
+
+constexpr int kThreads = 320;
+constexpr int kProducerWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr int kRows = 128;                // of a tile; keys of a step
+constexpr size_t kMinSmem = 116 * 1024;   // one CTA an SM: each allocates all of TMEM
+constexpr float kLog2e = 1.4426950408889634f;
+
+// First bounded wait that gave up (prism_device_status).
+__device__ int g_error = 0;
+enum WaitCode : int {
+  kErrFwdProducer = 501, kErrFwdMma = 502, kErrFwdSoftmax = 503,
+  kErrDkdvProducer = 511, kErrDkdvMma = 512, kErrDkdvSoftmax = 513,
+  kErrDqProducer = 521, kErrDqMma = 522, kErrDqSoftmax = 523,
+};
+
+__device__ __forceinline__ bool wait_one(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+  return mbar_wait(bar, parity, abort_flag, &g_error, code);
+}
+// Warp-uniform result (every lane must agree before a .sync.aligned operation).
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int code) {
+  const bool ok = __all_sync(0xffffffffu, wait_one(bar, parity, abort_flag, code));
+  if (!ok) *abort_flag = 1;
+  return ok;
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+// ------------------------------------------------------------------ element types
+// kShift: log2 of the largest p that a fresh maximum gives.  fp16 keeps p >= 2^-24 only, so its maximum is
+// put at 2^10 and keys down to 2^-34 of the largest count; kLag more (2^15 in all, below fp16's 65504)
+// until the maximum is raised.  kSum: a half tile's exponentials below it all are within that.
+template <typename T>
+struct Half;
+template <>
+struct Half<__nv_bfloat16> {
+  static constexpr float kShift = 0.0f, kLag = 8.0f, kSum = 65536.0f;
+  static constexpr uint32_t kFormat = 1;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16(lo, hi); }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
+};
+template <>
+struct Half<__half> {
+  static constexpr float kShift = 10.0f, kLag = 5.0f, kSum = 32768.0f;
+  static constexpr uint32_t kFormat = 0;
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
+  }
+};
+// Instruction descriptor as idesc_bf16's, both operands of type T.
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc(int N, bool b_mn) {
+  return (1u << 4) | (Half<T>::kFormat << 7) | (Half<T>::kFormat << 10) | ((b_mn ? 1u : 0u) << 16) |
+         ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+
+// ------------------------------------------------------------------ sequences
+struct Sequences {
+  const void *q, *k;       // offsets, count + 1 of them
+  int wide;                // 64-bit
+  int count;
+  int q_rows, k_rows;      // of the tensors
+};
+// Heads and the tiles that they give: n = tokens of a tile; pairs = upper bound of the pairs of tiles.
+struct Heads {
+  int keys, group, tokens, pairs;
+};
+
+enum Kind : int { kTile, kSpare, kBad };
+struct Place {
+  int kind;
+  int q0, nq, k0, nk;   // the sequence's rows
+  int tile;             // within the sequence; kSpare: number among the spare ones
+  int pairs;            // pairs of query tiles of the sequences before
+};
+
+__device__ __forceinline__ int64_t row_at(const void* offsets, int wide, int i) {
+  return wide ? static_cast<const long long*>(offsets)[i] : (int64_t)static_cast<const int*>(offsets)[i];
+}
+
+// Tile `my` of the grid (kKeys: of `per` keys, else of `per` queries) -> *place.  All threads of the CTA;
+// scratch: 2 ints a warp.  One round for up to blockDim sequences.
+template <bool kKeys>
+__device__ void find_place(const Sequences& s, int my, int per, int pair_tokens, Place* place, int* scratch) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  int base = 0, pairs_base = 0;
+  bool good = true;
+  if (tid == 0) place->kind = kSpare;
+  for (int b0 = 0; b0 < s.count; b0 += blockDim.x) {
+    const int b = b0 + tid;
+    int q0 = 0, nq = 0, k0 = 0, nk = 0;
+    bool fine = true;
+    if (b < s.count) {
+      const int64_t qa = row_at(s.q, s.wide, b), qb = row_at(s.q, s.wide, b + 1);
+      const int64_t ka = row_at(s.k, s.wide, b), kb = row_at(s.k, s.wide, b + 1);
+      fine = 0 <= qa && qa <= qb && qb <= s.q_rows && 0 <= ka && ka <= kb && kb <= s.k_rows;
+      if (fine) q0 = (int)qa, nq = (int)(qb - qa), k0 = (int)ka, nk = (int)(kb - ka);
+    }
+    const int pairs = (nq + pair_tokens - 1) / pair_tokens;
+    const int tiles = kKeys ? (nk + per - 1) / per : pairs;
+    int x = tiles, y = pairs;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {  // inclusive scans of the warp
+      const int xo = __shfl_up_sync(0xffffffffu, x, o), yo = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) x += xo, y += yo;
+    }
+    if (lane == 31) scratch[2 * warp] = x, scratch[2 * warp + 1] = y;
+    good = __syncthreads_and(fine) && good;
+    int before = base, pairs_before = pairs_base;
+    for (int w = 0; w < warps; ++w) {
+      if (w < warp) before += scratch[2 * w], pairs_before += scratch[2 * w + 1];
+      base += scratch[2 * w], pairs_base += scratch[2 * w + 1];
+    }
+    before += x - tiles, pairs_before += y - pairs;
+    if (my >= before && my < before + tiles) *place = {kTile, q0, nq, k0, nk, my - before, pairs_before};
+    __syncthreads();
+  }
+  if (tid == 0) {
+    if (!good) place->kind = kBad;
+    else if (my >= base) place->kind = kSpare, place->tile = my - base;
+  }
+  __syncthreads();
+}
+
+// A CTA without a tile: clears its share of the rows that no sequence holds (kSpare), or fills its share of
+// all rows with NaN (kBad).  Rows of `out` are [heads, width] elements; the CTA has those of key head h:
+// `width` elements from h * width on.
+template <typename T>
+__device__ void fill_rows(const Place& place, const void* offsets, const Sequences& s, int rows, int my, int per,
+                          T* out, int heads, int h, int width) {
+  const bool bad = place.kind == kBad;
+  const int head = bad ? 0 : (int)row_at(offsets, s.wide, 0), tail = bad ? 0 : (int)row_at(offsets, s.wide, s.count);
+  const int count = bad ? rows : head + rows - tail;
+  const int64_t first = (int64_t)(bad ? my : place.tile) * per;
+  const int64_t end = first + per < count ? first + per : count;
+  const uint32_t word = bad ? Half<T>::pack(__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u)) : 0u;
+  const int chunks = width / 8;
+  for (int64_t i = first * chunks + threadIdx.x; i < end * chunks; i += blockDim.x) {
+    const int64_t u = i / chunks;
+    const int64_t row = u < head ? u : tail + (u - head);
+    *reinterpret_cast<uint4*>(out + (row * heads + h) * width + (i - u * chunks) * 8) = make_uint4(word, word, word, word);
+  }
+}
+
+// Rows [from, 128) of a tile's sub-buffers set to zero, by a group of threads; the caller fences and
+// synchronises before the tensor core reads them.
+template <int kSub>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int from, int thread, int threads) {
+  const int chunks = (kRows - from) * 8;
+#pragma unroll
+  for (int s = 0; s < kSub; ++s)
+    for (int i = thread; i < chunks; i += threads)
+      *reinterpret_cast<uint4*>(tile + s * 16384 + from * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// r / group for r < 128 and group <= 128: (r * ceil(2^16 / group)) >> 16 is exact, the excess being
+// below r / 2^16 < 1 / group.
+__device__ __forceinline__ int over_group(int r, uint32_t inverse) { return (int)((uint32_t)r * inverse >> 16); }
+__device__ __forceinline__ uint32_t group_inverse(int group) { return (65536u + group - 1) / group; }
+
+// Columns from `lim` on -> -inf.
+__device__ __forceinline__ void mask_from(float (&s)[64], int lim) {
+#pragma unroll
+  for (int c = 0; c < 64; ++c)
+    if (c >= lim) s[c] = -INFINITY;
+}
+
+// p = exp2(s * scale - m) of 64 scores as 32 pairs of T; returns their fp32 sum.
+template <typename T>
+__device__ __forceinline__ float exp_pairs(const float (&s)[64], float scale, float m, uint32_t (&pk)[32]) {
+  const float2 sc = make_float2(scale, scale), nm = make_float2(-m, -m);
+  float su0 = 0.f, su1 = 0.f;
+#pragma unroll
+  for (int c = 0; c < 32; ++c) {
+    const float2 x = __ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sc, nm);
+    const float p0 = ex2(x.x), p1 = ex2(x.y);
+    su0 += p0;
+    su1 += p1;
+    pk[c] = Half<T>::pack(p0, p1);
+  }
+  return su0 + su1;
+}
+
+// ===================================================================== forward
+// CTA: two tiles of 128 rows (groups 0 and 1) of one key head, which share the stream of K and V steps, so
+// that the tensor core works on one group's products while the other group's softmax runs.
+template <int D>
+struct FwdLayout {
+  static constexpr int kRing = 2;
+  static constexpr int kSub = D / 64;
+  static constexpr int kTileBytes = kSub * 16384;
+  static constexpr int Q = 0;
+  static constexpr int K = Q + 2 * kTileBytes;
+  static constexpr int V = K + kRing * kTileBytes;
+  static constexpr int BAR = V + kRing * kTileBytes;
+  static constexpr int B_Q = 0, B_KF = 1, B_KE = B_KF + kRing, B_VF = B_KE + kRing, B_VE = B_VF + kRing,
+                       B_SF = B_VE + kRing,  // [g]: S of the group
+                       B_PF = B_SF + 2,      // [g]: P in TMEM (and O rescaled)
+                       B_OF = B_PF + 2,      // [g]: last P V done
+                       B_DRAIN = B_OF + 2, NBAR = B_DRAIN + 1;
+  static constexpr int TMEM_SLOT = BAR + NBAR * 8;
+  static constexpr int ABORT = TMEM_SLOT + 4;
+  static constexpr int PLACE = ABORT + 4;
+  static constexpr int SCRATCH = PLACE + (int)sizeof(Place);
+  static constexpr size_t kNeed = 1024 + SCRATCH + 2 * 4 * (kThreads / 32);
+  static constexpr size_t kBytes = kNeed > kMinSmem ? kNeed : kMinSmem;
+  // TMEM of group g at 256 g: S (128 fp32 columns; P as pairs over the first 64), O
+  static constexpr int T_S = 0, T_O = 128;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Sequences seqs, Heads hd, int causal,
+               float qk_scale, T* __restrict__ o, float* __restrict__ lse) {
+  using L = FwdLayout<D>;
+  using H = Half<T>;
+  constexpr int R = L::kRing;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = align1024(smem_raw);
+  const uint32_t sb = smem_u32(sm);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // a causal sequence's last tiles have the most keys: they go first
+  const int pair = hd.pairs - 1 - (int)(blockIdx.x / hd.keys), h = blockIdx.x % hd.keys;
+  const int n_tok = hd.tokens, rows = n_tok * hd.group;
+  auto bar = [&](int i) { return sb + L::BAR + 8 * i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::ABORT);
+
+  Place* shared_place = reinterpret_cast<Place*>(sm + L::PLACE);
+  find_place<false>(seqs, pair, 2 * n_tok, 2 * n_tok, shared_place, reinterpret_cast<int*>(sm + L::SCRATCH));
+  const Place at = *shared_place;
+  if (at.kind != kTile) {
+    fill_rows(at, seqs.q, seqs, seqs.q_rows, pair, 2 * n_tok, o, hd.keys, h, hd.group * D);
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar(L::B_Q), 1);
+    for (int i = 0; i < R; ++i) {
+      mbar_init(bar(L::B_KF + i), 1);
+      mbar_init(bar(L::B_KE + i), 1);
+      mbar_init(bar(L::B_VF + i), 1);
+      mbar_init(bar(L::B_VE + i), 1);
+    }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(bar(L::B_SF + g), 1);
+      mbar_init(bar(L::B_PF + g), 4);
+      mbar_init(bar(L::B_OF + g), 1);
+    }
+    mbar_init(bar(L::B_DRAIN), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (rows < kRows) {  // rows that no load fills
+    zero_rows<L::kSub>(sm + L::Q, rows, threadIdx.x, kThreads);
+    zero_rows<L::kSub>(sm + L::Q + L::kTileBytes, rows, threadIdx.x, kThreads);
+    fence_proxy_async_smem();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(sb + L::TMEM_SLOT, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + L::TMEM_SLOT);
+
+  const int tok0 = at.tile * 2 * n_tok, shift = at.nk - at.nq;
+  // keys and steps of each group, up to its last token's
+  int last[2], steps[2];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    last[g] = min(tok0 + (g + 1) * n_tok, at.nq) - 1;
+    const int keys = tok0 + g * n_tok >= at.nq ? 0 : causal ? min(max(last[g] + shift + 1, 0), at.nk) : at.nk;
+    steps[g] = (keys + kRows - 1) / kRows;
+  }
+  const int total = max(steps[0], steps[1]);
+
+  if (warp == kProducerWarp) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0 && total > 0) {
+      const int live = steps[1] > 0 ? 2 : 1;
+      mbar_expect_tx(bar(L::B_Q), live * rows * D * 2);
+      for (int g = 0; g < live; ++g)
+#pragma unroll
+        for (int s = 0; s < L::kSub; ++s)
+          tma_load_3d(sb + L::Q + g * L::kTileBytes + s * 16384, &tm_q, s * 64, h * hd.group,
+                      at.q0 + tok0 + g * n_tok, bar(L::B_Q));
+      int nk = 0, nv = 0;
+      for (int n = 0; n < total; ++n) {
+        const int st = n % R, key = at.k0 + n * kRows;
+        if (n >= R && !wait_one(bar(L::B_KE + st), ((n / R) - 1) & 1, abort_flag, kErrFwdProducer)) break;
+        mbar_expect_tx(bar(L::B_KF + st), L::kTileBytes);
+#pragma unroll
+        for (int s = 0; s < L::kSub; ++s)
+          tma_load_3d(sb + L::K + st * L::kTileBytes + s * 16384, &tm_k, s * 64, h, key, bar(L::B_KF + st));
+        ++nk;
+        if (n >= R && !wait_one(bar(L::B_VE + st), ((n / R) - 1) & 1, abort_flag, kErrFwdProducer)) break;
+        mbar_expect_tx(bar(L::B_VF + st), L::kTileBytes);
+#pragma unroll
+        for (int s = 0; s < L::kSub; ++s)
+          tma_load_3d(sb + L::V + st * L::kTileBytes + s * 16384, &tm_v, s * 64, h, key, bar(L::B_VF + st));
+        ++nv;
+      }
+      // every load has landed before the CTA may leave
+      for (int m = max(nk - R, 0); m < nk; ++m) wait_one(bar(L::B_KF + m % R), (m / R) & 1, abort_flag, kErrFwdProducer);
+      for (int m = max(nv - R, 0); m < nv; ++m) wait_one(bar(L::B_VF + m % R), (m / R) & 1, abort_flag, kErrFwdProducer);
+      wait_one(bar(L::B_Q), 0, abort_flag, kErrFwdProducer);
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------- MMA issuer
+    // Step n, for the groups that take part: P V of the group's step n - 1, then S of step n over the
+    // columns that held that P (one thread's products run in issue order).
+    constexpr uint32_t kIdS = idesc<T>(kRows, false), kIdO = idesc<T>(D, true);
+    const uint64_t dQ = desc_k_sw128(sb + L::Q), dK = desc_k_sw128(sb + L::K), dV = desc_mn_sw128(sb + L::V, 16384);
+    constexpr uint32_t kSlot = L::kTileBytes >> 4;
+    const auto pv = [&](int g, int j) -> bool {
+      if (!wait_warp(bar(L::B_PF + g), j & 1, abort_flag, kErrFwdMma)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint64_t b = dV + (j % R) * kSlot;
+        const uint32_t t = tmem + g * 256;
+        mma_ts_k64_mn(t + L::T_O, t + L::T_S, b, kIdO, j > 0 ? 1u : 0u);
+        mma_ts_k64_mn(t + L::T_O, t + L::T_S + 32, b + (8192 >> 4), kIdO, 1u);
+      }
+      __syncwarp();
+      return true;
+    };
+    // V of step j is there, its rows behind the sequence zero
+    const auto v_ready = [&](int j) -> bool {
+      if (!wait_warp(bar(L::B_VF + j % R), (j / R) & 1, abort_flag, kErrFwdMma)) return false;
+      if ((j + 1) * kRows > at.nk) {
+        zero_rows<L::kSub>(sm + L::V + (j % R) * L::kTileBytes, at.nk - j * kRows, lane, 32);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      return true;
+    };
+    bool ok = total == 0 || wait_warp(bar(L::B_Q), 0, abort_flag, kErrFwdMma);
+    tc_fence_after();
+    for (int n = 0; ok && n <= total && total > 0; ++n) {
+      const int st = n % R;
+      if ((n < total && !wait_warp(bar(L::B_KF + st), (n / R) & 1, abort_flag, kErrFwdMma)) ||
+          (n > 0 && !v_ready(n - 1))) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        if (n >= steps[g]) continue;
+        if (n > 0 && !pv(g, n - 1)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          mma_kd<L::kSub, 16384, 16384>(tmem + g * 256 + L::T_S, dQ + g * kSlot, dK + st * kSlot, kIdS, 0u);
+          mma_commit(bar(L::B_SF + g));
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
+      // a group's last P V, after the products that need not wait for it
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (n > 0 && n == steps[g]) {
+          if (!pv(g, n - 1)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mma_commit(bar(L::B_OF + g));
+          __syncwarp();
+        }
+      if (!ok) break;
+      if (lane == 0) {
+        if (n < total) mma_commit(bar(L::B_KE + st));
+        if (n > 0) mma_commit(bar(L::B_VE + (n - 1) % R));
+      }
+      __syncwarp();
+    }
+    // every product is done before TMEM is released
+    if (lane == 0) {
+      mma_commit(bar(L::B_DRAIN));
+      wait_one(bar(L::B_DRAIN), 0, abort_flag, kErrFwdMma);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------ softmax warps
+    const int g = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;  // row of the tile == TMEM lane
+    const uint32_t inverse = group_inverse(hd.group);
+    const int tok = tok0 + g * n_tok + over_group(r, inverse);
+    const bool valid = r < rows && tok < at.nq;
+    // keys that this row sees; rows without a token go along with the last one
+    const int seen = causal ? min(max(min(tok, last[g]) + shift + 1, 0), at.nk) : at.nk;
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * 256;
+    float m = -INFINITY, l = 1.0f;
+    bool ok = true;
+    for (int n = 0; n < steps[g]; ++n) {
+      // keys of the two halves of the step that the row sees; all / none of them for every row of the warp
+      const int lim0 = seen - n * kRows, lim1 = lim0 - 64;
+      const bool all0 = __all_sync(0xffffffffu, lim0 >= 64), all1 = __all_sync(0xffffffffu, lim1 >= 64);
+      const bool none0 = __all_sync(0xffffffffu, lim0 <= 0), none1 = __all_sync(0xffffffffu, lim1 <= 0);
+      if (!wait_warp(bar(L::B_SF + g), n & 1, abort_flag, kErrFwdSoftmax)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const auto scores = [&](int u, float(&s)[64]) {
+        tmem_load<2>(t_lane + L::T_S + u * 64, s);
+        if (!(u ? all1 : all0)) mask_from(s, u ? lim1 : lim0);
+      };
+      float sum0 = 0.f, sum1 = 0.f;
+      // Exponentials against the running maximum in one pass over S.  A row's first step, and a first half
+      // whose exponentials sum past kSum, take two passes (maximum, then exponentials; S is intact).  If only
+      // the second half passes the limit, P of the first half, l and O are scaled to the new maximum.
+      bool two_pass = __any_sync(0xffffffffu, m == -INFINITY);
+      uint32_t pk0[32];
+      if (!two_pass) {
+        if (none0) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) pk0[i] = 0u;
+        } else {
+          float s[64];
+          scores(0, s);
+          sum0 = exp_pairs<T>(s, qk_scale, m, pk0);
+        }
+        two_pass = __any_sync(0xffffffffu, !(sum0 <= H::kSum));
+      }
+      if (two_pass) {
+        sum0 = 0.f;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          if (u ? none1 : none0) continue;
+          float s[64];
+          scores(u, s);
+          mx = fmaxf(mx, tile_max(s));
+        }
+        mx = mx * qk_scale - H::kShift;
+        const bool need = mx > m + H::kLag;  // m = -inf: any key
+        if (__any_sync(0xffffffffu, need)) {
+          const float m_new = need ? mx : m;
+          const float alpha = need ? ex2(m - m_new) : 1.0f;  // m = -inf -> 0
+          const bool o_live = __any_sync(0xffffffffu, need && m != -INFINITY);
+          l *= alpha;
+          m = m_new;
+          // every earlier P V of the group is done: S was issued after them
+          if (n > 0 && o_live) scale_tmem_rows<D / 32>(t_lane + L::T_O, alpha);
+        }
+        const float mb = (m == -INFINITY) ? 0.0f : m;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t pk[32];
+          if (u ? none1 : none0) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) pk[i] = 0u;
+          } else {
+            float s[64];
+            scores(u, s);
+            const float t = exp_pairs<T>(s, qk_scale, mb, pk);
+            if (u) sum1 = t; else sum0 = t;
+          }
+          tmem_st32(t_lane + L::T_S + u * 32, pk);  // over scores of the first half, which are read
+        }
+      } else {
+        tmem_st32(t_lane + L::T_S, pk0);
+        uint32_t pk1[32];
+        if (none1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) pk1[i] = 0u;
+        } else {
+          float s[64];
+          scores(1, s);
+          sum1 = exp_pairs<T>(s, qk_scale, m, pk1);
+        }
+        const bool need = !(sum1 <= H::kSum);
+        if (__any_sync(0xffffffffu, need)) {  // rare
+          float s[64];
+          scores(1, s);
+          const float m_new = need ? fmaxf(m, tile_max(s) * qk_scale - H::kShift) : m;
+          const float alpha = ex2(m - m_new);
+          if (n > 0) scale_tmem_rows<D / 32>(t_lane + L::T_O, alpha);
+          tmem_wait_st();
+          uint32_t raw[32];
+          tmem_ld32(t_lane + L::T_S, raw);
+          tmem_wait_ld_dep(raw);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float2 p = H::unpack(raw[i]);
+            raw[i] = H::pack(p.x * alpha, p.y * alpha);
+          }
+          tmem_st32(t_lane + L::T_S, raw);
+          l = (l + sum0) * alpha;
+          sum0 = 0.f;
+          m = m_new;
+          sum1 = exp_pairs<T>(s, qk_scale, m, pk1);
+        }
+        tmem_st32(t_lane + L::T_S + 32, pk1);
+      }
+      l += sum0 + sum1;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(L::B_PF + g));
+    }
+    // epilogue
+    const bool empty = m == -INFINITY;  // no key
+    if (ok && lse != nullptr)
+      lse[(((int64_t)h * hd.pairs + pair) * 2 + g) * kRows + r] = valid && !empty ? m + __log2f(l) : INFINITY;
+    T* row = o + ((int64_t)(at.q0 + tok) * hd.keys * hd.group + h * hd.group + (r - (tok - tok0 - g * n_tok) * hd.group)) * D;
+    if (ok && steps[g] > 0 && wait_warp(bar(L::B_OF + g), 0, abort_flag, kErrFwdSoftmax)) {
+      tc_fence_after();
+      const float inv = 1.0f / l;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t raw[32], pk[16];
+        tmem_ld32(t_lane + L::T_O + c * 32, raw);
+        tmem_wait_ld_dep(raw);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pk[i] = empty ? 0u : H::pack(u2f(raw[2 * i]) * inv, u2f(raw[2 * i + 1]) * inv);
+        if (valid) {
+          uint4* dst = reinterpret_cast<uint4*>(row + c * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+        }
+      }
+    } else if (ok && steps[g] == 0 && valid) {
+      uint4* dst = reinterpret_cast<uint4*>(row);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ===================================================================== delta
+// delta = dO . O of every row of every tile, 0 for rows without a token, in the forward's tile order: D / 8
+// threads a row.  Bound by memory.
+constexpr int kDeltaThreads = 256;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kDeltaThreads)
+    delta_kernel(const __grid_constant__ Sequences seqs, Heads hd, const T* __restrict__ o, const T* __restrict__ go,
+                 int64_t go_row, int64_t go_head, float* __restrict__ delta) {
+  __shared__ Place shared_place;
+  __shared__ int scratch[2 * kDeltaThreads / 32];
+  const int pair = blockIdx.x / hd.keys, h = blockIdx.x % hd.keys;
+  find_place<false>(seqs, pair, 2 * hd.tokens, 2 * hd.tokens, &shared_place, scratch);
+  const Place at = shared_place;
+  if (at.kind != kTile) return;
+  constexpr int kLanes = D / 8, kStep = kDeltaThreads / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const uint32_t inverse = group_inverse(hd.group);
+#pragma unroll 4
+  for (int i = threadIdx.x / kLanes; i < 2 * kRows; i += kStep) {
+    const int g = i / kRows, r = i % kRows, t = over_group(r, inverse);
+    const int tok = (at.tile * 2 + g) * hd.tokens + t, head = h * hd.group + r - t * hd.group;
+    float sum = 0.0f;
+    if (t < hd.tokens && tok < at.nq) {
+      const int64_t row = at.q0 + tok;
+      const uint4 a = *reinterpret_cast<const uint4*>(o + (row * hd.keys * hd.group + head) * D + lane * 8);
+      const uint4 b = __ldg(reinterpret_cast<const uint4*>(go + row * go_row + head * go_head + lane * 8));
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 p = Half<T>::unpack(x[j]), q = Half<T>::unpack(y[j]);
+        sum = fmaf(p.x, q.x, sum);
+        sum = fmaf(p.y, q.y, sum);
+      }
+    }
+#pragma unroll
+    for (int off = kLanes / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+    if (lane == 0) delta[((int64_t)h * hd.pairs + pair) * 2 * kRows + i] = sum;
+  }
+}
+
+// ================================================================== dK and dV
+// CTA: 128 keys of one key head; a step is a tile of 128 query rows, so the sum over the heads that share
+// the keys is the products' own (no atomics, a fixed order).  S^T = K Q^T, dP^T = V dO^T; P^T and dS^T are
+// written over them in TMEM; dV += P^T dO, dK += dS^T Q.  Rows without a token have lse = +inf: p = 0.
+//
+// The softmax reads the 16x256b TMEM layout: a thread holds, in each 16-lane half, key lanes a and a + 8
+// (a = lane / 4) at columns 8 j + 2 (lane % 4) + {0, 1}, so that it needs 16 of a half tile's 64 lse and
+// delta values instead of all of them.
+template <int D>
+struct DkdvLayout {
+  static constexpr int kRing = 2;
+  static constexpr int kSub = D / 64;
+  static constexpr int kTileBytes = kSub * 16384;
+  static constexpr int K = 0;
+  static constexpr int V = K + kTileBytes;
+  static constexpr int Q = V + kTileBytes;
+  static constexpr int DO = Q + kRing * kTileBytes;
+  static constexpr int M = DO + kRing * kTileBytes;  // lse
+  static constexpr int DL = M + kRing * 512;         // delta
+  static constexpr int BAR = DL + kRing * 512;
+  static constexpr int B_KV = 0, B_QF = 1, B_QE = B_QF + kRing, B_SF = B_QE + kRing, B_DPF = B_SF + 1,
+                       B_PF = B_DPF + 1, B_DSF = B_PF + 1, B_FIN = B_DSF + 1, B_DRAIN = B_FIN + 1, NBAR = B_DRAIN + 1;
+  static constexpr int TMEM_SLOT = BAR + NBAR * 8;
+  static constexpr int ABORT = TMEM_SLOT + 4;
+  static constexpr int PLACE = ABORT + 4;
+  static constexpr int SCRATCH = PLACE + (int)sizeof(Place);
+  static constexpr size_t kNeed = 1024 + SCRATCH + 2 * 4 * (kThreads / 32);
+  static constexpr size_t kBytes = kNeed > kMinSmem ? kNeed : kMinSmem;
+  static constexpr int T_DK = 0, T_DV = D, T_S = 2 * D, T_DP = 2 * D + 128;
+  static_assert(T_DP + 128 <= 512, "TMEM budget");
+};
+
+// p = exp2(s scale - lse) of 64 columns for this warp's lanes, written as pairs over the first 32 columns.
+// kMasked: key lane `key` + 16 hl + 8 kk is 0 in columns whose `beyond` is not above it.
+template <typename T, bool kMasked>
+__device__ __forceinline__ void dkdv_p(uint32_t t_tile, const float* __restrict__ lse, float qk_scale, int lane,
+                                       const int* __restrict__ beyond, int key, float (&p)[64]) {
+  const int c2 = 2 * (lane & 3);
+  const float2 sc = make_float2(qk_scale, qk_scale);
+#pragma unroll
+  for (int hl = 0; hl < 2; ++hl) {
+    uint32_t raw[32], pk[16];
+    tmem_ld_16x256b_x8(t_tile + ((uint32_t)(16 * hl) << 16), raw);
+    tmem_wait_ld_dep(raw);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 ls = *reinterpret_cast<const float2*>(lse + 8 * j + c2), nl = make_float2(-ls.x, -ls.y);
+      int2 seen = make_int2(0, 0);
+      if constexpr (kMasked) seen = *reinterpret_cast<const int2*>(beyond + 8 * j + c2);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const float2 x = __ffma2_rn(make_float2(u2f(raw[4 * j + 2 * kk]), u2f(raw[4 * j + 2 * kk + 1])), sc, nl);
+        float e0 = ex2(x.x), e1 = ex2(x.y);
+        if constexpr (kMasked) {
+          const int row = key + 16 * hl + 8 * kk;
+          e0 = row < seen.x ? e0 : 0.0f;
+          e1 = row < seen.y ? e1 : 0.0f;
+        }
+        p[32 * hl + 4 * j + 2 * kk] = e0;
+        p[32 * hl + 4 * j + 2 * kk + 1] = e1;
+        pk[2 * j + kk] = Half<T>::pack(e0, e1);
+      }
+    }
+    tmem_st_16x128b_x8(t_tile + ((uint32_t)(16 * hl) << 16), pk);
+  }
+}
+
+// ds = p (dp - delta) as pairs over the first 32 columns of dP^T; 0 where p is 0 by the mask.
+template <typename T, bool kMasked>
+__device__ __forceinline__ void dkdv_ds(uint32_t t_tile, const float* __restrict__ delta, int lane,
+                                        const float (&p)[64]) {
+  const int c2 = 2 * (lane & 3);
+  const float2 neg1 = make_float2(-1.0f, -1.0f);
+#pragma unroll
+  for (int hl = 0; hl < 2; ++hl) {
+    uint32_t raw[32], pk[16];
+    tmem_ld_16x256b_x8(t_tile + ((uint32_t)(16 * hl) << 16), raw);
+    tmem_wait_ld_dep(raw);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float2 d2 = *reinterpret_cast<const float2*>(delta + 8 * j + c2);
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        const int i = 32 * hl + 4 * j + 2 * kk;
+        float2 ds = __fmul2_rn(make_float2(p[i], p[i + 1]),
+                               __ffma2_rn(d2, neg1, make_float2(u2f(raw[4 * j + 2 * kk]), u2f(raw[4 * j + 2 * kk + 1]))));
+        if constexpr (kMasked) ds = make_float2(p[i] == 0.0f ? 0.0f : ds.x, p[i + 1] == 0.0f ? 0.0f : ds.y);
+        pk[2 * j + kk] = Half<T>::pack(ds.x, ds.y);
+      }
+    }
+    tmem_st_16x128b_x8(t_tile + ((uint32_t)(16 * hl) << 16), pk);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                const __grid_constant__ Sequences seqs, Heads hd, int causal, float qk_scale, float scale,
+                const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
+                T* __restrict__ dv) {
+  using L = DkdvLayout<D>;
+  constexpr int R = L::kRing;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ int seen_keys[kRows];  // of a tile's rows, from this CTA's first key on
+  uint8_t* sm = align1024(smem_raw);
+  const uint32_t sb = smem_u32(sm);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int my = blockIdx.x / hd.keys, h = blockIdx.x % hd.keys;
+  const int n_tok = hd.tokens, rows = n_tok * hd.group;
+  auto bar = [&](int i) { return sb + L::BAR + 8 * i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::ABORT);
+
+  Place* shared_place = reinterpret_cast<Place*>(sm + L::PLACE);
+  find_place<true>(seqs, my, kRows, 2 * n_tok, shared_place, reinterpret_cast<int*>(sm + L::SCRATCH));
+  const Place at = *shared_place;
+  if (at.kind != kTile) {
+    fill_rows(at, seqs.k, seqs, seqs.k_rows, my, kRows, dk, hd.keys, h, D);
+    fill_rows(at, seqs.k, seqs, seqs.k_rows, my, kRows, dv, hd.keys, h, D);
+    return;
+  }
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar(L::B_KV), 1);
+    for (int i = 0; i < R; ++i) {
+      mbar_init(bar(L::B_QF + i), 1);
+      mbar_init(bar(L::B_QE + i), 1);
+    }
+    mbar_init(bar(L::B_SF), 1);
+    mbar_init(bar(L::B_DPF), 1);
+    mbar_init(bar(L::B_PF), 8);
+    mbar_init(bar(L::B_DSF), 8);
+    mbar_init(bar(L::B_FIN), 1);
+    mbar_init(bar(L::B_DRAIN), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  const int key0 = at.tile * kRows, shift = at.nk - at.nq;
+  const uint32_t inverse = group_inverse(hd.group);
+  // row r of tile i sees the keys below key0 + seen_keys[r] + i n
+  if (threadIdx.x < kRows) seen_keys[threadIdx.x] = over_group(threadIdx.x, inverse) + shift + 1 - key0;
+  if (rows < kRows) {  // rows that no load fills
+    for (int i = 0; i < R; ++i) {
+      zero_rows<L::kSub>(sm + L::Q + i * L::kTileBytes, rows, threadIdx.x, kThreads);
+      zero_rows<L::kSub>(sm + L::DO + i * L::kTileBytes, rows, threadIdx.x, kThreads);
+    }
+    fence_proxy_async_smem();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(sb + L::TMEM_SLOT, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + L::TMEM_SLOT);
+
+  // query tiles of the sequence, causal: from the one that sees the first key
+  const int tiles = (at.nq + n_tok - 1) / n_tok;
+  const int first = causal ? min(max(key0 - shift, 0) / n_tok, tiles) : 0, steps = tiles - first;
+  const int64_t stat0 = (((int64_t)h * hd.pairs + at.pairs) * 2 + first) * kRows;
+
+  if (warp == kProducerWarp) {
+    if (lane == 0 && steps > 0) {
+      mbar_expect_tx(bar(L::B_KV), 2 * L::kTileBytes);
+#pragma unroll
+      for (int s = 0; s < L::kSub; ++s) {
+        tma_load_3d(sb + L::K + s * 16384, &tm_k, s * 64, h, at.k0 + key0, bar(L::B_KV));
+        tma_load_3d(sb + L::V + s * 16384, &tm_v, s * 64, h, at.k0 + key0, bar(L::B_KV));
+      }
+      int n = 0;
+      for (; n < steps; ++n) {
+        const int st = n % R, tok = at.q0 + (first + n) * n_tok;
+        if (n >= R && !wait_one(bar(L::B_QE + st), ((n / R) - 1) & 1, abort_flag, kErrDkdvProducer)) break;
+        mbar_expect_tx(bar(L::B_QF + st), 2 * rows * D * 2 + 2 * 512);
+#pragma unroll
+        for (int s = 0; s < L::kSub; ++s) {
+          tma_load_3d(sb + L::Q + st * L::kTileBytes + s * 16384, &tm_q, s * 64, h * hd.group, tok, bar(L::B_QF + st));
+          tma_load_3d(sb + L::DO + st * L::kTileBytes + s * 16384, &tm_do, s * 64, h * hd.group, tok, bar(L::B_QF + st));
+        }
+        bulk_load(sb + L::M + st * 512, lse + stat0 + (int64_t)n * kRows, 512, bar(L::B_QF + st));
+        bulk_load(sb + L::DL + st * 512, delta + stat0 + (int64_t)n * kRows, 512, bar(L::B_QF + st));
+      }
+      for (int m = max(n - R, 0); m < n; ++m) wait_one(bar(L::B_QF + m % R), (m / R) & 1, abort_flag, kErrDkdvProducer);
+      wait_one(bar(L::B_KV), 0, abort_flag, kErrDkdvProducer);
+    }
+  } else if (warp == kMmaWarp) {
+    // Issue order: S^T(n) | dK(n-1) | dP^T(n) | dV(n).  The softmax computes P^T(n) while dK(n-1) and dP^T(n)
+    // run, dS^T(n) while dV(n) and S^T(n+1) do.  S^T(n) overwrites P^T(n-1), read by dV(n-1), dP^T(n)
+    // overwrites dS^T(n-1), read by dK(n-1): issued earlier, and one thread's products run in issue order.
+    constexpr uint32_t kIdS = idesc<T>(kRows, false), kIdG = idesc<T>(D, true);
+    const uint64_t dK = desc_k_sw128(sb + L::K), dV = desc_k_sw128(sb + L::V), dQk = desc_k_sw128(sb + L::Q),
+                   dDOk = desc_k_sw128(sb + L::DO), dQmn = desc_mn_sw128(sb + L::Q, 16384),
+                   dDOmn = desc_mn_sw128(sb + L::DO, 16384);
+    constexpr uint32_t kSlot = L::kTileBytes >> 4;
+    const auto dk_step = [&](int j) -> bool {
+      const uint32_t st = (uint32_t)j % R;
+      if (!wait_warp(bar(L::B_DSF), j & 1, abort_flag, kErrDkdvMma)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        mma_ts_k64_mn(tmem + L::T_DK, tmem + L::T_DP, dQmn + st * kSlot, kIdG, j > 0 ? 1u : 0u);
+        mma_ts_k64_mn(tmem + L::T_DK, tmem + L::T_DP + 64, dQmn + st * kSlot + 512, kIdG, 1u);
+        mma_commit(bar(L::B_QE + st));
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = steps == 0 || wait_warp(bar(L::B_KV), 0, abort_flag, kErrDkdvMma);
+    tc_fence_after();
+    for (int n = 0; ok && n < steps; ++n) {
+      const uint32_t st = (uint32_t)n % R;
+      if (!wait_warp(bar(L::B_QF + st), (n / R) & 1, abort_flag, kErrDkdvMma)) {
+        ok = false;
+        break;
+      }
+      const int valid = (at.nq - (first + n) * n_tok) * hd.group;
+      if (valid < rows) {  // the next sequence's rows
+        zero_rows<L::kSub>(sm + L::Q + st * L::kTileBytes, valid, lane, 32);
+        zero_rows<L::kSub>(sm + L::DO + st * L::kTileBytes, valid, lane, 32);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S, dK, dQk + st * kSlot, kIdS, 0u);
+        mma_commit(bar(L::B_SF));
+      }
+      __syncwarp();
+      if (n > 0 && !dk_step(n - 1)) {
+        ok = false;
+        break;
+      }
+      if (lane == 0) {
+        mma_kd<L::kSub, 16384, 16384>(tmem + L::T_DP, dV, dDOk + st * kSlot, kIdS, 0u);
+        mma_commit(bar(L::B_DPF));
+      }
+      __syncwarp();
+      if (!wait_warp(bar(L::B_PF), n & 1, abort_flag, kErrDkdvMma)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        mma_ts_k64_mn(tmem + L::T_DV, tmem + L::T_S, dDOmn + st * kSlot, kIdG, n > 0 ? 1u : 0u);
+        mma_ts_k64_mn(tmem + L::T_DV, tmem + L::T_S + 64, dDOmn + st * kSlot + 512, kIdG, 1u);
+      }
+      __syncwarp();
+    }
+    if (ok && steps > 0) dk_step(steps - 1);
+    if (lane == 0) {
+      mma_commit(bar(L::B_FIN));
+      mma_commit(bar(L::B_DRAIN));
+      wait_one(bar(L::B_DRAIN), 0, abort_flag, kErrDkdvMma);
+    }
+    __syncwarp();
+  } else {
+    // softmax warpgroup w: columns [64 w, 64 w + 64) of each tile
+    const int wg = warp >> 2, quarter = warp & 3;
+    const int r = quarter * 32 + lane;  // key row of the epilogue == TMEM lane
+    const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int key = quarter * 32 + (lane >> 2);  // this thread's first key lane
+    const float* sM = reinterpret_cast<const float*>(sm + L::M);
+    const float* sDl = reinterpret_cast<const float*>(sm + L::DL);
+    bool ok = true;
+    for (int n = 0; n < steps; ++n) {
+      const int st = n % R, tcol = wg * 64;
+      const int at_tile = (first + n) * n_tok;
+      // every row of the tile sees every key of the CTA from its first row's place on
+      const bool masked = causal && at_tile + shift + 1 - key0 < kRows;
+      if (!wait_warp(bar(L::B_QF + st), (n / R) & 1, abort_flag, kErrDkdvSoftmax) ||
+          !wait_warp(bar(L::B_SF), n & 1, abort_flag, kErrDkdvSoftmax)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      float p[64];
+      // key < seen + at_tile as key - at_tile < seen
+      if (masked) dkdv_p<T, true>(t_lane + L::T_S + tcol, sM + st * 128 + tcol, qk_scale, lane, seen_keys + tcol, key - at_tile, p);
+      else dkdv_p<T, false>(t_lane + L::T_S + tcol, sM + st * 128 + tcol, qk_scale, lane, nullptr, 0, p);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(L::B_PF));
+      if (!wait_warp(bar(L::B_DPF), n & 1, abort_flag, kErrDkdvSoftmax)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (masked) dkdv_ds<T, true>(t_lane + L::T_DP + tcol, sDl + st * 128 + tcol, lane, p);
+      else dkdv_ds<T, false>(t_lane + L::T_DP + tcol, sDl + st * 128 + tcol, lane, p);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(L::B_DSF));
+    }
+    // epilogue: warpgroup 0 writes dK, 1 dV
+    const bool valid = key0 + r < at.nk;
+    T* out = (wg == 0 ? dk : dv) + ((int64_t)(at.k0 + key0 + r) * hd.keys + h) * D;
+    const float by = wg == 0 ? scale : 1.0f;
+    if (ok && steps > 0 && wait_warp(bar(L::B_FIN), 0, abort_flag, kErrDkdvSoftmax)) {
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t raw[32], pk[16];
+        tmem_ld32(t_lane + (wg == 0 ? L::T_DK : L::T_DV) + c * 32, raw);
+        tmem_wait_ld_dep(raw);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) pk[i] = Half<T>::pack(u2f(raw[2 * i]) * by, u2f(raw[2 * i + 1]) * by);
+        if (valid) {
+          uint4* dst = reinterpret_cast<uint4*>(out + c * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+        }
+      }
+    } else if (ok && steps == 0 && valid) {
+      uint4* dst = reinterpret_cast<uint4*>(out);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ======================================================================= dQ
+// CTA: one tile of 128 query rows; a step is 128 keys: S = Q K^T and dP = dO V^T in TMEM, the softmax
+// warpgroups (64 keys each) write dS = P (dP - delta) into columns of its own, dQ += dS K reads them from
+// there.  S and dP of step n + 1 are issued as soon as those of step n are read.
+template <int D>
+struct DqLayout {
+  static constexpr int kRingK = 3, kRingV = 2;  // K serves two products
+  static constexpr int kSub = D / 64;
+  static constexpr int kTileBytes = kSub * 16384;
+  static constexpr int Q = 0;
+  static constexpr int DO = Q + kTileBytes;
+  static constexpr int K = DO + kTileBytes;
+  static constexpr int V = K + kRingK * kTileBytes;
+  static constexpr int BAR = V + kRingV * kTileBytes;
+  static constexpr int B_QD = 0, B_KF = 1, B_KE = B_KF + kRingK, B_VF = B_KE + kRingK, B_VE = B_VF + kRingV,
+                       B_SF = B_VE + kRingV, B_DPF = B_SF + 1, B_DPE = B_DPF + 1, B_DSF = B_DPE + 1,
+                       B_DSE = B_DSF + 1, B_FIN = B_DSE + 1, B_DRAIN = B_FIN + 1, NBAR = B_DRAIN + 1;
+  static constexpr int TMEM_SLOT = BAR + NBAR * 8;
+  static constexpr int ABORT = TMEM_SLOT + 4;
+  static constexpr int PLACE = ABORT + 4;
+  static constexpr int SCRATCH = PLACE + (int)sizeof(Place);
+  static constexpr size_t kNeed = 1024 + SCRATCH + 2 * 4 * (kThreads / 32);
+  static constexpr size_t kBytes = kNeed > kMinSmem ? kNeed : kMinSmem;
+  // dQ (D columns), S and dP (128 fp32 columns each), dS (64 columns of pairs)
+  static constexpr int T_DQ = 0, T_S = 128, T_DP = 256, T_DS = 384;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+              const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+              const __grid_constant__ Sequences seqs, Heads hd, int causal, float qk_scale, float scale,
+              const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dq) {
+  using L = DqLayout<D>;
+  constexpr int RK = L::kRingK, RV = L::kRingV;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = align1024(smem_raw);
+  const uint32_t sb = smem_u32(sm);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int my = 2 * hd.pairs - 1 - (int)(blockIdx.x / hd.keys), h = blockIdx.x % hd.keys;
+  const int pair = my >> 1, half = my & 1;
+  const int n_tok = hd.tokens, rows = n_tok * hd.group;
+  auto bar = [&](int i) { return sb + L::BAR + 8 * i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::ABORT);
+
+  Place* shared_place = reinterpret_cast<Place*>(sm + L::PLACE);
+  find_place<false>(seqs, pair, 2 * n_tok, 2 * n_tok, shared_place, reinterpret_cast<int*>(sm + L::SCRATCH));
+  const Place at = *shared_place;
+  if (at.kind != kTile) {
+    if (half == 0) fill_rows(at, seqs.q, seqs, seqs.q_rows, pair, 2 * n_tok, dq, hd.keys, h, hd.group * D);
+    return;
+  }
+  const int tok0 = (at.tile * 2 + half) * n_tok, shift = at.nk - at.nq;
+  if (tok0 >= at.nq) return;  // the pair's second tile, empty
+
+  if (threadIdx.x == 0) {
+    mbar_init(bar(L::B_QD), 1);
+    for (int i = 0; i < RK; ++i) {
+      mbar_init(bar(L::B_KF + i), 1);
+      mbar_init(bar(L::B_KE + i), 1);
+    }
+    for (int i = 0; i < RV; ++i) {
+      mbar_init(bar(L::B_VF + i), 1);
+      mbar_init(bar(L::B_VE + i), 1);
+    }
+    mbar_init(bar(L::B_SF), 1);
+    mbar_init(bar(L::B_DPF), 1);
+    mbar_init(bar(L::B_DPE), 8);
+    mbar_init(bar(L::B_DSF), 8);
+    mbar_init(bar(L::B_DSE), 1);
+    mbar_init(bar(L::B_FIN), 1);
+    mbar_init(bar(L::B_DRAIN), 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (rows < kRows) {  // rows that no load fills
+    zero_rows<L::kSub>(sm + L::Q, rows, threadIdx.x, kThreads);
+    zero_rows<L::kSub>(sm + L::DO, rows, threadIdx.x, kThreads);
+    fence_proxy_async_smem();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(sb + L::TMEM_SLOT, 512);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + L::TMEM_SLOT);
+
+  const int last = min(tok0 + n_tok, at.nq) - 1;
+  const int keys = causal ? min(max(last + shift + 1, 0), at.nk) : at.nk, steps = (keys + kRows - 1) / kRows;
+
+  if (warp == kProducerWarp) {
+    if (lane == 0 && steps > 0) {
+      mbar_expect_tx(bar(L::B_QD), 2 * rows * D * 2);
+#pragma unroll
+      for (int s = 0; s < L::kSub; ++s) {
+        tma_load_3d(sb + L::Q + s * 16384, &tm_q, s * 64, h * hd.group, at.q0 + tok0, bar(L::B_QD));
+        tma_load_3d(sb + L::DO + s * 16384, &tm_do, s * 64, h * hd.group, at.q0 + tok0, bar(L::B_QD));
+      }
+      int nk = 0, nv = 0;
+      for (int n = 0; n < steps; ++n) {
+        const int sk = n % RK, sv = n % RV, key = at.k0 + n * kRows;
+        if (n >= RK && !wait_one(bar(L::B_KE + sk), ((n / RK) - 1) & 1, abort_flag, kErrDqProducer)) break;
+        mbar_expect_tx(bar(L::B_KF + sk), L::kTileBytes);
+#pragma unroll
+        for (int s = 0; s < L::kSub; ++s)
+          tma_load_3d(sb + L::K + sk * L::kTileBytes + s * 16384, &tm_k, s * 64, h, key, bar(L::B_KF + sk));
+        ++nk;
+        if (n >= RV && !wait_one(bar(L::B_VE + sv), ((n / RV) - 1) & 1, abort_flag, kErrDqProducer)) break;
+        mbar_expect_tx(bar(L::B_VF + sv), L::kTileBytes);
+#pragma unroll
+        for (int s = 0; s < L::kSub; ++s)
+          tma_load_3d(sb + L::V + sv * L::kTileBytes + s * 16384, &tm_v, s * 64, h, key, bar(L::B_VF + sv));
+        ++nv;
+      }
+      for (int m = max(nk - RK, 0); m < nk; ++m) wait_one(bar(L::B_KF + m % RK), (m / RK) & 1, abort_flag, kErrDqProducer);
+      for (int m = max(nv - RV, 0); m < nv; ++m) wait_one(bar(L::B_VF + m % RV), (m / RV) & 1, abort_flag, kErrDqProducer);
+      wait_one(bar(L::B_QD), 0, abort_flag, kErrDqProducer);
+    }
+  } else if (warp == kMmaWarp) {
+    // Issue order: S(0) dP(0) | S(1) dP(1) dQ(0) | S(2) dP(2) dQ(1) | ...
+    constexpr uint32_t kIdS = idesc<T>(kRows, false), kIdG = idesc<T>(D, true);
+    const uint64_t dQ = desc_k_sw128(sb + L::Q), dDO = desc_k_sw128(sb + L::DO), dKk = desc_k_sw128(sb + L::K),
+                   dVk = desc_k_sw128(sb + L::V), dKmn = desc_mn_sw128(sb + L::K, 16384);
+    constexpr uint32_t kSlot = L::kTileBytes >> 4;
+    const auto dq_step = [&](int j) -> bool {
+      if (!wait_warp(bar(L::B_DSF), j & 1, abort_flag, kErrDqMma)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint64_t b = dKmn + (j % RK) * kSlot;
+        mma_ts_k64_mn(tmem + L::T_DQ, tmem + L::T_DS, b, kIdG, j > 0 ? 1u : 0u);
+        mma_ts_k64_mn(tmem + L::T_DQ, tmem + L::T_DS + 32, b + (8192 >> 4), kIdG, 1u);
+        mma_commit(bar(L::B_DSE));
+        mma_commit(bar(L::B_KE + j % RK));
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = steps == 0 || wait_warp(bar(L::B_QD), 0, abort_flag, kErrDqMma);
+    tc_fence_after();
+    for (int n = 0; ok && n < steps; ++n) {
+      const int sk = n % RK, sv = n % RV;
+      if (!wait_warp(bar(L::B_KF + sk), (n / RK) & 1, abort_flag, kErrDqMma) ||
+          (n > 0 && !wait_warp(bar(L::B_DPE), (n - 1) & 1, abort_flag, kErrDqMma))) {
+        ok = false;
+        break;
+      }
+      if ((n + 1) * kRows > at.nk) {  // the next sequence's keys, which dQ sums over
+        zero_rows<L::kSub>(sm + L::K + sk * L::kTileBytes, at.nk - n * kRows, lane, 32);
+        fence_proxy_async_smem();
+        __syncwarp();
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S, dQ, dKk + sk * kSlot, kIdS, 0u);
+        mma_commit(bar(L::B_SF));
+      }
+      __syncwarp();
+      if (!wait_warp(bar(L::B_VF + sv), (n / RV) & 1, abort_flag, kErrDqMma)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (lane == 0) {
+        mma_kd<L::kSub, 16384, 16384>(tmem + L::T_DP, dDO, dVk + sv * kSlot, kIdS, 0u);
+        mma_commit(bar(L::B_DPF));
+        mma_commit(bar(L::B_VE + sv));
+      }
+      __syncwarp();
+      if (n > 0 && !dq_step(n - 1)) {
+        ok = false;
+        break;
+      }
+    }
+    if (ok && steps > 0) dq_step(steps - 1);
+    if (lane == 0) {
+      mma_commit(bar(L::B_FIN));
+      mma_commit(bar(L::B_DRAIN));
+      wait_one(bar(L::B_DRAIN), 0, abort_flag, kErrDqMma);
+    }
+    __syncwarp();
+  } else {
+    // softmax warpgroup w: keys [64 w, 64 w + 64) of each step
+    const int wg = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;  // row of the tile == TMEM lane
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int t = over_group(r, group_inverse(hd.group)), tok = tok0 + t;
+    const bool valid = r < rows && tok < at.nq;
+    const int seen = causal ? min(max(min(tok, last) + shift + 1, 0), at.nk) : at.nk;
+    const int64_t stat = (((int64_t)h * hd.pairs + pair) * 2 + half) * kRows + r;
+    const float mrow = lse[stat], drow = delta[stat];
+    bool ok = true;
+    for (int n = 0; n < steps; ++n) {
+      const int lim = seen - n * kRows - wg * 64;
+      const bool all = __all_sync(0xffffffffu, lim >= 64), none = __all_sync(0xffffffffu, lim <= 0);
+      if (!wait_warp(bar(L::B_SF), n & 1, abort_flag, kErrDqSoftmax)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      // S(n) and dP(n) are both read before the exponentials and released at once; dS(n) overwrites dS(n-1),
+      // so its stores wait for dQ(n-1); it is written in two parts to bound registers
+      float p[64], dp[64];
+      if (!none) tmem_load<2>(t_lane + L::T_S + wg * 64, p);
+      if (!wait_warp(bar(L::B_DPF), n & 1, abort_flag, kErrDqSoftmax)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      if (!none) tmem_load<2>(t_lane + L::T_DP + wg * 64, dp);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(L::B_DPE));
+      if (!none && !all) {  // masked keys: p = 0, whatever their V rows hold
+        mask_from(p, lim);
+#pragma unroll
+        for (int c = 0; c < 64; ++c)
+          if (c >= lim) dp[c] = 0.0f;
+      }
+      const float2 sc = make_float2(qk_scale, qk_scale), nm = make_float2(-mrow, -mrow), nd = make_float2(-drow, -drow);
+#pragma unroll
+      for (int part = 0; part < 2; ++part) {
+        uint32_t pk[16];
+        if (!none) {
+#pragma unroll
+          for (int c = 32 * part; c < 32 * part + 32; c += 2) {
+            const float2 x = __ffma2_rn(make_float2(p[c], p[c + 1]), sc, nm);
+            const float2 ds = __fmul2_rn(make_float2(ex2(x.x), ex2(x.y)), __fadd2_rn(make_float2(dp[c], dp[c + 1]), nd));
+            pk[(c - 32 * part) / 2] = Half<T>::pack(ds.x, ds.y);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pk[i] = 0u;
+        }
+        if (part == 0) {
+          if (n > 0 && !wait_warp(bar(L::B_DSE), (n - 1) & 1, abort_flag, kErrDqSoftmax)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+        }
+        tmem_st16(t_lane + L::T_DS + wg * 32 + 16 * part, pk);
+      }
+      if (!ok) break;
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(L::B_DSF));
+    }
+    // epilogue: warpgroup w writes columns [w D / 2, (w + 1) D / 2); a row without keys has none of its own
+    const bool empty = seen == 0;
+    T* row = dq + ((int64_t)(at.q0 + tok) * hd.keys * hd.group + h * hd.group + (r - t * hd.group)) * D + wg * (D / 2);
+    if (ok && steps > 0 && wait_warp(bar(L::B_FIN), 0, abort_flag, kErrDqSoftmax)) {
+      tc_fence_after();
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) {
+        uint32_t raw[32], pk[16];
+        tmem_ld32(t_lane + L::T_DQ + wg * (D / 2) + c * 32, raw);
+        tmem_wait_ld_dep(raw);
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          pk[i] = empty ? 0u : Half<T>::pack(u2f(raw[2 * i]) * scale, u2f(raw[2 * i + 1]) * scale);
+        if (valid) {
+          uint4* dst = reinterpret_cast<uint4*>(row + c * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+        }
+      }
+    } else if (ok && steps == 0 && valid) {
+      uint4* dst = reinterpret_cast<uint4*>(row);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ================================================================ host side
+using EncodeFn = PFN_cuTensorMapEncodeTiled_v12000;
+
+static EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+  });
+  return fn;
+}
+
+// Makes the device's context the thread's: encoding a tensor map needs one, and a thread of autograd's whose
+// first call this is has none yet.
+static prism_status_t bind_context(const char* what) {
+  int device = 0;
+  PRISM_CHECK_CUDA(cudaGetDevice(&device), what);
+  PRISM_CHECK_CUDA(cudaSetDevice(device), what);
+  return PRISM_OK;
+}
+
+// [rows, heads, D] with row and head strides in elements; boxes of 64 columns x box_heads x box_rows.
+static prism_status_t make_map(CUtensorMap* map, const void* ptr, int64_t rows, int heads, int D, const int64_t* strides,
+                               int box_heads, int box_rows, int dtype) {
+  EncodeFn enc = encode_fn();
+  if (enc == nullptr) {
+    set_error("prism_packed_attention: cuTensorMapEncodeTiled is unavailable from the driver");
+    return PRISM_ERR_CUDA;
+  }
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t bytes[2] = {(cuuint64_t)strides[1] * 2, (cuuint64_t)strides[0] * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(map, dtype == PRISM_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                   const_cast<void*>(ptr), dims, bytes, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error("prism_packed_attention: cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return PRISM_ERR_CUDA;
+  }
+  return PRISM_OK;
+}
+
+static int64_t pair_bound(int64_t rows, int64_t count, int group) {
+  const int64_t per = 2 * (kRows / group);
+  return (rows + per - 1) / per + count;
+}
+
+struct Shape {
+  const void *q_offsets, *k_offsets;
+  int wide;
+  int64_t count, q_rows, k_rows;
+  int q_heads, k_heads, D, causal, dtype;
+  float scale;
+  Sequences sequences() const {
+    return {q_offsets, k_offsets, wide, (int)count, (int)q_rows, (int)k_rows};
+  }
+  Heads heads() const {
+    const int group = q_heads / k_heads;
+    return {k_heads, group, kRows / group, (int)pair_bound(q_rows, count, group)};
+  }
+  int64_t key_tiles() const { return (k_rows + kRows - 1) / kRows + count; }
+};
+
+static prism_status_t check(const Shape& s, const char* what) {
+  constexpr int64_t kMost = (int64_t)1 << 30;
+  PRISM_CHECK_ARG(s.D == 64 || s.D == 128, "%s: head dim %d not supported (64, 128)", what, s.D);
+  PRISM_CHECK_ARG(s.k_heads >= 1 && s.q_heads >= 1 && s.q_heads % s.k_heads == 0 && s.q_heads / s.k_heads <= kRows,
+                  "%s: %d query heads do not share %d key heads in equal groups of up to %d", what, s.q_heads,
+                  s.k_heads, kRows);
+  PRISM_CHECK_ARG(s.dtype == PRISM_BF16 || s.dtype == PRISM_FP16, "%s: element type %d (bf16 or fp16)", what, s.dtype);
+  PRISM_CHECK_ARG(s.count >= 0 && s.q_rows >= 0 && s.k_rows >= 0 && s.count < kMost && s.q_rows < kMost && s.k_rows < kMost,
+                  "%s: bad sizes", what);
+  // the grids, the largest of which has two CTAs a pair of tiles and key head
+  PRISM_CHECK_ARG(2 * pair_bound(s.q_rows, s.count, s.q_heads / s.k_heads) * s.k_heads < 2 * kMost &&
+                      s.key_tiles() * s.k_heads < 2 * kMost,
+                  "%s: too many rows, sequences or heads", what);
+  PRISM_CHECK_ARG(s.scale > 0.0f && s.scale < 1.0e30f, "%s: the scale must be positive and finite", what);
+  return PRISM_OK;
+}
+
+// Row and head strides, in elements, that a tensor map takes.
+static prism_status_t check_rows(const void* p, const int64_t* strides, const char* what, const char* name) {
+  PRISM_CHECK_ARG(p != nullptr && strides != nullptr, "%s: null pointer (%s)", what, name);
+  PRISM_CHECK_ARG(aligned16(p) && strides[0] > 0 && strides[1] > 0 && strides[0] % 8 == 0 && strides[1] % 8 == 0 &&
+                      strides[0] < ((int64_t)1 << 38) && strides[1] < ((int64_t)1 << 38),
+                  "%s: %s must start on 16 bytes, with positive row and head strides of whole 16 bytes", what, name);
+  return PRISM_OK;
+}
+
+#define PRISM_TRY(x)                       \
+  do {                                     \
+    prism_status_t st_ = (x);              \
+    if (st_ != PRISM_OK) return st_;       \
+  } while (0)
+
+struct Input {
+  const void* p;
+  const int64_t* strides;
+};
+
+template <typename T, int D>
+static prism_status_t launch_fwd(const Shape& s, const Input& q, const Input& k, const Input& v, void* o, float* lse,
+                                 cudaStream_t stream) {
+  constexpr const char* what = "prism_packed_attention";
+  const Heads hd = s.heads();
+  PRISM_TRY(bind_context(what));
+  CUtensorMap mq, mk, mv;
+  PRISM_TRY(make_map(&mq, q.p, s.q_rows, s.q_heads, D, q.strides, hd.group, hd.tokens, s.dtype));
+  // without key rows nothing is loaded: any valid map does
+  const Input& kk = s.k_rows > 0 ? k : q;
+  const Input& vv = s.k_rows > 0 ? v : q;
+  const int64_t k_rows = s.k_rows > 0 ? s.k_rows : s.q_rows;
+  PRISM_TRY(make_map(&mk, kk.p, k_rows, s.k_heads, D, kk.strides, 1, kRows, s.dtype));
+  PRISM_TRY(make_map(&mv, vv.p, k_rows, s.k_heads, D, vv.strides, 1, kRows, s.dtype));
+  const auto kernel = fwd_kernel<T, D>;
+  constexpr size_t bytes = FwdLayout<D>::kBytes;
+  static_assert(bytes <= 227 * 1024, "shared memory");
+  PRISM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
+  kernel<<<(unsigned)(hd.pairs * hd.keys), kThreads, bytes, stream>>>(mq, mk, mv, s.sequences(), hd, s.causal,
+                                                                      s.scale * kLog2e, (T*)o, lse);
+  PRISM_CHECK_LAUNCH(what);
+  return PRISM_OK;
+}
+
+template <typename T, int D>
+static prism_status_t launch_bwd(const Shape& s, const Input& q, const Input& k, const Input& v, const void* o,
+                                 const Input& go, const float* lse, float* delta, void* dq, void* dk, void* dv,
+                                 cudaStream_t stream) {
+  constexpr const char* what = "prism_packed_attention_bwd";
+  const Heads hd = s.heads();
+  const Sequences seqs = s.sequences();
+  PRISM_TRY(bind_context(what));
+  CUtensorMap mq, mk, mv, mdo;
+  PRISM_TRY(make_map(&mq, q.p, s.q_rows, s.q_heads, D, q.strides, hd.group, hd.tokens, s.dtype));
+  PRISM_TRY(make_map(&mdo, go.p, s.q_rows, s.q_heads, D, go.strides, hd.group, hd.tokens, s.dtype));
+  PRISM_TRY(make_map(&mk, k.p, s.k_rows, s.k_heads, D, k.strides, 1, kRows, s.dtype));
+  PRISM_TRY(make_map(&mv, v.p, s.k_rows, s.k_heads, D, v.strides, 1, kRows, s.dtype));
+  delta_kernel<T, D><<<(unsigned)(hd.pairs * hd.keys), kDeltaThreads, 0, stream>>>(
+      seqs, hd, (const T*)o, (const T*)go.p, go.strides[0], go.strides[1], delta);
+  PRISM_CHECK_LAUNCH(what);
+  if (dk != nullptr) {
+    constexpr size_t bytes = DkdvLayout<D>::kBytes;
+    static_assert(bytes + 512 <= 227 * 1024, "shared memory");
+    const auto kernel = dkdv_kernel<T, D>;
+    PRISM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
+    kernel<<<(unsigned)(s.key_tiles() * hd.keys), kThreads, bytes, stream>>>(
+        mq, mk, mv, mdo, seqs, hd, s.causal, s.scale * kLog2e, s.scale, lse, delta, (T*)dk, (T*)dv);
+    PRISM_CHECK_LAUNCH(what);
+  }
+  if (dq != nullptr) {
+    constexpr size_t bytes = DqLayout<D>::kBytes;
+    static_assert(bytes <= 227 * 1024, "shared memory");
+    const auto kernel = dq_kernel<T, D>;
+    PRISM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
+    kernel<<<(unsigned)(2 * hd.pairs * hd.keys), kThreads, bytes, stream>>>(
+        mq, mk, mv, mdo, seqs, hd, s.causal, s.scale * kLog2e, s.scale, lse, delta, (T*)dq);
+    PRISM_CHECK_LAUNCH(what);
+  }
+  return PRISM_OK;
+}
+
+}  // namespace packed
+}  // namespace prism
+
+using namespace prism;
+
+int prism_packed_device_status_internal(void) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, packed::g_error, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(packed::g_error, &zero, sizeof(int));
+  }
+  return v;
+}
+
+extern "C" {
+
+size_t prism_packed_attention_stats_bytes(int64_t q_rows, int64_t count, int q_heads, int k_heads) {
+  if (q_rows < 0 || count < 0 || k_heads < 1 || q_heads < k_heads || q_heads / k_heads > packed::kRows) return 0;
+  return (size_t)packed::pair_bound(q_rows, count, q_heads / k_heads) * 2 * packed::kRows * k_heads * sizeof(float);
+}
+
+prism_status_t prism_packed_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                      const void* v, const int64_t* v_strides, const void* q_offsets,
+                                      const void* k_offsets, int offsets_64, int64_t count, int64_t q_rows,
+                                      int64_t k_rows, int q_heads, int k_heads, int D, int causal, float scale,
+                                      int dtype, void* o, float* lse, cudaStream_t stream) {
+  constexpr const char* what = "prism_packed_attention";
+  const packed::Shape s = {q_offsets, k_offsets, offsets_64, count, q_rows, k_rows,
+                           q_heads,   k_heads,   D,          causal != 0, dtype, scale};
+  PRISM_TRY(packed::check(s, what));
+  if (q_rows == 0) return PRISM_OK;
+  PRISM_CHECK_ARG(q_offsets && k_offsets && o && aligned16(o) && (!lse || aligned16(lse)), "%s: null pointer, or an output off 16 bytes", what);
+  PRISM_TRY(packed::check_rows(q, q_strides, what, "q"));
+  if (k_rows > 0) {
+    PRISM_TRY(packed::check_rows(k, k_strides, what, "k"));
+    PRISM_TRY(packed::check_rows(v, v_strides, what, "v"));
+  }
+  const packed::Input iq = {q, q_strides}, ik = {k, k_strides}, iv = {v, v_strides};
+  if (dtype == PRISM_FP16)
+    return D == 64 ? packed::launch_fwd<__half, 64>(s, iq, ik, iv, o, lse, stream)
+                   : packed::launch_fwd<__half, 128>(s, iq, ik, iv, o, lse, stream);
+  return D == 64 ? packed::launch_fwd<__nv_bfloat16, 64>(s, iq, ik, iv, o, lse, stream)
+                 : packed::launch_fwd<__nv_bfloat16, 128>(s, iq, ik, iv, o, lse, stream);
+}
+
+prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
+                                          const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                          const void* o, const void* dout, const int64_t* dout_strides,
+                                          const float* lse, const void* q_offsets, const void* k_offsets,
+                                          int offsets_64, int64_t count, int64_t q_rows, int64_t k_rows, int q_heads,
+                                          int k_heads, int D, int causal, float scale, void* workspace, void* dq,
+                                          void* dk, void* dv, cudaStream_t stream) {
+  constexpr const char* what = "prism_packed_attention_bwd";
+  const packed::Shape s = {q_offsets, k_offsets, offsets_64, count, q_rows, k_rows,
+                           q_heads,   k_heads,   D,          causal != 0, PRISM_BF16, scale};
+  PRISM_TRY(packed::check(s, what));
+  PRISM_CHECK_ARG(q_rows > 0 && k_rows > 0, "%s: no rows (all gradients are zero)", what);
+  PRISM_CHECK_ARG(q_offsets && k_offsets && o && lse && workspace && (dk == nullptr) == (dv == nullptr),
+                  "%s: null pointer", what);
+  PRISM_CHECK_ARG(aligned16(o) && aligned16(lse) && aligned16(workspace) && aligned16(dq) && aligned16(dk) && aligned16(dv),
+                  "%s: buffers must start on 16 bytes", what);
+  PRISM_TRY(packed::check_rows(q, q_strides, what, "q"));
+  PRISM_TRY(packed::check_rows(k, k_strides, what, "k"));
+  PRISM_TRY(packed::check_rows(v, v_strides, what, "v"));
+  PRISM_TRY(packed::check_rows(dout, dout_strides, what, "dout"));
+  const packed::Input iq = {q, q_strides}, ik = {k, k_strides}, iv = {v, v_strides}, ig = {dout, dout_strides};
+  float* delta = static_cast<float*>(workspace);
+  return D == 64 ? packed::launch_bwd<__nv_bfloat16, 64>(s, iq, ik, iv, o, ig, lse, delta, dq, dk, dv, stream)
+                 : packed::launch_bwd<__nv_bfloat16, 128>(s, iq, ik, iv, o, ig, lse, delta, dq, dk, dv, stream);
+}
+
+}  // extern "C"

@@ -1,4 +1,4 @@
-// The torch side of the norm, rotary, 8-bit projection and clipping operators: argument checks,
+// The torch side of the norm, rotary, 8-bit projection, clipping and packed and paged attention operators: argument checks,
 // outputs and workspaces from torch's allocator, the current stream, autograd nodes, and the call of
 // the C entry point.  In C++ because at one token the host's share of a call is longer than the
 // kernel's (one row's norm: 14 us through Python attributes and ctypes), and a list of a thousand
@@ -9,8 +9,10 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <array>
 #include <cmath>
 #include <optional>
+#include <stdexcept>
 #include <string>
 #include <vector>
 
@@ -24,8 +26,9 @@ using torch::autograd::variable_list;
 using Optional = std::optional<Tensor>;
 
 // ------------------------------------------------------------------ errors
-struct PrismFailure {
-  std::string what;
+// A std::exception: autograd's threads carry those to the caller, and end the process on any other.
+struct PrismFailure : std::runtime_error {
+  using std::runtime_error::runtime_error;
 };
 
 void check(prism_status_t status, const char* name) {
@@ -138,14 +141,16 @@ std::tuple<Tensor, Tensor, Tensor> norm_forward(const Tensor& x, const Tensor& r
 
 // The gradients as parts of a graph that raises where it is differentiated.  `from`: what they depend on; the
 // node leads there, or a derivative with respect to these alone would go past it.
-std::pair<Tensor, Tensor> without_derivative(Tensor dx, Tensor dw, std::initializer_list<Tensor> from) {
+variable_list without_derivative(const variable_list& grads, std::initializer_list<Tensor> from, const char* what) {
   const at::AutoGradMode grad(true);
-  variable_list in = {dx.requires_grad_(), dw.defined() ? dw.requires_grad_() : Tensor()};
+  variable_list in;
+  for (const Tensor& g : grads) in.push_back(g.defined() ? g.requires_grad_() : g);
   in.insert(in.end(), from);
-  const auto node = std::make_shared<torch::autograd::DelayedError>("add_rms_norm: its gradient has no gradient",
-                                                                   (int64_t)in.size());
-  const variable_list out = (*node)(std::move(in));
-  return {out[0], out[1]};
+  const auto node =
+      std::make_shared<torch::autograd::DelayedError>(std::string(what) + ": its gradient has no gradient", (int64_t)in.size());
+  variable_list out = (*node)(std::move(in));
+  out.resize(grads.size());
+  return out;
 }
 
 struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
@@ -187,7 +192,10 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
                                    at(workspace), (float*)at(dw), launch.stream),
             "prism_add_rms_norm_bwd");
       if (want_w) dw = dw.to(w.scalar_type());
-      if (graph) std::tie(dx, dw) = without_derivative(dx, dw, {gy, gh, h, w});
+      if (graph) {
+        const variable_list out = without_derivative({dx, dw}, {gy, gh, h, w}, "add_rms_norm");
+        dx = out[0], dw = out[1];
+      }
     }
     const bool want_r = has_r && ctx->needs_input_grad(1);
     return {ctx->needs_input_grad(0) ? dx : Tensor(), want_r ? dx : Tensor(), dw, Tensor()};
@@ -383,6 +391,142 @@ Tensor linear_fp8(const Tensor& x8, const Tensor& x_scale, const Tensor& w8, con
   return out.view(shape);
 }
 
+// ------------------------------------------------------------------ attention over packed sequences
+// t [rows, heads, D], or a contiguous copy where a tensor map does not take its strides.
+Tensor mappable(const Tensor& t) {
+  const auto fits = [&](int64_t d) { return t.size(d) <= 1 || (t.stride(d) > 0 && t.stride(d) % 8 == 0); };
+  return t.stride(2) == 1 && fits(0) && fits(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0
+             ? t
+             : t.clone(at::MemoryFormat::Contiguous);
+}
+// {row, head} strides; those of a dimension of one element are never used, but have to be fit for a map.
+std::array<int64_t, 2> map_strides(const Tensor& t) {
+  const int64_t head = t.size(1) > 1 ? t.stride(1) : t.size(2);
+  return {t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2), head};
+}
+
+struct PackedCall {
+  Tensor offsets, k_offsets;
+  bool causal;
+  double scale;
+};
+
+Tensor stats_like(const Tensor& q, const Tensor& k, const PackedCall& c) {
+  const size_t bytes = prism_packed_attention_stats_bytes(q.size(0), c.offsets.size(0) - 1, (int)q.size(1), (int)k.size(1));
+  return fp32({(int64_t)(bytes / sizeof(float))}, q);
+}
+
+// (o, lse)
+std::pair<Tensor, Tensor> packed_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const PackedCall& c,
+                                         bool want_lse) {
+  const Launch launch(q_in.get_device());
+  const Tensor q = mappable(q_in), k = mappable(k_in), v = mappable(v_in);
+  Tensor o = new_like(q), lse = want_lse ? stats_like(q, k, c) : Tensor();
+  const auto sq = map_strides(q), sk = map_strides(k), sv = map_strides(v);
+  check(prism_packed_attention(at(q), sq.data(), at(k), sk.data(), at(v), sv.data(), at(c.offsets), at(c.k_offsets),
+                               c.offsets.scalar_type() == at::kLong, c.offsets.size(0) - 1, q.size(0), k.size(0),
+                               (int)q.size(1), (int)k.size(1), (int)q.size(2), c.causal, (float)c.scale,
+                               dtype_code(q, "packed_attention"), at(o), (float*)at(lse), launch.stream),
+        "prism_packed_attention");
+  return {o, lse};
+}
+
+struct PackedAttention : torch::autograd::Function<PackedAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const PackedCall& c) {
+    auto [o, lse] = packed_forward(q, k, v, c, true);
+    ctx->save_for_backward({q, k, v, o, lse, c.offsets, c.k_offsets});
+    ctx->saved_data["causal"] = c.causal;
+    ctx->saved_data["scale"] = c.scale;
+    ctx->set_materialize_grads(false);
+    return o;
+  }
+
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& go_in = grads[0];
+    if (!go_in.defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const bool graph = at::GradMode::is_enabled();
+    variable_list out(3);
+    {
+      const at::NoGradGuard no_grad;
+      const Launch launch(saved[0].get_device());
+      const Tensor q = mappable(saved[0]), k = mappable(saved[1]), v = mappable(saved[2]), go = mappable(go_in);
+      const Tensor &o = saved[3], &lse = saved[4];
+      const PackedCall c = {saved[5], saved[6], ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble()};
+      const bool want_q = ctx->needs_input_grad(0), want_k = ctx->needs_input_grad(1), want_v = ctx->needs_input_grad(2);
+      const bool pair = want_k || want_v;
+      if (q.size(0) == 0 || k.size(0) == 0) {
+        out = {at::zeros_like(q), at::zeros_like(k), at::zeros_like(v)};
+      } else {
+        if (want_q) out[0] = new_like(q);
+        if (pair) out[1] = new_like(k), out[2] = new_like(v);
+        const Tensor workspace = stats_like(q, k, c);
+        const auto sq = map_strides(q), sk = map_strides(k), sv = map_strides(v), sg = map_strides(go);
+        check(prism_packed_attention_bwd(at(q), sq.data(), at(k), sk.data(), at(v), sv.data(), at(o), at(go), sg.data(),
+                                         (const float*)at(lse), at(c.offsets), at(c.k_offsets),
+                                         c.offsets.scalar_type() == at::kLong, c.offsets.size(0) - 1, q.size(0),
+                                         k.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), c.causal,
+                                         (float)c.scale, at(workspace), at(out[0]), at(out[1]), at(out[2]),
+                                         launch.stream),
+              "prism_packed_attention_bwd");
+      }
+      if (!want_q) out[0] = Tensor();
+      if (!want_k) out[1] = Tensor();
+      if (!want_v) out[2] = Tensor();
+    }
+    if (graph) out = without_derivative(out, {go_in, saved[0], saved[1], saved[2]}, "packed_attention");
+    return {out[0], out[1], out[2], Tensor()};
+  }
+};
+
+void check_offsets(const Tensor& t, const char* name) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, name, " must be int32 or int64, got ",
+                   t.scalar_type());
+  TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) >= 1, name, " must hold one row number more than there are sequences, got shape ",
+                    t.sizes());
+}
+
+void check_scale(const std::optional<double>& scale, const char* what) {
+  TORCH_CHECK_VALUE(!scale.has_value() || (*scale > 0.0 && *scale < 1e30), what, ": scale must be positive and finite, got ",
+                    scale.value_or(0.0));
+}
+
+Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& offsets,
+                        const Optional& k_offsets_in, bool causal, const std::optional<double>& scale) {
+  constexpr const char* what = "packed_attention";
+  TORCH_CHECK_VALUE(q.dim() == 3 && k.dim() == 3 && v.sizes() == k.sizes() && q.size(2) == k.size(2), what,
+                    ": q must be [T, Hq, D], k and v [Tk, Hk, D], got ", q.sizes(), ", ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_TYPE((q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) && k.scalar_type() == q.scalar_type() &&
+                       v.scalar_type() == q.scalar_type(),
+                   what, " expects q, k and v all bf16 or all fp16, got ", q.scalar_type(), ", ", k.scalar_type(), " and ",
+                   v.scalar_type());
+  TORCH_CHECK_VALUE(q.size(2) == 64 || q.size(2) == 128, what, ": head dim ", q.size(2), " not supported (64, 128)");
+  TORCH_CHECK_VALUE(k.size(1) >= 1 && q.size(1) >= 1 && q.size(1) % k.size(1) == 0 && q.size(1) / k.size(1) <= 128, what, ": ",
+                    q.size(1), " query heads do not share ", k.size(1), " key heads in equal groups of up to 128");
+  TORCH_CHECK_VALUE(q.size(0) < (1 << 30) && k.size(0) < (1 << 30) && q.size(1) < (1 << 30), what, ": sizes of 2^30 and more");
+  check_offsets(offsets, "offsets");
+  const bool own_keys = k_offsets_in.has_value();
+  if (own_keys) {
+    check_offsets(*k_offsets_in, "k_offsets");
+    TORCH_CHECK_VALUE(k_offsets_in->sizes() == offsets.sizes() && k_offsets_in->scalar_type() == offsets.scalar_type(),
+                      "k_offsets must have the shape and type of offsets");
+  } else {
+    TORCH_CHECK_VALUE(k.size(0) == q.size(0), what, ": without k_offsets k must have q's rows, got ", k.size(0), " and ",
+                      q.size(0));
+  }
+  check_scale(scale, what);
+  refuse_tangents({q, k, v}, what);
+  PackedCall c = {offsets.contiguous(), Tensor(), causal, scale.value_or(1.0 / std::sqrt((double)q.size(2)))};
+  c.k_offsets = own_keys ? k_offsets_in->contiguous() : c.offsets;
+  device_of({q, k, v, c.offsets, c.k_offsets});
+  if (wants_grad({q, k, v})) {
+    // fp16 holds p (dp - delta) down to 6e-8 only: gradients of long rows would be lost without a sign
+    TORCH_CHECK_NOT_IMPLEMENTED(q.scalar_type() == at::kBFloat16, what, " has gradients in bf16 only");
+    return PackedAttention::apply(q, k, v, c);
+  }
+  return packed_forward(q, k, v, c, false).first;
+}
+
 // ------------------------------------------------------------------ clipping
 // Over lists of contiguous tensors (outs may be grads): the norm, 0-dim fp32.  None where the lists
 // are not of contiguous CUDA tensors of the three types on one device, alike in type and number of
@@ -429,7 +573,7 @@ PYBIND11_MODULE(prism_torch_ops, m) {
     try {
       if (p) std::rethrow_exception(p);
     } catch (const PrismFailure& e) {
-      PyErr_SetString(prism_error ? prism_error : PyExc_RuntimeError, e.what.c_str());
+      PyErr_SetString(prism_error ? prism_error : PyExc_RuntimeError, e.what());
     }
   });
   const auto free = py::call_guard<py::gil_scoped_release>();
@@ -438,4 +582,5 @@ PYBIND11_MODULE(prism_torch_ops, m) {
   m.def("apply_rotary", &apply_rotary, free);
   m.def("linear_fp8", &linear_fp8, free);
   m.def("clip_grad_norm", &clip_grad_norm, free);
+  m.def("packed_attention", &packed_attention, free);
 }
