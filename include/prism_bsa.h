@@ -591,6 +591,45 @@ prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_stride
                                           int k_heads, int D, int causal, float scale, void* workspace,
                                           void* dq, void* dk, void* dv, cudaStream_t stream);
 
+/* A paged cache: keys and values as [pages, page_size, k_heads, D] each (strides {page, place, head} in
+ * elements; columns contiguous), token j of sequence b at place j % page_size of page
+ * page_table[b * table_row + j / page_size] (int32, table_width entries a sequence; entries behind the last
+ * token are not read).  lengths [batch] int32: tokens of each sequence, the new ones among them.
+ *
+ * prism_append_paged: k and v [tokens, k_heads, dim] (strides {token, head}; bf16 or fp16) go to their places,
+ * k rotated, and q [tokens, q_heads, dim] (q_heads = 0: none) rotated to q_out, contiguous.  Sequence b's new
+ * tokens are the rows [offsets[b], offsets[b + 1]) (batch + 1 int32, or int64 with offsets_64), or
+ * tokens / batch rows each with offsets NULL; the last of them is token lengths[b] - 1.  Rotation: the first
+ * rot columns form pairs, (2j, 2j + 1) if interleaved, else (j, j + rot / 2), and pair j, as a complex number,
+ * is multiplied by scale * exp(i p freqs[j]), p the token's number; the other columns are copied.  dim <= 256.  A
+ * token of no sequence, or with a negative number (lengths[b] below its new tokens: an empty slot of a padded
+ * batch), writes nothing and its q_out is 0; one whose page lies outside the table or the cache writes
+ * nothing and its q_out is NaN.  Places must differ: two tokens of one call on one place race.
+ *
+ * prism_paged_attention: q [batch, tokens, q_heads, D] (strides {sequence, token, head}; the last `tokens` of
+ * each sequence; D = 64 or 128) -> o alike, contiguous: query i of sequence b attends the keys
+ * j <= lengths[b] - tokens + i, softmax(scale q k) v, scale > 0; 0 without a key, NaN for a sequence whose
+ * length or one of whose pages is outside the table or the cache.  What lies in the cache behind a sequence's end is
+ * not read.  Rows of the caches start on 16 bytes, of q on 4.  workspace:
+ * prism_paged_attention_workspace_bytes(D).  Both read lengths and the table on the device. */
+prism_status_t prism_append_paged(const void* q, const int64_t* q_strides, int q_heads, const void* k,
+                                  const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                  int k_heads, int64_t tokens, int dim, const void* offsets,
+                                  int offsets_64, int batch, void* k_cache,
+                                  const int64_t* k_cache_strides, void* v_cache,
+                                  const int64_t* v_cache_strides, int pages, int page_size,
+                                  const int* page_table, int64_t table_row, int table_width,
+                                  const int* lengths, int rot, int interleaved, const double* freqs,
+                                  float scale, int dtype, void* q_out, cudaStream_t stream);
+size_t prism_paged_attention_workspace_bytes(int D);
+prism_status_t prism_paged_attention(const void* q, const int64_t* q_strides, int batch, int tokens,
+                                     int q_heads, int k_heads, int D, const void* k_cache,
+                                     const int64_t* k_cache_strides, const void* v_cache,
+                                     const int64_t* v_cache_strides, int pages, int page_size,
+                                     const int* page_table, int64_t table_row, int table_width,
+                                     const int* lengths, float scale, int dtype, void* o,
+                                     void* workspace, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,9 @@ attention package):
   linear_fp8                  projection of 8-bit rows (linear.py)
   apply_rotary, rotary_frequencies   rotary positions (rotary.py)
   clip_grad_norm              global gradient norm and clipping (grad_clip.py)
+Dense attention (the reference leaves it to its framework):
+  packed_attention            sequences of different lengths, with gradients (packed.py)
+  append_paged, paged_attention   a paged cache of keys and values, and attention over it (paged.py)
 The kernels live in libprism_bsa.so (C ABI: include/prism_bsa.h).
 """
 from .bias_rectification import bsa_rectified_sparse_attn, bsa_taylor_sparse_attn  # noqa: F401
@@ -44,6 +47,7 @@ from .linear import linear_fp8  # noqa: F401
 from .norm import add_rms_norm, add_rms_norm_fp8, quantize_rows_fp8  # noqa: F401
 from .ops import token_norms  # noqa: F401
 from .packed import packed_attention  # noqa: F401
+from .paged import append_paged, paged_attention  # noqa: F401
 from .rotary import apply_rotary, rotary_frequencies  # noqa: F401
 
 __version__ = "0.1.0"

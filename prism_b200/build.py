@@ -37,6 +37,7 @@ SOURCES = {
     "rotary_kernels.cu": [],
     "clip_kernels.cu": [],
     "packed_attention.cu": [],
+    "paged_kernels.cu": [],
 }
 
 

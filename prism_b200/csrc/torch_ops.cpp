@@ -527,6 +527,125 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
   return packed_forward(q, k, v, c, false).first;
 }
 
+// ------------------------------------------------------------------ paged cache
+struct PagedCache {
+  std::array<int64_t, 3> k_strides, v_strides;
+  int pages, page_size;
+};
+
+// The caches [pages, page_size, Hk, D] and what addresses them: in place, so nothing here is copied into shape.
+PagedCache check_cache(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths, const char* what) {
+  TORCH_CHECK_VALUE(k.dim() == 4 && v.sizes() == k.sizes() && k.size(1) >= 1 && k.size(2) >= 1, what,
+                    ": the caches must both be [pages, page_size, Hk, D], got ", k.sizes(), " and ", v.sizes());
+  TORCH_CHECK_TYPE((k.scalar_type() == at::kBFloat16 || k.scalar_type() == at::kHalf) && v.scalar_type() == k.scalar_type(),
+                   what, " expects caches both bf16 or both fp16, got ", k.scalar_type(), " and ", v.scalar_type());
+  TORCH_CHECK_VALUE(k.stride(3) == 1 && v.stride(3) == 1, what, ": the caches' columns must be contiguous");
+  TORCH_CHECK_TYPE(table.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt, what,
+                   " expects an int32 page_table and int32 lengths, got ", table.scalar_type(), " and ", lengths.scalar_type());
+  TORCH_CHECK_VALUE(table.dim() == 2 && lengths.dim() == 1 && table.size(0) == lengths.size(0), what,
+                    ": page_table must be [sequences, pages of each], lengths [sequences], got ", table.sizes(), " and ",
+                    lengths.sizes());
+  TORCH_CHECK_VALUE(k.size(0) < (1 << 30) && k.size(1) < (1 << 30) && k.size(2) < (1 << 20) && table.size(0) < (1 << 28) &&
+                        table.size(1) * k.size(1) < (int64_t(1) << 31) - 64,
+                    what, ": too many pages, heads, sequences or keys of a sequence");
+  PagedCache c;
+  for (int d = 0; d < 3; ++d) c.k_strides[d] = k.stride(d), c.v_strides[d] = v.stride(d);
+  c.pages = (int)k.size(0), c.page_size = (int)k.size(1);
+  return c;
+}
+Tensor unit_columns(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// t [B, H, D] (one token a sequence) or [B, n, H, D] as rows [tokens, H, D], or [T, H, D] with offsets.
+Tensor token_rows(const Tensor& t) { return unit_columns(t.dim() == 4 ? t.flatten(0, 1) : t); }
+
+Optional append_paged(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache, const Tensor& v_cache,
+                      const Tensor& table_in, const Tensor& lengths_in, const Optional& offsets_in, const Optional& q_in,
+                      const Optional& freqs_in, const std::string& layout, double scale) {
+  constexpr const char* what = "append_paged";
+  const Tensor q_given = or_undefined(q_in), offsets = or_undefined(offsets_in), freqs = or_undefined(freqs_in);
+  TORCH_CHECK_VALUE(layout == "interleaved" || layout == "half", "layout must be 'interleaved' or 'half', got '", layout, "'");
+  const PagedCache c = check_cache(k_cache, v_cache, table_in, lengths_in, what);
+  const int64_t dims = k_in.dim(), batch = lengths_in.size(0), D = k_cache.size(3);
+  TORCH_CHECK_VALUE((dims == 3 || (dims == 4 && !offsets.defined())) && v_in.sizes() == k_in.sizes() && k_in.size(-1) == D &&
+                        k_in.size(-2) == k_cache.size(2),
+                    what, ": k and v must be [B, Hk, D] or [B, n, Hk, D], or [T, Hk, D] with offsets, of the caches' heads, got ",
+                    k_in.sizes(), " and ", v_in.sizes(), " for caches ", k_cache.sizes());
+  TORCH_CHECK_TYPE(k_in.scalar_type() == k_cache.scalar_type() && v_in.scalar_type() == k_cache.scalar_type(), what,
+                   ": k and v must have the caches' type");
+  TORCH_CHECK_VALUE(D <= 256, what, ": head dims up to 256, got ", D);
+  if (q_given.defined()) {
+    TORCH_CHECK_VALUE(q_given.dim() == dims && q_given.sizes().slice(0, dims - 2) == k_in.sizes().slice(0, dims - 2) &&
+                          q_given.size(-1) == D && q_given.scalar_type() == k_cache.scalar_type(),
+                      what, ": q must have k's tokens, head dim and type, got ", q_given.sizes());
+    TORCH_CHECK_VALUE(q_given.size(-2) < (1 << 20), what, ": too many heads");
+  }
+  if (offsets.defined()) {
+    check_offsets(offsets, "offsets");
+    TORCH_CHECK_VALUE(offsets.size(0) == batch + 1, what, ": offsets must hold one row number more than there are sequences, got ",
+                      offsets.size(0), " for ", batch);
+  } else {
+    TORCH_CHECK_VALUE(k_in.size(0) == batch, what, ": ", k_in.size(0), " sequences of k, ", batch, " of lengths");
+  }
+  if (freqs.defined()) {
+    TORCH_CHECK_TYPE(freqs.scalar_type() == at::kDouble && freqs.dim() == 1, "freqs must be a float64 vector (rotary_frequencies)");
+    TORCH_CHECK_VALUE(2 * freqs.size(0) <= D, freqs.size(0), " pairs do not fit a head of ", D, " columns");
+  }
+  refuse_tangents({k_in, v_in, q_given, k_cache, v_cache, freqs}, what);
+  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({k_in, v_in, q_given, k_cache, v_cache, freqs}), what, " is inference only");
+  const Launch launch(device_of({k_in, v_in, k_cache, v_cache, table_in, lengths_in, offsets, q_given, freqs}));
+  const Tensor k = token_rows(k_in), v = token_rows(v_in), q = q_given.defined() ? token_rows(q_given) : Tensor();
+  const Tensor table = unit_columns(table_in), lengths = lengths_in.contiguous(), at_rows = offsets.defined() ? offsets.contiguous() : offsets;
+  const Tensor f = freqs.defined() ? freqs.contiguous() : freqs;
+  TORCH_CHECK_VALUE(k.size(0) < (1 << 30), what, ": too many tokens");
+  const Tensor out = q.defined() ? new_like(q_given) : Tensor();
+  const auto strides = [](const Tensor& t) { return t.defined() ? t.strides().data() : nullptr; };
+  check(prism_append_paged(at(q), strides(q), q.defined() ? (int)q.size(1) : 0, at(k), strides(k), at(v), strides(v),
+                           (int)k.size(1), k.size(0), (int)D, at(at_rows), at_rows.defined() && at_rows.scalar_type() == at::kLong,
+                           (int)batch, at(k_cache), c.k_strides.data(), at(v_cache), c.v_strides.data(), c.pages, c.page_size,
+                           (const int*)at(table), table.stride(0), (int)table.size(1), (const int*)at(lengths),
+                           f.defined() ? 2 * (int)f.size(0) : 0, layout == "interleaved", (const double*)at(f), (float)scale,
+                           dtype_code(k, what), at(out), launch.stream),
+        "prism_append_paged");
+  for (const Tensor& t : {k_cache, v_cache})
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return out.defined() ? Optional(out) : std::nullopt;
+}
+
+Tensor paged_attention(const Tensor& q_in, const Tensor& k_cache, const Tensor& v_cache, const Tensor& table_in,
+                       const Tensor& lengths_in, const std::optional<double>& scale) {
+  constexpr const char* what = "paged_attention";
+  const PagedCache c = check_cache(k_cache, v_cache, table_in, lengths_in, what);
+  const int64_t D = k_cache.size(3), Hk = k_cache.size(2);
+  TORCH_CHECK_VALUE((q_in.dim() == 3 || q_in.dim() == 4) && q_in.size(0) == lengths_in.size(0) && q_in.size(-1) == D, what,
+                    ": q must be [B, Hq, D] or [B, n, Hq, D] with the sequences of lengths and the caches' head dim, got ",
+                    q_in.sizes());
+  TORCH_CHECK_TYPE(q_in.scalar_type() == k_cache.scalar_type(), what, ": q must have the caches' type, got ", q_in.scalar_type());
+  TORCH_CHECK_VALUE(D == 64 || D == 128, what, ": head dim ", D, " not supported (64, 128)");
+  TORCH_CHECK_VALUE(q_in.size(-2) >= 1 && q_in.size(-2) % Hk == 0, what, ": ", q_in.size(-2), " query heads do not share ", Hk,
+                    " key heads in equal groups");
+  TORCH_CHECK_VALUE(q_in.numel() / D < (1 << 28), what, ": too many rows");
+  check_scale(scale, what);
+  refuse_tangents({q_in, k_cache, v_cache}, what);
+  TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({q_in, k_cache, v_cache}), what, " is inference only");
+  const auto fits = [](const Tensor& t) {
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.stride(0) | t.stride(1) | t.stride(2)) % 8 == 0;
+  };
+  const Launch launch(device_of({q_in, k_cache, v_cache, table_in, lengths_in}));
+  TORCH_CHECK_VALUE(fits(k_cache) && fits(v_cache), what, ": the caches' rows must start on 16 bytes");
+  Tensor q = q_in.dim() == 4 ? q_in : q_in.unsqueeze(1);
+  if (q.stride(3) != 1 || (q.stride(0) | q.stride(1) | q.stride(2)) % 2 != 0 || reinterpret_cast<uintptr_t>(q.data_ptr()) % 4 != 0)
+    q = q.clone(at::MemoryFormat::Contiguous);
+  const Tensor table = unit_columns(table_in), lengths = lengths_in.contiguous(), out = new_like(q_in);
+  const Tensor workspace = at::empty({(int64_t)prism_paged_attention_workspace_bytes((int)D)}, q_in.options().dtype(at::kByte));
+  check(prism_paged_attention(at(q), q.strides().data(), (int)q.size(0), (int)q.size(1), (int)q.size(2), (int)Hk, (int)D,
+                              at(k_cache), c.k_strides.data(), at(v_cache), c.v_strides.data(), c.pages, c.page_size,
+                              (const int*)at(table), table.stride(0), (int)table.size(1), (const int*)at(lengths),
+                              (float)scale.value_or(1.0 / std::sqrt((double)D)), dtype_code(q, what), at(out), at(workspace),
+                              launch.stream),
+        "prism_paged_attention");
+  return out;
+}
+
 // ------------------------------------------------------------------ clipping
 // Over lists of contiguous tensors (outs may be grads): the norm, 0-dim fp32.  None where the lists
 // are not of contiguous CUDA tensors of the three types on one device, alike in type and number of
@@ -583,4 +702,6 @@ PYBIND11_MODULE(prism_torch_ops, m) {
   m.def("linear_fp8", &linear_fp8, free);
   m.def("clip_grad_norm", &clip_grad_norm, free);
   m.def("packed_attention", &packed_attention, free);
+  m.def("append_paged", &append_paged, free);
+  m.def("paged_attention", &paged_attention, free);
 }
