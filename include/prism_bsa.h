@@ -611,7 +611,7 @@ prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_stride
  * j <= lengths[b] - tokens + i, softmax(scale q k) v, scale > 0; 0 without a key, NaN for a sequence whose
  * length or one of whose pages is outside the table or the cache.  What lies in the cache behind a sequence's end is
  * not read.  Rows of the caches start on 16 bytes, of q on 4.  workspace:
- * prism_paged_attention_workspace_bytes(D).  Both read lengths and the table on the device. */
+ * prism_paged_attention_workspace_bytes (NULL where that is 0).  Both read lengths and the table on the device. */
 prism_status_t prism_append_paged(const void* q, const int64_t* q_strides, int q_heads, const void* k,
                                   const int64_t* k_strides, const void* v, const int64_t* v_strides,
                                   int k_heads, int64_t tokens, int dim, const void* offsets,
@@ -621,7 +621,7 @@ prism_status_t prism_append_paged(const void* q, const int64_t* q_strides, int q
                                   const int* page_table, int64_t table_row, int table_width,
                                   const int* lengths, int rot, int interleaved, const double* freqs,
                                   float scale, int dtype, void* q_out, cudaStream_t stream);
-size_t prism_paged_attention_workspace_bytes(int D);
+size_t prism_paged_attention_workspace_bytes(int D, int page_size, int table_width);
 prism_status_t prism_paged_attention(const void* q, const int64_t* q_strides, int batch, int tokens,
                                      int q_heads, int k_heads, int D, const void* k_cache,
                                      const int64_t* k_cache_strides, const void* v_cache,

@@ -74,7 +74,7 @@ SIGNATURES = {
                                         _I, _I, _F, _P, _P, _P, _P, _P]),
     "prism_append_paged": (_I, [_P, _P, _I, _P, _P, _P, _P, _I, _I64, _I, _P, _I, _I, _P, _P, _P, _P, _I, _I, _P, _I64,
                                 _I, _P, _I, _I, _P, _F, _I, _P, _P]),
-    "prism_paged_attention_workspace_bytes": (_SZ, [_I]),
+    "prism_paged_attention_workspace_bytes": (_SZ, [_I, _I, _I]),
     "prism_paged_attention": (_I, [_P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _I, _I, _P, _I64, _I, _P, _F, _I, _P, _P,
                                    _P]),
     "prism_bsa_fwd_qk": (_I, [_P, _P, _P, _I, _I64, _I64, _I, _F, _P, _P, _P, _P, _P, _P]),

@@ -251,9 +251,9 @@ struct Layout {
   static constexpr int kStages = D == 64 ? 6 : 3;      // 96 KB a CTA
   static constexpr int kWarpBytes = 16 * D * 2 * 2;    // 16 keys and values
   static constexpr int kRing = kStages * kWarps * kWarpBytes;
-  static constexpr int kPitch = D + 4;                 // of a row of partial sums, in floats
-  static constexpr int kJoin = 2 * kRows * kPitch * 4;
-  static constexpr int kBytes = kRing + kJoin;
+  static constexpr int kPitch = D + 4;                 // of a row of the warps' sums, in floats
+  static constexpr int kJoin = kWarps * 8 * kPitch * 4, kJoinMl = kWarps * 8 * 8;
+  static constexpr int kBytes = kRing + kJoin + kJoinMl;  // two CTAs an SM
 };
 
 template <typename T>
@@ -270,6 +270,9 @@ struct Mma<__nv_bfloat16> {
     const __nv_bfloat162 p = __floats2bfloat162_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&p);
   }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+  }
 };
 // fp16's p starts at 2^10 (keys down to 2^-34 of the largest count) and may grow to 2^15 before the maximum
 // is raised, as in packed_attention.cu.
@@ -284,6 +287,9 @@ struct Mma<__half> {
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
     const __half2 p = __floats2half2_rn(x, y);
     return *reinterpret_cast<const uint32_t*>(&p);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&u));
   }
 };
 
@@ -404,7 +410,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * L::kWarpBytes;
   constexpr uint32_t kStageBytes = kWarps * L::kWarpBytes;
-  float* join = reinterpret_cast<float*>(smem + L::kRing);
+  float* join = reinterpret_cast<float*>(smem + L::kRing);  // [warp][row of 8]
+  float2* join_ml = reinterpret_cast<float2*>(smem + L::kRing + L::kJoin);
   const int units = s.heads * s.row_tiles;
 
   Cursor at = {0, 0, 0, 0, 0};
@@ -489,16 +496,16 @@ __global__ void __launch_bounds__(kThreads, 2)
   int lim0 = 0, lim1 = 0;  // keys that rows lane / 4 and lane / 4 + 8 see
   bool bad = false;
   const int r0 = lane >> 2, c2 = 2 * (lane & 3);
-  const auto begin = [&] {
-    const int head = at.unit / s.row_tiles, base = (at.unit - head * s.row_tiles) * kRows, all = s.tokens * s.group;
-    const T* q = static_cast<const T*>(s.q) + at.b * s.q_b;
+  const auto load_queries = [&](const Cursor& u) {
+    const int head = u.unit / s.row_tiles, base = (u.unit - head * s.row_tiles) * kRows, all = s.tokens * s.group;
+    const T* q = static_cast<const T*>(s.q) + u.b * s.q_b;
     const T* row[2];
     int lim[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {  // rows behind the last one go along with it
       const int r = min(base + r0 + 8 * i, all - 1), token = r / s.group;
       row[i] = q + token * s.q_t + (head * s.group + (r - token * s.group)) * s.q_h;
-      lim[i] = at.length - s.tokens + token + 1;
+      lim[i] = u.length - s.tokens + token + 1;
     }
     lim0 = lim[0], lim1 = lim[1];
 #pragma unroll
@@ -506,6 +513,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         qf[k][i] = *reinterpret_cast<const uint32_t*>(row[i & 1] + 16 * k + 8 * (i >> 1) + c2);
+  };
+  const auto clear = [&] {
 #pragma unroll
     for (int i = 0; i < D / 8; ++i)
 #pragma unroll
@@ -516,7 +525,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   int piece_tile = at.tile;     // the piece's first tile
   bool at_start = true;         // ... is the share's first
-  begin();
+  load_queries(at);
+  clear();
   int stage = 0;
   for (int64_t step = 0; step < steps; ++step, stage = stage + 1 == kStages ? 0 : stage + 1) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -565,13 +575,15 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int i = 0; i < D / 8; ++i) acc[i][0] *= a0, acc[i][1] *= a0, acc[i][2] *= a1, acc[i][3] *= a1;
       }
       const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
-      uint32_t p[4];
+      uint32_t p[4], p_rest[4];  // p is taken in two 16-bit parts: the products are there for the taking
 #pragma unroll
       for (int nb = 0; nb < 2; ++nb) {
         const float p0 = ex2(fmaf(sc[nb][0], scale, -b0)), p1 = ex2(fmaf(sc[nb][1], scale, -b0));
         const float p2 = ex2(fmaf(sc[nb][2], scale, -b1)), p3 = ex2(fmaf(sc[nb][3], scale, -b1));
         l0 += p0 + p1, l1 += p2 + p3;
-        p[2 * nb] = M::pack(p0, p1), p[2 * nb + 1] = M::pack(p2, p3);  // rounded for the product with V
+        p[2 * nb] = M::pack(p0, p1), p[2 * nb + 1] = M::pack(p2, p3);
+        const float2 h0 = M::unpack(p[2 * nb]), h1 = M::unpack(p[2 * nb + 1]);
+        p_rest[2 * nb] = M::pack(p0 - h0.x, p1 - h0.y), p_rest[2 * nb + 1] = M::pack(p2 - h1.x, p3 - h1.y);
       }
       // O += P V
       {
@@ -582,135 +594,135 @@ __global__ void __launch_bounds__(kThreads, 2)
           ldmatrix_t(b, values + row * (D * 2) + (((2 * n + part) ^ (row & 7)) << 4));
           M::run(acc[2 * n], p, b[0], b[1]);
           M::run(acc[2 * n + 1], p, b[2], b[3]);
+          M::run(acc[2 * n], p_rest, b[0], b[1]);
+          M::run(acc[2 * n + 1], p_rest, b[2], b[3]);
         }
       }
     }
 
     const bool unit_ends = at.tile + 1 == at.tiles;
-    if (unit_ends || step + 1 == steps) {
-      // ---- the four warps' sums, joined in a fixed order
-#pragma unroll
-      for (int off = 1; off <= 2; off <<= 1) {
-        l0 += __shfl_xor_sync(0xffffffffu, l0, off);
-        l1 += __shfl_xor_sync(0xffffffffu, l1, off);
-      }
-      if (bad) l0 = l1 = __int_as_float(0x7fc00000);
-      float2* ml = reinterpret_cast<float2*>(join);
-      if ((lane & 3) == 0) ml[warp * kRows + r0] = make_float2(m0, l0), ml[warp * kRows + r0 + 8] = make_float2(m1, l1);
-      __syncthreads();
-      float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) top[i] = fmaxf(top[i], ml[w * kRows + r0 + 8 * i].x);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float2 x = ml[w * kRows + r0 + 8 * i];
-          sum[i] += x.x == -INFINITY ? x.y : x.y * ex2(x.x - top[i]);
-        }
-      const float f0 = m0 == -INFINITY ? 0.0f : ex2(m0 - top[0]), f1 = m1 == -INFINITY ? 0.0f : ex2(m1 - top[1]);
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) acc[i][0] *= f0, acc[i][1] *= f0, acc[i][2] *= f1, acc[i][3] *= f1;
-      __syncthreads();
-      const auto put = [&](float* to) {
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          *reinterpret_cast<float2*>(to + r0 * L::kPitch + 8 * i + c2) = make_float2(acc[i][0], acc[i][1]);
-          *reinterpret_cast<float2*>(to + (r0 + 8) * L::kPitch + 8 * i + c2) = make_float2(acc[i][2], acc[i][3]);
-        }
-      };
-      const auto add = [&](const float* from) {
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          const float2 a = *reinterpret_cast<const float2*>(from + r0 * L::kPitch + 8 * i + c2);
-          const float2 b = *reinterpret_cast<const float2*>(from + (r0 + 8) * L::kPitch + 8 * i + c2);
-          acc[i][0] += a.x, acc[i][1] += a.y, acc[i][2] += b.x, acc[i][3] += b.y;
-        }
-      };
-      float* const buffer[2] = {join, join + kRows * L::kPitch};
-      if (warp >= 2) put(buffer[warp - 2]);
-      __syncthreads();
-      if (warp < 2) add(buffer[warp]);
-      __syncthreads();
-      if (warp == 1) put(buffer[0]);
-      __syncthreads();
-      if (warp == 0) {
-        add(buffer[0]);
-        const int rows = rows_of(s, at.unit);
-        if (piece_tile == 0 && unit_ends) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int r = r0 + 8 * half;
-            if (r >= rows) continue;
-            const float inv = sum[half] == 0.0f ? 0.0f : 1.0f / sum[half];  // a row without keys
-            T* out = o + out_row(s, at.b, at.unit, r) * D + c2;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-              *reinterpret_cast<uint32_t*>(out + 8 * i) = M::pack(acc[i][2 * half] * inv, acc[i][2 * half + 1] * inv);
-          }
-        } else {
-          const int64_t slot = (int64_t)blockIdx.x * 2 + (at_start ? 0 : 1);
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int r = r0 + 8 * half;
-            if (r >= rows) continue;
-            float* out = part_o + (slot * kRows + r) * D + c2;
-#pragma unroll
-            for (int i = 0; i < D / 8; ++i)
-              *reinterpret_cast<float2*>(out + 8 * i) = make_float2(acc[i][2 * half], acc[i][2 * half + 1]);
-            if ((lane & 3) == 0) part_ml[slot * kRows + r] = make_float2(top[half], sum[half]);
-          }
-        }
-      }
-      __syncthreads();
-      at.next(c, s.batch, units);
-      piece_tile = at.tile, at_start = false;
-      if (step + 1 < steps) begin();
-    } else {
+    if (!unit_ends && step + 1 < steps) {
       ++at.tile;
+      continue;
     }
+    // ---- the end of a piece: the four warps' sums, joined in order, 8 rows at a time
+    const Cursor done = at;
+    at.next(c, s.batch, units);
+    if (step + 1 < steps) load_queries(at);  // on their way meanwhile
+#pragma unroll
+    for (int off = 1; off <= 2; off <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+    }
+    if (bad) l0 = l1 = __int_as_float(0x7fc00000);
+    const int rows = rows_of(s, done.unit);
+    const bool whole = piece_tile == 0 && unit_ends;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (8 * half >= rows) break;
+      __syncthreads();
+      float* to = join + (warp * 8 + r0) * L::kPitch + c2;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+        *reinterpret_cast<float2*>(to + 8 * i) = make_float2(acc[i][2 * half], acc[i][2 * half + 1]);
+      if ((lane & 3) == 0) join_ml[warp * 8 + r0] = half ? make_float2(m1, l1) : make_float2(m0, l0);
+      __syncthreads();
+      for (int i = threadIdx.x; i < min(rows - 8 * half, 8) * (D / 4); i += kThreads) {
+        const int r = i / (D / 4), col = (i - r * (D / 4)) * 4;
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, join_ml[w * 8 + r].x);
+        float4 all = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float2 x = join_ml[w * 8 + r];
+          const float4 v = *reinterpret_cast<const float4*>(join + (w * 8 + r) * L::kPitch + col);
+          const float f = x.x == -INFINITY ? 0.0f : ex2(x.x - top);
+          sum += x.x == -INFINITY ? x.y : x.y * f;  // no key: 0, or NaN for a wrong page
+          all.x = fmaf(v.x, f, all.x), all.y = fmaf(v.y, f, all.y), all.z = fmaf(v.z, f, all.z), all.w = fmaf(v.w, f, all.w);
+        }
+        if (whole) {
+          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row without keys
+          *reinterpret_cast<uint2*>(o + out_row(s, done.b, done.unit, 8 * half + r) * D + col) =
+              make_uint2(M::pack(all.x * inv, all.y * inv), M::pack(all.z * inv, all.w * inv));
+        } else {
+          const int64_t slot = ((int64_t)blockIdx.x * 2 + (at_start ? 0 : 1)) * kRows + 8 * half + r;
+          *reinterpret_cast<float4*>(part_o + slot * D + col) = all;
+          if (col == 0) part_ml[slot] = make_float2(top, sum);
+        }
+      }
+    }
+    piece_tile = at.tile, at_start = false;
+    if (step + 1 < steps) clear();
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // Joins the pieces of a divided unit: o = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c over the shares that
-// hold one, in order.  A CTA takes a unit.
+// hold one, in order.  A CTA takes a row of a unit (one row of 37 pieces each for 8 CTAs took 29 us behind
+// 131,001 keys, where the attention takes 83): the pieces' factors first, a thread a piece, then their sums, D / 4
+// columns of every kGroups-th piece a thread.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads)
     join_kernel(const __grid_constant__ Queries s, const __grid_constant__ Cache c, T* __restrict__ o,
                 const float* __restrict__ part_o, const float2* __restrict__ part_ml) {
+  constexpr int kCols = D / 4, kGroups = kThreads / kCols;
   __shared__ int64_t scratch[kWarps];
-  const int units = s.heads * s.row_tiles, b = blockIdx.x / units, unit = blockIdx.x - b * units;
+  __shared__ float factor[kCtas];
+  __shared__ float of_warps[2][kWarps];
+  __shared__ float4 of_groups[kThreads];
+  const int units = s.heads * s.row_tiles, b = blockIdx.x / units, unit = blockIdx.x - b * units, r = blockIdx.y;
   const int tiles = tiles_of(length_of(c, b));
   const Deal deal(tiles_before(c, s.batch, units, scratch));
   const int64_t first = tiles_before(c, b, units, scratch) + (int64_t)unit * tiles;
   cudaGridDependencySynchronize();  // in every CTA: what follows in the stream waits for the attention too
-  if (tiles == 0) return;
-  const int c0 = deal.owner(first), c1 = deal.owner(first + tiles - 1);
-  if (c0 == c1) return;  // written by that share
-  constexpr int kCols = D / 4;
-  const auto slot = [&](int cta) { return 2 * (int64_t)cta + (cta == c0 && deal.start(c0) != first ? 1 : 0); };
-  for (int i = threadIdx.x; i < rows_of(s, unit) * kCols; i += kThreads) {
-    const int r = i / kCols, col = (i - r * kCols) * 4;
-    float top = -INFINITY;
-#pragma unroll 4
-    for (int cta = c0; cta <= c1; ++cta) top = fmaxf(top, part_ml[slot(cta) * kRows + r].x);
-    float sum = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int cta = c0; cta <= c1; ++cta) {
-      const float2 x = part_ml[slot(cta) * kRows + r];
-      const float4 v = *reinterpret_cast<const float4*>(part_o + (slot(cta) * kRows + r) * D + col);
-      const float f = x.x == -INFINITY ? 0.0f : ex2(x.x - top);
-      sum += x.x == -INFINITY ? x.y : x.y * f;
-      acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
-    }
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    *reinterpret_cast<uint2*>(o + out_row(s, b, unit, r) * D + col) =
-        make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv), Mma<T>::pack(acc.z * inv, acc.w * inv));
+  if (tiles == 0 || r >= rows_of(s, unit)) return;
+  const int c0 = deal.owner(first), pieces = deal.owner(first + tiles - 1) - c0 + 1;
+  if (pieces == 1) return;  // written by that share
+  // the first piece is its share's last one, unless it begins there; the others are their shares' first
+  const bool inside = deal.start(c0) != first;
+  const auto slot = [&](int i) { return ((int64_t)(c0 + i) * 2 + (i == 0 && inside)) * kRows + r; };
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float top = -INFINITY;
+  for (int i = threadIdx.x; i < pieces; i += kThreads) top = fmaxf(top, part_ml[slot(i)].x);
+#pragma unroll
+  for (int off = 16; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  if (lane == 0) of_warps[0][warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) top = fmaxf(top, of_warps[0][w]);
+  float sum = 0.0f;
+  for (int i = threadIdx.x; i < pieces; i += kThreads) {
+    const float2 x = part_ml[slot(i)];
+    const float f = x.x == -INFINITY ? 0.0f : ex2(x.x - top);
+    factor[i] = f;
+    sum += x.x == -INFINITY ? x.y : x.y * f;  // no key: 0, or NaN for a wrong page
   }
+  sum = warp_sum(sum);
+  if (lane == 0) of_warps[1][warp] = sum;
+  __syncthreads();
+  sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) sum += of_warps[1][w];
+  const int col = threadIdx.x % kCols;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int i = threadIdx.x / kCols; i < pieces; i += kGroups) {
+    const float4 v = *reinterpret_cast<const float4*>(part_o + slot(i) * D + col * 4);
+    const float f = factor[i];
+    acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+  }
+  of_groups[threadIdx.x] = acc;
+  __syncthreads();
+  if (threadIdx.x >= kCols) return;
+#pragma unroll
+  for (int g = 1; g < kGroups; ++g) {
+    const float4 v = of_groups[g * kCols + threadIdx.x];
+    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  *reinterpret_cast<uint2*>(o + out_row(s, b, unit, r) * D + col * 4) =
+      make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv), Mma<T>::pack(acc.z * inv, acc.w * inv));
 }
 
 template <typename T, int D>
@@ -731,7 +743,7 @@ static cudaError_t launch_attention(Queries s, const Cache& c, float scale, void
   cudaLaunchAttribute overlap = {};
   overlap.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   overlap.val.programmaticStreamSerializationAllowed = 1;
-  config.gridDim = dim3((unsigned)all), config.blockDim = dim3(kThreads), config.stream = stream;
+  config.gridDim = dim3((unsigned)all, (unsigned)min(kRows, s.tokens * s.group)), config.blockDim = dim3(kThreads), config.stream = stream;
   config.attrs = &overlap, config.numAttrs = 1;
   return cudaLaunchKernelEx(&config, join_kernel<T, D>, (const Queries)s, (const Cache)c, (T*)o, (const float*)part, (const float2*)ml);
 }
@@ -797,8 +809,8 @@ prism_status_t prism_append_paged(const void* q, const int64_t* q_strides, int q
   return PRISM_OK;
 }
 
-size_t prism_paged_attention_workspace_bytes(int D) {
-  if (D < 1) return 0;
+size_t prism_paged_attention_workspace_bytes(int D, int page_size, int table_width) {
+  if (D < 1 || (int64_t)page_size * table_width <= paged::kWhole) return 0;
   return (size_t)2 * paged::kCtas * paged::kRows * (sizeof(float2) + D * sizeof(float));
 }
 
@@ -819,7 +831,7 @@ prism_status_t prism_paged_attention(const void* q, const int64_t* q_strides, in
   const prism_status_t st = paged::check_cache(c, k_cache_strides, v_cache_strides, batch, what);
   if (st != PRISM_OK) return st;
   if ((int64_t)batch * tokens == 0) return PRISM_OK;
-  PRISM_CHECK_ARG(q && q_strides && o && workspace && aligned16(o) && aligned16(workspace), "%s: null pointer, or a buffer off 16 bytes", what);
+  PRISM_CHECK_ARG(q && q_strides && o && (workspace || prism_paged_attention_workspace_bytes(D, page_size, table_width) == 0) && aligned16(o) && aligned16(workspace), "%s: null pointer, or a buffer off 16 bytes", what);
   c.k_page = k_cache_strides[0], c.k_place = k_cache_strides[1], c.k_head = k_cache_strides[2];
   c.v_page = v_cache_strides[0], c.v_place = v_cache_strides[1], c.v_head = v_cache_strides[2];
   PRISM_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache) &&

@@ -636,7 +636,8 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_cache, const Tensor& 
   if (q.stride(3) != 1 || (q.stride(0) | q.stride(1) | q.stride(2)) % 2 != 0 || reinterpret_cast<uintptr_t>(q.data_ptr()) % 4 != 0)
     q = q.clone(at::MemoryFormat::Contiguous);
   const Tensor table = unit_columns(table_in), lengths = lengths_in.contiguous(), out = new_like(q_in);
-  const Tensor workspace = at::empty({(int64_t)prism_paged_attention_workspace_bytes((int)D)}, q_in.options().dtype(at::kByte));
+  const int64_t bytes = (int64_t)prism_paged_attention_workspace_bytes((int)D, c.page_size, (int)table.size(1));
+  const Tensor workspace = bytes > 0 ? at::empty({bytes}, q_in.options().dtype(at::kByte)) : Tensor();
   check(prism_paged_attention(at(q), q.strides().data(), (int)q.size(0), (int)q.size(1), (int)q.size(2), (int)Hk, (int)D,
                               at(k_cache), c.k_strides.data(), at(v_cache), c.v_strides.data(), c.pages, c.page_size,
                               (const int*)at(table), table.stride(0), (int)table.size(1), (const int*)at(lengths),
