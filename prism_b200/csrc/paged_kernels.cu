@@ -25,6 +25,7 @@ struct Cache {
   const int* table;
   int64_t table_row;
   int table_width, page_size, pages;
+  uint32_t page_inverse;      // floor((2^32 - 1) / page_size)
   const int* lengths;
 };
 
@@ -226,8 +227,9 @@ static cudaError_t dispatch_append(const Append& a, const Cache& c, const double
 // are all there is, so the tensor cores are idle most of the time whichever instruction feeds them, and
 // fragments in registers need no trip through TMEM.
 //   * A unit is a sequence, a key head and up to 16 rows (query i, head g), row i G + g.  Its keys come in
-//     tiles of 64, 16 for each of 4 warps; a warp loads its own keys into its own ring with cp.async and
-//     keeps its own running maximum and sum: no barrier in the loop.
+//     tiles of 32 KB, a quarter for each of 4 warps (16 keys of 128 columns, 32 of 64: with 16, a step's fixed
+//     costs held 64 columns at 0.6 of the memory's rate); a warp loads its own keys into its own ring with
+//     cp.async and keeps its own running maximum and sum: no barrier in the loop.
 //   * All tiles of all units, in order, are dealt out in equal shares to a fixed number of CTAs (two an
 //     SM), whatever the lengths are: a share may end inside a unit and hold several.  A unit that lies in
 //     one share is written at once; the pieces of a divided one go to the workspace, two places a CTA, and
@@ -235,7 +237,7 @@ static cudaError_t dispatch_append(const Append& a, const Cache& c, const double
 //   * Where no sequence can have more than kWhole keys (the table's width), a CTA takes one unit and there
 //     is no second launch.
 //   * Keys behind a sequence's end are not read (zero-filled), so what lies there does not matter.
-constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 64, kRows = 16, kCtas = 2 * kSms;
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kRows = 16, kCtas = 2 * kSms;
 constexpr int kWhole = 512;
 
 struct Queries {
@@ -248,8 +250,10 @@ struct Queries {
 
 template <int D>
 struct Layout {
-  static constexpr int kStages = D == 64 ? 6 : 3;      // 96 KB a CTA
-  static constexpr int kWarpBytes = 16 * D * 2 * 2;    // 16 keys and values
+  static constexpr int kStages = 3;                    // 96 KB a CTA
+  static constexpr int kKeys = 2048 / D;               // of a warp's step
+  static constexpr int kTile = kWarps * kKeys;
+  static constexpr int kWarpBytes = kKeys * D * 2 * 2;  // keys and values
   static constexpr int kRing = kStages * kWarps * kWarpBytes;
   static constexpr int kPitch = D + 4;                 // of a row of the warps' sums, in floats
   static constexpr int kJoin = kWarps * 8 * kPitch * 4, kJoinMl = kWarps * 8 * 8;
@@ -314,14 +318,16 @@ __device__ __forceinline__ void ldmatrix_t(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ int length_of(const Cache& c, int b) {
   return min(max(c.lengths[b], 0), c.table_width * c.page_size);
 }
+template <int kTile>
 __device__ __forceinline__ int tiles_of(int length) { return (length + kTile - 1) / kTile; }
 
 // A tile: of sequence b, unit `unit` (key head * row_tiles + row tile) of it.
+template <int kTile>
 struct Cursor {
   int b, unit, tile, tiles, length;
   __device__ __forceinline__ void enter(const Cache& c, int batch) {  // from b on, the next sequence with keys
     for (; b < batch; ++b) {
-      length = length_of(c, b), tiles = tiles_of(length);
+      length = length_of(c, b), tiles = tiles_of<kTile>(length);
       if (tiles > 0) return;
     }
   }
@@ -346,10 +352,57 @@ struct Deal {
   __device__ __forceinline__ int owner(int64_t tile) const { return (int)(((tile + 1) * shares - 1) / total); }
 };
 
+// The share of this CTA: its first tile, and that tile's sequence with the tiles before it.  All threads; up to
+// kThreads sequences take one round, more a second one once the total is known.
+struct Share {
+  int64_t first, steps, before;
+  int b;
+};
+template <int kTile>
+__device__ Share share_of(const Cache& c, int batch, int units, int64_t* scratch) {
+  __shared__ int64_t found_before;
+  __shared__ int found_b;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Share share = {0, 0, 0, 0};
+  int64_t total = 0;
+  for (int pass = batch <= kThreads ? 1 : 0; pass < 2; ++pass) {
+    int64_t base = 0;
+    for (int b0 = 0; b0 < batch; b0 += kThreads) {
+      const int b = b0 + threadIdx.x;
+      const int64_t tiles = b < batch ? (int64_t)tiles_of<kTile>(length_of(c, b)) * units : 0;
+      int64_t sum = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += y;
+      }
+      if (lane == 31) scratch[warp] = sum;
+      __syncthreads();
+      int64_t start = base + sum - tiles;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) start += scratch[w];
+        base += scratch[w];
+      }
+      if (pass == 1) {
+        if (batch <= kThreads) total = base;
+        const Deal deal(total);
+        share.first = deal.start(blockIdx.x), share.steps = deal.start(blockIdx.x + 1) - share.first;
+        if (share.steps > 0 && share.first >= start && share.first < start + tiles) found_b = b, found_before = start;
+      }
+      __syncthreads();
+    }
+    total = base;
+  }
+  if (share.steps > 0) share.b = found_b, share.before = found_before;
+  return share;
+}
+
 // Tiles before sequence b (b = batch: all), summed by the CTA's threads.
+template <int kTile>
 __device__ int64_t tiles_before(const Cache& c, int b, int units, int64_t* scratch) {
   int64_t sum = 0;
-  for (int i = threadIdx.x; i < b; i += kThreads) sum += tiles_of(length_of(c, i));
+  for (int i = threadIdx.x; i < b; i += kThreads) sum += tiles_of<kTile>(length_of(c, i));
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = sum;
@@ -359,32 +412,6 @@ __device__ int64_t tiles_before(const Cache& c, int b, int units, int64_t* scrat
   for (int w = 0; w < kWarps; ++w) sum += scratch[w];
   __syncthreads();
   return sum * units;
-}
-
-// The sequence of tile x, and the tiles before it.
-__device__ void find_sequence(const Cache& c, int batch, int units, int64_t x, int64_t* scratch, int* found, int64_t* before) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t base = 0;
-  for (int b0 = 0; b0 < batch; b0 += kThreads) {
-    const int b = b0 + threadIdx.x;
-    const int64_t tiles = b < batch ? (int64_t)tiles_of(length_of(c, b)) * units : 0;
-    int64_t sum = tiles;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += y;
-    }
-    if (lane == 31) scratch[warp] = sum;
-    __syncthreads();
-    int64_t start = base + sum - tiles;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) start += scratch[w];
-      base += scratch[w];
-    }
-    if (x >= start && x < start + tiles) *found = b, *before = start;
-    __syncthreads();
-  }
 }
 
 // Rows of a unit in o, [batch, tokens, heads * group, D].
@@ -403,10 +430,9 @@ __global__ void __launch_bounds__(kThreads, 2)
   using L = Layout<D>;
   using M = Mma<T>;
   constexpr int kStages = L::kStages;
+  constexpr int kTile = L::kTile, kKeys = L::kKeys;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t scratch[kWarps];
-  __shared__ int64_t found_before;
-  __shared__ int found_b;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * L::kWarpBytes;
   constexpr uint32_t kStageBytes = kWarps * L::kWarpBytes;
@@ -414,11 +440,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   float2* join_ml = reinterpret_cast<float2*>(smem + L::kRing + L::kJoin);
   const int units = s.heads * s.row_tiles;
 
-  Cursor at = {0, 0, 0, 0, 0};
+  Cursor<kTile> at = {0, 0, 0, 0, 0};
   int64_t steps;
   if (s.whole) {
     at.b = blockIdx.x / units, at.unit = blockIdx.x - at.b * units;
-    at.length = length_of(c, at.b), at.tiles = tiles_of(at.length);
+    at.length = length_of(c, at.b), at.tiles = tiles_of<kTile>(at.length);
     steps = at.tiles;
     if (steps == 0) {
       for (int i = threadIdx.x; i < rows_of(s, at.unit) * (D / 8); i += kThreads)
@@ -432,54 +458,54 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (c.lengths[b] <= 0)
         for (int i = threadIdx.x; i < chunks; i += kThreads)
           reinterpret_cast<uint4*>(o + (int64_t)b * chunks * 8)[i] = make_uint4(0, 0, 0, 0);
-    const Deal deal(tiles_before(c, s.batch, units, scratch));
-    const int64_t first = deal.start(blockIdx.x);
-    steps = deal.start(blockIdx.x + 1) - first;
+    const Share share = share_of<kTile>(c, s.batch, units, scratch);
+    steps = share.steps;
     if (steps == 0) return;
-    find_sequence(c, s.batch, units, first, scratch, &found_b, &found_before);
-    at.b = found_b;
-    at.length = length_of(c, at.b), at.tiles = tiles_of(at.length);
-    const int64_t in = first - found_before;
+    at.b = share.b;
+    at.length = length_of(c, at.b), at.tiles = tiles_of<kTile>(at.length);
+    const int64_t in = share.first - share.before;
     at.unit = (int)(in / at.tiles), at.tile = (int)(in - (int64_t)at.unit * at.tiles);
   }
 
-  // ---- loads: `ahead` is the next tile to load, its table entry on its way.  Lane w * 16 + i looks up key i
-  // of the warp's 16, for K (w = 0) and V (w = 1).
-  Cursor ahead = at;
+  // ---- loads: `ahead` is the next tile to load, its table entries on their way.  Lane i looks up key i of the
+  // warp's; rows are addressed in 16-byte units (32 bits of them: 64 GiB a cache).
+  constexpr uint32_t kAbsent = 0xffffffffu;
+  Cursor<kTile> ahead = at;
   int64_t loaded = 0;
   uint32_t bad_stages = 0;  // stages with a page that the cache does not have
-  const int mine = lane & 15;
   int entry = 0, place = 0;
   bool inside = false;
   const auto look_up = [&] {
-    const int key = ahead.tile * kTile + warp * 16 + mine;
+    const int key = ahead.tile * kTile + warp * kKeys + (kKeys == 32 ? lane : lane & 15);
     inside = key < ahead.length;
-    const int e = key / c.page_size;
+    int e = __umulhi((uint32_t)key, c.page_inverse);  // at most 1 below key / page_size
     place = key - e * c.page_size;
+    if (place >= c.page_size) place -= c.page_size, ++e;
     entry = inside ? __ldg(c.table + ahead.b * c.table_row + e) : 0;
   };
   const auto issue = [&](int stage) {
     if (loaded < steps) {
       const bool wrong = inside && (entry < 0 || entry >= c.pages);
       const int head = ahead.unit / s.row_tiles;
-      const char* row = nullptr;
-      if (inside && !wrong)
-        row = lane < 16 ? static_cast<const char*>(c.k) + 2 * (entry * c.k_page + place * c.k_place + head * c.k_head)
-                        : static_cast<const char*>(c.v) + 2 * (entry * c.v_page + place * c.v_place + head * c.v_head);
+      uint32_t k_row = kAbsent, v_row = kAbsent;
+      if (inside && !wrong) {
+        k_row = (uint32_t)((entry * c.k_page + place * c.k_place + head * c.k_head) >> 3);
+        v_row = (uint32_t)((entry * c.v_page + place * c.v_place + head * c.v_head) >> 3);
+      }
       bad_stages = (bad_stages & ~(1u << stage)) | ((uint32_t)(__any_sync(0xffffffffu, wrong) != 0) << stage);
       constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks;  // 16-byte chunks of a row; rows of a warp's load
       const int chunk = lane % kChunks;
       const uint32_t dst = ring + stage * kStageBytes;
+      const char* const k = static_cast<const char*>(c.k) + chunk * 16;
+      const char* const v = static_cast<const char*>(c.v) + chunk * 16;
 #pragma unroll
-      for (int which = 0; which < 2; ++which)
-#pragma unroll
-        for (int r0 = 0; r0 < 16; r0 += kAtOnce) {
-          const int r = r0 + lane / kChunks;
-          const char* p = reinterpret_cast<const char*>(
-              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(row), which * 16 + r));
-          load16(dst + which * (16 * D * 2) + r * (D * 2) + ((chunk ^ (r & 7)) << 4),
-                 p != nullptr ? p + chunk * 16 : static_cast<const char*>(c.k), p != nullptr);
-        }
+      for (int row0 = 0; row0 < kKeys; row0 += kAtOnce) {
+        const int r = row0 + lane / kChunks;
+        const uint32_t to = dst + r * (D * 2) + ((chunk ^ (r & 7)) << 4);
+        const uint32_t kr = __shfl_sync(0xffffffffu, k_row, r), vr = __shfl_sync(0xffffffffu, v_row, r);
+        load16(to, kr != kAbsent ? k + ((uint64_t)kr << 4) : k, kr != kAbsent);
+        load16(to + kKeys * D * 2, vr != kAbsent ? v + ((uint64_t)vr << 4) : v, vr != kAbsent);
+      }
       ++loaded;
       ahead.next(c, s.batch, units);
       if (loaded < steps) look_up();
@@ -496,7 +522,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   int lim0 = 0, lim1 = 0;  // keys that rows lane / 4 and lane / 4 + 8 see
   bool bad = false;
   const int r0 = lane >> 2, c2 = 2 * (lane & 3);
-  const auto load_queries = [&](const Cursor& u) {
+  const auto load_queries = [&](const Cursor<kTile>& u) {
     const int head = u.unit / s.row_tiles, base = (u.unit - head * s.row_tiles) * kRows, all = s.tokens * s.group;
     const T* q = static_cast<const T*>(s.q) + u.b * s.q_b;
     const T* row[2];
@@ -534,24 +560,27 @@ __global__ void __launch_bounds__(kThreads, 2)
     bad |= (bad_stages >> stage) & 1u;
     issue(stage == 0 ? kStages - 1 : stage - 1);  // over the stage of the step before
 
-    const int key0 = at.tile * kTile + warp * 16;
+    const int key0 = at.tile * kTile + warp * kKeys;
     if (key0 < at.length) {
-      const uint32_t keys = ring + stage * kStageBytes, values = keys + 16 * D * 2;
-      // S = Q K^T: two blocks of 8 keys
-      float sc[2][4] = {};
+      constexpr int kBlocks = kKeys / 8;
+      const uint32_t keys = ring + stage * kStageBytes, values = keys + kKeys * D * 2;
+      // S = Q K^T: blocks of 8 keys
+      float sc[kBlocks][4] = {};
       {
         const int row = ((lane >> 4) << 3) + (lane & 7), part = (lane >> 3) & 1;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          uint32_t b[4];
-          ldmatrix(b, keys + row * (D * 2) + (((2 * k + part) ^ (row & 7)) << 4));
-          M::run(sc[0], qf[k], b[0], b[1]);
-          M::run(sc[1], qf[k], b[2], b[3]);
-        }
-      }
-      if (key0 + 16 > at.length - s.tokens + 1) {
+        for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-        for (int nb = 0; nb < 2; ++nb)
+          for (int nb = 0; nb < kBlocks; nb += 2) {
+            uint32_t b[4];
+            ldmatrix(b, keys + (8 * nb + row) * (D * 2) + (((2 * k + part) ^ (row & 7)) << 4));
+            M::run(sc[nb], qf[k], b[0], b[1]);
+            M::run(sc[nb + 1], qf[k], b[2], b[3]);
+          }
+      }
+      if (key0 + kKeys > at.length - s.tokens + 1) {
+#pragma unroll
+        for (int nb = 0; nb < kBlocks; ++nb)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int key = key0 + 8 * nb + c2 + e;
@@ -560,8 +589,11 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
       }
       // the running maximum is raised when a score lies 2^kLag above it
-      float x0 = fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[1][0], sc[1][1])) * scale - M::kShift;
-      float x1 = fmaxf(fmaxf(sc[0][2], sc[0][3]), fmaxf(sc[1][2], sc[1][3])) * scale - M::kShift;
+      float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+      for (int nb = 0; nb < kBlocks; ++nb)
+        x0 = fmaxf(x0, fmaxf(sc[nb][0], sc[nb][1])), x1 = fmaxf(x1, fmaxf(sc[nb][2], sc[nb][3]));
+      x0 = x0 * scale - M::kShift, x1 = x1 * scale - M::kShift;
       if (__any_sync(0xffffffffu, x0 > m0 + M::kLag || x1 > m1 + M::kLag)) {
 #pragma unroll
         for (int off = 1; off <= 2; off <<= 1) {
@@ -575,23 +607,25 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int i = 0; i < D / 8; ++i) acc[i][0] *= a0, acc[i][1] *= a0, acc[i][2] *= a1, acc[i][3] *= a1;
       }
       const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
-      uint32_t p[4], p_rest[4];  // p is taken in two 16-bit parts: the products are there for the taking
 #pragma unroll
-      for (int nb = 0; nb < 2; ++nb) {
-        const float p0 = ex2(fmaf(sc[nb][0], scale, -b0)), p1 = ex2(fmaf(sc[nb][1], scale, -b0));
-        const float p2 = ex2(fmaf(sc[nb][2], scale, -b1)), p3 = ex2(fmaf(sc[nb][3], scale, -b1));
-        l0 += p0 + p1, l1 += p2 + p3;
-        p[2 * nb] = M::pack(p0, p1), p[2 * nb + 1] = M::pack(p2, p3);
-        const float2 h0 = M::unpack(p[2 * nb]), h1 = M::unpack(p[2 * nb + 1]);
-        p_rest[2 * nb] = M::pack(p0 - h0.x, p1 - h0.y), p_rest[2 * nb + 1] = M::pack(p2 - h1.x, p3 - h1.y);
-      }
-      // O += P V
-      {
+      for (int kb = 0; kb < kBlocks; kb += 2) {  // 16 keys of the product with V
+        uint32_t p[4], p_rest[4];  // p is taken in two 16-bit parts: the products are there for the taking
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float(&x)[4] = sc[kb + i];
+          const float p0 = ex2(fmaf(x[0], scale, -b0)), p1 = ex2(fmaf(x[1], scale, -b0));
+          const float p2 = ex2(fmaf(x[2], scale, -b1)), p3 = ex2(fmaf(x[3], scale, -b1));
+          l0 += p0 + p1, l1 += p2 + p3;
+          p[2 * i] = M::pack(p0, p1), p[2 * i + 1] = M::pack(p2, p3);
+          const float2 h0 = M::unpack(p[2 * i]), h1 = M::unpack(p[2 * i + 1]);
+          p_rest[2 * i] = M::pack(p0 - h0.x, p1 - h0.y), p_rest[2 * i + 1] = M::pack(p2 - h1.x, p3 - h1.y);
+        }
+        // O += P V
         const int row = (((lane >> 3) & 1) << 3) + (lane & 7), part = lane >> 4;
 #pragma unroll
         for (int n = 0; n < D / 16; ++n) {
           uint32_t b[4];
-          ldmatrix_t(b, values + row * (D * 2) + (((2 * n + part) ^ (row & 7)) << 4));
+          ldmatrix_t(b, values + (8 * kb + row) * (D * 2) + (((2 * n + part) ^ (row & 7)) << 4));
           M::run(acc[2 * n], p, b[0], b[1]);
           M::run(acc[2 * n + 1], p, b[2], b[3]);
           M::run(acc[2 * n], p_rest, b[0], b[1]);
@@ -606,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       continue;
     }
     // ---- the end of a piece: the four warps' sums, joined in order, 8 rows at a time
-    const Cursor done = at;
+    const Cursor<kTile> done = at;
     at.next(c, s.batch, units);
     if (step + 1 < steps) load_queries(at);  // on their way meanwhile
 #pragma unroll
@@ -671,10 +705,11 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ float factor[kCtas];
   __shared__ float of_warps[2][kWarps];
   __shared__ float4 of_groups[kThreads];
+  constexpr int kTile = Layout<D>::kTile;
   const int units = s.heads * s.row_tiles, b = blockIdx.x / units, unit = blockIdx.x - b * units, r = blockIdx.y;
-  const int tiles = tiles_of(length_of(c, b));
-  const Deal deal(tiles_before(c, s.batch, units, scratch));
-  const int64_t first = tiles_before(c, b, units, scratch) + (int64_t)unit * tiles;
+  const int tiles = tiles_of<kTile>(length_of(c, b));
+  const Deal deal(tiles_before<kTile>(c, s.batch, units, scratch));
+  const int64_t first = tiles_before<kTile>(c, b, units, scratch) + (int64_t)unit * tiles;
   cudaGridDependencySynchronize();  // in every CTA: what follows in the stream waits for the attention too
   if (tiles == 0 || r >= rows_of(s, unit)) return;
   const int c0 = deal.owner(first), pieces = deal.owner(first + tiles - 1) - c0 + 1;
@@ -751,7 +786,7 @@ static cudaError_t launch_attention(Queries s, const Cache& c, float scale, void
 static prism_status_t check_cache(const Cache& c, const int64_t* k_strides, const int64_t* v_strides, int batch,
                                   const char* what) {
   PRISM_CHECK_ARG(c.page_size >= 1 && c.table_width >= 0 && c.pages >= 0 && batch >= 0 &&
-                      (int64_t)c.page_size * c.table_width < ((int64_t)1 << 31) - kTile,
+                      (int64_t)c.page_size * c.table_width < ((int64_t)1 << 31) - 256,
                   "%s: bad sizes (page size at least 1, fewer than 2^31 keys a sequence)", what);
   PRISM_CHECK_ARG(k_strides && v_strides && (batch == 0 || c.lengths) && (batch == 0 || c.table_width == 0 || c.table) &&
                       (c.pages == 0 || (c.k && c.v)),
@@ -828,6 +863,7 @@ prism_status_t prism_paged_attention(const void* q, const int64_t* q_strides, in
   paged::Cache c = {};
   c.k = const_cast<void*>(k_cache), c.v = const_cast<void*>(v_cache), c.table = page_table, c.table_row = table_row;
   c.table_width = table_width, c.page_size = page_size, c.pages = pages, c.lengths = lengths;
+  if (page_size >= 1) c.page_inverse = 0xffffffffu / (uint32_t)page_size;
   const prism_status_t st = paged::check_cache(c, k_cache_strides, v_cache_strides, batch, what);
   if (st != PRISM_OK) return st;
   if ((int64_t)batch * tokens == 0) return PRISM_OK;
@@ -837,6 +873,10 @@ prism_status_t prism_paged_attention(const void* q, const int64_t* q_strides, in
   PRISM_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache) &&
                       ((c.k_page | c.k_place | c.k_head | c.v_page | c.v_place | c.v_head) & 7) == 0,
                   "%s: the caches' rows must start on 16 bytes", what);
+  constexpr int64_t kMost = (int64_t)1 << 35;  // elements: 2^32 units of 16 bytes
+  PRISM_CHECK_ARG((pages - 1) * c.k_page + (page_size - 1) * c.k_place + k_heads * c.k_head < kMost &&
+                      (pages - 1) * c.v_page + (page_size - 1) * c.v_place + k_heads * c.v_head < kMost,
+                  "%s: caches of 64 GiB and more", what);
   PRISM_CHECK_ARG(aligned_to(q, 4) && ((q_strides[0] | q_strides[1] | q_strides[2]) & 1) == 0, "%s: q's rows must start on 4 bytes", what);
   paged::Queries s = {q, q_strides[0], q_strides[1], q_strides[2], batch, tokens, k_heads, q_heads / k_heads, 0, 0};
   s.row_tiles = (int)(((int64_t)tokens * s.group + paged::kRows - 1) / paged::kRows);
