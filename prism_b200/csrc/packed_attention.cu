@@ -23,12 +23,16 @@
 //     a NaN in one sequence stays there, 0 * NaN being NaN.
 //   * Scores in log2 units; fp32 statistics and accumulators; P and dS rounded to the inputs' 16 bits
 //     for the second products, as the matrix instruction takes them.
-//   * A CTA finds its sequence by itself, with a scan of the offsets (no host copy of the lengths, no
-//     plan kernel); a grid has the upper bound of tiles that the row counts allow, and its spare CTAs
-//     clear the rows that no sequence holds.  Offsets that decrease or leave the tensors give NaN.
+//   * The tiles of a grid are its CTAs' work items; a grid has the upper bound of tiles that the row counts
+//     allow, and its spare items clear the rows that no sequence holds.  Offsets that decrease or leave the
+//     tensors give NaN.  The lengths are read on the device only: no host copy, no plan kernel.
+//   * A CTA that is running takes over the items of CTAs that have not started (cluster launch control), so
+//     that barriers and TMEM are set up once an SM, the next item's loads and first scores run under this
+//     one's epilogue, and the hardware's order (long causal tiles first) still balances the SMs.
 //
 // Warp roles (320 threads): warps 0-7 softmax and epilogue (thread i of a warpgroup owns TMEM lane i),
-// warp 8 TMA producer, warp 9 MMA issuer (lane 0 issues; all lanes clear tail rows) and TMEM owner.
+// warp 8 TMA producer, which also takes the items and finds their sequences, warp 9 MMA issuer (lane 0
+// issues; all lanes clear tail rows) and TMEM owner.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -49,11 +53,15 @@ namespace packed {
 using namespace tc;
 
 constexpr int kThreads = 320;
+constexpr int kSoftmaxThreads = 256;
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
+constexpr int kItemReaders = 9;           // the warps other than the producer
 constexpr int kRows = 128;                // of a tile; keys of a step
 constexpr size_t kMinSmem = 116 * 1024;   // one CTA an SM: each allocates all of TMEM
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSms = 148;
+constexpr int kWaves = 6;
 
 // First bounded wait that gave up (prism_device_status).
 __device__ int g_error = 0;
@@ -183,24 +191,232 @@ __device__ void find_place(const Sequences& s, int my, int per, int pair_tokens,
   __syncthreads();
 }
 
-// A CTA without a tile: clears its share of the rows that no sequence holds (kSpare), or fills its share of
-// all rows with NaN (kBad).  Rows of `out` are [heads, width] elements; the CTA has those of key head h:
+// An item without a tile: clears its share of the rows that no sequence holds (kSpare), or fills its share of
+// all rows with NaN (kBad).  Rows of `out` are [heads, width] elements; the item has those of key head h:
 // `width` elements from h * width on.
 template <typename T>
-__device__ void fill_rows(const Place& place, const void* offsets, const Sequences& s, int rows, int my, int per,
-                          T* out, int heads, int h, int width) {
-  const bool bad = place.kind == kBad;
+__device__ void fill_rows(int kind, int share, const void* offsets, const Sequences& s, int rows, int per, T* out,
+                          int heads, int h, int width) {
+  const bool bad = kind == kBad;
   const int head = bad ? 0 : (int)row_at(offsets, s.wide, 0), tail = bad ? 0 : (int)row_at(offsets, s.wide, s.count);
   const int count = bad ? rows : head + rows - tail;
-  const int64_t first = (int64_t)(bad ? my : place.tile) * per;
+  const int64_t first = (int64_t)share * per;
   const int64_t end = first + per < count ? first + per : count;
   const uint32_t word = bad ? Half<T>::pack(__uint_as_float(0x7fc00000u), __uint_as_float(0x7fc00000u)) : 0u;
   const int chunks = width / 8;
-  for (int64_t i = first * chunks + threadIdx.x; i < end * chunks; i += blockDim.x) {
+  for (int64_t i = first * chunks + threadIdx.x; i < end * chunks; i += kSoftmaxThreads) {
     const int64_t u = i / chunks;
     const int64_t row = u < head ? u : tail + (u - head);
     *reinterpret_cast<uint4*>(out + (row * heads + h) * width + (i - u * chunks) * 8) = make_uint4(word, word, word, word);
   }
+}
+
+// The same for the (maximum, sum) of a part's rows.
+__device__ __forceinline__ void fill_parts(int kind, int share, const Sequences& s, int per, float2* ml, const Heads& hd, int h) {
+  const bool bad = kind == kBad;
+  const int head = bad ? 0 : (int)row_at(s.q, s.wide, 0), tail = bad ? 0 : (int)row_at(s.q, s.wide, s.count);
+  const int count = bad ? s.q_rows : head + s.q_rows - tail;
+  const int64_t first = (int64_t)share * per, end = first + per < count ? first + per : count;
+  for (int64_t i = first * hd.group + threadIdx.x; i < end * hd.group; i += kSoftmaxThreads) {
+    const int64_t u = i / hd.group, row = u < head ? u : tail + (u - head);
+    ml[(row * hd.keys + h) * hd.group + (i - u * hd.group)] = make_float2(-INFINITY, bad ? __uint_as_float(0x7fc00000u) : 0.0f);
+  }
+}
+
+// ------------------------------------------------------------------ items
+struct Item {
+  int kind;
+  int q0, nq, k0, nk;   // the sequence's rows
+  int tile;             // within the sequence; kSpare, kBad: the share of the rows to fill
+  int pairs;            // pairs of query tiles of the sequences before
+  int index, h, part;   // the tile's number in the grid, the key head, the part of its steps
+};
+
+// What the scan of all offsets finds: whether they are in order, and the tiles and pairs of query tiles.
+struct Survey {
+  int good, tiles, pairs;
+};
+template <bool kKeys>
+__device__ Survey survey(const Sequences& s, int pair_tokens, int* scratch) {
+  int tiles = 0, pairs = 0;
+  bool good = true;
+  for (int b = threadIdx.x; b < s.count; b += kThreads) {
+    const int64_t qa = row_at(s.q, s.wide, b), qb = row_at(s.q, s.wide, b + 1);
+    const int64_t ka = row_at(s.k, s.wide, b), kb = row_at(s.k, s.wide, b + 1);
+    if (0 <= qa && qa <= qb && qb <= s.q_rows && 0 <= ka && ka <= kb && kb <= s.k_rows) {
+      const int p = ((int)(qb - qa) + pair_tokens - 1) / pair_tokens;
+      pairs += p, tiles += kKeys ? ((int)(kb - ka) + kRows - 1) / kRows : p;
+    } else {
+      good = false;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    pairs += __shfl_xor_sync(0xffffffffu, pairs, o);
+  }
+  if ((threadIdx.x & 31) == 0) scratch[2 * (threadIdx.x >> 5)] = tiles, scratch[2 * (threadIdx.x >> 5) + 1] = pairs;
+  Survey all = {__syncthreads_and(good), 0, 0};
+  for (int w = 0; w < kThreads / 32; ++w) all.tiles += scratch[2 * w], all.pairs += scratch[2 * w + 1];
+  return all;
+}
+
+// A warp's way through the sequences, 32 at a time; items come in order, so that it goes through them once.
+template <bool kKeys>
+struct Walker {
+  int chunk, base, tiles, pairs_base, pairs;  // the 32 sequences, tiles before and in them
+  int q0, nq, k0, nk, start, count, pairs_start;  // this lane's sequence
+  __device__ __forceinline__ void load(const Sequences& s, int pair_tokens, int lane) {
+    const int b = chunk * 32 + lane;
+    q0 = nq = k0 = nk = 0;
+    if (b < s.count) {
+      q0 = (int)row_at(s.q, s.wide, b), nq = (int)row_at(s.q, s.wide, b + 1) - q0;
+      k0 = (int)row_at(s.k, s.wide, b), nk = (int)row_at(s.k, s.wide, b + 1) - k0;
+    }
+    const int p = (nq + pair_tokens - 1) / pair_tokens;
+    count = kKeys ? (nk + kRows - 1) / kRows : p;
+    int x = count, y = p;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int xo = __shfl_up_sync(0xffffffffu, x, o), yo = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) x += xo, y += yo;
+    }
+    start = x - count, pairs_start = y - p;  // within the 32
+    tiles = __shfl_sync(0xffffffffu, x, 31), pairs = __shfl_sync(0xffffffffu, y, 31);
+  }
+  __device__ __forceinline__ void begin(const Sequences& s, int pair_tokens, int lane, const Survey& all, int my) {
+    const bool back = my > all.tiles / 2;
+    chunk = back ? (s.count - 1) / 32 : 0;
+    load(s, pair_tokens, lane);
+    base = back ? all.tiles - tiles : 0, pairs_base = back ? all.pairs - pairs : 0;
+  }
+  // tile `my` of good sequences' tiles
+  __device__ __forceinline__ void find(const Sequences& s, int pair_tokens, int lane, int my, Item& item) {
+    while (my < base) {
+      --chunk;
+      load(s, pair_tokens, lane);
+      base -= tiles, pairs_base -= pairs;
+    }
+    while (my >= base + tiles) {
+      ++chunk, base += tiles, pairs_base += pairs;
+      load(s, pair_tokens, lane);
+    }
+    const int in = my - base;
+    const int at = __ffs(__ballot_sync(0xffffffffu, in >= start && in < start + count)) - 1;
+    const auto of = [&](int v) { return __shfl_sync(0xffffffffu, v, at); };
+    item.q0 = of(q0), item.nq = of(nq), item.k0 = of(k0), item.nk = of(nk);
+    item.tile = in - of(start), item.pairs = pairs_base + of(pairs_start);
+  }
+};
+
+// Asks for an item of a CTA that has not started: 16 bytes to `response`, completing on `bar`.
+__device__ __forceinline__ void request_item(uint32_t response, uint32_t bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(response),
+               "r"(bar)
+               : "memory");
+}
+// The block index of the CTA that will not start, or -1: none is left.
+__device__ __forceinline__ int requested_item(uint32_t response) {
+  uint32_t got, index;
+  asm volatile(
+      "{\n .reg .pred p;\n .reg .b128 r;\n"
+      " ld.shared.b128 r, [%2];\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n"
+      " selp.u32 %0, 1, 0, p;\n mov.u32 %1, 0;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n}\n"
+      : "=r"(got), "=r"(index)
+      : "r"(response)
+      : "memory");
+  return got ? (int)index : -1;
+}
+
+// Shared memory of the items, at a 16-byte boundary: two of them in turn, each with a barrier that it is
+// there and one that all readers have it.
+struct ItemRing {
+  static constexpr int RESPONSE = 0, FULL = 16, EMPTY = FULL + 16, ANSWER = EMPTY + 16, ITEMS = ANSWER + 16;
+  static constexpr int kBytes = ITEMS + 2 * (int)sizeof(Item);
+  __device__ static void init(uint32_t at) {
+    for (int i = 0; i < 2; ++i) mbar_init(at + FULL + 8 * i, 1), mbar_init(at + EMPTY + 8 * i, kItemReaders);
+    mbar_init(at + ANSWER, 1);
+  }
+};
+
+enum : int { kStop = 3 };  // an Item's kind: no more
+
+// How a grid's items follow from the block index: parts of a tile next to each other, then key heads, then
+// tiles, the last ones first where `backwards`.
+struct Grid {
+  int tiles, parts, backwards;
+};
+
+// The producer warp's side.  The next item is asked for when the last load of an item is issued, and not
+// before: an item taken early is one that an idle SM does not get (nine causal sequences of up to 4,093
+// tokens, 1,200 items: 312 us forward with each item asked for at the start of the one before, 256 so).
+template <bool kKeys>
+struct ItemSource {
+  const Sequences& s;
+  const Heads& hd;
+  const Grid& grid;
+  const Survey& all;
+  uint8_t* sm_ring;
+  uint32_t ring;
+  volatile int* abort_flag;
+  int lane, code;
+  Walker<kKeys> walker;
+  bool begun = false;
+  int n = 0;  // items so far
+
+  // The next item, given to the other warps too; false: none, or a wait gave up.
+  __device__ __forceinline__ bool next(Item& item) {
+    int block = blockIdx.x;
+    if (n > 0) {
+      if (lane == 0) request_item(ring + ItemRing::RESPONSE, ring + ItemRing::ANSWER);
+      __syncwarp();
+      if (!wait_warp(ring + ItemRing::ANSWER, (n - 1) & 1, abort_flag, code)) return false;
+      block = requested_item(ring + ItemRing::RESPONSE);
+      fence_proxy_async_smem();  // read, before the next answer is written over it
+      __syncwarp();
+    }
+    item.kind = kStop;
+    if (block >= 0) {
+      const int of_head = block / grid.parts, rank = of_head / hd.keys;
+      item.part = block - of_head * grid.parts, item.h = of_head - rank * hd.keys;
+      const int my = grid.backwards ? grid.tiles - 1 - rank : rank;
+      item.index = my;
+      item.kind = !all.good ? kBad : my >= all.tiles ? kSpare : kTile;
+      item.tile = item.kind == kSpare ? my - all.tiles : my;
+      if (item.kind == kTile) {
+        if (!begun) walker.begin(s, 2 * hd.tokens, lane, all, my);
+        begun = true;
+        walker.find(s, 2 * hd.tokens, lane, my, item);
+      }
+    }
+    const int slot = n & 1;
+    if (n >= 2 && !wait_warp(ring + ItemRing::EMPTY + 8 * slot, ((n >> 1) - 1) & 1, abort_flag, code)) return false;
+    if (lane == 0) {
+      *reinterpret_cast<Item*>(sm_ring + ItemRing::ITEMS + slot * sizeof(Item)) = item;
+      mbar_arrive(ring + ItemRing::FULL + 8 * slot);
+    }
+    __syncwarp();
+    ++n;
+    return item.kind != kStop;
+  }
+};
+
+__device__ __forceinline__ bool item_ready(int n, uint32_t ring) {
+  return mbar_try(ring + ItemRing::FULL + 8 * (n & 1), (n >> 1) & 1);
+}
+// The next item, for a warp; false: the wait gave up, or there is none.
+__device__ __forceinline__ bool next_item(Item& item, int& n, const uint8_t* sm_ring, uint32_t ring,
+                                          volatile int* abort_flag, int lane, int code) {
+  const int slot = n & 1;
+  if (!wait_warp(ring + ItemRing::FULL + 8 * slot, (n >> 1) & 1, abort_flag, code)) return false;
+  item = *reinterpret_cast<const Item*>(sm_ring + ItemRing::ITEMS + slot * sizeof(Item));
+  __syncwarp();
+  if (lane == 0) mbar_arrive(ring + ItemRing::EMPTY + 8 * slot);
+  ++n;
+  return item.kind != kStop;
 }
 
 // Rows [from, 128) of a tile's sub-buffers set to zero, by a group of threads; the caller fences and
@@ -243,8 +459,9 @@ __device__ __forceinline__ float exp_pairs(const float (&s)[64], float scale, fl
 }
 
 // ===================================================================== forward
-// CTA: two tiles of 128 rows (groups 0 and 1) of one key head, which share the stream of K and V steps, so
-// that the tensor core works on one group's products while the other group's softmax runs.
+// An item: two tiles of 128 rows (groups 0 and 1) of one key head, which share the stream of K and V steps, so
+// that the tensor core works on one group's products while the other group's softmax runs.  Where there are
+// few tiles and long keys, an item is a part of the steps, and join_kernel adds the parts up.
 template <int D>
 struct FwdLayout {
   static constexpr int kRing = 2;
@@ -253,27 +470,56 @@ struct FwdLayout {
   static constexpr int Q = 0;
   static constexpr int K = Q + 2 * kTileBytes;
   static constexpr int V = K + kRing * kTileBytes;
-  static constexpr int BAR = V + kRing * kTileBytes;
-  static constexpr int B_Q = 0, B_KF = 1, B_KE = B_KF + kRing, B_VF = B_KE + kRing, B_VE = B_VF + kRing,
-                       B_SF = B_VE + kRing,  // [g]: S of the group
-                       B_PF = B_SF + 2,      // [g]: P in TMEM (and O rescaled)
-                       B_OF = B_PF + 2,      // [g]: last P V done
-                       B_DRAIN = B_OF + 2, NBAR = B_DRAIN + 1;
+  static constexpr int ITEMS = V + kRing * kTileBytes;
+  static constexpr int BAR = ITEMS + (ItemRing::kBytes + 15) / 16 * 16;
+  static constexpr int B_QF = 0, B_QE = 2,    // [g]: Q of the group; its last S done
+                       B_KF = 4, B_KE = B_KF + kRing, B_VF = B_KE + kRing, B_VE = B_VF + kRing,
+                       B_SF = B_VE + kRing,   // [g]: S of the group
+                       B_PF = B_SF + 2,       // [g]: P in TMEM (and O rescaled)
+                       B_OF = B_PF + 2,       // [g]: last P V of an item done
+                       B_OE = B_OF + 2,       // [g]: O read
+                       B_DRAIN = B_OE + 2, NBAR = B_DRAIN + 1;
   static constexpr int TMEM_SLOT = BAR + NBAR * 8;
   static constexpr int ABORT = TMEM_SLOT + 4;
-  static constexpr int PLACE = ABORT + 4;
-  static constexpr int SCRATCH = PLACE + (int)sizeof(Place);
+  static constexpr int SCRATCH = ABORT + 4;
   static constexpr size_t kNeed = 1024 + SCRATCH + 2 * 4 * (kThreads / 32);
   static constexpr size_t kBytes = kNeed > kMinSmem ? kNeed : kMinSmem;
   // TMEM of group g at 256 g: S (128 fp32 columns; P as pairs over the first 64), O
   static constexpr int T_S = 0, T_O = 128;
 };
 
+// The steps of an item: groups' last tokens, the part's first step and each group's number of them.
+struct FwdSteps {
+  int tok0, shift, last[2], from, n[2], total;
+  __device__ __forceinline__ FwdSteps(const Item& at, int n_tok, int causal, int parts) {
+    tok0 = at.tile * 2 * n_tok, shift = at.nk - at.nq;
+    int all[2];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      last[g] = min(tok0 + (g + 1) * n_tok, at.nq) - 1;
+      const int keys = tok0 + g * n_tok >= at.nq ? 0 : causal ? min(max(last[g] + shift + 1, 0), at.nk) : at.nk;
+      all[g] = (keys + kRows - 1) / kRows;
+    }
+    const int most = max(all[0], all[1]);
+    from = (int)((int64_t)most * at.part / parts);
+    const int end = (int)((int64_t)most * (at.part + 1) / parts);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) n[g] = max(0, min(end, all[g]) - from);
+    total = max(n[0], n[1]);
+  }
+};
+
+// What the parts of a row leave: sums [part][row][head][D] and (maximum, sum) [part][row][head].
+struct Parts {
+  float* o;
+  float2* ml;
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Sequences seqs, Heads hd, int causal,
-               float qk_scale, T* __restrict__ o, float* __restrict__ lse) {
+               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Sequences seqs, Heads hd, Grid grid,
+               int causal, float qk_scale, T* __restrict__ o, float* __restrict__ lse, Parts parts) {
   using L = FwdLayout<D>;
   using H = Half<T>;
   constexpr int R = L::kRing;
@@ -281,22 +527,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sm = align1024(smem_raw);
   const uint32_t sb = smem_u32(sm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // a causal sequence's last tiles have the most keys: they go first
-  const int pair = hd.pairs - 1 - (int)(blockIdx.x / hd.keys), h = blockIdx.x % hd.keys;
   const int n_tok = hd.tokens, rows = n_tok * hd.group;
   auto bar = [&](int i) { return sb + L::BAR + 8 * i; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::ABORT);
-
-  Place* shared_place = reinterpret_cast<Place*>(sm + L::PLACE);
-  find_place<false>(seqs, pair, 2 * n_tok, 2 * n_tok, shared_place, reinterpret_cast<int*>(sm + L::SCRATCH));
-  const Place at = *shared_place;
-  if (at.kind != kTile) {
-    fill_rows(at, seqs.q, seqs, seqs.q_rows, pair, 2 * n_tok, o, hd.keys, h, hd.group * D);
-    return;
-  }
+  const uint32_t ring = sb + L::ITEMS;
 
   if (threadIdx.x == 0) {
-    mbar_init(bar(L::B_Q), 1);
+    ItemRing::init(ring);
     for (int i = 0; i < R; ++i) {
       mbar_init(bar(L::B_KF + i), 1);
       mbar_init(bar(L::B_KE + i), 1);
@@ -304,9 +541,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(L::B_VE + i), 1);
     }
     for (int g = 0; g < 2; ++g) {
+      mbar_init(bar(L::B_QF + g), 1);
+      mbar_init(bar(L::B_QE + g), 1);
       mbar_init(bar(L::B_SF + g), 1);
       mbar_init(bar(L::B_PF + g), 4);
       mbar_init(bar(L::B_OF + g), 1);
+      mbar_init(bar(L::B_OE + g), 4);
     }
     mbar_init(bar(L::B_DRAIN), 1);
     *abort_flag = 0;
@@ -322,123 +562,181 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
     tc_fence_before();
   }
+  const Survey all = survey<false>(seqs, 2 * n_tok, reinterpret_cast<int*>(sm + L::SCRATCH));
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + L::TMEM_SLOT);
 
-  const int tok0 = at.tile * 2 * n_tok, shift = at.nk - at.nq;
-  // keys and steps of each group, up to its last token's
-  int last[2], steps[2];
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    last[g] = min(tok0 + (g + 1) * n_tok, at.nq) - 1;
-    const int keys = tok0 + g * n_tok >= at.nq ? 0 : causal ? min(max(last[g] + shift + 1, 0), at.nk) : at.nk;
-    steps[g] = (keys + kRows - 1) / kRows;
-  }
-  const int total = max(steps[0], steps[1]);
-
+  Item at;
+  int items = 0;
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------ producer
-    if (lane == 0 && total > 0) {
-      const int live = steps[1] > 0 ? 2 : 1;
-      mbar_expect_tx(bar(L::B_Q), live * rows * D * 2);
-      for (int g = 0; g < live; ++g)
+    int nk = 0, nv = 0, nq[2] = {0, 0};
+    bool ok = true;
+    ItemSource<false> source = {seqs, hd, grid, all, sm + L::ITEMS, ring, abort_flag, lane, kErrFwdProducer};
+    while (ok && source.next(at)) {
+      if (at.kind != kTile) continue;
+      const FwdSteps w(at, n_tok, causal, grid.parts);
+      if (lane == 0) {
 #pragma unroll
-        for (int s = 0; s < L::kSub; ++s)
-          tma_load_3d(sb + L::Q + g * L::kTileBytes + s * 16384, &tm_q, s * 64, h * hd.group,
-                      at.q0 + tok0 + g * n_tok, bar(L::B_Q));
-      int nk = 0, nv = 0;
-      for (int n = 0; n < total; ++n) {
-        const int st = n % R, key = at.k0 + n * kRows;
-        if (n >= R && !wait_one(bar(L::B_KE + st), ((n / R) - 1) & 1, abort_flag, kErrFwdProducer)) break;
-        mbar_expect_tx(bar(L::B_KF + st), L::kTileBytes);
+        for (int g = 0; g < 2; ++g) {
+          if (!ok || w.n[g] == 0) continue;
+          ok = nq[g] == 0 || wait_one(bar(L::B_QE + g), (nq[g] - 1) & 1, abort_flag, kErrFwdProducer);
+          if (!ok) continue;
+          mbar_expect_tx(bar(L::B_QF + g), rows * D * 2);
 #pragma unroll
-        for (int s = 0; s < L::kSub; ++s)
-          tma_load_3d(sb + L::K + st * L::kTileBytes + s * 16384, &tm_k, s * 64, h, key, bar(L::B_KF + st));
-        ++nk;
-        if (n >= R && !wait_one(bar(L::B_VE + st), ((n / R) - 1) & 1, abort_flag, kErrFwdProducer)) break;
-        mbar_expect_tx(bar(L::B_VF + st), L::kTileBytes);
+          for (int s = 0; s < L::kSub; ++s)
+            tma_load_3d(sb + L::Q + g * L::kTileBytes + s * 16384, &tm_q, s * 64, at.h * hd.group,
+                        at.q0 + w.tok0 + g * n_tok, bar(L::B_QF + g));
+          ++nq[g];
+        }
+        for (int n = 0; ok && n < w.total; ++n) {
+          const int key = at.k0 + (w.from + n) * kRows;
+          ok = nk < R || wait_one(bar(L::B_KE + nk % R), ((nk / R) - 1) & 1, abort_flag, kErrFwdProducer);
+          if (!ok) break;
+          mbar_expect_tx(bar(L::B_KF + nk % R), L::kTileBytes);
 #pragma unroll
-        for (int s = 0; s < L::kSub; ++s)
-          tma_load_3d(sb + L::V + st * L::kTileBytes + s * 16384, &tm_v, s * 64, h, key, bar(L::B_VF + st));
-        ++nv;
+          for (int s = 0; s < L::kSub; ++s)
+            tma_load_3d(sb + L::K + (nk % R) * L::kTileBytes + s * 16384, &tm_k, s * 64, at.h, key, bar(L::B_KF + nk % R));
+          ++nk;
+          ok = nv < R || wait_one(bar(L::B_VE + nv % R), ((nv / R) - 1) & 1, abort_flag, kErrFwdProducer);
+          if (!ok) break;
+          mbar_expect_tx(bar(L::B_VF + nv % R), L::kTileBytes);
+#pragma unroll
+          for (int s = 0; s < L::kSub; ++s)
+            tma_load_3d(sb + L::V + (nv % R) * L::kTileBytes + s * 16384, &tm_v, s * 64, at.h, key, bar(L::B_VF + nv % R));
+          ++nv;
+        }
       }
-      // every load has landed before the CTA may leave
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+    if (lane == 0) {  // every load has landed before the CTA may leave
       for (int m = max(nk - R, 0); m < nk; ++m) wait_one(bar(L::B_KF + m % R), (m / R) & 1, abort_flag, kErrFwdProducer);
       for (int m = max(nv - R, 0); m < nv; ++m) wait_one(bar(L::B_VF + m % R), (m / R) & 1, abort_flag, kErrFwdProducer);
-      wait_one(bar(L::B_Q), 0, abort_flag, kErrFwdProducer);
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        if (nq[g] > 0) wait_one(bar(L::B_QF + g), (nq[g] - 1) & 1, abort_flag, kErrFwdProducer);
     }
+    __syncwarp();
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------- MMA issuer
-    // Step n, for the groups that take part: P V of the group's step n - 1, then S of step n over the
-    // columns that held that P (one thread's products run in issue order).
+    // Steps of all items in one stream, by lane 0: every instruction between a P and its products is time that
+    // the tensor core idles (32,768 causal tokens took 8.9 ms with votes of the warp in each wait, 8.4 without
+    // and 8.2 with inner()).  Step n, group by group: P V of the group's step before it, then S of step n over the columns that
+    // held that P (one thread's products run in issue order).
     constexpr uint32_t kIdS = idesc<T>(kRows, false), kIdO = idesc<T>(D, true);
     const uint64_t dQ = desc_k_sw128(sb + L::Q), dK = desc_k_sw128(sb + L::K), dV = desc_mn_sw128(sb + L::V, 16384);
     constexpr uint32_t kSlot = L::kTileBytes >> 4;
-    const auto pv = [&](int g, int j) -> bool {
-      if (!wait_warp(bar(L::B_PF + g), j & 1, abort_flag, kErrFwdMma)) return false;
-      tc_fence_after();
-      if (lane == 0) {
-        const uint64_t b = dV + (j % R) * kSlot;
-        const uint32_t t = tmem + g * 256;
-        mma_ts_k64_mn(t + L::T_O, t + L::T_S, b, kIdO, j > 0 ? 1u : 0u);
-        mma_ts_k64_mn(t + L::T_O, t + L::T_S + 32, b + (8192 >> 4), kIdO, 1u);
-      }
-      __syncwarp();
-      return true;
-    };
-    // V of step j is there, its rows behind the sequence zero
-    const auto v_ready = [&](int j) -> bool {
-      if (!wait_warp(bar(L::B_VF + j % R), (j / R) & 1, abort_flag, kErrFwdMma)) return false;
-      if ((j + 1) * kRows > at.nk) {
-        zero_rows<L::kSub>(sm + L::V + (j % R) * L::kTileBytes, at.nk - j * kRows, lane, 32);
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      return true;
-    };
-    bool ok = total == 0 || wait_warp(bar(L::B_Q), 0, abort_flag, kErrFwdMma);
-    tc_fence_after();
-    for (int n = 0; ok && n <= total && total > 0; ++n) {
-      const int st = n % R;
-      if ((n < total && !wait_warp(bar(L::B_KF + st), (n / R) & 1, abort_flag, kErrFwdMma)) ||
-          (n > 0 && !v_ready(n - 1))) {
-        ok = false;
-        break;
+    int ns = 0, v_rows = 0;                        // steps so far; keys of the last one, 0: its P V is issued
+    int n_s[2] = {0, 0}, n_q[2] = {0, 0}, n_o[2] = {0, 0};
+    bool waiting[2] = {false, false}, first[2] = {}, last[2] = {};  // P V of the last step still to come
+    const auto wait = [&](int i, int parity) { return wait_one(bar(i), parity & 1, abort_flag, kErrFwdMma); };
+    const auto pv = [&](int g) -> bool {
+      const int before = (ns - 1) % R;
+      const uint32_t t = tmem + g * 256;
+      if (!wait(L::B_PF + g, n_s[g] - 1)) return false;
+      if (first[g]) {  // over the O of an earlier item
+        if (n_o[g] > 0 && !wait(L::B_OE + g, n_o[g] - 1)) return false;
+        ++n_o[g];
       }
       tc_fence_after();
+      const uint64_t b = dV + before * kSlot;
+      mma_ts_k64_mn(t + L::T_O, t + L::T_S, b, kIdO, first[g] ? 0u : 1u);
+      mma_ts_k64_mn(t + L::T_O, t + L::T_S + 32, b + (8192 >> 4), kIdO, 1u);
+      if (last[g]) mma_commit(bar(L::B_OF + g));
+      waiting[g] = false;
+      return true;
+    };
+    const auto step = [&](int n, int n0, int n1) -> bool {
+      const int st = ns % R, before = (ns - 1) % R;
+      const bool any = waiting[0] || waiting[1];
+      if (!wait(L::B_KF + st, ns / R) || (any && !wait(L::B_VF + before, (ns - 1) / R))) return false;
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        if (n >= steps[g]) continue;
-        if (n > 0 && !pv(g, n - 1)) {
-          ok = false;
-          break;
+        const int of_group = g ? n1 : n0;
+        if (waiting[g] && !pv(g)) return false;
+        if (n >= of_group) continue;
+        first[g] = n == 0, last[g] = n + 1 == of_group;
+        if (first[g]) {
+          if (!wait(L::B_QF + g, n_q[g])) return false;
+          tc_fence_after();
         }
-        if (lane == 0) {
-          mma_kd<L::kSub, 16384, 16384>(tmem + g * 256 + L::T_S, dQ + g * kSlot, dK + st * kSlot, kIdS, 0u);
-          mma_commit(bar(L::B_SF + g));
-        }
-        __syncwarp();
+        mma_kd<L::kSub, 16384, 16384>(tmem + g * 256 + L::T_S, dQ + g * kSlot, dK + st * kSlot, kIdS, 0u);
+        mma_commit(bar(L::B_SF + g));
+        if (last[g]) mma_commit(bar(L::B_QE + g)), ++n_q[g];
+        ++n_s[g];
+        waiting[g] = true;
       }
-      if (!ok) break;
-      // a group's last P V, after the products that need not wait for it
+      mma_commit(bar(L::B_KE + st));
+      if (any) mma_commit(bar(L::B_VE + before));
+      ++ns;
+      return true;
+    };
+    // a step that is neither the first two nor the last one of either group: the same, without the cases
+    const auto inner = [&]() -> bool {
+      const int st = ns % R, before = (ns - 1) % R;
+      if (!wait(L::B_KF + st, ns / R) || !wait(L::B_VF + before, (ns - 1) / R)) return false;
 #pragma unroll
-      for (int g = 0; g < 2; ++g)
-        if (n > 0 && n == steps[g]) {
-          if (!pv(g, n - 1)) {
-            ok = false;
-            break;
-          }
-          if (lane == 0) mma_commit(bar(L::B_OF + g));
-          __syncwarp();
-        }
-      if (!ok) break;
-      if (lane == 0) {
-        if (n < total) mma_commit(bar(L::B_KE + st));
-        if (n > 0) mma_commit(bar(L::B_VE + (n - 1) % R));
+      for (int g = 0; g < 2; ++g) {
+        const uint32_t t = tmem + g * 256;
+        if (!wait(L::B_PF + g, n_s[g] - 1)) return false;
+        tc_fence_after();
+        const uint64_t b = dV + before * kSlot;
+        mma_ts_k64_mn(t + L::T_O, t + L::T_S, b, kIdO, 1u);
+        mma_ts_k64_mn(t + L::T_O, t + L::T_S + 32, b + (8192 >> 4), kIdO, 1u);
+        mma_kd<L::kSub, 16384, 16384>(t + L::T_S, dQ + g * kSlot, dK + st * kSlot, kIdS, 0u);
+        mma_commit(bar(L::B_SF + g));
+        ++n_s[g];
       }
+      mma_commit(bar(L::B_KE + st));
+      mma_commit(bar(L::B_VE + before));
+      ++ns;
+      return true;
+    };
+    // all lanes: the last step's V is there, its rows behind the sequence zero
+    const auto clear_tail = [&]() -> bool {
+      if (v_rows == 0 || v_rows == kRows) return true;
+      const int before = (ns - 1) % R;
+      if (!wait_warp(bar(L::B_VF + before), ((ns - 1) / R) & 1, abort_flag, kErrFwdMma)) return false;
+      zero_rows<L::kSub>(sm + L::V + before * L::kTileBytes, v_rows, lane, 32);
+      fence_proxy_async_smem();
       __syncwarp();
+      return true;
+    };
+    const auto flush = [&]() -> bool {
+      bool ok = clear_tail();
+      if (lane == 0 && ok && v_rows > 0) {
+        const int before = (ns - 1) % R;
+        ok = wait(L::B_VF + before, (ns - 1) / R);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) ok = ok && (!waiting[g] || pv(g));
+        if (ok) mma_commit(bar(L::B_VE + before));
+      }
+      v_rows = 0;
+      return __all_sync(0xffffffffu, ok);
+    };
+    bool ok = true;
+    while (ok) {
+      // an item that is not there yet is not waited for with products to issue
+      if (v_rows > 0 && !__any_sync(0xffffffffu, item_ready(items, ring))) ok = flush();
+      if (!ok || !next_item(at, items, sm + L::ITEMS, ring, abort_flag, lane, kErrFwdMma)) break;
+      if (at.kind != kTile) continue;
+      const FwdSteps w(at, n_tok, causal, grid.parts);
+      if (w.total == 0) continue;
+      ok = clear_tail();
+      const int both = min(w.n[0], w.n[1]);
+      if (lane == 0) {
+        for (int n = 0; ok && n < w.total; ++n) {
+          ok = step(n, w.n[0], w.n[1]);
+          if (n == 1)
+            for (; ok && n + 2 < both; ++n) ok = inner();
+        }
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      if (lane != 0) ns += w.total;
+      v_rows = min(at.nk - (w.from + w.total - 1) * kRows, kRows);
     }
+    if (ok) flush();
     // every product is done before TMEM is released
     if (lane == 0) {
       mma_commit(bar(L::B_DRAIN));
@@ -449,147 +747,183 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------ softmax warps
     const int g = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the tile == TMEM lane
-    const uint32_t inverse = group_inverse(hd.group);
-    const int tok = tok0 + g * n_tok + over_group(r, inverse);
-    const bool valid = r < rows && tok < at.nq;
-    // keys that this row sees; rows without a token go along with the last one
-    const int seen = causal ? min(max(min(tok, last[g]) + shift + 1, 0), at.nk) : at.nk;
+    const int t_of_row = over_group(r, group_inverse(hd.group)), head_of_row = r - t_of_row * hd.group;
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * 256;
-    float m = -INFINITY, l = 1.0f;
+    const int heads = hd.keys * hd.group;
+    int n_s = 0, n_o = 0;
     bool ok = true;
-    for (int n = 0; n < steps[g]; ++n) {
-      // keys of the two halves of the step that the row sees; all / none of them for every row of the warp
-      const int lim0 = seen - n * kRows, lim1 = lim0 - 64;
-      const bool all0 = __all_sync(0xffffffffu, lim0 >= 64), all1 = __all_sync(0xffffffffu, lim1 >= 64);
-      const bool none0 = __all_sync(0xffffffffu, lim0 <= 0), none1 = __all_sync(0xffffffffu, lim1 <= 0);
-      if (!wait_warp(bar(L::B_SF + g), n & 1, abort_flag, kErrFwdSoftmax)) {
-        ok = false;
-        break;
+    while (ok && next_item(at, items, sm + L::ITEMS, ring, abort_flag, lane, kErrFwdSoftmax)) {
+      if (at.kind != kTile) {
+        if (grid.parts == 1) {
+          fill_rows(at.kind, at.tile, seqs.q, seqs, seqs.q_rows, 2 * n_tok, o, hd.keys, at.h, hd.group * D);
+        } else {  // rows without a key in this part, or NaN
+          fill_parts(at.kind, at.tile, seqs, 2 * n_tok, parts.ml + (int64_t)at.part * seqs.q_rows * heads, hd, at.h);
+        }
+        continue;
       }
-      tc_fence_after();
-      const auto scores = [&](int u, float(&s)[64]) {
-        tmem_load<2>(t_lane + L::T_S + u * 64, s);
-        if (!(u ? all1 : all0)) mask_from(s, u ? lim1 : lim0);
-      };
-      float sum0 = 0.f, sum1 = 0.f;
-      // Exponentials against the running maximum in one pass over S.  A row's first step, and a first half
-      // whose exponentials sum past kSum, take two passes (maximum, then exponentials; S is intact).  If only
-      // the second half passes the limit, P of the first half, l and O are scaled to the new maximum.
-      bool two_pass = __any_sync(0xffffffffu, m == -INFINITY);
-      uint32_t pk0[32];
-      if (!two_pass) {
-        if (none0) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) pk0[i] = 0u;
-        } else {
-          float s[64];
-          scores(0, s);
-          sum0 = exp_pairs<T>(s, qk_scale, m, pk0);
+      const FwdSteps w(at, n_tok, causal, grid.parts);
+      const int n_steps = g ? w.n[1] : w.n[0], last = g ? w.last[1] : w.last[0];
+      const int tok = w.tok0 + g * n_tok + t_of_row;
+      const bool valid = r < rows && tok < at.nq;
+      // keys that this row sees; rows without a token go along with the last one
+      const int seen = causal ? min(max(min(tok, last) + w.shift + 1, 0), at.nk) : at.nk;
+      float m = -INFINITY, l = 1.0f;
+      for (int n = 0; n < n_steps; ++n) {
+        // keys of the two halves of the step that the row sees; all / none of them for every row of the warp
+        const int lim0 = seen - (w.from + n) * kRows, lim1 = lim0 - 64;
+        const bool all0 = __all_sync(0xffffffffu, lim0 >= 64), all1 = __all_sync(0xffffffffu, lim1 >= 64);
+        const bool none0 = __all_sync(0xffffffffu, lim0 <= 0), none1 = __all_sync(0xffffffffu, lim1 <= 0);
+        if (!wait_warp(bar(L::B_SF + g), n_s & 1, abort_flag, kErrFwdSoftmax)) {
+          ok = false;
+          break;
         }
-        two_pass = __any_sync(0xffffffffu, !(sum0 <= H::kSum));
-      }
-      if (two_pass) {
-        sum0 = 0.f;
-        float mx = -INFINITY;
+        ++n_s;
+        tc_fence_after();
+        const auto scores = [&](int u, float(&s)[64]) {
+          tmem_load<2>(t_lane + L::T_S + u * 64, s);
+          if (!(u ? all1 : all0)) mask_from(s, u ? lim1 : lim0);
+        };
+        float sum0 = 0.f, sum1 = 0.f;
+        // Exponentials against the running maximum in one pass over S.  A row's first step, and a first half
+        // whose exponentials sum past kSum, take two passes (maximum, then exponentials; S is intact).  If only
+        // the second half passes the limit, P of the first half, l and O are scaled to the new maximum.
+        bool two_pass = __any_sync(0xffffffffu, m == -INFINITY);
+        uint32_t pk0[32];
+        if (!two_pass) {
+          if (none0) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (u ? none1 : none0) continue;
-          float s[64];
-          scores(u, s);
-          mx = fmaxf(mx, tile_max(s));
-        }
-        mx = mx * qk_scale - H::kShift;
-        const bool need = mx > m + H::kLag;  // m = -inf: any key
-        if (__any_sync(0xffffffffu, need)) {
-          const float m_new = need ? mx : m;
-          const float alpha = need ? ex2(m - m_new) : 1.0f;  // m = -inf -> 0
-          const bool o_live = __any_sync(0xffffffffu, need && m != -INFINITY);
-          l *= alpha;
-          m = m_new;
-          // every earlier P V of the group is done: S was issued after them
-          if (n > 0 && o_live) scale_tmem_rows<D / 32>(t_lane + L::T_O, alpha);
-        }
-        const float mb = (m == -INFINITY) ? 0.0f : m;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t pk[32];
-          if (u ? none1 : none0) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) pk[i] = 0u;
+            for (int i = 0; i < 32; ++i) pk0[i] = 0u;
           } else {
             float s[64];
-            scores(u, s);
-            const float t = exp_pairs<T>(s, qk_scale, mb, pk);
-            if (u) sum1 = t; else sum0 = t;
+            scores(0, s);
+            sum0 = exp_pairs<T>(s, qk_scale, m, pk0);
           }
-          tmem_st32(t_lane + L::T_S + u * 32, pk);  // over scores of the first half, which are read
+          two_pass = __any_sync(0xffffffffu, !(sum0 <= H::kSum));
         }
-      } else {
-        tmem_st32(t_lane + L::T_S, pk0);
-        uint32_t pk1[32];
-        if (none1) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) pk1[i] = 0u;
-        } else {
-          float s[64];
-          scores(1, s);
-          sum1 = exp_pairs<T>(s, qk_scale, m, pk1);
-        }
-        const bool need = !(sum1 <= H::kSum);
-        if (__any_sync(0xffffffffu, need)) {  // rare
-          float s[64];
-          scores(1, s);
-          const float m_new = need ? fmaxf(m, tile_max(s) * qk_scale - H::kShift) : m;
-          const float alpha = ex2(m - m_new);
-          if (n > 0) scale_tmem_rows<D / 32>(t_lane + L::T_O, alpha);
-          tmem_wait_st();
-          uint32_t raw[32];
-          tmem_ld32(t_lane + L::T_S, raw);
-          tmem_wait_ld_dep(raw);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float2 p = H::unpack(raw[i]);
-            raw[i] = H::pack(p.x * alpha, p.y * alpha);
-          }
-          tmem_st32(t_lane + L::T_S, raw);
-          l = (l + sum0) * alpha;
+        if (two_pass) {
           sum0 = 0.f;
-          m = m_new;
-          sum1 = exp_pairs<T>(s, qk_scale, m, pk1);
+          float mx = -INFINITY;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            if (u ? none1 : none0) continue;
+            float s[64];
+            scores(u, s);
+            mx = fmaxf(mx, tile_max(s));
+          }
+          mx = mx * qk_scale - H::kShift;
+          const bool need = mx > m + H::kLag;  // m = -inf: any key
+          if (__any_sync(0xffffffffu, need)) {
+            const float m_new = need ? mx : m;
+            const float alpha = need ? ex2(m - m_new) : 1.0f;  // m = -inf -> 0
+            const bool o_live = __any_sync(0xffffffffu, need && m != -INFINITY);
+            l *= alpha;
+            m = m_new;
+            // every earlier P V of the group is done: S was issued after them
+            if (n > 0 && o_live) scale_tmem_rows<D / 32>(t_lane + L::T_O, alpha);
+          }
+          const float mb = (m == -INFINITY) ? 0.0f : m;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            uint32_t pk[32];
+            if (u ? none1 : none0) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) pk[i] = 0u;
+            } else {
+              float s[64];
+              scores(u, s);
+              const float t = exp_pairs<T>(s, qk_scale, mb, pk);
+              if (u) sum1 = t; else sum0 = t;
+            }
+            tmem_st32(t_lane + L::T_S + u * 32, pk);  // over scores of the first half, which are read
+          }
+        } else {
+          tmem_st32(t_lane + L::T_S, pk0);
+          uint32_t pk1[32];
+          if (none1) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) pk1[i] = 0u;
+          } else {
+            float s[64];
+            scores(1, s);
+            sum1 = exp_pairs<T>(s, qk_scale, m, pk1);
+          }
+          const bool need = !(sum1 <= H::kSum);
+          if (__any_sync(0xffffffffu, need)) {  // rare
+            float s[64];
+            scores(1, s);
+            const float m_new = need ? fmaxf(m, tile_max(s) * qk_scale - H::kShift) : m;
+            const float alpha = ex2(m - m_new);
+            if (n > 0) scale_tmem_rows<D / 32>(t_lane + L::T_O, alpha);
+            tmem_wait_st();
+            uint32_t raw[32];
+            tmem_ld32(t_lane + L::T_S, raw);
+            tmem_wait_ld_dep(raw);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float2 p = H::unpack(raw[i]);
+              raw[i] = H::pack(p.x * alpha, p.y * alpha);
+            }
+            tmem_st32(t_lane + L::T_S, raw);
+            l = (l + sum0) * alpha;
+            sum0 = 0.f;
+            m = m_new;
+            sum1 = exp_pairs<T>(s, qk_scale, m, pk1);
+          }
+          tmem_st32(t_lane + L::T_S + 32, pk1);
         }
-        tmem_st32(t_lane + L::T_S + 32, pk1);
+        l += sum0 + sum1;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::B_PF + g));
       }
-      l += sum0 + sum1;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(L::B_PF + g));
-    }
-    // epilogue
-    const bool empty = m == -INFINITY;  // no key
-    if (ok && lse != nullptr)
-      lse[(((int64_t)h * hd.pairs + pair) * 2 + g) * kRows + r] = valid && !empty ? m + __log2f(l) : INFINITY;
-    T* row = o + ((int64_t)(at.q0 + tok) * hd.keys * hd.group + h * hd.group + (r - (tok - tok0 - g * n_tok) * hd.group)) * D;
-    if (ok && steps[g] > 0 && wait_warp(bar(L::B_OF + g), 0, abort_flag, kErrFwdSoftmax)) {
-      tc_fence_after();
-      const float inv = 1.0f / l;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t raw[32], pk[16];
-        tmem_ld32(t_lane + L::T_O + c * 32, raw);
-        tmem_wait_ld_dep(raw);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) pk[i] = empty ? 0u : H::pack(u2f(raw[2 * i]) * inv, u2f(raw[2 * i + 1]) * inv);
-        if (valid) {
-          uint4* dst = reinterpret_cast<uint4*>(row + c * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+      if (!ok) break;
+      // epilogue
+      const bool empty = m == -INFINITY;  // no key
+      const int64_t out_row = (int64_t)(at.q0 + tok) * heads + at.h * hd.group + head_of_row;
+      if (lse != nullptr)
+        lse[(((int64_t)at.h * hd.pairs + at.index) * 2 + g) * kRows + r] = valid && !empty ? m + __log2f(l) : INFINITY;
+      if (grid.parts > 1 && valid)
+        parts.ml[(int64_t)at.part * seqs.q_rows * heads + out_row] = make_float2(m, empty ? 0.0f : l);
+      if (n_steps > 0) {
+        if (!wait_warp(bar(L::B_OF + g), n_o & 1, abort_flag, kErrFwdSoftmax)) {
+          ok = false;
+          break;
         }
-      }
-    } else if (ok && steps[g] == 0 && valid) {
-      uint4* dst = reinterpret_cast<uint4*>(row);
+        ++n_o;
+        tc_fence_after();
+        const float inv = 1.0f / l;
 #pragma unroll
-      for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t raw[32];
+          tmem_ld32(t_lane + L::T_O + c * 32, raw);
+          tmem_wait_ld_dep(raw);
+          if (grid.parts > 1) {
+            float4* dst = reinterpret_cast<float4*>(parts.o + ((int64_t)at.part * seqs.q_rows * heads + out_row) * D + c * 32);
+            if (valid) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                dst[i] = make_float4(u2f(raw[4 * i]), u2f(raw[4 * i + 1]), u2f(raw[4 * i + 2]), u2f(raw[4 * i + 3]));
+            }
+            continue;
+          }
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pk[i] = empty ? 0u : H::pack(u2f(raw[2 * i]) * inv, u2f(raw[2 * i + 1]) * inv);
+          if (valid) {
+            uint4* dst = reinterpret_cast<uint4*>(o + out_row * D + c * 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::B_OE + g));
+      } else if (grid.parts == 1 && valid) {
+        uint4* dst = reinterpret_cast<uint4*>(o + out_row * D);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+      }
     }
   }
   tc_fence_before();
@@ -598,6 +932,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+}
+
+// o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over a row's parts, in order; D / 4 threads a row.  Bound by
+// memory.
+constexpr int kJoinThreads = 256;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(Parts parts, int count, int64_t rows, T* __restrict__ o) {
+  const int64_t i = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x, row = i / (D / 4);
+  const int col = (int)(i - row * (D / 4)) * 4;
+  if (row >= rows) return;
+  float top = -INFINITY;
+#pragma unroll 4
+  for (int p = 0; p < count; ++p) top = fmaxf(top, parts.ml[p * rows + row].x);
+  float sum = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int p = 0; p < count; ++p) {
+    const float2 x = parts.ml[p * rows + row];
+    if (x.x == -INFINITY) {  // no key; its sums were not written
+      sum += x.y;            // 0, or NaN for wrong offsets
+      continue;
+    }
+    const float f = ex2(x.x - top);
+    const float4 v = *reinterpret_cast<const float4*>(parts.o + (p * rows + row) * D + col);
+    sum = fmaf(x.y, f, sum);
+    acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+  }
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  *reinterpret_cast<uint2*>(o + row * D + col) =
+      make_uint2(Half<T>::pack(acc.x * inv, acc.y * inv), Half<T>::pack(acc.z * inv, acc.w * inv));
 }
 
 // ===================================================================== delta
@@ -758,8 +1123,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   find_place<true>(seqs, my, kRows, 2 * n_tok, shared_place, reinterpret_cast<int*>(sm + L::SCRATCH));
   const Place at = *shared_place;
   if (at.kind != kTile) {
-    fill_rows(at, seqs.k, seqs, seqs.k_rows, my, kRows, dk, hd.keys, h, D);
-    fill_rows(at, seqs.k, seqs, seqs.k_rows, my, kRows, dv, hd.keys, h, D);
+    if (threadIdx.x < kSoftmaxThreads) {
+      const int share = at.kind == kBad ? my : at.tile;
+      fill_rows(at.kind, share, seqs.k, seqs, seqs.k_rows, kRows, dk, hd.keys, h, D);
+      fill_rows(at.kind, share, seqs.k, seqs, seqs.k_rows, kRows, dv, hd.keys, h, D);
+    }
     return;
   }
 
@@ -896,7 +1264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       wait_one(bar(L::B_DRAIN), 0, abort_flag, kErrDkdvMma);
     }
     __syncwarp();
-  } else {
+  } else if (warp < kProducerWarp) {
     // softmax warpgroup w: columns [64 w, 64 w + 64) of each tile
     const int wg = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;  // key row of the epilogue == TMEM lane
@@ -1018,7 +1386,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   find_place<false>(seqs, pair, 2 * n_tok, 2 * n_tok, shared_place, reinterpret_cast<int*>(sm + L::SCRATCH));
   const Place at = *shared_place;
   if (at.kind != kTile) {
-    if (half == 0) fill_rows(at, seqs.q, seqs, seqs.q_rows, pair, 2 * n_tok, dq, hd.keys, h, hd.group * D);
+    if (half == 0 && threadIdx.x < kSoftmaxThreads)
+      fill_rows(at.kind, at.kind == kBad ? pair : at.tile, seqs.q, seqs, seqs.q_rows, 2 * n_tok, dq, hd.keys, h, hd.group * D);
     return;
   }
   const int tok0 = (at.tile * 2 + half) * n_tok, shift = at.nk - at.nq;
@@ -1151,7 +1520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       wait_one(bar(L::B_DRAIN), 0, abort_flag, kErrDqMma);
     }
     __syncwarp();
-  } else {
+  } else if (warp < kProducerWarp) {
     // softmax warpgroup w: keys [64 w, 64 w + 64) of each step
     const int wg = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the tile == TMEM lane
@@ -1318,6 +1687,16 @@ struct Shape {
     return {k_heads, group, kRows / group, (int)pair_bound(q_rows, count, group)};
   }
   int64_t key_tiles() const { return (k_rows + kRows - 1) / kRows + count; }
+  // Parts of the forward's steps: as many as give every SM kWaves items, while a part has four steps of an
+  // average sequence.
+  int parts() const {
+    const int64_t items = pair_bound(q_rows, count, q_heads / k_heads) * k_heads;
+    const int64_t steps = count > 0 ? k_rows / count / kRows : 0;
+    const int64_t want = (kWaves * kSms + items - 1) / (items > 0 ? items : 1);
+    const int64_t most = steps / 4 < 16 ? steps / 4 : 16;
+    const int64_t n = want < most ? want : most;
+    return n > 1 ? (int)n : 1;
+  }
 };
 
 static prism_status_t check(const Shape& s, const char* what) {
@@ -1359,7 +1738,7 @@ struct Input {
 
 template <typename T, int D>
 static prism_status_t launch_fwd(const Shape& s, const Input& q, const Input& k, const Input& v, void* o, float* lse,
-                                 cudaStream_t stream) {
+                                 void* workspace, cudaStream_t stream) {
   constexpr const char* what = "prism_packed_attention";
   const Heads hd = s.heads();
   PRISM_TRY(bind_context(what));
@@ -1375,9 +1754,18 @@ static prism_status_t launch_fwd(const Shape& s, const Input& q, const Input& k,
   constexpr size_t bytes = FwdLayout<D>::kBytes;
   static_assert(bytes <= 227 * 1024, "shared memory");
   PRISM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
-  kernel<<<(unsigned)(hd.pairs * hd.keys), kThreads, bytes, stream>>>(mq, mk, mv, s.sequences(), hd, s.causal,
-                                                                      s.scale * kLog2e, (T*)o, lse);
+  const Grid grid = {hd.pairs, lse != nullptr ? 1 : s.parts(), s.causal};
+  const int64_t rows = s.q_rows * s.q_heads;
+  Parts parts = {nullptr, nullptr};
+  if (grid.parts > 1) parts.o = static_cast<float*>(workspace), parts.ml = reinterpret_cast<float2*>(parts.o + grid.parts * rows * D);
+  kernel<<<(unsigned)(hd.pairs * hd.keys * grid.parts), kThreads, bytes, stream>>>(
+      mq, mk, mv, s.sequences(), hd, grid, s.causal, s.scale * kLog2e, (T*)o, lse, parts);
   PRISM_CHECK_LAUNCH(what);
+  if (grid.parts > 1) {
+    join_kernel<T, D><<<(unsigned)((rows * (D / 4) + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, stream>>>(
+        parts, grid.parts, rows, (T*)o);
+    PRISM_CHECK_LAUNCH(what);
+  }
   return PRISM_OK;
 }
 
@@ -1440,17 +1828,27 @@ size_t prism_packed_attention_stats_bytes(int64_t q_rows, int64_t count, int q_h
   return (size_t)packed::pair_bound(q_rows, count, q_heads / k_heads) * 2 * packed::kRows * k_heads * sizeof(float);
 }
 
+size_t prism_packed_attention_workspace_bytes(int64_t q_rows, int64_t k_rows, int64_t count, int q_heads, int k_heads,
+                                              int D) {
+  if (q_rows < 0 || k_rows < 0 || count < 0 || D < 1 || k_heads < 1 || q_heads < k_heads || q_heads / k_heads > packed::kRows)
+    return 0;
+  const packed::Shape s = {nullptr, nullptr, 0, count, q_rows, k_rows, q_heads, k_heads, D, 0, PRISM_BF16, 1.0f};
+  const int parts = s.parts();
+  return parts == 1 ? 0 : (size_t)parts * q_rows * q_heads * (D * sizeof(float) + sizeof(float2));
+}
+
 prism_status_t prism_packed_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                       const void* v, const int64_t* v_strides, const void* q_offsets,
                                       const void* k_offsets, int offsets_64, int64_t count, int64_t q_rows,
                                       int64_t k_rows, int q_heads, int k_heads, int D, int causal, float scale,
-                                      int dtype, void* o, float* lse, cudaStream_t stream) {
+                                      int dtype, void* o, float* lse, void* workspace, cudaStream_t stream) {
   constexpr const char* what = "prism_packed_attention";
   const packed::Shape s = {q_offsets, k_offsets, offsets_64, count, q_rows, k_rows,
                            q_heads,   k_heads,   D,          causal != 0, dtype, scale};
   PRISM_TRY(packed::check(s, what));
   if (q_rows == 0) return PRISM_OK;
   PRISM_CHECK_ARG(q_offsets && k_offsets && o && aligned16(o) && (!lse || aligned16(lse)), "%s: null pointer, or an output off 16 bytes", what);
+  PRISM_CHECK_ARG(lse || s.parts() == 1 || (workspace && aligned16(workspace)), "%s: no workspace", what);
   PRISM_TRY(packed::check_rows(q, q_strides, what, "q"));
   if (k_rows > 0) {
     PRISM_TRY(packed::check_rows(k, k_strides, what, "k"));
@@ -1458,10 +1856,10 @@ prism_status_t prism_packed_attention(const void* q, const int64_t* q_strides, c
   }
   const packed::Input iq = {q, q_strides}, ik = {k, k_strides}, iv = {v, v_strides};
   if (dtype == PRISM_FP16)
-    return D == 64 ? packed::launch_fwd<__half, 64>(s, iq, ik, iv, o, lse, stream)
-                   : packed::launch_fwd<__half, 128>(s, iq, ik, iv, o, lse, stream);
-  return D == 64 ? packed::launch_fwd<__nv_bfloat16, 64>(s, iq, ik, iv, o, lse, stream)
-                 : packed::launch_fwd<__nv_bfloat16, 128>(s, iq, ik, iv, o, lse, stream);
+    return D == 64 ? packed::launch_fwd<__half, 64>(s, iq, ik, iv, o, lse, workspace, stream)
+                   : packed::launch_fwd<__half, 128>(s, iq, ik, iv, o, lse, workspace, stream);
+  return D == 64 ? packed::launch_fwd<__nv_bfloat16, 64>(s, iq, ik, iv, o, lse, workspace, stream)
+                 : packed::launch_fwd<__nv_bfloat16, 128>(s, iq, ik, iv, o, lse, workspace, stream);
 }
 
 prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_strides, const void* k,

@@ -423,10 +423,15 @@ std::pair<Tensor, Tensor> packed_forward(const Tensor& q_in, const Tensor& k_in,
   const Tensor q = mappable(q_in), k = mappable(k_in), v = mappable(v_in);
   Tensor o = new_like(q), lse = want_lse ? stats_like(q, k, c) : Tensor();
   const auto sq = map_strides(q), sk = map_strides(k), sv = map_strides(v);
+  const int64_t bytes = want_lse ? 0
+                                 : (int64_t)prism_packed_attention_workspace_bytes(
+                                       q.size(0), k.size(0), c.offsets.size(0) - 1, (int)q.size(1), (int)k.size(1), (int)q.size(2));
+  const Tensor workspace = bytes > 0 ? at::empty({bytes}, q.options().dtype(at::kByte)) : Tensor();
   check(prism_packed_attention(at(q), sq.data(), at(k), sk.data(), at(v), sv.data(), at(c.offsets), at(c.k_offsets),
                                c.offsets.scalar_type() == at::kLong, c.offsets.size(0) - 1, q.size(0), k.size(0),
                                (int)q.size(1), (int)k.size(1), (int)q.size(2), c.causal, (float)c.scale,
-                               dtype_code(q, "packed_attention"), at(o), (float*)at(lse), launch.stream),
+                               dtype_code(q, "packed_attention"), at(o), (float*)at(lse), at(workspace),
+                               launch.stream),
         "prism_packed_attention");
   return {o, lse};
 }
