@@ -568,31 +568,35 @@ prism_status_t prism_linear_fp8(const void* x8, int64_t ldx, const float* x_scal
  * queries and m keys, query i attends all keys, or with causal != 0 the keys j <= i + m - n:
  *   o_i = sum_j p_ij v_j,  p_ij = softmax_j(scale q_i . k_j), scale > 0;  o_i = 0 without a key.
  * o [q_rows, q_heads, D] contiguous, 0 in rows that no sequence holds.  Strides {row, head} in elements, whole
- * 16 bytes; columns contiguous.  A NaN or an infinity in one sequence reaches no other.  lse (NULL: not
- * wanted): what the backward reads, of prism_packed_attention_stats_bytes.  workspace:
+ * 16 bytes; columns contiguous.  A NaN or an infinity in one sequence reaches no other.  workspace:
  * prism_packed_attention_workspace_bytes (NULL where that is 0, or with lse).  Sums and statistics fp32.
+ * For the backward (bf16; both or neither): lse, of prism_packed_attention_stats_bytes, and rest, a byte an
+ * element of o: what o's rounding left.
  *
  * prism_packed_attention_bwd (bf16): dout = dL/do -> dq, dk, dv in the layouts of o and of contiguous k, v, each
- * sum in a fixed order; dq or the pair dk, dv may be NULL (not wanted).  o and lse are the forward's;
- * workspace: prism_packed_attention_stats_bytes.  No rows on either side is refused: the gradients are zero.
- * Bounded waits report through prism_device_status (501-523). */
+ * sum in a fixed order; dq or the pair dk, dv may be NULL (not wanted).  o, rest and lse are the forward's;
+ * workspace: prism_packed_attention_bwd_workspace_bytes.  No rows on either side is refused: the gradients
+ * are zero.  Bounded waits report through prism_device_status (501-523). */
 size_t prism_packed_attention_workspace_bytes(int64_t q_rows, int64_t k_rows, int64_t count, int q_heads,
                                               int k_heads, int D);
 size_t prism_packed_attention_stats_bytes(int64_t q_rows, int64_t count, int q_heads, int k_heads);
+size_t prism_packed_attention_bwd_workspace_bytes(int64_t q_rows, int64_t k_rows, int64_t count,
+                                                  int q_heads, int k_heads, int D);
 prism_status_t prism_packed_attention(const void* q, const int64_t* q_strides, const void* k,
                                       const int64_t* k_strides, const void* v, const int64_t* v_strides,
                                       const void* q_offsets, const void* k_offsets, int offsets_64,
                                       int64_t count, int64_t q_rows, int64_t k_rows, int q_heads,
                                       int k_heads, int D, int causal, float scale, int dtype, void* o,
-                                      float* lse, void* workspace, cudaStream_t stream);
+                                      float* lse, void* rest, void* workspace, cudaStream_t stream);
 prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
                                           const int64_t* k_strides, const void* v,
-                                          const int64_t* v_strides, const void* o, const void* dout,
-                                          const int64_t* dout_strides, const float* lse,
-                                          const void* q_offsets, const void* k_offsets, int offsets_64,
-                                          int64_t count, int64_t q_rows, int64_t k_rows, int q_heads,
-                                          int k_heads, int D, int causal, float scale, void* workspace,
-                                          void* dq, void* dk, void* dv, cudaStream_t stream);
+                                          const int64_t* v_strides, const void* o, const void* rest,
+                                          const void* dout, const int64_t* dout_strides,
+                                          const float* lse, const void* q_offsets,
+                                          const void* k_offsets, int offsets_64, int64_t count,
+                                          int64_t q_rows, int64_t k_rows, int q_heads, int k_heads,
+                                          int D, int causal, float scale, void* workspace, void* dq,
+                                          void* dk, void* dv, cudaStream_t stream);
 
 /* A paged cache: keys and values as [pages, page_size, k_heads, D] each (strides {page, place, head} in
  * elements; columns contiguous), token j of sequence b at place j % page_size of page

@@ -67,11 +67,12 @@ SIGNATURES = {
     "prism_clip_grad_norm_workspace_bytes": (_SZ, [_I64]),
     "prism_clip_grad_norm": (_I, [_P, _P, _P, _P, _I64, _F, _P, _P, _P]),
     "prism_linear_fp8": (_I, [_P, _I64, _P, _P, _I64, _P, _P, _I, _I, _I, _P, _I64, _P]),
-    "prism_packed_attention_stats_bytes": (_SZ, [_I64, _I64, _I, _I]),
-    "prism_packed_attention": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _I, _I, _I, _F, _I, _P,
-                                    _P, _P, _P]),
     "prism_packed_attention_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I, _I, _I]),
-    "prism_packed_attention_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _I,
+    "prism_packed_attention_stats_bytes": (_SZ, [_I64, _I64, _I, _I]),
+    "prism_packed_attention_bwd_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I, _I, _I]),
+    "prism_packed_attention": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _I, _I, _I, _F, _I, _P,
+                                    _P, _P, _P, _P]),
+    "prism_packed_attention_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _I,
                                         _I, _I, _F, _P, _P, _P, _P, _P]),
     "prism_append_paged": (_I, [_P, _P, _I, _P, _P, _P, _P, _I, _I64, _I, _P, _I, _I, _P, _P, _P, _P, _I, _I, _P, _I64,
                                 _I, _P, _I, _I, _P, _F, _I, _P, _P]),

@@ -135,60 +135,10 @@ struct Heads {
   int keys, group, tokens, pairs;
 };
 
-enum Kind : int { kTile, kSpare, kBad };
-struct Place {
-  int kind;
-  int q0, nq, k0, nk;   // the sequence's rows
-  int tile;             // within the sequence; kSpare: number among the spare ones
-  int pairs;            // pairs of query tiles of the sequences before
-};
+enum Kind : int { kTile, kSpare, kBad, kStop };  // kStop: no more items
 
 __device__ __forceinline__ int64_t row_at(const void* offsets, int wide, int i) {
   return wide ? static_cast<const long long*>(offsets)[i] : (int64_t)static_cast<const int*>(offsets)[i];
-}
-
-// Tile `my` of the grid (kKeys: of `per` keys, else of `per` queries) -> *place.  All threads of the CTA;
-// scratch: 2 ints a warp.  One round for up to blockDim sequences.
-template <bool kKeys>
-__device__ void find_place(const Sequences& s, int my, int per, int pair_tokens, Place* place, int* scratch) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-  int base = 0, pairs_base = 0;
-  bool good = true;
-  if (tid == 0) place->kind = kSpare;
-  for (int b0 = 0; b0 < s.count; b0 += blockDim.x) {
-    const int b = b0 + tid;
-    int q0 = 0, nq = 0, k0 = 0, nk = 0;
-    bool fine = true;
-    if (b < s.count) {
-      const int64_t qa = row_at(s.q, s.wide, b), qb = row_at(s.q, s.wide, b + 1);
-      const int64_t ka = row_at(s.k, s.wide, b), kb = row_at(s.k, s.wide, b + 1);
-      fine = 0 <= qa && qa <= qb && qb <= s.q_rows && 0 <= ka && ka <= kb && kb <= s.k_rows;
-      if (fine) q0 = (int)qa, nq = (int)(qb - qa), k0 = (int)ka, nk = (int)(kb - ka);
-    }
-    const int pairs = (nq + pair_tokens - 1) / pair_tokens;
-    const int tiles = kKeys ? (nk + per - 1) / per : pairs;
-    int x = tiles, y = pairs;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {  // inclusive scans of the warp
-      const int xo = __shfl_up_sync(0xffffffffu, x, o), yo = __shfl_up_sync(0xffffffffu, y, o);
-      if (lane >= o) x += xo, y += yo;
-    }
-    if (lane == 31) scratch[2 * warp] = x, scratch[2 * warp + 1] = y;
-    good = __syncthreads_and(fine) && good;
-    int before = base, pairs_before = pairs_base;
-    for (int w = 0; w < warps; ++w) {
-      if (w < warp) before += scratch[2 * w], pairs_before += scratch[2 * w + 1];
-      base += scratch[2 * w], pairs_base += scratch[2 * w + 1];
-    }
-    before += x - tiles, pairs_before += y - pairs;
-    if (my >= before && my < before + tiles) *place = {kTile, q0, nq, k0, nk, my - before, pairs_before};
-    __syncthreads();
-  }
-  if (tid == 0) {
-    if (!good) place->kind = kBad;
-    else if (my >= base) place->kind = kSpare, place->tile = my - base;
-  }
-  __syncthreads();
 }
 
 // An item without a tile: clears its share of the rows that no sequence holds (kSpare), or fills its share of
@@ -342,8 +292,6 @@ struct ItemRing {
   }
 };
 
-enum : int { kStop = 3 };  // an Item's kind: no more
-
 // How a grid's items follow from the block index: parts of a tile next to each other, then key heads, then
 // tiles, the last ones first where `backwards`.
 struct Grid {
@@ -477,8 +425,7 @@ struct FwdLayout {
                        B_SF = B_VE + kRing,   // [g]: S of the group
                        B_PF = B_SF + 2,       // [g]: P in TMEM (and O rescaled)
                        B_OF = B_PF + 2,       // [g]: last P V of an item done
-                       B_OE = B_OF + 2,       // [g]: O read
-                       B_DRAIN = B_OE + 2, NBAR = B_DRAIN + 1;
+                       B_DRAIN = B_OF + 2, NBAR = B_DRAIN + 1;
   static constexpr int TMEM_SLOT = BAR + NBAR * 8;
   static constexpr int ABORT = TMEM_SLOT + 4;
   static constexpr int SCRATCH = ABORT + 4;
@@ -509,17 +456,34 @@ struct FwdSteps {
   }
 };
 
+// What a forward leaves besides o: nothing; what the backward reads; a part's sums in o's place.
+enum Mode : int { kInfer, kTrain, kPart };
+
+// What rounding a value to 16 bits leaves, in units of 2^-8 of the 16 bits' last place: the difference of the
+// bit patterns, to 8 bits (the last half step, which they cannot hold, is cut).  32 values' worth of them.
+__device__ __forceinline__ uint32_t rest_of(float x, uint32_t high) {
+  return (uint32_t)min((int)(__float_as_uint(x) - high) + 128, 32767);
+}
+__device__ __forceinline__ uint32_t rest_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0051), __byte_perm(c, d, 0x0051), 0x5410);
+}
+// ... and the value again, from its 16 bits and byte i of `left`.
+__device__ __forceinline__ float with_rest(uint32_t high, uint32_t left, int i) {
+  return __uint_as_float(high + (uint32_t)((int)(int8_t)(left >> (8 * i)) * 256));
+}
+
 // What the parts of a row leave: sums [part][row][head][D] and (maximum, sum) [part][row][head].
 struct Parts {
   float* o;
   float2* ml;
 };
 
-template <typename T, int D>
+template <typename T, int D, int kMode>
 __global__ void __launch_bounds__(kThreads, 1)
     fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Sequences seqs, Heads hd, Grid grid,
-               int causal, float qk_scale, T* __restrict__ o, float* __restrict__ lse, Parts parts) {
+               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ Sequences seqs,
+               const __grid_constant__ Heads hd, const __grid_constant__ Grid grid, int causal, float qk_scale,
+               T* __restrict__ o, float* __restrict__ lse, int8_t* __restrict__ rest, Parts parts) {
   using L = FwdLayout<D>;
   using H = Half<T>;
   constexpr int R = L::kRing;
@@ -546,7 +510,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(L::B_SF + g), 1);
       mbar_init(bar(L::B_PF + g), 4);
       mbar_init(bar(L::B_OF + g), 1);
-      mbar_init(bar(L::B_OE + g), 4);
     }
     mbar_init(bar(L::B_DRAIN), 1);
     *abort_flag = 0;
@@ -623,22 +586,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Steps of all items in one stream, by lane 0: every instruction between a P and its products is time that
     // the tensor core idles (32,768 causal tokens took 8.9 ms with votes of the warp in each wait, 8.4 without
     // and 8.2 with inner()).  Step n, group by group: P V of the group's step before it, then S of step n over the columns that
-    // held that P (one thread's products run in issue order).
+    // held that P (one thread's products run in issue order).  An item's first P V overwrites an O that the
+    // epilogue of the item before has read: the P that it waits for is written after it.
     constexpr uint32_t kIdS = idesc<T>(kRows, false), kIdO = idesc<T>(D, true);
     const uint64_t dQ = desc_k_sw128(sb + L::Q), dK = desc_k_sw128(sb + L::K), dV = desc_mn_sw128(sb + L::V, 16384);
     constexpr uint32_t kSlot = L::kTileBytes >> 4;
     int ns = 0, v_rows = 0;                        // steps so far; keys of the last one, 0: its P V is issued
-    int n_s[2] = {0, 0}, n_q[2] = {0, 0}, n_o[2] = {0, 0};
+    int n_s[2] = {0, 0}, n_q[2] = {0, 0};
     bool waiting[2] = {false, false}, first[2] = {}, last[2] = {};  // P V of the last step still to come
     const auto wait = [&](int i, int parity) { return wait_one(bar(i), parity & 1, abort_flag, kErrFwdMma); };
     const auto pv = [&](int g) -> bool {
       const int before = (ns - 1) % R;
       const uint32_t t = tmem + g * 256;
       if (!wait(L::B_PF + g, n_s[g] - 1)) return false;
-      if (first[g]) {  // over the O of an earlier item
-        if (n_o[g] > 0 && !wait(L::B_OE + g, n_o[g] - 1)) return false;
-        ++n_o[g];
-      }
       tc_fence_after();
       const uint64_t b = dV + before * kSlot;
       mma_ts_k64_mn(t + L::T_O, t + L::T_S, b, kIdO, first[g] ? 0u : 1u);
@@ -754,7 +714,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     while (ok && next_item(at, items, sm + L::ITEMS, ring, abort_flag, lane, kErrFwdSoftmax)) {
       if (at.kind != kTile) {
-        if (grid.parts == 1) {
+        if constexpr (kMode != kPart) {
           fill_rows(at.kind, at.tile, seqs.q, seqs, seqs.q_rows, 2 * n_tok, o, hd.keys, at.h, hd.group * D);
         } else {  // rows without a key in this part, or NaN
           fill_parts(at.kind, at.tile, seqs, 2 * n_tok, parts.ml + (int64_t)at.part * seqs.q_rows * heads, hd, at.h);
@@ -881,9 +841,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // epilogue
       const bool empty = m == -INFINITY;  // no key
       const int64_t out_row = (int64_t)(at.q0 + tok) * heads + at.h * hd.group + head_of_row;
-      if (lse != nullptr)
+      if constexpr (kMode == kTrain)
         lse[(((int64_t)at.h * hd.pairs + at.index) * 2 + g) * kRows + r] = valid && !empty ? m + __log2f(l) : INFINITY;
-      if (grid.parts > 1 && valid)
+      if (kMode == kPart && valid)
         parts.ml[(int64_t)at.part * seqs.q_rows * heads + out_row] = make_float2(m, empty ? 0.0f : l);
       if (n_steps > 0) {
         if (!wait_warp(bar(L::B_OF + g), n_o & 1, abort_flag, kErrFwdSoftmax)) {
@@ -898,28 +858,43 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t raw[32];
           tmem_ld32(t_lane + L::T_O + c * 32, raw);
           tmem_wait_ld_dep(raw);
-          if (grid.parts > 1) {
+          if constexpr (kMode == kPart) {
             float4* dst = reinterpret_cast<float4*>(parts.o + ((int64_t)at.part * seqs.q_rows * heads + out_row) * D + c * 32);
             if (valid) {
 #pragma unroll
               for (int i = 0; i < 8; ++i)
                 dst[i] = make_float4(u2f(raw[4 * i]), u2f(raw[4 * i + 1]), u2f(raw[4 * i + 2]), u2f(raw[4 * i + 3]));
             }
-            continue;
-          }
-          uint32_t pk[16];
+          } else {
+            uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) pk[i] = empty ? 0u : H::pack(u2f(raw[2 * i]) * inv, u2f(raw[2 * i + 1]) * inv);
-          if (valid) {
-            uint4* dst = reinterpret_cast<uint4*>(o + out_row * D + c * 32);
+            for (int i = 0; i < 16; ++i) pk[i] = empty ? 0u : H::pack(u2f(raw[2 * i]) * inv, u2f(raw[2 * i + 1]) * inv);
+            if (valid) {
+              uint4* dst = reinterpret_cast<uint4*>(o + out_row * D + c * 32);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+              for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+            }
+            if constexpr (kMode == kTrain) {
+              uint32_t left[8];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                uint32_t d[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t word = pk[2 * i + e / 2], high = (e & 1) ? word & 0xffff0000u : word << 16;
+                  d[e] = rest_of(empty ? 0.0f : u2f(raw[4 * i + e]) * inv, high);
+                }
+                left[i] = rest_bytes(d[0], d[1], d[2], d[3]);
+              }
+              if (valid) {
+                uint4* dst = reinterpret_cast<uint4*>(rest + out_row * D + c * 32);
+                dst[0] = make_uint4(left[0], left[1], left[2], left[3]), dst[1] = make_uint4(left[4], left[5], left[6], left[7]);
+              }
+            }
           }
         }
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(L::B_OE + g));
-      } else if (grid.parts == 1 && valid) {
+      } else if (kMode != kPart && valid) {
         uint4* dst = reinterpret_cast<uint4*>(o + out_row * D);
 #pragma unroll
         for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
@@ -965,21 +940,64 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Parts parts, int cou
       make_uint2(Half<T>::pack(acc.x * inv, acc.y * inv), Half<T>::pack(acc.z * inv, acc.w * inv));
 }
 
+// Pair `my` of the query tiles (of `per` tokens), for kernels whose CTAs each have one: found by all threads;
+// scratch: one int a warp.  Not there: more pairs than that, or offsets that are not in order.
+struct Place {
+  int there, q0, nq, tile;
+};
+__device__ void find_place(const Sequences& s, int my, int per, Place* place, int* scratch) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+  int base = 0;
+  bool good = true;
+  if (tid == 0) place->there = 0;
+  for (int b0 = 0; b0 < s.count; b0 += blockDim.x) {
+    const int b = b0 + tid;
+    int q0 = 0, nq = 0;
+    bool fine = true;
+    if (b < s.count) {
+      const int64_t qa = row_at(s.q, s.wide, b), qb = row_at(s.q, s.wide, b + 1);
+      const int64_t ka = row_at(s.k, s.wide, b), kb = row_at(s.k, s.wide, b + 1);
+      fine = 0 <= qa && qa <= qb && qb <= s.q_rows && 0 <= ka && ka <= kb && kb <= s.k_rows;
+      if (fine) q0 = (int)qa, nq = (int)(qb - qa);
+    }
+    const int tiles = (nq + per - 1) / per;
+    int x = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int xo = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += xo;
+    }
+    if (lane == 31) scratch[warp] = x;
+    good = __syncthreads_and(fine) && good;
+    int before = base + x - tiles;
+    for (int w = 0; w < warps; ++w) {
+      if (w < warp) before += scratch[w];
+      base += scratch[w];
+    }
+    if (my >= before && my < before + tiles) *place = {1, q0, nq, my - before};
+    __syncthreads();
+  }
+  if (tid == 0 && !good) place->there = 0;
+  __syncthreads();
+}
+
 // ===================================================================== delta
 // delta = dO . O of every row of every tile, 0 for rows without a token, in the forward's tile order: D / 8
-// threads a row.  Bound by memory.
+// threads a row.  O with the 8 bits that the forward kept of what its rounding left: delta enters ds next to
+// do . v, and o's rounding alone would be as large an error as that of ds.  Bound by memory.
 constexpr int kDeltaThreads = 256;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kDeltaThreads)
-    delta_kernel(const __grid_constant__ Sequences seqs, Heads hd, const T* __restrict__ o, const T* __restrict__ go,
-                 int64_t go_row, int64_t go_head, float* __restrict__ delta) {
+    delta_kernel(const __grid_constant__ Sequences seqs, Heads hd, const T* __restrict__ o,
+                 const int8_t* __restrict__ rest, const T* __restrict__ go, int64_t go_row, int64_t go_head,
+                 float* __restrict__ delta) {
   __shared__ Place shared_place;
-  __shared__ int scratch[2 * kDeltaThreads / 32];
+  __shared__ int scratch[kDeltaThreads / 32];
   const int pair = blockIdx.x / hd.keys, h = blockIdx.x % hd.keys;
-  find_place<false>(seqs, pair, 2 * hd.tokens, 2 * hd.tokens, &shared_place, scratch);
+  find_place(seqs, pair, 2 * hd.tokens, &shared_place, scratch);
   const Place at = shared_place;
-  if (at.kind != kTile) return;
+  if (!at.there) return;
   constexpr int kLanes = D / 8, kStep = kDeltaThreads / kLanes;
   const int lane = threadIdx.x % kLanes;
   const uint32_t inverse = group_inverse(hd.group);
@@ -989,15 +1007,16 @@ __global__ void __launch_bounds__(kDeltaThreads)
     const int tok = (at.tile * 2 + g) * hd.tokens + t, head = h * hd.group + r - t * hd.group;
     float sum = 0.0f;
     if (t < hd.tokens && tok < at.nq) {
-      const int64_t row = at.q0 + tok;
-      const uint4 a = *reinterpret_cast<const uint4*>(o + (row * hd.keys * hd.group + head) * D + lane * 8);
+      const int64_t row = at.q0 + tok, place = (row * hd.keys * hd.group + head) * D + lane * 8;
+      const uint4 a = __ldg(reinterpret_cast<const uint4*>(o + place));
+      const uint2 e = __ldg(reinterpret_cast<const uint2*>(rest + place));
       const uint4 b = __ldg(reinterpret_cast<const uint4*>(go + row * go_row + head * go_head + lane * 8));
-      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+      const uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w}, left[2] = {e.x, e.y};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 p = Half<T>::unpack(x[j]), q = Half<T>::unpack(y[j]);
-        sum = fmaf(p.x, q.x, sum);
-        sum = fmaf(p.y, q.y, sum);
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t high = (j & 1) ? x[j / 2] & 0xffff0000u : x[j / 2] << 16;
+        const float2 q = Half<T>::unpack(y[j / 2]);
+        sum = fmaf(with_rest(high, left[j / 4], j % 4), (j & 1) ? q.y : q.x, sum);
       }
     }
 #pragma unroll
@@ -1007,9 +1026,10 @@ __global__ void __launch_bounds__(kDeltaThreads)
 }
 
 // ================================================================== dK and dV
-// CTA: 128 keys of one key head; a step is a tile of 128 query rows, so the sum over the heads that share
-// the keys is the products' own (no atomics, a fixed order).  S^T = K Q^T, dP^T = V dO^T; P^T and dS^T are
-// written over them in TMEM; dV += P^T dO, dK += dS^T Q.  Rows without a token have lse = +inf: p = 0.
+// An item: 128 keys of one key head and a part of the tiles of 128 query rows that see them (all of them,
+// unless there are few key tiles); a step is one such tile, so the sum over the heads that share the keys is
+// the products' own (no atomics, a fixed order).  S^T = K Q^T, dP^T = V dO^T; P^T and dS^T are written over
+// them in TMEM; dV += P^T dO, dK += dS^T Q.  Rows without a token have lse = +inf: p = 0.
 //
 // The softmax reads the 16x256b TMEM layout: a thread holds, in each 16-lane half, key lanes a and a + 8
 // (a = lane / 4) at columns 8 j + 2 (lane % 4) + {0, 1}, so that it needs 16 of a half tile's 64 lse and
@@ -1025,17 +1045,35 @@ struct DkdvLayout {
   static constexpr int DO = Q + kRing * kTileBytes;
   static constexpr int M = DO + kRing * kTileBytes;  // lse
   static constexpr int DL = M + kRing * 512;         // delta
-  static constexpr int BAR = DL + kRing * 512;
-  static constexpr int B_KV = 0, B_QF = 1, B_QE = B_QF + kRing, B_SF = B_QE + kRing, B_DPF = B_SF + 1,
-                       B_PF = B_DPF + 1, B_DSF = B_PF + 1, B_FIN = B_DSF + 1, B_DRAIN = B_FIN + 1, NBAR = B_DRAIN + 1;
+  static constexpr int TOKENS = DL + kRing * 512;    // of a tile's rows
+  static constexpr int ITEMS = TOKENS + kRows * 4;
+  static constexpr int BAR = ITEMS + (ItemRing::kBytes + 15) / 16 * 16;
+  static constexpr int B_KV = 0, B_KVE = 1,   // an item's keys; its last S^T and dP^T done
+                       B_QF = 2, B_QE = B_QF + kRing, B_SF = B_QE + kRing, B_DPF = B_SF + 1, B_PF = B_DPF + 1,
+                       B_DSF = B_PF + 1, B_FIN = B_DSF + 1, B_DRAIN = B_FIN + 1, NBAR = B_DRAIN + 1;
   static constexpr int TMEM_SLOT = BAR + NBAR * 8;
   static constexpr int ABORT = TMEM_SLOT + 4;
-  static constexpr int PLACE = ABORT + 4;
-  static constexpr int SCRATCH = PLACE + (int)sizeof(Place);
+  static constexpr int SCRATCH = ABORT + 4;
   static constexpr size_t kNeed = 1024 + SCRATCH + 2 * 4 * (kThreads / 32);
   static constexpr size_t kBytes = kNeed > kMinSmem ? kNeed : kMinSmem;
   static constexpr int T_DK = 0, T_DV = D, T_S = 2 * D, T_DP = 2 * D + 128;
   static_assert(T_DP + 128 <= 512, "TMEM budget");
+};
+
+// The steps of an item: its first key, and the first of its query tiles and their number.
+struct DkdvSteps {
+  int key0, shift, first, steps;
+  bool tail;  // the last one ends with another sequence's rows
+  __device__ __forceinline__ DkdvSteps(const Item& at, int n_tok, int causal, int parts) {
+    key0 = at.tile * kRows, shift = at.nk - at.nq;
+    const int tiles = (at.nq + n_tok - 1) / n_tok;
+    // causal: from the tile that sees the first key
+    const int from = causal ? min(max(key0 - shift, 0) / n_tok, tiles) : 0, all = tiles - from;
+    first = from + (int)((int64_t)all * at.part / parts);
+    const int end = from + (int)((int64_t)all * (at.part + 1) / parts);
+    steps = end - first;
+    tail = end == tiles && tiles * n_tok > at.nq;
+  }
 };
 
 // p = exp2(s scale - lse) of 64 columns for this warp's lanes, written as pairs over the first 32 columns.
@@ -1100,39 +1138,31 @@ __device__ __forceinline__ void dkdv_ds(uint32_t t_tile, const float* __restrict
   }
 }
 
-template <typename T, int D>
+// kParts: sums of a part, fp32, to sums[part][0: dK, 1: dV][row][key head][D]; else dk and dv.
+template <typename T, int D, bool kParts>
 __global__ void __launch_bounds__(kThreads, 1)
     dkdv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                const __grid_constant__ Sequences seqs, Heads hd, int causal, float qk_scale, float scale,
+                const __grid_constant__ Sequences seqs, const __grid_constant__ Heads hd,
+                const __grid_constant__ Grid grid, int causal, float qk_scale, float scale,
                 const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dk,
-                T* __restrict__ dv) {
+                T* __restrict__ dv, float* __restrict__ sums) {
   using L = DkdvLayout<D>;
   constexpr int R = L::kRing;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ int seen_keys[kRows];  // of a tile's rows, from this CTA's first key on
   uint8_t* sm = align1024(smem_raw);
   const uint32_t sb = smem_u32(sm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int my = blockIdx.x / hd.keys, h = blockIdx.x % hd.keys;
   const int n_tok = hd.tokens, rows = n_tok * hd.group;
   auto bar = [&](int i) { return sb + L::BAR + 8 * i; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::ABORT);
-
-  Place* shared_place = reinterpret_cast<Place*>(sm + L::PLACE);
-  find_place<true>(seqs, my, kRows, 2 * n_tok, shared_place, reinterpret_cast<int*>(sm + L::SCRATCH));
-  const Place at = *shared_place;
-  if (at.kind != kTile) {
-    if (threadIdx.x < kSoftmaxThreads) {
-      const int share = at.kind == kBad ? my : at.tile;
-      fill_rows(at.kind, share, seqs.k, seqs, seqs.k_rows, kRows, dk, hd.keys, h, D);
-      fill_rows(at.kind, share, seqs.k, seqs, seqs.k_rows, kRows, dv, hd.keys, h, D);
-    }
-    return;
-  }
+  const uint32_t ring = sb + L::ITEMS;
+  int* tokens = reinterpret_cast<int*>(sm + L::TOKENS);
 
   if (threadIdx.x == 0) {
+    ItemRing::init(ring);
     mbar_init(bar(L::B_KV), 1);
+    mbar_init(bar(L::B_KVE), 1);
     for (int i = 0; i < R; ++i) {
       mbar_init(bar(L::B_QF + i), 1);
       mbar_init(bar(L::B_QE + i), 1);
@@ -1146,10 +1176,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort_flag = 0;
     fence_barrier_init();
   }
-  const int key0 = at.tile * kRows, shift = at.nk - at.nq;
-  const uint32_t inverse = group_inverse(hd.group);
-  // row r of tile i sees the keys below key0 + seen_keys[r] + i n
-  if (threadIdx.x < kRows) seen_keys[threadIdx.x] = over_group(threadIdx.x, inverse) + shift + 1 - key0;
+  if (threadIdx.x < kRows) tokens[threadIdx.x] = over_group(threadIdx.x, group_inverse(hd.group));
   if (rows < kRows) {  // rows that no load fills
     for (int i = 0; i < R; ++i) {
       zero_rows<L::kSub>(sm + L::Q + i * L::kTileBytes, rows, threadIdx.x, kThreads);
@@ -1162,171 +1189,236 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
     tc_fence_before();
   }
+  const Survey all = survey<true>(seqs, 2 * n_tok, reinterpret_cast<int*>(sm + L::SCRATCH));
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + L::TMEM_SLOT);
 
-  // query tiles of the sequence, causal: from the one that sees the first key
-  const int tiles = (at.nq + n_tok - 1) / n_tok;
-  const int first = causal ? min(max(key0 - shift, 0) / n_tok, tiles) : 0, steps = tiles - first;
-  const int64_t stat0 = (((int64_t)h * hd.pairs + at.pairs) * 2 + first) * kRows;
-
+  Item at;
+  int items = 0;
   if (warp == kProducerWarp) {
-    if (lane == 0 && steps > 0) {
-      mbar_expect_tx(bar(L::B_KV), 2 * L::kTileBytes);
+    // ------------------------------------------------------------ producer
+    int ns = 0, n_kv = 0;
+    bool ok = true;
+    ItemSource<true> source = {seqs, hd, grid, all, sm + L::ITEMS, ring, abort_flag, lane, kErrDkdvProducer};
+    while (ok && source.next(at)) {
+      if (at.kind != kTile) continue;
+      const DkdvSteps w(at, n_tok, causal, grid.parts);
+      if (w.steps == 0) continue;
+      if (lane == 0) {
+        ok = n_kv == 0 || wait_one(bar(L::B_KVE), (n_kv - 1) & 1, abort_flag, kErrDkdvProducer);
+        if (ok) {
+          mbar_expect_tx(bar(L::B_KV), 2 * L::kTileBytes);
 #pragma unroll
-      for (int s = 0; s < L::kSub; ++s) {
-        tma_load_3d(sb + L::K + s * 16384, &tm_k, s * 64, h, at.k0 + key0, bar(L::B_KV));
-        tma_load_3d(sb + L::V + s * 16384, &tm_v, s * 64, h, at.k0 + key0, bar(L::B_KV));
-      }
-      int n = 0;
-      for (; n < steps; ++n) {
-        const int st = n % R, tok = at.q0 + (first + n) * n_tok;
-        if (n >= R && !wait_one(bar(L::B_QE + st), ((n / R) - 1) & 1, abort_flag, kErrDkdvProducer)) break;
-        mbar_expect_tx(bar(L::B_QF + st), 2 * rows * D * 2 + 2 * 512);
-#pragma unroll
-        for (int s = 0; s < L::kSub; ++s) {
-          tma_load_3d(sb + L::Q + st * L::kTileBytes + s * 16384, &tm_q, s * 64, h * hd.group, tok, bar(L::B_QF + st));
-          tma_load_3d(sb + L::DO + st * L::kTileBytes + s * 16384, &tm_do, s * 64, h * hd.group, tok, bar(L::B_QF + st));
+          for (int s = 0; s < L::kSub; ++s) {
+            tma_load_3d(sb + L::K + s * 16384, &tm_k, s * 64, at.h, at.k0 + w.key0, bar(L::B_KV));
+            tma_load_3d(sb + L::V + s * 16384, &tm_v, s * 64, at.h, at.k0 + w.key0, bar(L::B_KV));
+          }
+          ++n_kv;
         }
-        bulk_load(sb + L::M + st * 512, lse + stat0 + (int64_t)n * kRows, 512, bar(L::B_QF + st));
-        bulk_load(sb + L::DL + st * 512, delta + stat0 + (int64_t)n * kRows, 512, bar(L::B_QF + st));
+        const int64_t stat0 = (((int64_t)at.h * hd.pairs + at.pairs) * 2 + w.first) * kRows;
+        for (int n = 0; ok && n < w.steps; ++n) {
+          const int st = ns % R, tok = at.q0 + (w.first + n) * n_tok;
+          ok = ns < R || wait_one(bar(L::B_QE + st), ((ns / R) - 1) & 1, abort_flag, kErrDkdvProducer);
+          if (!ok) break;
+          mbar_expect_tx(bar(L::B_QF + st), 2 * rows * D * 2 + 2 * 512);
+#pragma unroll
+          for (int s = 0; s < L::kSub; ++s) {
+            tma_load_3d(sb + L::Q + st * L::kTileBytes + s * 16384, &tm_q, s * 64, at.h * hd.group, tok, bar(L::B_QF + st));
+            tma_load_3d(sb + L::DO + st * L::kTileBytes + s * 16384, &tm_do, s * 64, at.h * hd.group, tok, bar(L::B_QF + st));
+          }
+          bulk_load(sb + L::M + st * 512, lse + stat0 + (int64_t)n * kRows, 512, bar(L::B_QF + st));
+          bulk_load(sb + L::DL + st * 512, delta + stat0 + (int64_t)n * kRows, 512, bar(L::B_QF + st));
+          ++ns;
+        }
       }
-      for (int m = max(n - R, 0); m < n; ++m) wait_one(bar(L::B_QF + m % R), (m / R) & 1, abort_flag, kErrDkdvProducer);
-      wait_one(bar(L::B_KV), 0, abort_flag, kErrDkdvProducer);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
     }
+    if (lane == 0) {  // every load has landed before the CTA may leave
+      for (int m = max(ns - R, 0); m < ns; ++m) wait_one(bar(L::B_QF + m % R), (m / R) & 1, abort_flag, kErrDkdvProducer);
+      if (n_kv > 0) wait_one(bar(L::B_KV), (n_kv - 1) & 1, abort_flag, kErrDkdvProducer);
+    }
+    __syncwarp();
   } else if (warp == kMmaWarp) {
-    // Issue order: S^T(n) | dK(n-1) | dP^T(n) | dV(n).  The softmax computes P^T(n) while dK(n-1) and dP^T(n)
-    // run, dS^T(n) while dV(n) and S^T(n+1) do.  S^T(n) overwrites P^T(n-1), read by dV(n-1), dP^T(n)
-    // overwrites dS^T(n-1), read by dK(n-1): issued earlier, and one thread's products run in issue order.
+    // ---------------------------------------------------------- MMA issuer
+    // Steps of all items in one stream: S^T(n) | dK(n-1) | dP^T(n) | dV(n).  The softmax computes P^T(n) while
+    // dK(n-1) and dP^T(n) run, dS^T(n) while dV(n) and S^T(n+1) do.  S^T(n) overwrites P^T(n-1), read by
+    // dV(n-1), dP^T(n) overwrites dS^T(n-1), read by dK(n-1): issued earlier, and one thread's products run in
+    // issue order.  An item's first dV and dK overwrite sums that the epilogue of the item before has read: the
+    // P^T and dS^T that they wait for are written after it.
     constexpr uint32_t kIdS = idesc<T>(kRows, false), kIdG = idesc<T>(D, true);
     const uint64_t dK = desc_k_sw128(sb + L::K), dV = desc_k_sw128(sb + L::V), dQk = desc_k_sw128(sb + L::Q),
                    dDOk = desc_k_sw128(sb + L::DO), dQmn = desc_mn_sw128(sb + L::Q, 16384),
                    dDOmn = desc_mn_sw128(sb + L::DO, 16384);
     constexpr uint32_t kSlot = L::kTileBytes >> 4;
-    const auto dk_step = [&](int j) -> bool {
-      const uint32_t st = (uint32_t)j % R;
-      if (!wait_warp(bar(L::B_DSF), j & 1, abort_flag, kErrDkdvMma)) return false;
+    int ns = 0, n_kv = 0;
+    bool waiting = false, first = false, last = false;  // dK of the last step still to come
+    const auto wait = [&](int i, int parity) { return wait_one(bar(i), parity & 1, abort_flag, kErrDkdvMma); };
+    const auto dk_step = [&]() -> bool {
+      const uint32_t st = (uint32_t)(ns - 1) % R;
+      if (!wait(L::B_DSF, ns - 1)) return false;
       tc_fence_after();
-      if (lane == 0) {
-        mma_ts_k64_mn(tmem + L::T_DK, tmem + L::T_DP, dQmn + st * kSlot, kIdG, j > 0 ? 1u : 0u);
-        mma_ts_k64_mn(tmem + L::T_DK, tmem + L::T_DP + 64, dQmn + st * kSlot + 512, kIdG, 1u);
-        mma_commit(bar(L::B_QE + st));
-      }
-      __syncwarp();
+      mma_ts_k64_mn(tmem + L::T_DK, tmem + L::T_DP, dQmn + st * kSlot, kIdG, first ? 0u : 1u);
+      mma_ts_k64_mn(tmem + L::T_DK, tmem + L::T_DP + 64, dQmn + st * kSlot + 512, kIdG, 1u);
+      mma_commit(bar(L::B_QE + st));
+      if (last) mma_commit(bar(L::B_FIN));
+      waiting = false;
       return true;
     };
-    bool ok = steps == 0 || wait_warp(bar(L::B_KV), 0, abort_flag, kErrDkdvMma);
-    tc_fence_after();
-    for (int n = 0; ok && n < steps; ++n) {
-      const uint32_t st = (uint32_t)n % R;
-      if (!wait_warp(bar(L::B_QF + st), (n / R) & 1, abort_flag, kErrDkdvMma)) {
-        ok = false;
-        break;
+    const auto step = [&](int n, int steps) -> bool {
+      const uint32_t st = (uint32_t)ns % R;
+      if (n == 0 && !wait(L::B_KV, n_kv)) return false;
+      if (!wait(L::B_QF + st, ns / R)) return false;
+      tc_fence_after();
+      mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S, dK, dQk + st * kSlot, kIdS, 0u);
+      mma_commit(bar(L::B_SF));
+      if (waiting && !dk_step()) return false;
+      mma_kd<L::kSub, 16384, 16384>(tmem + L::T_DP, dV, dDOk + st * kSlot, kIdS, 0u);
+      mma_commit(bar(L::B_DPF));
+      first = n == 0, last = n + 1 == steps;
+      if (last) mma_commit(bar(L::B_KVE)), ++n_kv;
+      if (!wait(L::B_PF, ns)) return false;
+      tc_fence_after();
+      mma_ts_k64_mn(tmem + L::T_DV, tmem + L::T_S, dDOmn + st * kSlot, kIdG, first ? 0u : 1u);
+      mma_ts_k64_mn(tmem + L::T_DV, tmem + L::T_S + 64, dDOmn + st * kSlot + 512, kIdG, 1u);
+      ++ns;
+      waiting = true;
+      return true;
+    };
+    bool ok = true, any = false;
+    while (ok) {
+      // an item that is not there yet is not waited for with products to issue
+      if (any && !__any_sync(0xffffffffu, item_ready(items, ring))) {
+        if (lane == 0 && waiting) ok = dk_step();
+        ok = __all_sync(0xffffffffu, ok), any = false;
       }
-      const int valid = (at.nq - (first + n) * n_tok) * hd.group;
-      if (valid < rows) {  // the next sequence's rows
-        zero_rows<L::kSub>(sm + L::Q + st * L::kTileBytes, valid, lane, 32);
-        zero_rows<L::kSub>(sm + L::DO + st * L::kTileBytes, valid, lane, 32);
-        fence_proxy_async_smem();
+      if (!ok || !next_item(at, items, sm + L::ITEMS, ring, abort_flag, lane, kErrDkdvMma)) break;
+      if (at.kind != kTile) continue;
+      const DkdvSteps w(at, n_tok, causal, grid.parts);
+      if (w.steps == 0) continue;
+      any = true;
+      const int plain = w.tail ? w.steps - 1 : w.steps;
+      if (lane == 0)
+        for (int n = 0; ok && n < plain; ++n) ok = step(n, w.steps);
+      ok = __all_sync(0xffffffffu, ok);
+      if (lane != 0) ns += plain;
+      if (w.tail && ok) {  // the next sequence's rows, which dK and dV sum over
+        const int st = ns % R;
+        ok = wait_warp(bar(L::B_QF + st), (ns / R) & 1, abort_flag, kErrDkdvMma);
+        const int valid = (at.nq - (w.first + plain) * n_tok) * hd.group;
+        if (ok) {
+          zero_rows<L::kSub>(sm + L::Q + st * L::kTileBytes, valid, lane, 32);
+          zero_rows<L::kSub>(sm + L::DO + st * L::kTileBytes, valid, lane, 32);
+          fence_proxy_async_smem();
+        }
         __syncwarp();
+        if (lane == 0 && ok) ok = step(plain, w.steps);
+        ok = __all_sync(0xffffffffu, ok);
+        if (lane != 0) ++ns;
       }
-      tc_fence_after();
-      if (lane == 0) {
-        mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S, dK, dQk + st * kSlot, kIdS, 0u);
-        mma_commit(bar(L::B_SF));
-      }
-      __syncwarp();
-      if (n > 0 && !dk_step(n - 1)) {
-        ok = false;
-        break;
-      }
-      if (lane == 0) {
-        mma_kd<L::kSub, 16384, 16384>(tmem + L::T_DP, dV, dDOk + st * kSlot, kIdS, 0u);
-        mma_commit(bar(L::B_DPF));
-      }
-      __syncwarp();
-      if (!wait_warp(bar(L::B_PF), n & 1, abort_flag, kErrDkdvMma)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (lane == 0) {
-        mma_ts_k64_mn(tmem + L::T_DV, tmem + L::T_S, dDOmn + st * kSlot, kIdG, n > 0 ? 1u : 0u);
-        mma_ts_k64_mn(tmem + L::T_DV, tmem + L::T_S + 64, dDOmn + st * kSlot + 512, kIdG, 1u);
-      }
-      __syncwarp();
     }
-    if (ok && steps > 0) dk_step(steps - 1);
     if (lane == 0) {
-      mma_commit(bar(L::B_FIN));
+      if (ok && waiting) dk_step();
       mma_commit(bar(L::B_DRAIN));
       wait_one(bar(L::B_DRAIN), 0, abort_flag, kErrDkdvMma);
     }
     __syncwarp();
-  } else if (warp < kProducerWarp) {
-    // softmax warpgroup w: columns [64 w, 64 w + 64) of each tile
+  } else {
+    // ------------------------------------------------------ softmax warps
+    // warpgroup w: columns [64 w, 64 w + 64) of each tile
     const int wg = warp >> 2, quarter = warp & 3;
     const int r = quarter * 32 + lane;  // key row of the epilogue == TMEM lane
     const uint32_t t_lane = tmem + ((uint32_t)(quarter * 32) << 16);
-    const int key = quarter * 32 + (lane >> 2);  // this thread's first key lane
-    const float* sM = reinterpret_cast<const float*>(sm + L::M);
-    const float* sDl = reinterpret_cast<const float*>(sm + L::DL);
+    const int key = quarter * 32 + (lane >> 2), tcol = wg * 64;  // this thread's first key lane
+    const float* sM = reinterpret_cast<const float*>(sm + L::M) + tcol;
+    const float* sDl = reinterpret_cast<const float*>(sm + L::DL) + tcol;
+    const int64_t part_rows = (int64_t)seqs.k_rows * hd.keys;
+    int ns = 0, n_fin = 0;
     bool ok = true;
-    for (int n = 0; n < steps; ++n) {
-      const int st = n % R, tcol = wg * 64;
-      const int at_tile = (first + n) * n_tok;
-      // every row of the tile sees every key of the CTA from its first row's place on
-      const bool masked = causal && at_tile + shift + 1 - key0 < kRows;
-      if (!wait_warp(bar(L::B_QF + st), (n / R) & 1, abort_flag, kErrDkdvSoftmax) ||
-          !wait_warp(bar(L::B_SF), n & 1, abort_flag, kErrDkdvSoftmax)) {
+    while (ok && next_item(at, items, sm + L::ITEMS, ring, abort_flag, lane, kErrDkdvSoftmax)) {
+      float* part = kParts ? sums + (int64_t)at.part * 2 * part_rows * D : nullptr;
+      if (at.kind != kTile) {
+        if constexpr (kParts) {  // fp32 zeros or NaN, as pairs of 16-bit ones
+          fill_rows(at.kind, at.tile, seqs.k, seqs, seqs.k_rows, kRows, reinterpret_cast<T*>(part), hd.keys, at.h, 2 * D);
+          fill_rows(at.kind, at.tile, seqs.k, seqs, seqs.k_rows, kRows, reinterpret_cast<T*>(part + part_rows * D), hd.keys, at.h, 2 * D);
+        } else {
+          fill_rows(at.kind, at.tile, seqs.k, seqs, seqs.k_rows, kRows, dk, hd.keys, at.h, D);
+          fill_rows(at.kind, at.tile, seqs.k, seqs, seqs.k_rows, kRows, dv, hd.keys, at.h, D);
+        }
+        continue;
+      }
+      const DkdvSteps w(at, n_tok, causal, grid.parts);
+      for (int n = 0; n < w.steps; ++n) {
+        const int st = ns % R;
+        // the keys that the tile's first row sees, from the item's first one on: all of them, or masked
+        const int seen = (w.first + n) * n_tok + w.shift + 1 - w.key0;
+        const bool masked = causal && seen < kRows;
+        if (!wait_warp(bar(L::B_QF + st), (ns / R) & 1, abort_flag, kErrDkdvSoftmax) ||
+            !wait_warp(bar(L::B_SF), ns & 1, abort_flag, kErrDkdvSoftmax)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        float p[64];
+        // key < seen + tokens[column]
+        if (masked) dkdv_p<T, true>(t_lane + L::T_S + tcol, sM + st * 128, qk_scale, lane, tokens + tcol, key - seen, p);
+        else dkdv_p<T, false>(t_lane + L::T_S + tcol, sM + st * 128, qk_scale, lane, nullptr, 0, p);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::B_PF));
+        if (!wait_warp(bar(L::B_DPF), ns & 1, abort_flag, kErrDkdvSoftmax)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (masked) dkdv_ds<T, true>(t_lane + L::T_DP + tcol, sDl + st * 128, lane, p);
+        else dkdv_ds<T, false>(t_lane + L::T_DP + tcol, sDl + st * 128, lane, p);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::B_DSF));
+        ++ns;
+      }
+      if (!ok) break;
+      // epilogue: warpgroup 0 writes dK, 1 dV
+      const bool valid = w.key0 + r < at.nk;
+      const int64_t row = (int64_t)(at.k0 + w.key0 + r) * hd.keys + at.h;
+      T* out = (wg == 0 ? dk : dv) + row * D;
+      float* sum = kParts ? part + (wg * part_rows + row) * D : nullptr;
+      const float by = wg == 0 ? scale : 1.0f;
+      if (w.steps > 0 && !wait_warp(bar(L::B_FIN), n_fin & 1, abort_flag, kErrDkdvSoftmax)) {
         ok = false;
         break;
       }
-      tc_fence_after();
-      float p[64];
-      // key < seen + at_tile as key - at_tile < seen
-      if (masked) dkdv_p<T, true>(t_lane + L::T_S + tcol, sM + st * 128 + tcol, qk_scale, lane, seen_keys + tcol, key - at_tile, p);
-      else dkdv_p<T, false>(t_lane + L::T_S + tcol, sM + st * 128 + tcol, qk_scale, lane, nullptr, 0, p);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(L::B_PF));
-      if (!wait_warp(bar(L::B_DPF), n & 1, abort_flag, kErrDkdvSoftmax)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (masked) dkdv_ds<T, true>(t_lane + L::T_DP + tcol, sDl + st * 128 + tcol, lane, p);
-      else dkdv_ds<T, false>(t_lane + L::T_DP + tcol, sDl + st * 128 + tcol, lane, p);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(L::B_DSF));
-    }
-    // epilogue: warpgroup 0 writes dK, 1 dV
-    const bool valid = key0 + r < at.nk;
-    T* out = (wg == 0 ? dk : dv) + ((int64_t)(at.k0 + key0 + r) * hd.keys + h) * D;
-    const float by = wg == 0 ? scale : 1.0f;
-    if (ok && steps > 0 && wait_warp(bar(L::B_FIN), 0, abort_flag, kErrDkdvSoftmax)) {
+      if (w.steps > 0) ++n_fin;
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        uint32_t raw[32], pk[16];
-        tmem_ld32(t_lane + (wg == 0 ? L::T_DK : L::T_DV) + c * 32, raw);
-        tmem_wait_ld_dep(raw);
+        uint32_t raw[32];
+        if (w.steps > 0) {
+          tmem_ld32(t_lane + (wg == 0 ? L::T_DK : L::T_DV) + c * 32, raw);
+          tmem_wait_ld_dep(raw);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) pk[i] = Half<T>::pack(u2f(raw[2 * i]) * by, u2f(raw[2 * i + 1]) * by);
-        if (valid) {
+          for (int i = 0; i < 32; ++i) raw[i] = 0u;
+        }
+        if (!valid) continue;
+        if constexpr (kParts) {
+          float4* dst = reinterpret_cast<float4*>(sum + c * 32);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            dst[i] = make_float4(u2f(raw[4 * i]), u2f(raw[4 * i + 1]), u2f(raw[4 * i + 2]), u2f(raw[4 * i + 3]));
+        } else {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) pk[i] = Half<T>::pack(u2f(raw[2 * i]) * by, u2f(raw[2 * i + 1]) * by);
           uint4* dst = reinterpret_cast<uint4*>(out + c * 32);
 #pragma unroll
           for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
         }
       }
-    } else if (ok && steps == 0 && valid) {
-      uint4* dst = reinterpret_cast<uint4*>(out);
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+      tc_fence_before();
     }
   }
   tc_fence_before();
@@ -1337,8 +1429,27 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
+// dK and dV from the sums of their parts, in order.  Bound by memory.
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads)
+    add_parts_kernel(const float* __restrict__ sums, int parts, int64_t count, float scale, T* __restrict__ dk,
+                     T* __restrict__ dv) {
+  const int64_t i = ((int64_t)blockIdx.x * kJoinThreads + threadIdx.x) * 4;
+  const int which = blockIdx.y;  // 0: dK, 1: dV
+  if (i >= count) return;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+  for (int p = 0; p < parts; ++p) {
+    const float4 v = *reinterpret_cast<const float4*>(sums + (2 * p + which) * count + i);
+    acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+  }
+  const float by = which == 0 ? scale : 1.0f;
+  *reinterpret_cast<uint2*>((which == 0 ? dk : dv) + i) =
+      make_uint2(Half<T>::pack(acc.x * by, acc.y * by), Half<T>::pack(acc.z * by, acc.w * by));
+}
+
 // ======================================================================= dQ
-// CTA: one tile of 128 query rows; a step is 128 keys: S = Q K^T and dP = dO V^T in TMEM, the softmax
+// An item: one tile of 128 query rows; a step is 128 keys: S = Q K^T and dP = dO V^T in TMEM, the softmax
 // warpgroups (64 keys each) write dS = P (dP - delta) into columns of its own, dQ += dS K reads them from
 // there.  S and dP of step n + 1 are issued as soon as those of step n are read.
 template <int D>
@@ -1350,25 +1461,40 @@ struct DqLayout {
   static constexpr int DO = Q + kTileBytes;
   static constexpr int K = DO + kTileBytes;
   static constexpr int V = K + kRingK * kTileBytes;
-  static constexpr int BAR = V + kRingV * kTileBytes;
-  static constexpr int B_QD = 0, B_KF = 1, B_KE = B_KF + kRingK, B_VF = B_KE + kRingK, B_VE = B_VF + kRingV,
+  static constexpr int ITEMS = V + kRingV * kTileBytes;
+  static constexpr int BAR = ITEMS + (ItemRing::kBytes + 15) / 16 * 16;
+  static constexpr int B_QD = 0, B_QE = 1,   // an item's rows; its last S and dP done
+                       B_KF = 2, B_KE = B_KF + kRingK, B_VF = B_KE + kRingK, B_VE = B_VF + kRingV,
                        B_SF = B_VE + kRingV, B_DPF = B_SF + 1, B_DPE = B_DPF + 1, B_DSF = B_DPE + 1,
                        B_DSE = B_DSF + 1, B_FIN = B_DSE + 1, B_DRAIN = B_FIN + 1, NBAR = B_DRAIN + 1;
   static constexpr int TMEM_SLOT = BAR + NBAR * 8;
   static constexpr int ABORT = TMEM_SLOT + 4;
-  static constexpr int PLACE = ABORT + 4;
-  static constexpr int SCRATCH = PLACE + (int)sizeof(Place);
+  static constexpr int SCRATCH = ABORT + 4;
   static constexpr size_t kNeed = 1024 + SCRATCH + 2 * 4 * (kThreads / 32);
   static constexpr size_t kBytes = kNeed > kMinSmem ? kNeed : kMinSmem;
   // dQ (D columns), S and dP (128 fp32 columns each), dS (64 columns of pairs)
   static constexpr int T_DQ = 0, T_S = 128, T_DP = 256, T_DS = 384;
 };
 
+// The steps of an item (its part: which tile of the pair).
+struct DqSteps {
+  int tok0, shift, last, steps;
+  bool tail;  // the last one ends with another sequence's keys
+  __device__ __forceinline__ DqSteps(const Item& at, int n_tok, int causal) {
+    tok0 = (at.tile * 2 + at.part) * n_tok, shift = at.nk - at.nq;
+    last = min(tok0 + n_tok, at.nq) - 1;
+    const int keys = tok0 >= at.nq ? 0 : causal ? min(max(last + shift + 1, 0), at.nk) : at.nk;
+    steps = (keys + kRows - 1) / kRows;
+    tail = steps * kRows > at.nk;
+  }
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
               const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-              const __grid_constant__ Sequences seqs, Heads hd, int causal, float qk_scale, float scale,
+              const __grid_constant__ Sequences seqs, const __grid_constant__ Heads hd,
+              const __grid_constant__ Grid grid, int causal, float qk_scale, float scale,
               const float* __restrict__ lse, const float* __restrict__ delta, T* __restrict__ dq) {
   using L = DqLayout<D>;
   constexpr int RK = L::kRingK, RV = L::kRingV;
@@ -1376,25 +1502,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sm = align1024(smem_raw);
   const uint32_t sb = smem_u32(sm);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int my = 2 * hd.pairs - 1 - (int)(blockIdx.x / hd.keys), h = blockIdx.x % hd.keys;
-  const int pair = my >> 1, half = my & 1;
   const int n_tok = hd.tokens, rows = n_tok * hd.group;
   auto bar = [&](int i) { return sb + L::BAR + 8 * i; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + L::ABORT);
-
-  Place* shared_place = reinterpret_cast<Place*>(sm + L::PLACE);
-  find_place<false>(seqs, pair, 2 * n_tok, 2 * n_tok, shared_place, reinterpret_cast<int*>(sm + L::SCRATCH));
-  const Place at = *shared_place;
-  if (at.kind != kTile) {
-    if (half == 0 && threadIdx.x < kSoftmaxThreads)
-      fill_rows(at.kind, at.kind == kBad ? pair : at.tile, seqs.q, seqs, seqs.q_rows, 2 * n_tok, dq, hd.keys, h, hd.group * D);
-    return;
-  }
-  const int tok0 = (at.tile * 2 + half) * n_tok, shift = at.nk - at.nq;
-  if (tok0 >= at.nq) return;  // the pair's second tile, empty
+  const uint32_t ring = sb + L::ITEMS;
 
   if (threadIdx.x == 0) {
+    ItemRing::init(ring);
     mbar_init(bar(L::B_QD), 1);
+    mbar_init(bar(L::B_QE), 1);
     for (int i = 0; i < RK; ++i) {
       mbar_init(bar(L::B_KF + i), 1);
       mbar_init(bar(L::B_KE + i), 1);
@@ -1423,194 +1539,246 @@ __global__ void __launch_bounds__(kThreads, 1)
     tmem_relinquish();
     tc_fence_before();
   }
+  const Survey all = survey<false>(seqs, 2 * n_tok, reinterpret_cast<int*>(sm + L::SCRATCH));
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(sm + L::TMEM_SLOT);
 
-  const int last = min(tok0 + n_tok, at.nq) - 1;
-  const int keys = causal ? min(max(last + shift + 1, 0), at.nk) : at.nk, steps = (keys + kRows - 1) / kRows;
-
+  Item at;
+  int items = 0;
   if (warp == kProducerWarp) {
-    if (lane == 0 && steps > 0) {
-      mbar_expect_tx(bar(L::B_QD), 2 * rows * D * 2);
+    // ------------------------------------------------------------ producer
+    int nk = 0, nv = 0, n_q = 0;
+    bool ok = true;
+    ItemSource<false> source = {seqs, hd, grid, all, sm + L::ITEMS, ring, abort_flag, lane, kErrDqProducer};
+    while (ok && source.next(at)) {
+      if (at.kind != kTile) continue;
+      const DqSteps w(at, n_tok, causal);
+      if (w.steps == 0) continue;
+      if (lane == 0) {
+        ok = n_q == 0 || wait_one(bar(L::B_QE), (n_q - 1) & 1, abort_flag, kErrDqProducer);
+        if (ok) {
+          mbar_expect_tx(bar(L::B_QD), 2 * rows * D * 2);
 #pragma unroll
-      for (int s = 0; s < L::kSub; ++s) {
-        tma_load_3d(sb + L::Q + s * 16384, &tm_q, s * 64, h * hd.group, at.q0 + tok0, bar(L::B_QD));
-        tma_load_3d(sb + L::DO + s * 16384, &tm_do, s * 64, h * hd.group, at.q0 + tok0, bar(L::B_QD));
+          for (int s = 0; s < L::kSub; ++s) {
+            tma_load_3d(sb + L::Q + s * 16384, &tm_q, s * 64, at.h * hd.group, at.q0 + w.tok0, bar(L::B_QD));
+            tma_load_3d(sb + L::DO + s * 16384, &tm_do, s * 64, at.h * hd.group, at.q0 + w.tok0, bar(L::B_QD));
+          }
+          ++n_q;
+        }
+        for (int n = 0; ok && n < w.steps; ++n) {
+          const int sk = nk % RK, sv = nv % RV, key = at.k0 + n * kRows;
+          ok = nk < RK || wait_one(bar(L::B_KE + sk), ((nk / RK) - 1) & 1, abort_flag, kErrDqProducer);
+          if (!ok) break;
+          mbar_expect_tx(bar(L::B_KF + sk), L::kTileBytes);
+#pragma unroll
+          for (int s = 0; s < L::kSub; ++s)
+            tma_load_3d(sb + L::K + sk * L::kTileBytes + s * 16384, &tm_k, s * 64, at.h, key, bar(L::B_KF + sk));
+          ++nk;
+          ok = nv < RV || wait_one(bar(L::B_VE + sv), ((nv / RV) - 1) & 1, abort_flag, kErrDqProducer);
+          if (!ok) break;
+          mbar_expect_tx(bar(L::B_VF + sv), L::kTileBytes);
+#pragma unroll
+          for (int s = 0; s < L::kSub; ++s)
+            tma_load_3d(sb + L::V + sv * L::kTileBytes + s * 16384, &tm_v, s * 64, at.h, key, bar(L::B_VF + sv));
+          ++nv;
+        }
       }
-      int nk = 0, nv = 0;
-      for (int n = 0; n < steps; ++n) {
-        const int sk = n % RK, sv = n % RV, key = at.k0 + n * kRows;
-        if (n >= RK && !wait_one(bar(L::B_KE + sk), ((n / RK) - 1) & 1, abort_flag, kErrDqProducer)) break;
-        mbar_expect_tx(bar(L::B_KF + sk), L::kTileBytes);
-#pragma unroll
-        for (int s = 0; s < L::kSub; ++s)
-          tma_load_3d(sb + L::K + sk * L::kTileBytes + s * 16384, &tm_k, s * 64, h, key, bar(L::B_KF + sk));
-        ++nk;
-        if (n >= RV && !wait_one(bar(L::B_VE + sv), ((n / RV) - 1) & 1, abort_flag, kErrDqProducer)) break;
-        mbar_expect_tx(bar(L::B_VF + sv), L::kTileBytes);
-#pragma unroll
-        for (int s = 0; s < L::kSub; ++s)
-          tma_load_3d(sb + L::V + sv * L::kTileBytes + s * 16384, &tm_v, s * 64, h, key, bar(L::B_VF + sv));
-        ++nv;
-      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+    if (lane == 0) {  // every load has landed before the CTA may leave
       for (int m = max(nk - RK, 0); m < nk; ++m) wait_one(bar(L::B_KF + m % RK), (m / RK) & 1, abort_flag, kErrDqProducer);
       for (int m = max(nv - RV, 0); m < nv; ++m) wait_one(bar(L::B_VF + m % RV), (m / RV) & 1, abort_flag, kErrDqProducer);
-      wait_one(bar(L::B_QD), 0, abort_flag, kErrDqProducer);
+      if (n_q > 0) wait_one(bar(L::B_QD), (n_q - 1) & 1, abort_flag, kErrDqProducer);
     }
+    __syncwarp();
   } else if (warp == kMmaWarp) {
-    // Issue order: S(0) dP(0) | S(1) dP(1) dQ(0) | S(2) dP(2) dQ(1) | ...
+    // ---------------------------------------------------------- MMA issuer
+    // Steps of all items in one stream: S(0) dP(0) | S(1) dP(1) dQ(0) | S(2) dP(2) dQ(1) | ...  An item's first
+    // dQ overwrites one that the epilogue of the item before has read: the dS that it waits for is written
+    // after it.
     constexpr uint32_t kIdS = idesc<T>(kRows, false), kIdG = idesc<T>(D, true);
     const uint64_t dQ = desc_k_sw128(sb + L::Q), dDO = desc_k_sw128(sb + L::DO), dKk = desc_k_sw128(sb + L::K),
                    dVk = desc_k_sw128(sb + L::V), dKmn = desc_mn_sw128(sb + L::K, 16384);
     constexpr uint32_t kSlot = L::kTileBytes >> 4;
-    const auto dq_step = [&](int j) -> bool {
-      if (!wait_warp(bar(L::B_DSF), j & 1, abort_flag, kErrDqMma)) return false;
+    int ns = 0, n_q = 0;
+    bool waiting = false, first = false, last = false;  // dQ of the last step still to come
+    const auto wait = [&](int i, int parity) { return wait_one(bar(i), parity & 1, abort_flag, kErrDqMma); };
+    const auto dq_step = [&](int j, bool begins, bool ends) -> bool {
+      if (!wait(L::B_DSF, j)) return false;
       tc_fence_after();
-      if (lane == 0) {
-        const uint64_t b = dKmn + (j % RK) * kSlot;
-        mma_ts_k64_mn(tmem + L::T_DQ, tmem + L::T_DS, b, kIdG, j > 0 ? 1u : 0u);
-        mma_ts_k64_mn(tmem + L::T_DQ, tmem + L::T_DS + 32, b + (8192 >> 4), kIdG, 1u);
-        mma_commit(bar(L::B_DSE));
-        mma_commit(bar(L::B_KE + j % RK));
-      }
-      __syncwarp();
+      const uint64_t b = dKmn + (j % RK) * kSlot;
+      mma_ts_k64_mn(tmem + L::T_DQ, tmem + L::T_DS, b, kIdG, begins ? 0u : 1u);
+      mma_ts_k64_mn(tmem + L::T_DQ, tmem + L::T_DS + 32, b + (8192 >> 4), kIdG, 1u);
+      mma_commit(bar(L::B_DSE));
+      mma_commit(bar(L::B_KE + j % RK));
+      if (ends) mma_commit(bar(L::B_FIN));
       return true;
     };
-    bool ok = steps == 0 || wait_warp(bar(L::B_QD), 0, abort_flag, kErrDqMma);
-    tc_fence_after();
-    for (int n = 0; ok && n < steps; ++n) {
-      const int sk = n % RK, sv = n % RV;
-      if (!wait_warp(bar(L::B_KF + sk), (n / RK) & 1, abort_flag, kErrDqMma) ||
-          (n > 0 && !wait_warp(bar(L::B_DPE), (n - 1) & 1, abort_flag, kErrDqMma))) {
-        ok = false;
-        break;
+    const auto step = [&](int n, int steps) -> bool {
+      const int sk = ns % RK, sv = ns % RV;
+      if (n == 0 && !wait(L::B_QD, n_q)) return false;
+      if (!wait(L::B_KF + sk, ns / RK) || (ns > 0 && !wait(L::B_DPE, ns - 1))) return false;
+      tc_fence_after();
+      mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S, dQ, dKk + sk * kSlot, kIdS, 0u);
+      mma_commit(bar(L::B_SF));
+      if (!wait(L::B_VF + sv, ns / RV)) return false;
+      tc_fence_after();
+      mma_kd<L::kSub, 16384, 16384>(tmem + L::T_DP, dDO, dVk + sv * kSlot, kIdS, 0u);
+      mma_commit(bar(L::B_DPF));
+      mma_commit(bar(L::B_VE + sv));
+      const bool ends = n + 1 == steps;
+      if (ends) mma_commit(bar(L::B_QE)), ++n_q;
+      if (waiting && !dq_step(ns - 1, first, last)) return false;
+      ++ns;
+      waiting = true, first = n == 0, last = ends;
+      return true;
+    };
+    bool ok = true, any = false;
+    while (ok) {
+      // an item that is not there yet is not waited for with products to issue
+      if (any && !__any_sync(0xffffffffu, item_ready(items, ring))) {
+        if (lane == 0 && waiting) ok = dq_step(ns - 1, first, last), waiting = false;
+        ok = __all_sync(0xffffffffu, ok), any = false;
       }
-      if ((n + 1) * kRows > at.nk) {  // the next sequence's keys, which dQ sums over
-        zero_rows<L::kSub>(sm + L::K + sk * L::kTileBytes, at.nk - n * kRows, lane, 32);
-        fence_proxy_async_smem();
+      if (!ok || !next_item(at, items, sm + L::ITEMS, ring, abort_flag, lane, kErrDqMma)) break;
+      if (at.kind != kTile) continue;
+      const DqSteps w(at, n_tok, causal);
+      if (w.steps == 0) continue;
+      any = true;
+      const int plain = w.tail ? w.steps - 1 : w.steps;
+      if (lane == 0)
+        for (int n = 0; ok && n < plain; ++n) ok = step(n, w.steps);
+      ok = __all_sync(0xffffffffu, ok);
+      if (lane != 0) ns += plain;
+      if (w.tail && ok) {  // the next sequence's keys, which dQ sums over
+        const int sk = ns % RK;
+        ok = wait_warp(bar(L::B_KF + sk), (ns / RK) & 1, abort_flag, kErrDqMma);
+        if (ok) {
+          zero_rows<L::kSub>(sm + L::K + sk * L::kTileBytes, at.nk - plain * kRows, lane, 32);
+          fence_proxy_async_smem();
+        }
         __syncwarp();
-      }
-      tc_fence_after();
-      if (lane == 0) {
-        mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S, dQ, dKk + sk * kSlot, kIdS, 0u);
-        mma_commit(bar(L::B_SF));
-      }
-      __syncwarp();
-      if (!wait_warp(bar(L::B_VF + sv), (n / RV) & 1, abort_flag, kErrDqMma)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (lane == 0) {
-        mma_kd<L::kSub, 16384, 16384>(tmem + L::T_DP, dDO, dVk + sv * kSlot, kIdS, 0u);
-        mma_commit(bar(L::B_DPF));
-        mma_commit(bar(L::B_VE + sv));
-      }
-      __syncwarp();
-      if (n > 0 && !dq_step(n - 1)) {
-        ok = false;
-        break;
+        if (lane == 0 && ok) ok = step(plain, w.steps);
+        ok = __all_sync(0xffffffffu, ok);
+        if (lane != 0) ++ns;
       }
     }
-    if (ok && steps > 0) dq_step(steps - 1);
     if (lane == 0) {
-      mma_commit(bar(L::B_FIN));
+      if (ok && waiting) dq_step(ns - 1, first, last);
       mma_commit(bar(L::B_DRAIN));
       wait_one(bar(L::B_DRAIN), 0, abort_flag, kErrDqMma);
     }
     __syncwarp();
-  } else if (warp < kProducerWarp) {
-    // softmax warpgroup w: keys [64 w, 64 w + 64) of each step
+  } else {
+    // ------------------------------------------------------ softmax warps
+    // warpgroup w: keys [64 w, 64 w + 64) of each step
     const int wg = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the tile == TMEM lane
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    const int t = over_group(r, group_inverse(hd.group)), tok = tok0 + t;
-    const bool valid = r < rows && tok < at.nq;
-    const int seen = causal ? min(max(min(tok, last) + shift + 1, 0), at.nk) : at.nk;
-    const int64_t stat = (((int64_t)h * hd.pairs + pair) * 2 + half) * kRows + r;
-    const float mrow = lse[stat], drow = delta[stat];
+    const int t = over_group(r, group_inverse(hd.group)), head = r - t * hd.group;
+    int ns = 0, n_fin = 0;
     bool ok = true;
-    for (int n = 0; n < steps; ++n) {
-      const int lim = seen - n * kRows - wg * 64;
-      const bool all = __all_sync(0xffffffffu, lim >= 64), none = __all_sync(0xffffffffu, lim <= 0);
-      if (!wait_warp(bar(L::B_SF), n & 1, abort_flag, kErrDqSoftmax)) {
-        ok = false;
-        break;
+    while (ok && next_item(at, items, sm + L::ITEMS, ring, abort_flag, lane, kErrDqSoftmax)) {
+      if (at.kind != kTile) {
+        if (at.part == 0) fill_rows(at.kind, at.tile, seqs.q, seqs, seqs.q_rows, 2 * n_tok, dq, hd.keys, at.h, hd.group * D);
+        continue;
       }
-      tc_fence_after();
-      // S(n) and dP(n) are both read before the exponentials and released at once; dS(n) overwrites dS(n-1),
-      // so its stores wait for dQ(n-1); it is written in two parts to bound registers
-      float p[64], dp[64];
-      if (!none) tmem_load<2>(t_lane + L::T_S + wg * 64, p);
-      if (!wait_warp(bar(L::B_DPF), n & 1, abort_flag, kErrDqSoftmax)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (!none) tmem_load<2>(t_lane + L::T_DP + wg * 64, dp);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(L::B_DPE));
-      if (!none && !all) {  // masked keys: p = 0, whatever their V rows hold
-        mask_from(p, lim);
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c >= lim) dp[c] = 0.0f;
-      }
-      const float2 sc = make_float2(qk_scale, qk_scale), nm = make_float2(-mrow, -mrow), nd = make_float2(-drow, -drow);
-#pragma unroll
-      for (int part = 0; part < 2; ++part) {
-        uint32_t pk[16];
-        if (!none) {
-#pragma unroll
-          for (int c = 32 * part; c < 32 * part + 32; c += 2) {
-            const float2 x = __ffma2_rn(make_float2(p[c], p[c + 1]), sc, nm);
-            const float2 ds = __fmul2_rn(make_float2(ex2(x.x), ex2(x.y)), __fadd2_rn(make_float2(dp[c], dp[c + 1]), nd));
-            pk[(c - 32 * part) / 2] = Half<T>::pack(ds.x, ds.y);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) pk[i] = 0u;
+      const DqSteps w(at, n_tok, causal);
+      const int tok = w.tok0 + t;
+      const bool valid = r < rows && tok < at.nq;
+      const int seen = causal ? min(max(min(tok, w.last) + w.shift + 1, 0), at.nk) : at.nk;
+      const int64_t stat = (((int64_t)at.h * hd.pairs + at.index) * 2 + at.part) * kRows + r;
+      const float mrow = lse[stat], drow = delta[stat];
+      for (int n = 0; n < w.steps; ++n) {
+        const int lim = seen - n * kRows - wg * 64;
+        const bool all_seen = __all_sync(0xffffffffu, lim >= 64), none = __all_sync(0xffffffffu, lim <= 0);
+        if (!wait_warp(bar(L::B_SF), ns & 1, abort_flag, kErrDqSoftmax)) {
+          ok = false;
+          break;
         }
-        if (part == 0) {
-          if (n > 0 && !wait_warp(bar(L::B_DSE), (n - 1) & 1, abort_flag, kErrDqSoftmax)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+        tc_fence_after();
+        // S and dP are both read before the exponentials and released at once; dS overwrites that of the step
+        // before, so its stores wait for that step's dQ; it is written in two parts to bound registers
+        float p[64], dp[64];
+        if (!none) tmem_load<2>(t_lane + L::T_S + wg * 64, p);
+        if (!wait_warp(bar(L::B_DPF), ns & 1, abort_flag, kErrDqSoftmax)) {
+          ok = false;
+          break;
         }
-        tmem_st16(t_lane + L::T_DS + wg * 32 + 16 * part, pk);
+        tc_fence_after();
+        if (!none) tmem_load<2>(t_lane + L::T_DP + wg * 64, dp);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::B_DPE));
+        if (!none && !all_seen) {  // masked keys: p = 0, whatever their V rows hold
+          mask_from(p, lim);
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c >= lim) dp[c] = 0.0f;
+        }
+        const float2 sc = make_float2(qk_scale, qk_scale), nm = make_float2(-mrow, -mrow), nd = make_float2(-drow, -drow);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[16];
+          if (!none) {
+#pragma unroll
+            for (int c = 32 * half; c < 32 * half + 32; c += 2) {
+              const float2 x = __ffma2_rn(make_float2(p[c], p[c + 1]), sc, nm);
+              const float2 ds = __fmul2_rn(make_float2(ex2(x.x), ex2(x.y)), __fadd2_rn(make_float2(dp[c], dp[c + 1]), nd));
+              pk[(c - 32 * half) / 2] = Half<T>::pack(ds.x, ds.y);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk[i] = 0u;
+          }
+          if (half == 0) {
+            if (ns > 0 && !wait_warp(bar(L::B_DSE), (ns - 1) & 1, abort_flag, kErrDqSoftmax)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
+          tmem_st16(t_lane + L::T_DS + wg * 32 + 16 * half, pk);
+        }
+        if (!ok) break;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(L::B_DSF));
+        ++ns;
       }
       if (!ok) break;
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(L::B_DSF));
-    }
-    // epilogue: warpgroup w writes columns [w D / 2, (w + 1) D / 2); a row without keys has none of its own
-    const bool empty = seen == 0;
-    T* row = dq + ((int64_t)(at.q0 + tok) * hd.keys * hd.group + h * hd.group + (r - t * hd.group)) * D + wg * (D / 2);
-    if (ok && steps > 0 && wait_warp(bar(L::B_FIN), 0, abort_flag, kErrDqSoftmax)) {
-      tc_fence_after();
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
-        uint32_t raw[32], pk[16];
-        tmem_ld32(t_lane + L::T_DQ + wg * (D / 2) + c * 32, raw);
-        tmem_wait_ld_dep(raw);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          pk[i] = empty ? 0u : Half<T>::pack(u2f(raw[2 * i]) * scale, u2f(raw[2 * i + 1]) * scale);
-        if (valid) {
-          uint4* dst = reinterpret_cast<uint4*>(row + c * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+      // epilogue: warpgroup w writes columns [w D / 2, (w + 1) D / 2); a row without keys has none of its own
+      const bool empty = seen == 0;
+      T* row = dq + ((int64_t)(at.q0 + tok) * hd.keys * hd.group + at.h * hd.group + head) * D + wg * (D / 2);
+      if (w.steps > 0) {
+        if (!wait_warp(bar(L::B_FIN), n_fin & 1, abort_flag, kErrDqSoftmax)) {
+          ok = false;
+          break;
         }
-      }
-    } else if (ok && steps == 0 && valid) {
-      uint4* dst = reinterpret_cast<uint4*>(row);
+        ++n_fin;
+        tc_fence_after();
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+        for (int c = 0; c < D / 64; ++c) {
+          uint32_t raw[32], pk[16];
+          tmem_ld32(t_lane + L::T_DQ + wg * (D / 2) + c * 32, raw);
+          tmem_wait_ld_dep(raw);
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            pk[i] = empty ? 0u : Half<T>::pack(u2f(raw[2 * i]) * scale, u2f(raw[2 * i + 1]) * scale);
+          if (valid) {
+            uint4* dst = reinterpret_cast<uint4*>(row + c * 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+          }
+        }
+        tc_fence_before();
+      } else if (valid) {
+        uint4* dst = reinterpret_cast<uint4*>(row);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) dst[i] = make_uint4(0, 0, 0, 0);
+      }
     }
   }
   tc_fence_before();
@@ -1687,15 +1855,20 @@ struct Shape {
     return {k_heads, group, kRows / group, (int)pair_bound(q_rows, count, group)};
   }
   int64_t key_tiles() const { return (k_rows + kRows - 1) / kRows + count; }
-  // Parts of the forward's steps: as many as give every SM kWaves items, while a part has four steps of an
-  // average sequence.
-  int parts() const {
-    const int64_t items = pair_bound(q_rows, count, q_heads / k_heads) * k_heads;
-    const int64_t steps = count > 0 ? k_rows / count / kRows : 0;
-    const int64_t want = (kWaves * kSms + items - 1) / (items > 0 ? items : 1);
-    const int64_t most = steps / 4 < 16 ? steps / 4 : 16;
+  // Values of lse, or of delta: of all rows of all tiles.
+  int64_t stats() const { return pair_bound(q_rows, count, q_heads / k_heads) * 2 * kRows * k_heads; }
+  // Parts of the items' steps: as many as give every SM kWaves items, while a part has four steps of an average
+  // sequence.
+  static int parts(int64_t items, int64_t steps) {
+    const int64_t want = items > 0 ? (kWaves * kSms + items - 1) / items : 1, most = steps / 4 < 16 ? steps / 4 : 16;
     const int64_t n = want < most ? want : most;
     return n > 1 ? (int)n : 1;
+  }
+  int forward_parts() const {
+    return count == 0 ? 1 : parts(pair_bound(q_rows, count, q_heads / k_heads) * k_heads, k_rows / count / kRows);
+  }
+  int dkdv_parts() const {
+    return count == 0 ? 1 : parts(key_tiles() * k_heads, q_rows / count / (kRows / (q_heads / k_heads)));
   }
 };
 
@@ -1738,7 +1911,7 @@ struct Input {
 
 template <typename T, int D>
 static prism_status_t launch_fwd(const Shape& s, const Input& q, const Input& k, const Input& v, void* o, float* lse,
-                                 void* workspace, cudaStream_t stream) {
+                                 int8_t* rest, void* workspace, cudaStream_t stream) {
   constexpr const char* what = "prism_packed_attention";
   const Heads hd = s.heads();
   PRISM_TRY(bind_context(what));
@@ -1750,16 +1923,21 @@ static prism_status_t launch_fwd(const Shape& s, const Input& q, const Input& k,
   const int64_t k_rows = s.k_rows > 0 ? s.k_rows : s.q_rows;
   PRISM_TRY(make_map(&mk, kk.p, k_rows, s.k_heads, D, kk.strides, 1, kRows, s.dtype));
   PRISM_TRY(make_map(&mv, vv.p, k_rows, s.k_heads, D, vv.strides, 1, kRows, s.dtype));
-  const auto kernel = fwd_kernel<T, D>;
   constexpr size_t bytes = FwdLayout<D>::kBytes;
   static_assert(bytes <= 227 * 1024, "shared memory");
-  PRISM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
-  const Grid grid = {hd.pairs, lse != nullptr ? 1 : s.parts(), s.causal};
+  const Grid grid = {hd.pairs, lse != nullptr ? 1 : s.forward_parts(), s.causal};
   const int64_t rows = s.q_rows * s.q_heads;
   Parts parts = {nullptr, nullptr};
-  if (grid.parts > 1) parts.o = static_cast<float*>(workspace), parts.ml = reinterpret_cast<float2*>(parts.o + grid.parts * rows * D);
+  auto kernel = fwd_kernel<T, D, kInfer>;
+  if (grid.parts > 1) {
+    parts.o = static_cast<float*>(workspace), parts.ml = reinterpret_cast<float2*>(parts.o + grid.parts * rows * D);
+    kernel = fwd_kernel<T, D, kPart>;
+  }
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    if (lse != nullptr) kernel = fwd_kernel<T, D, kTrain>;
+  PRISM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
   kernel<<<(unsigned)(hd.pairs * hd.keys * grid.parts), kThreads, bytes, stream>>>(
-      mq, mk, mv, s.sequences(), hd, grid, s.causal, s.scale * kLog2e, (T*)o, lse, parts);
+      mq, mk, mv, s.sequences(), hd, grid, s.causal, s.scale * kLog2e, (T*)o, lse, rest, parts);
   PRISM_CHECK_LAUNCH(what);
   if (grid.parts > 1) {
     join_kernel<T, D><<<(unsigned)((rows * (D / 4) + kJoinThreads - 1) / kJoinThreads), kJoinThreads, 0, stream>>>(
@@ -1771,11 +1949,13 @@ static prism_status_t launch_fwd(const Shape& s, const Input& q, const Input& k,
 
 template <typename T, int D>
 static prism_status_t launch_bwd(const Shape& s, const Input& q, const Input& k, const Input& v, const void* o,
-                                 const Input& go, const float* lse, float* delta, void* dq, void* dk, void* dv,
-                                 cudaStream_t stream) {
+                                 const int8_t* rest, const Input& go, const float* lse, void* workspace, void* dq,
+                                 void* dk, void* dv, cudaStream_t stream) {
   constexpr const char* what = "prism_packed_attention_bwd";
   const Heads hd = s.heads();
   const Sequences seqs = s.sequences();
+  float* delta = static_cast<float*>(workspace);
+  float* sums = delta + s.stats();
   PRISM_TRY(bind_context(what));
   CUtensorMap mq, mk, mv, mdo;
   PRISM_TRY(make_map(&mq, q.p, s.q_rows, s.q_heads, D, q.strides, hd.group, hd.tokens, s.dtype));
@@ -1783,24 +1963,32 @@ static prism_status_t launch_bwd(const Shape& s, const Input& q, const Input& k,
   PRISM_TRY(make_map(&mk, k.p, s.k_rows, s.k_heads, D, k.strides, 1, kRows, s.dtype));
   PRISM_TRY(make_map(&mv, v.p, s.k_rows, s.k_heads, D, v.strides, 1, kRows, s.dtype));
   delta_kernel<T, D><<<(unsigned)(hd.pairs * hd.keys), kDeltaThreads, 0, stream>>>(
-      seqs, hd, (const T*)o, (const T*)go.p, go.strides[0], go.strides[1], delta);
+      seqs, hd, (const T*)o, rest, (const T*)go.p, go.strides[0], go.strides[1], delta);
   PRISM_CHECK_LAUNCH(what);
   if (dk != nullptr) {
     constexpr size_t bytes = DkdvLayout<D>::kBytes;
-    static_assert(bytes + 512 <= 227 * 1024, "shared memory");
-    const auto kernel = dkdv_kernel<T, D>;
+    static_assert(bytes <= 227 * 1024, "shared memory");
+    const Grid grid = {(int)s.key_tiles(), s.dkdv_parts(), 0};
+    const auto kernel = grid.parts > 1 ? dkdv_kernel<T, D, true> : dkdv_kernel<T, D, false>;
     PRISM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
-    kernel<<<(unsigned)(s.key_tiles() * hd.keys), kThreads, bytes, stream>>>(
-        mq, mk, mv, mdo, seqs, hd, s.causal, s.scale * kLog2e, s.scale, lse, delta, (T*)dk, (T*)dv);
+    kernel<<<(unsigned)(grid.tiles * hd.keys * grid.parts), kThreads, bytes, stream>>>(
+        mq, mk, mv, mdo, seqs, hd, grid, s.causal, s.scale * kLog2e, s.scale, lse, delta, (T*)dk, (T*)dv, sums);
     PRISM_CHECK_LAUNCH(what);
+    if (grid.parts > 1) {
+      const int64_t count = s.k_rows * s.k_heads * D;
+      const unsigned blocks = (unsigned)((count / 4 + kJoinThreads - 1) / kJoinThreads);
+      add_parts_kernel<T><<<dim3(blocks, 2), kJoinThreads, 0, stream>>>(sums, grid.parts, count, s.scale, (T*)dk, (T*)dv);
+      PRISM_CHECK_LAUNCH(what);
+    }
   }
   if (dq != nullptr) {
     constexpr size_t bytes = DqLayout<D>::kBytes;
     static_assert(bytes <= 227 * 1024, "shared memory");
     const auto kernel = dq_kernel<T, D>;
+    const Grid grid = {hd.pairs, 2, s.causal};
     PRISM_CHECK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes), what);
     kernel<<<(unsigned)(2 * hd.pairs * hd.keys), kThreads, bytes, stream>>>(
-        mq, mk, mv, mdo, seqs, hd, s.causal, s.scale * kLog2e, s.scale, lse, delta, (T*)dq);
+        mq, mk, mv, mdo, seqs, hd, grid, s.causal, s.scale * kLog2e, s.scale, lse, delta, (T*)dq);
     PRISM_CHECK_LAUNCH(what);
   }
   return PRISM_OK;
@@ -1833,7 +2021,7 @@ size_t prism_packed_attention_workspace_bytes(int64_t q_rows, int64_t k_rows, in
   if (q_rows < 0 || k_rows < 0 || count < 0 || D < 1 || k_heads < 1 || q_heads < k_heads || q_heads / k_heads > packed::kRows)
     return 0;
   const packed::Shape s = {nullptr, nullptr, 0, count, q_rows, k_rows, q_heads, k_heads, D, 0, PRISM_BF16, 1.0f};
-  const int parts = s.parts();
+  const int parts = s.forward_parts();
   return parts == 1 ? 0 : (size_t)parts * q_rows * q_heads * (D * sizeof(float) + sizeof(float2));
 }
 
@@ -1841,14 +2029,16 @@ prism_status_t prism_packed_attention(const void* q, const int64_t* q_strides, c
                                       const void* v, const int64_t* v_strides, const void* q_offsets,
                                       const void* k_offsets, int offsets_64, int64_t count, int64_t q_rows,
                                       int64_t k_rows, int q_heads, int k_heads, int D, int causal, float scale,
-                                      int dtype, void* o, float* lse, void* workspace, cudaStream_t stream) {
+                                      int dtype, void* o, float* lse, void* rest, void* workspace, cudaStream_t stream) {
   constexpr const char* what = "prism_packed_attention";
   const packed::Shape s = {q_offsets, k_offsets, offsets_64, count, q_rows, k_rows,
                            q_heads,   k_heads,   D,          causal != 0, dtype, scale};
   PRISM_TRY(packed::check(s, what));
   if (q_rows == 0) return PRISM_OK;
   PRISM_CHECK_ARG(q_offsets && k_offsets && o && aligned16(o) && (!lse || aligned16(lse)), "%s: null pointer, or an output off 16 bytes", what);
-  PRISM_CHECK_ARG(lse || s.parts() == 1 || (workspace && aligned16(workspace)), "%s: no workspace", what);
+  PRISM_CHECK_ARG((lse == nullptr) == (rest == nullptr) && (!lse || (dtype == PRISM_BF16 && aligned16(rest))),
+                  "%s: lse and rest belong together, of bf16", what);
+  PRISM_CHECK_ARG(lse || s.forward_parts() == 1 || (workspace && aligned16(workspace)), "%s: no workspace", what);
   PRISM_TRY(packed::check_rows(q, q_strides, what, "q"));
   if (k_rows > 0) {
     PRISM_TRY(packed::check_rows(k, k_strides, what, "k"));
@@ -1856,16 +2046,25 @@ prism_status_t prism_packed_attention(const void* q, const int64_t* q_strides, c
   }
   const packed::Input iq = {q, q_strides}, ik = {k, k_strides}, iv = {v, v_strides};
   if (dtype == PRISM_FP16)
-    return D == 64 ? packed::launch_fwd<__half, 64>(s, iq, ik, iv, o, lse, workspace, stream)
-                   : packed::launch_fwd<__half, 128>(s, iq, ik, iv, o, lse, workspace, stream);
-  return D == 64 ? packed::launch_fwd<__nv_bfloat16, 64>(s, iq, ik, iv, o, lse, workspace, stream)
-                 : packed::launch_fwd<__nv_bfloat16, 128>(s, iq, ik, iv, o, lse, workspace, stream);
+    return D == 64 ? packed::launch_fwd<__half, 64>(s, iq, ik, iv, o, lse, (int8_t*)rest, workspace, stream)
+                   : packed::launch_fwd<__half, 128>(s, iq, ik, iv, o, lse, (int8_t*)rest, workspace, stream);
+  return D == 64 ? packed::launch_fwd<__nv_bfloat16, 64>(s, iq, ik, iv, o, lse, (int8_t*)rest, workspace, stream)
+                 : packed::launch_fwd<__nv_bfloat16, 128>(s, iq, ik, iv, o, lse, (int8_t*)rest, workspace, stream);
+}
+
+size_t prism_packed_attention_bwd_workspace_bytes(int64_t q_rows, int64_t k_rows, int64_t count, int q_heads,
+                                                  int k_heads, int D) {
+  if (q_rows < 0 || k_rows < 0 || count < 0 || D < 1 || k_heads < 1 || q_heads < k_heads || q_heads / k_heads > packed::kRows)
+    return 0;
+  const packed::Shape s = {nullptr, nullptr, 0, count, q_rows, k_rows, q_heads, k_heads, D, 0, PRISM_BF16, 1.0f};
+  const int parts = s.dkdv_parts();
+  return (size_t)(s.stats() + (parts == 1 ? 0 : 2 * (int64_t)parts * k_rows * k_heads * D)) * sizeof(float);
 }
 
 prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_strides, const void* k,
                                           const int64_t* k_strides, const void* v, const int64_t* v_strides,
-                                          const void* o, const void* dout, const int64_t* dout_strides,
-                                          const float* lse, const void* q_offsets, const void* k_offsets,
+                                          const void* o, const void* rest, const void* dout,
+                                          const int64_t* dout_strides, const float* lse, const void* q_offsets, const void* k_offsets,
                                           int offsets_64, int64_t count, int64_t q_rows, int64_t k_rows, int q_heads,
                                           int k_heads, int D, int causal, float scale, void* workspace, void* dq,
                                           void* dk, void* dv, cudaStream_t stream) {
@@ -1874,18 +2073,17 @@ prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_stride
                            q_heads,   k_heads,   D,          causal != 0, PRISM_BF16, scale};
   PRISM_TRY(packed::check(s, what));
   PRISM_CHECK_ARG(q_rows > 0 && k_rows > 0, "%s: no rows (all gradients are zero)", what);
-  PRISM_CHECK_ARG(q_offsets && k_offsets && o && lse && workspace && (dk == nullptr) == (dv == nullptr),
+  PRISM_CHECK_ARG(q_offsets && k_offsets && o && rest && lse && workspace && (dk == nullptr) == (dv == nullptr),
                   "%s: null pointer", what);
-  PRISM_CHECK_ARG(aligned16(o) && aligned16(lse) && aligned16(workspace) && aligned16(dq) && aligned16(dk) && aligned16(dv),
+  PRISM_CHECK_ARG(aligned16(o) && aligned16(rest) && aligned16(lse) && aligned16(workspace) && aligned16(dq) && aligned16(dk) && aligned16(dv),
                   "%s: buffers must start on 16 bytes", what);
   PRISM_TRY(packed::check_rows(q, q_strides, what, "q"));
   PRISM_TRY(packed::check_rows(k, k_strides, what, "k"));
   PRISM_TRY(packed::check_rows(v, v_strides, what, "v"));
   PRISM_TRY(packed::check_rows(dout, dout_strides, what, "dout"));
   const packed::Input iq = {q, q_strides}, ik = {k, k_strides}, iv = {v, v_strides}, ig = {dout, dout_strides};
-  float* delta = static_cast<float*>(workspace);
-  return D == 64 ? packed::launch_bwd<__nv_bfloat16, 64>(s, iq, ik, iv, o, ig, lse, delta, dq, dk, dv, stream)
-                 : packed::launch_bwd<__nv_bfloat16, 128>(s, iq, ik, iv, o, ig, lse, delta, dq, dk, dv, stream);
+  return D == 64 ? packed::launch_bwd<__nv_bfloat16, 64>(s, iq, ik, iv, o, (const int8_t*)rest, ig, lse, workspace, dq, dk, dv, stream)
+                 : packed::launch_bwd<__nv_bfloat16, 128>(s, iq, ik, iv, o, (const int8_t*)rest, ig, lse, workspace, dq, dk, dv, stream);
 }
 
 }  // extern "C"

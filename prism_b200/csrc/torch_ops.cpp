@@ -416,30 +416,30 @@ Tensor stats_like(const Tensor& q, const Tensor& k, const PackedCall& c) {
   return fp32({(int64_t)(bytes / sizeof(float))}, q);
 }
 
-// (o, lse)
-std::pair<Tensor, Tensor> packed_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const PackedCall& c,
-                                         bool want_lse) {
+// (o, lse, rest); the last two for the backward.
+std::tuple<Tensor, Tensor, Tensor> packed_forward(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const PackedCall& c,
+                                                  bool train) {
   const Launch launch(q_in.get_device());
   const Tensor q = mappable(q_in), k = mappable(k_in), v = mappable(v_in);
-  Tensor o = new_like(q), lse = want_lse ? stats_like(q, k, c) : Tensor();
+  Tensor o = new_like(q), lse = train ? stats_like(q, k, c) : Tensor(), rest = train ? new_like(q, at::kChar) : Tensor();
   const auto sq = map_strides(q), sk = map_strides(k), sv = map_strides(v);
-  const int64_t bytes = want_lse ? 0
+  const int64_t bytes = train ? 0
                                  : (int64_t)prism_packed_attention_workspace_bytes(
                                        q.size(0), k.size(0), c.offsets.size(0) - 1, (int)q.size(1), (int)k.size(1), (int)q.size(2));
   const Tensor workspace = bytes > 0 ? at::empty({bytes}, q.options().dtype(at::kByte)) : Tensor();
   check(prism_packed_attention(at(q), sq.data(), at(k), sk.data(), at(v), sv.data(), at(c.offsets), at(c.k_offsets),
                                c.offsets.scalar_type() == at::kLong, c.offsets.size(0) - 1, q.size(0), k.size(0),
                                (int)q.size(1), (int)k.size(1), (int)q.size(2), c.causal, (float)c.scale,
-                               dtype_code(q, "packed_attention"), at(o), (float*)at(lse), at(workspace),
+                               dtype_code(q, "packed_attention"), at(o), (float*)at(lse), at(rest), at(workspace),
                                launch.stream),
         "prism_packed_attention");
-  return {o, lse};
+  return {o, lse, rest};
 }
 
 struct PackedAttention : torch::autograd::Function<PackedAttention> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const PackedCall& c) {
-    auto [o, lse] = packed_forward(q, k, v, c, true);
-    ctx->save_for_backward({q, k, v, o, lse, c.offsets, c.k_offsets});
+    auto [o, lse, rest] = packed_forward(q, k, v, c, true);
+    ctx->save_for_backward({q, k, v, o, lse, c.offsets, c.k_offsets, rest});
     ctx->saved_data["causal"] = c.causal;
     ctx->saved_data["scale"] = c.scale;
     ctx->set_materialize_grads(false);
@@ -456,7 +456,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
       const at::NoGradGuard no_grad;
       const Launch launch(saved[0].get_device());
       const Tensor q = mappable(saved[0]), k = mappable(saved[1]), v = mappable(saved[2]), go = mappable(go_in);
-      const Tensor &o = saved[3], &lse = saved[4];
+      const Tensor &o = saved[3], &lse = saved[4], &rest = saved[7];
       const PackedCall c = {saved[5], saved[6], ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble()};
       const bool want_q = ctx->needs_input_grad(0), want_k = ctx->needs_input_grad(1), want_v = ctx->needs_input_grad(2);
       const bool pair = want_k || want_v;
@@ -465,9 +465,12 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
       } else {
         if (want_q) out[0] = new_like(q);
         if (pair) out[1] = new_like(k), out[2] = new_like(v);
-        const Tensor workspace = stats_like(q, k, c);
+        const Tensor workspace = at::empty({(int64_t)prism_packed_attention_bwd_workspace_bytes(
+                                               q.size(0), k.size(0), c.offsets.size(0) - 1, (int)q.size(1), (int)k.size(1),
+                                               (int)q.size(2))},
+                                           q.options().dtype(at::kByte));
         const auto sq = map_strides(q), sk = map_strides(k), sv = map_strides(v), sg = map_strides(go);
-        check(prism_packed_attention_bwd(at(q), sq.data(), at(k), sk.data(), at(v), sv.data(), at(o), at(go), sg.data(),
+        check(prism_packed_attention_bwd(at(q), sq.data(), at(k), sk.data(), at(v), sv.data(), at(o), at(rest), at(go), sg.data(),
                                          (const float*)at(lse), at(c.offsets), at(c.k_offsets),
                                          c.offsets.scalar_type() == at::kLong, c.offsets.size(0) - 1, q.size(0),
                                          k.size(0), (int)q.size(1), (int)k.size(1), (int)q.size(2), c.causal,
@@ -529,7 +532,7 @@ Tensor packed_attention(const Tensor& q, const Tensor& k, const Tensor& v, const
     TORCH_CHECK_NOT_IMPLEMENTED(q.scalar_type() == at::kBFloat16, what, " has gradients in bf16 only");
     return PackedAttention::apply(q, k, v, c);
   }
-  return packed_forward(q, k, v, c, false).first;
+  return std::get<0>(packed_forward(q, k, v, c, false));
 }
 
 // ------------------------------------------------------------------ paged cache
