@@ -568,7 +568,8 @@ prism_status_t prism_linear_fp8(const void* x8, int64_t ldx, const float* x_scal
  * queries and m keys, query i attends all keys, or with causal != 0 the keys j <= i + m - n:
  *   o_i = sum_j p_ij v_j,  p_ij = softmax_j(scale q_i . k_j), scale > 0;  o_i = 0 without a key.
  * o [q_rows, q_heads, D] contiguous, 0 in rows that no sequence holds.  Strides {row, head} in elements, whole
- * 16 bytes; columns contiguous.  A NaN or an infinity in one sequence reaches no other.  workspace:
+ * 16 bytes; columns contiguous.  Outputs and workspaces start on 32 bytes.  A NaN or an infinity in one
+ * sequence reaches no other.  workspace:
  * prism_packed_attention_workspace_bytes (NULL where that is 0, or with lse).  Sums and statistics fp32.
  * For the backward (bf16; both or neither): lse, of prism_packed_attention_stats_bytes, and rest, a byte an
  * element of o: what o's rounding left.

@@ -89,10 +89,18 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
+// 32 bytes to global memory: a sector, whole.
+__device__ __forceinline__ void store32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
 // ------------------------------------------------------------------ element types
 // kShift: log2 of the largest p that a fresh maximum gives.  fp16 keeps p >= 2^-24 only, so its maximum is
-// put at 2^10 and keys down to 2^-34 of the largest count; kLag more (2^15 in all, below fp16's 65504)
-// until the maximum is raised.  kSum: a half tile's exponentials below it all are within that.
+// put at 2^8 and keys down to 2^-32 of the largest count; kLag more (2^15 in all, below fp16's 65504)
+// until the maximum is raised.  kSum: a half step's exponentials below it all are within that; 64 equal
+// scores are.
 template <typename T>
 struct Half;
 template <>
@@ -106,7 +114,7 @@ struct Half<__nv_bfloat16> {
 };
 template <>
 struct Half<__half> {
-  static constexpr float kShift = 10.0f, kLag = 5.0f, kSum = 32768.0f;
+  static constexpr float kShift = 8.0f, kLag = 7.0f, kSum = 32768.0f;
   static constexpr uint32_t kFormat = 0;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -744,21 +752,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!(u ? all1 : all0)) mask_from(s, u ? lim1 : lim0);
         };
         float sum0 = 0.f, sum1 = 0.f;
-        // Exponentials against the running maximum in one pass over S.  A row's first step, and a first half
-        // whose exponentials sum past kSum, take two passes (maximum, then exponentials; S is intact).  If only
-        // the second half passes the limit, P of the first half, l and O are scaled to the new maximum.
-        bool two_pass = __any_sync(0xffffffffu, m == -INFINITY);
+        // Exponentials against the running maximum in one pass over S; a row's first maximum is that of its
+        // first half step.  A first half whose exponentials sum past kSum, and a row that has seen no key yet,
+        // take two passes (maximum, then exponentials; S is intact).  If only the second half passes the limit,
+        // P of the first half, l and O are scaled to the new maximum.
+        bool two_pass = false;
         uint32_t pk0[32];
-        if (!two_pass) {
-          if (none0) {
+        if (none0) {
+          two_pass = __any_sync(0xffffffffu, m == -INFINITY);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) pk0[i] = 0u;
-          } else {
-            float s[64];
-            scores(0, s);
-            sum0 = exp_pairs<T>(s, qk_scale, m, pk0);
+          for (int i = 0; i < 32; ++i) pk0[i] = 0u;
+        } else {
+          float s[64];
+          scores(0, s);
+          if (__any_sync(0xffffffffu, m == -INFINITY)) {
+            if (m == -INFINITY) m = tile_max(s) * qk_scale - H::kShift, l = 0.0f;
+            if (m == -INFINITY) l = 1.0f;
+            two_pass = __any_sync(0xffffffffu, m == -INFINITY);
           }
-          two_pass = __any_sync(0xffffffffu, !(sum0 <= H::kSum));
+          sum0 = exp_pairs<T>(s, qk_scale, m, pk0);
+          two_pass = two_pass || __any_sync(0xffffffffu, !(sum0 <= H::kSum));
         }
         if (two_pass) {
           sum0 = 0.f;
@@ -859,20 +872,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_ld32(t_lane + L::T_O + c * 32, raw);
           tmem_wait_ld_dep(raw);
           if constexpr (kMode == kPart) {
-            float4* dst = reinterpret_cast<float4*>(parts.o + ((int64_t)at.part * seqs.q_rows * heads + out_row) * D + c * 32);
+            float* dst = parts.o + ((int64_t)at.part * seqs.q_rows * heads + out_row) * D + c * 32;
             if (valid) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i)
-                dst[i] = make_float4(u2f(raw[4 * i]), u2f(raw[4 * i + 1]), u2f(raw[4 * i + 2]), u2f(raw[4 * i + 3]));
+              for (int i = 0; i < 4; ++i) store32(dst + 8 * i, raw + 8 * i);
             }
           } else {
             uint32_t pk[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) pk[i] = empty ? 0u : H::pack(u2f(raw[2 * i]) * inv, u2f(raw[2 * i + 1]) * inv);
             if (valid) {
-              uint4* dst = reinterpret_cast<uint4*>(o + out_row * D + c * 32);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+              T* dst = o + out_row * D + c * 32;
+              store32(dst, pk), store32(dst + 16, pk + 8);
             }
             if constexpr (kMode == kTrain) {
               uint32_t left[8];
@@ -886,10 +897,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 left[i] = rest_bytes(d[0], d[1], d[2], d[3]);
               }
-              if (valid) {
-                uint4* dst = reinterpret_cast<uint4*>(rest + out_row * D + c * 32);
-                dst[0] = make_uint4(left[0], left[1], left[2], left[3]), dst[1] = make_uint4(left[4], left[5], left[6], left[7]);
-              }
+              if (valid) store32(rest + out_row * D + c * 32, left);
             }
           }
         }
@@ -1405,17 +1413,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!valid) continue;
         if constexpr (kParts) {
-          float4* dst = reinterpret_cast<float4*>(sum + c * 32);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(u2f(raw[4 * i]), u2f(raw[4 * i + 1]), u2f(raw[4 * i + 2]), u2f(raw[4 * i + 3]));
+          for (int i = 0; i < 4; ++i) store32(sum + c * 32 + 8 * i, raw + 8 * i);
         } else {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) pk[i] = Half<T>::pack(u2f(raw[2 * i]) * by, u2f(raw[2 * i + 1]) * by);
-          uint4* dst = reinterpret_cast<uint4*>(out + c * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
+          store32(out + c * 32, pk), store32(out + c * 32 + 16, pk + 8);
         }
       }
       tc_fence_before();
@@ -1767,11 +1771,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int i = 0; i < 16; ++i)
             pk[i] = empty ? 0u : Half<T>::pack(u2f(raw[2 * i]) * scale, u2f(raw[2 * i + 1]) * scale);
-          if (valid) {
-            uint4* dst = reinterpret_cast<uint4*>(row + c * 32);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pk[4 * i], pk[4 * i + 1], pk[4 * i + 2], pk[4 * i + 3]);
-          }
+          if (valid) store32(row + c * 32, pk), store32(row + c * 32 + 16, pk + 8);
         }
         tc_fence_before();
       } else if (valid) {
@@ -2035,10 +2035,10 @@ prism_status_t prism_packed_attention(const void* q, const int64_t* q_strides, c
                            q_heads,   k_heads,   D,          causal != 0, dtype, scale};
   PRISM_TRY(packed::check(s, what));
   if (q_rows == 0) return PRISM_OK;
-  PRISM_CHECK_ARG(q_offsets && k_offsets && o && aligned16(o) && (!lse || aligned16(lse)), "%s: null pointer, or an output off 16 bytes", what);
-  PRISM_CHECK_ARG((lse == nullptr) == (rest == nullptr) && (!lse || (dtype == PRISM_BF16 && aligned16(rest))),
+  PRISM_CHECK_ARG(q_offsets && k_offsets && o && aligned_to(o, 32) && aligned16(lse), "%s: null pointer, or o off 32 bytes", what);
+  PRISM_CHECK_ARG((lse == nullptr) == (rest == nullptr) && (!lse || (dtype == PRISM_BF16 && aligned_to(rest, 32))),
                   "%s: lse and rest belong together, of bf16", what);
-  PRISM_CHECK_ARG(lse || s.forward_parts() == 1 || (workspace && aligned16(workspace)), "%s: no workspace", what);
+  PRISM_CHECK_ARG(lse || s.forward_parts() == 1 || (workspace && aligned_to(workspace, 32)), "%s: no workspace, or one off 32 bytes", what);
   PRISM_TRY(packed::check_rows(q, q_strides, what, "q"));
   if (k_rows > 0) {
     PRISM_TRY(packed::check_rows(k, k_strides, what, "k"));
@@ -2075,8 +2075,9 @@ prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_stride
   PRISM_CHECK_ARG(q_rows > 0 && k_rows > 0, "%s: no rows (all gradients are zero)", what);
   PRISM_CHECK_ARG(q_offsets && k_offsets && o && rest && lse && workspace && (dk == nullptr) == (dv == nullptr),
                   "%s: null pointer", what);
-  PRISM_CHECK_ARG(aligned16(o) && aligned16(rest) && aligned16(lse) && aligned16(workspace) && aligned16(dq) && aligned16(dk) && aligned16(dv),
-                  "%s: buffers must start on 16 bytes", what);
+  PRISM_CHECK_ARG(aligned16(o) && aligned16(rest) && aligned16(lse) && aligned_to(workspace, 32) && aligned_to(dq, 32) && aligned_to(dk, 32) &&
+                      aligned_to(dv, 32),
+                  "%s: buffers must start on 32 bytes", what);
   PRISM_TRY(packed::check_rows(q, q_strides, what, "q"));
   PRISM_TRY(packed::check_rows(k, k_strides, what, "k"));
   PRISM_TRY(packed::check_rows(v, v_strides, what, "v"));

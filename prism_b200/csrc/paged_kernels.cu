@@ -278,11 +278,11 @@ struct Mma<__nv_bfloat16> {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   }
 };
-// fp16's p starts at 2^10 (keys down to 2^-34 of the largest count) and may grow to 2^15 before the maximum
+// fp16's p starts at 2^8 (keys down to 2^-32 of the largest count) and may grow to 2^15 before the maximum
 // is raised, as in packed_attention.cu.
 template <>
 struct Mma<__half> {
-  static constexpr float kShift = 10.0f, kLag = 5.0f;
+  static constexpr float kShift = 8.0f, kLag = 7.0f;
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
