@@ -467,17 +467,15 @@ struct FwdSteps {
 // What a forward leaves besides o: nothing; what the backward reads; a part's sums in o's place.
 enum Mode : int { kInfer, kTrain, kPart };
 
-// What rounding a value to 16 bits leaves, in units of 2^-8 of the 16 bits' last place: the difference of the
-// bit patterns, to 8 bits (the last half step, which they cannot hold, is cut).  32 values' worth of them.
-__device__ __forceinline__ uint32_t rest_of(float x, uint32_t high) {
-  return (uint32_t)min((int)(__float_as_uint(x) - high) + 128, 32767);
-}
+// What rounding an fp32 value to bf16 leaves, in 8 bits: the second byte of its bit pattern, signed.  The
+// lower half of the pattern is what was rounded off, up where its first bit is set (but for a value in the very
+// middle that went down, one in 2^17, which comes back a place too low).  The bytes of four values:
 __device__ __forceinline__ uint32_t rest_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0051), __byte_perm(c, d, 0x0051), 0x5410);
 }
-// ... and the value again, from its 16 bits and byte i of `left`.
+// ... and a value again, from its bf16 and byte i of `left`, to 2^-9 of bf16's last place.
 __device__ __forceinline__ float with_rest(uint32_t high, uint32_t left, int i) {
-  return __uint_as_float(high + (uint32_t)((int)(int8_t)(left >> (8 * i)) * 256));
+  return __uint_as_float(high + (uint32_t)((int)(int8_t)(left >> (8 * i)) * 256 + 128));
 }
 
 // What the parts of a row leave: sums [part][row][head][D] and (maximum, sum) [part][row][head].
@@ -878,9 +876,15 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int i = 0; i < 4; ++i) store32(dst + 8 * i, raw + 8 * i);
             }
           } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) raw[i] = __float_as_uint(u2f(raw[i]) * inv);
+            if (__any_sync(0xffffffffu, empty)) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) raw[i] = empty ? 0u : raw[i];
+            }
             uint32_t pk[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = empty ? 0u : H::pack(u2f(raw[2 * i]) * inv, u2f(raw[2 * i + 1]) * inv);
+            for (int i = 0; i < 16; ++i) pk[i] = H::pack(u2f(raw[2 * i]), u2f(raw[2 * i + 1]));
             if (valid) {
               T* dst = o + out_row * D + c * 32;
               store32(dst, pk), store32(dst + 16, pk + 8);
@@ -888,15 +892,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (kMode == kTrain) {
               uint32_t left[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                uint32_t d[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const uint32_t word = pk[2 * i + e / 2], high = (e & 1) ? word & 0xffff0000u : word << 16;
-                  d[e] = rest_of(empty ? 0.0f : u2f(raw[4 * i + e]) * inv, high);
-                }
-                left[i] = rest_bytes(d[0], d[1], d[2], d[3]);
-              }
+              for (int i = 0; i < 8; ++i) left[i] = rest_bytes(raw[4 * i], raw[4 * i + 1], raw[4 * i + 2], raw[4 * i + 3]);
               if (valid) store32(rest + out_row * D + c * 32, left);
             }
           }
