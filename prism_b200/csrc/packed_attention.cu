@@ -1040,7 +1040,10 @@ __global__ void __launch_bounds__(kDeltaThreads)
 // delta values instead of all of them.
 template <int D>
 struct DkdvLayout {
-  static constexpr int kRing = 2;
+  // 64 columns leave room in TMEM for a second S^T: that of step n + 1 is issued before P^T of step n is there
+  static constexpr bool kEarly = D == 64;
+  static constexpr int kScores = kEarly ? 2 : 1;
+  static constexpr int kRing = kEarly ? 3 : 2;
   static constexpr int kSub = D / 64;
   static constexpr int kTileBytes = kSub * 16384;
   static constexpr int K = 0;
@@ -1053,14 +1056,15 @@ struct DkdvLayout {
   static constexpr int ITEMS = TOKENS + kRows * 4;
   static constexpr int BAR = ITEMS + (ItemRing::kBytes + 15) / 16 * 16;
   static constexpr int B_KV = 0, B_KVE = 1,   // an item's keys; its last S^T and dP^T done
-                       B_QF = 2, B_QE = B_QF + kRing, B_SF = B_QE + kRing, B_DPF = B_SF + 1, B_PF = B_DPF + 1,
-                       B_DSF = B_PF + 1, B_FIN = B_DSF + 1, B_DRAIN = B_FIN + 1, NBAR = B_DRAIN + 1;
+                       B_QF = 2, B_QE = B_QF + kRing,
+                       B_SF = B_QE + kRing,   // [buffer]
+                       B_DPF = B_SF + kScores, B_PF = B_DPF + 1, B_DSF = B_PF + 1, B_FIN = B_DSF + 1, B_DRAIN = B_FIN + 1, NBAR = B_DRAIN + 1;
   static constexpr int TMEM_SLOT = BAR + NBAR * 8;
   static constexpr int ABORT = TMEM_SLOT + 4;
   static constexpr int SCRATCH = ABORT + 4;
   static constexpr size_t kNeed = 1024 + SCRATCH + 2 * 4 * (kThreads / 32);
   static constexpr size_t kBytes = kNeed > kMinSmem ? kNeed : kMinSmem;
-  static constexpr int T_DK = 0, T_DV = D, T_S = 2 * D, T_DP = 2 * D + 128;
+  static constexpr int T_DK = 0, T_DV = D, T_S = 2 * D, T_DP = T_S + 128 * kScores;
   static_assert(T_DP + 128 <= 512, "TMEM budget");
 };
 
@@ -1171,7 +1175,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(L::B_QF + i), 1);
       mbar_init(bar(L::B_QE + i), 1);
     }
-    mbar_init(bar(L::B_SF), 1);
+    for (int i = 0; i < L::kScores; ++i) mbar_init(bar(L::B_SF + i), 1);
     mbar_init(bar(L::B_DPF), 1);
     mbar_init(bar(L::B_PF), 8);
     mbar_init(bar(L::B_DSF), 8);
@@ -1245,7 +1249,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------- MMA issuer
-    // Steps of all items in one stream: S^T(n) | dK(n-1) | dP^T(n) | dV(n).  The softmax computes P^T(n) while
+    // Steps of all items in one stream: S^T(n) | dK(n-1) | dP^T(n) | dV(n), or, with two S^T, within an item
+    // dK(n-1) | S^T(n+1) | dP^T(n) | dV(n).  The softmax computes P^T(n) while
     // dK(n-1) and dP^T(n) run, dS^T(n) while dV(n) and S^T(n+1) do.  S^T(n) overwrites P^T(n-1), read by
     // dV(n-1), dP^T(n) overwrites dS^T(n-1), read by dK(n-1): issued earlier, and one thread's products run in
     // issue order.  An item's first dV and dK overwrite sums that the epilogue of the item before has read: the
@@ -1269,22 +1274,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       waiting = false;
       return true;
     };
-    const auto step = [&](int n, int steps) -> bool {
+    const auto scores = [&](int j) -> bool {  // S^T of step j
+      const uint32_t st = (uint32_t)j % R, buffer = (uint32_t)j % L::kScores;
+      if (!wait(L::B_QF + st, j / R)) return false;
+      tc_fence_after();
+      mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S + 128 * buffer, dK, dQk + st * kSlot, kIdS, 0u);
+      mma_commit(bar(L::B_SF + buffer));
+      return true;
+    };
+    // step n of `steps`; early: S^T of it is issued; next: S^T of the one behind it may be
+    const auto step = [&](int n, int steps, bool early, bool next) -> bool {
       const uint32_t st = (uint32_t)ns % R;
       if (n == 0 && !wait(L::B_KV, n_kv)) return false;
-      if (!wait(L::B_QF + st, ns / R)) return false;
-      tc_fence_after();
-      mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S, dK, dQk + st * kSlot, kIdS, 0u);
-      mma_commit(bar(L::B_SF));
+      if (!early && !scores(ns)) return false;
       if (waiting && !dk_step()) return false;
+      if (next && !scores(ns + 1)) return false;
       mma_kd<L::kSub, 16384, 16384>(tmem + L::T_DP, dV, dDOk + st * kSlot, kIdS, 0u);
       mma_commit(bar(L::B_DPF));
       first = n == 0, last = n + 1 == steps;
       if (last) mma_commit(bar(L::B_KVE)), ++n_kv;
       if (!wait(L::B_PF, ns)) return false;
       tc_fence_after();
-      mma_ts_k64_mn(tmem + L::T_DV, tmem + L::T_S, dDOmn + st * kSlot, kIdG, first ? 0u : 1u);
-      mma_ts_k64_mn(tmem + L::T_DV, tmem + L::T_S + 64, dDOmn + st * kSlot + 512, kIdG, 1u);
+      const uint32_t p = tmem + L::T_S + 128 * ((uint32_t)ns % L::kScores);
+      mma_ts_k64_mn(tmem + L::T_DV, p, dDOmn + st * kSlot, kIdG, first ? 0u : 1u);
+      mma_ts_k64_mn(tmem + L::T_DV, p + 64, dDOmn + st * kSlot + 512, kIdG, 1u);
       ++ns;
       waiting = true;
       return true;
@@ -1303,7 +1316,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       any = true;
       const int plain = w.tail ? w.steps - 1 : w.steps;
       if (lane == 0)
-        for (int n = 0; ok && n < plain; ++n) ok = step(n, w.steps);
+        for (int n = 0; ok && n < plain; ++n)
+          ok = step(n, w.steps, L::kEarly && n > 0, L::kEarly && n + 1 < plain);
       ok = __all_sync(0xffffffffu, ok);
       if (lane != 0) ns += plain;
       if (w.tail && ok) {  // the next sequence's rows, which dK and dV sum over
@@ -1316,7 +1330,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           fence_proxy_async_smem();
         }
         __syncwarp();
-        if (lane == 0 && ok) ok = step(plain, w.steps);
+        if (lane == 0 && ok) ok = step(plain, w.steps, false, false);
         ok = __all_sync(0xffffffffu, ok);
         if (lane != 0) ++ns;
       }
@@ -1358,15 +1372,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int seen = (w.first + n) * n_tok + w.shift + 1 - w.key0;
         const bool masked = causal && seen < kRows;
         if (!wait_warp(bar(L::B_QF + st), (ns / R) & 1, abort_flag, kErrDkdvSoftmax) ||
-            !wait_warp(bar(L::B_SF), ns & 1, abort_flag, kErrDkdvSoftmax)) {
+            !wait_warp(bar(L::B_SF + ns % L::kScores), (ns / L::kScores) & 1, abort_flag, kErrDkdvSoftmax)) {
           ok = false;
           break;
         }
         tc_fence_after();
         float p[64];
+        const uint32_t t_scores = t_lane + L::T_S + 128 * (ns % L::kScores) + tcol;
         // key < seen + tokens[column]
-        if (masked) dkdv_p<T, true>(t_lane + L::T_S + tcol, sM + st * 128, qk_scale, lane, tokens + tcol, key - seen, p);
-        else dkdv_p<T, false>(t_lane + L::T_S + tcol, sM + st * 128, qk_scale, lane, nullptr, 0, p);
+        if (masked) dkdv_p<T, true>(t_scores, sM + st * 128, qk_scale, lane, tokens + tcol, key - seen, p);
+        else dkdv_p<T, false>(t_scores, sM + st * 128, qk_scale, lane, nullptr, 0, p);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
