@@ -402,16 +402,16 @@ __device__ __forceinline__ void mask_from(float (&s)[64], int lim) {
 template <typename T>
 __device__ __forceinline__ float exp_pairs(const float (&s)[64], float scale, float m, uint32_t (&pk)[32]) {
   const float2 sc = make_float2(scale, scale), nm = make_float2(-m, -m);
-  float su0 = 0.f, su1 = 0.f;
+  float2 even = make_float2(0.f, 0.f), odd = even;
 #pragma unroll
   for (int c = 0; c < 32; ++c) {
     const float2 x = __ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sc, nm);
-    const float p0 = ex2(x.x), p1 = ex2(x.y);
-    su0 += p0;
-    su1 += p1;
-    pk[c] = Half<T>::pack(p0, p1);
+    const float2 p = make_float2(ex2(x.x), ex2(x.y));
+    if (c & 1) odd = __fadd2_rn(odd, p);
+    else even = __fadd2_rn(even, p);
+    pk[c] = Half<T>::pack(p.x, p.y);
   }
-  return su0 + su1;
+  return (even.x + even.y) + (odd.x + odd.y);
 }
 
 // ===================================================================== forward
@@ -420,6 +420,8 @@ __device__ __forceinline__ float exp_pairs(const float (&s)[64], float scale, fl
 // few tiles and long keys, an item is a part of the steps, and join_kernel adds the parts up.
 template <int D>
 struct FwdLayout {
+  // 64 columns leave room in TMEM for a third S: that of a group's next step is issued before its P is there
+  static constexpr int kScores = D == 64 ? 3 : 2;
   static constexpr int kRing = 2;
   static constexpr int kSub = D / 64;
   static constexpr int kTileBytes = kSub * 16384;
@@ -430,17 +432,23 @@ struct FwdLayout {
   static constexpr int BAR = ITEMS + (ItemRing::kBytes + 15) / 16 * 16;
   static constexpr int B_QF = 0, B_QE = 2,    // [g]: Q of the group; its last S done
                        B_KF = 4, B_KE = B_KF + kRing, B_VF = B_KE + kRing, B_VE = B_VF + kRing,
-                       B_SF = B_VE + kRing,   // [g]: S of the group
-                       B_PF = B_SF + 2,       // [g]: P in TMEM (and O rescaled)
-                       B_OF = B_PF + 2,       // [g]: last P V of an item done
+                       B_SF = B_VE + kRing,   // [barrier()]: S of the group
+                       B_PF = B_SF + 4,       // [barrier()]: P in TMEM (and O rescaled)
+                       B_PV = B_PF + 4,       // [g]: P V done
+                       B_OF = B_PV + 2,       // [g]: last P V of an item done
                        B_DRAIN = B_OF + 2, NBAR = B_DRAIN + 1;
   static constexpr int TMEM_SLOT = BAR + NBAR * 8;
   static constexpr int ABORT = TMEM_SLOT + 4;
   static constexpr int SCRATCH = ABORT + 4;
   static constexpr size_t kNeed = 1024 + SCRATCH + 2 * 4 * (kThreads / 32);
   static constexpr size_t kBytes = kNeed > kMinSmem ? kNeed : kMinSmem;
-  // TMEM of group g at 256 g: S (128 fp32 columns; P as pairs over the first 64), O
-  static constexpr int T_S = 0, T_O = 128;
+  // TMEM: O of each group (D columns), then the S (128 fp32 columns each; P as pairs over the first 64)
+  static constexpr int T_O = 0, T_S = 2 * D;
+  static_assert(T_S + 128 * kScores <= 512, "TMEM budget");
+  // With three S a group may be a step ahead of what the issuer has waited for: its steps take two barriers in
+  // turn, or a second phase would look like none.
+  static __device__ __forceinline__ int barrier(int g, int step) { return 2 * g + (kScores > 2 ? step & 1 : 0); }
+  static __device__ __forceinline__ int phase(int step) { return (kScores > 2 ? step >> 1 : step) & 1; }
 };
 
 // The steps of an item: groups' last tokens, the part's first step and each group's number of them.
@@ -513,8 +521,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int g = 0; g < 2; ++g) {
       mbar_init(bar(L::B_QF + g), 1);
       mbar_init(bar(L::B_QE + g), 1);
-      mbar_init(bar(L::B_SF + g), 1);
-      mbar_init(bar(L::B_PF + g), 4);
+      mbar_init(bar(L::B_SF + 2 * g), 1);
+      mbar_init(bar(L::B_SF + 2 * g + 1), 1);
+      mbar_init(bar(L::B_PF + 2 * g), 4);
+      mbar_init(bar(L::B_PF + 2 * g + 1), 4);
+      mbar_init(bar(L::B_PV + g), 1);
       mbar_init(bar(L::B_OF + g), 1);
     }
     mbar_init(bar(L::B_DRAIN), 1);
@@ -589,120 +600,229 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------- MMA issuer
-    // Steps of all items in one stream, by lane 0: every instruction between a P and its products is time that
-    // the tensor core idles (32,768 causal tokens took 8.9 ms with votes of the warp in each wait, 8.4 without
-    // and 8.2 with inner()).  Step n, group by group: P V of the group's step before it, then S of step n over the columns that
-    // held that P (one thread's products run in issue order).  An item's first P V overwrites an O that the
+    // Steps of both groups and of all items in one stream, by lane 0: every instruction between a P and its
+    // products is time that the tensor core idles (32,768 causal tokens took 8.9 ms with votes of the warp in
+    // each wait).  One thread's products run in issue order.  An item's first P V overwrites an O that the
     // epilogue of the item before has read: the P that it waits for is written after it.
     constexpr uint32_t kIdS = idesc<T>(kRows, false), kIdO = idesc<T>(D, true);
     const uint64_t dQ = desc_k_sw128(sb + L::Q), dK = desc_k_sw128(sb + L::K), dV = desc_mn_sw128(sb + L::V, 16384);
     constexpr uint32_t kSlot = L::kTileBytes >> 4;
-    int ns = 0, v_rows = 0;                        // steps so far; keys of the last one, 0: its P V is issued
-    int n_s[2] = {0, 0}, n_q[2] = {0, 0};
-    bool waiting[2] = {false, false}, first[2] = {}, last[2] = {};  // P V of the last step still to come
+    int v_rows = kRows, steps = 0;                 // keys of the last item's last step; all steps so far
     const auto wait = [&](int i, int parity) { return wait_one(bar(i), parity & 1, abort_flag, kErrFwdMma); };
-    const auto pv = [&](int g) -> bool {
-      const int before = (ns - 1) % R;
-      const uint32_t t = tmem + g * 256;
-      if (!wait(L::B_PF + g, n_s[g] - 1)) return false;
-      tc_fence_after();
-      const uint64_t b = dV + before * kSlot;
-      mma_ts_k64_mn(t + L::T_O, t + L::T_S, b, kIdO, first[g] ? 0u : 1u);
-      mma_ts_k64_mn(t + L::T_O, t + L::T_S + 32, b + (8192 >> 4), kIdO, 1u);
-      if (last[g]) mma_commit(bar(L::B_OF + g));
-      waiting[g] = false;
-      return true;
-    };
-    const auto step = [&](int n, int n0, int n1) -> bool {
-      const int st = ns % R, before = (ns - 1) % R;
-      const bool any = waiting[0] || waiting[1];
-      if (!wait(L::B_KF + st, ns / R) || (any && !wait(L::B_VF + before, (ns - 1) / R))) return false;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const int of_group = g ? n1 : n0;
-        if (waiting[g] && !pv(g)) return false;
-        if (n >= of_group) continue;
-        first[g] = n == 0, last[g] = n + 1 == of_group;
-        if (first[g]) {
-          if (!wait(L::B_QF + g, n_q[g])) return false;
-          tc_fence_after();
+    // the items: item_steps issues an item's steps, finish what is still open
+    const auto run = [&](const auto& item_steps, const auto& finish) {
+      // all lanes: the last item's last V is there, its rows behind the sequence zero
+      const auto clear_tail = [&]() -> bool {
+        if (v_rows == kRows) return true;
+        const int slot = (steps - 1) % R;
+        const bool ok = wait_warp(bar(L::B_VF + slot), ((steps - 1) / R) & 1, abort_flag, kErrFwdMma);
+        if (ok) {
+          zero_rows<L::kSub>(sm + L::V + slot * L::kTileBytes, v_rows, lane, 32);
+          fence_proxy_async_smem();
         }
-        mma_kd<L::kSub, 16384, 16384>(tmem + g * 256 + L::T_S, dQ + g * kSlot, dK + st * kSlot, kIdS, 0u);
-        mma_commit(bar(L::B_SF + g));
-        if (last[g]) mma_commit(bar(L::B_QE + g)), ++n_q[g];
-        ++n_s[g];
-        waiting[g] = true;
+        v_rows = kRows;
+        __syncwarp();
+        return ok;
+      };
+      const auto flush = [&]() -> bool {
+        bool ok = clear_tail();
+        if (lane == 0 && ok) ok = finish();
+        return __all_sync(0xffffffffu, ok);
+      };
+      bool ok = true;
+      while (ok) {
+        // an item that is not there yet is not waited for with products to issue
+        if (!__any_sync(0xffffffffu, item_ready(items, ring))) ok = flush();
+        if (!ok || !next_item(at, items, sm + L::ITEMS, ring, abort_flag, lane, kErrFwdMma)) break;
+        if (at.kind != kTile) continue;
+        const FwdSteps w(at, n_tok, causal, grid.parts);
+        if (w.total == 0) continue;
+        ok = clear_tail();
+        if (lane == 0 && ok) ok = item_steps(w.n[0], w.n[1]);
+        ok = __all_sync(0xffffffffu, ok);
+        steps += w.total;
+        v_rows = min(at.nk - (w.from + w.total - 1) * kRows, kRows);
       }
-      mma_commit(bar(L::B_KE + st));
-      if (any) mma_commit(bar(L::B_VE + before));
-      ++ns;
-      return true;
+      if (ok) flush();
     };
-    // a step that is neither the first two nor the last one of either group: the same, without the cases
-    const auto inner = [&]() -> bool {
-      const int st = ns % R, before = (ns - 1) % R;
-      if (!wait(L::B_KF + st, ns / R) || !wait(L::B_VF + before, (ns - 1) / R)) return false;
-#pragma unroll
-      for (int g = 0; g < 2; ++g) {
-        const uint32_t t = tmem + g * 256;
-        if (!wait(L::B_PF + g, n_s[g] - 1)) return false;
+    if constexpr (L::kScores == 2) {
+      // Step n, group by group: P V of the group's step before it, then S of step n over the columns that held
+      // that P.
+      int ns = 0;                                    // steps so far
+      int n_s[2] = {0, 0}, n_q[2] = {0, 0};
+      bool waiting[2] = {false, false}, first[2] = {}, last[2] = {};  // P V of the last step still to come
+      const auto pv = [&](int g) -> bool {
+        const int before = (ns - 1) % R;
+        const uint32_t t_o = tmem + L::T_O + g * D, t_s = tmem + L::T_S + 128 * g;
+        if (!wait(L::B_PF + 2 * g, n_s[g] - 1)) return false;
         tc_fence_after();
         const uint64_t b = dV + before * kSlot;
-        mma_ts_k64_mn(t + L::T_O, t + L::T_S, b, kIdO, 1u);
-        mma_ts_k64_mn(t + L::T_O, t + L::T_S + 32, b + (8192 >> 4), kIdO, 1u);
-        mma_kd<L::kSub, 16384, 16384>(t + L::T_S, dQ + g * kSlot, dK + st * kSlot, kIdS, 0u);
-        mma_commit(bar(L::B_SF + g));
-        ++n_s[g];
-      }
-      mma_commit(bar(L::B_KE + st));
-      mma_commit(bar(L::B_VE + before));
-      ++ns;
-      return true;
-    };
-    // all lanes: the last step's V is there, its rows behind the sequence zero
-    const auto clear_tail = [&]() -> bool {
-      if (v_rows == 0 || v_rows == kRows) return true;
-      const int before = (ns - 1) % R;
-      if (!wait_warp(bar(L::B_VF + before), ((ns - 1) / R) & 1, abort_flag, kErrFwdMma)) return false;
-      zero_rows<L::kSub>(sm + L::V + before * L::kTileBytes, v_rows, lane, 32);
-      fence_proxy_async_smem();
-      __syncwarp();
-      return true;
-    };
-    const auto flush = [&]() -> bool {
-      bool ok = clear_tail();
-      if (lane == 0 && ok && v_rows > 0) {
-        const int before = (ns - 1) % R;
-        ok = wait(L::B_VF + before, (ns - 1) / R);
+        mma_ts_k64_mn(t_o, t_s, b, kIdO, first[g] ? 0u : 1u);
+        mma_ts_k64_mn(t_o, t_s + 32, b + (8192 >> 4), kIdO, 1u);
+        if (last[g]) mma_commit(bar(L::B_OF + g));
+        waiting[g] = false;
+        return true;
+      };
+      const auto step = [&](int n, int n0, int n1) -> bool {
+        const int st = ns % R, before = (ns - 1) % R;
+        const bool any = waiting[0] || waiting[1];
+        if (!wait(L::B_KF + st, ns / R) || (any && !wait(L::B_VF + before, (ns - 1) / R))) return false;
 #pragma unroll
-        for (int g = 0; g < 2; ++g) ok = ok && (!waiting[g] || pv(g));
-        if (ok) mma_commit(bar(L::B_VE + before));
-      }
-      v_rows = 0;
-      return __all_sync(0xffffffffu, ok);
-    };
-    bool ok = true;
-    while (ok) {
-      // an item that is not there yet is not waited for with products to issue
-      if (v_rows > 0 && !__any_sync(0xffffffffu, item_ready(items, ring))) ok = flush();
-      if (!ok || !next_item(at, items, sm + L::ITEMS, ring, abort_flag, lane, kErrFwdMma)) break;
-      if (at.kind != kTile) continue;
-      const FwdSteps w(at, n_tok, causal, grid.parts);
-      if (w.total == 0) continue;
-      ok = clear_tail();
-      const int both = min(w.n[0], w.n[1]);
-      if (lane == 0) {
-        for (int n = 0; ok && n < w.total; ++n) {
-          ok = step(n, w.n[0], w.n[1]);
-          if (n == 1)
-            for (; ok && n + 2 < both; ++n) ok = inner();
+        for (int g = 0; g < 2; ++g) {
+          const int of_group = g ? n1 : n0;
+          if (waiting[g] && !pv(g)) return false;
+          if (n >= of_group) continue;
+          first[g] = n == 0, last[g] = n + 1 == of_group;
+          if (first[g]) {
+            if (!wait(L::B_QF + g, n_q[g])) return false;
+            tc_fence_after();
+          }
+          mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S + 128 * g, dQ + g * kSlot, dK + st * kSlot, kIdS, 0u);
+          mma_commit(bar(L::B_SF + 2 * g));
+          if (last[g]) mma_commit(bar(L::B_QE + g)), ++n_q[g];
+          ++n_s[g];
+          waiting[g] = true;
         }
-      }
-      ok = __all_sync(0xffffffffu, ok);
-      if (lane != 0) ns += w.total;
-      v_rows = min(at.nk - (w.from + w.total - 1) * kRows, kRows);
+        mma_commit(bar(L::B_KE + st));
+        if (any) mma_commit(bar(L::B_VE + before));
+        ++ns;
+        return true;
+      };
+      // a step that is neither the first two nor the last one of either group: the same, without the cases
+      const auto inner = [&]() -> bool {
+        const int st = ns % R, before = (ns - 1) % R;
+        if (!wait(L::B_KF + st, ns / R) || !wait(L::B_VF + before, (ns - 1) / R)) return false;
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const uint32_t t_o = tmem + L::T_O + g * D, t_s = tmem + L::T_S + 128 * g;
+          if (!wait(L::B_PF + 2 * g, n_s[g] - 1)) return false;
+          tc_fence_after();
+          const uint64_t b = dV + before * kSlot;
+          mma_ts_k64_mn(t_o, t_s, b, kIdO, 1u);
+          mma_ts_k64_mn(t_o, t_s + 32, b + (8192 >> 4), kIdO, 1u);
+          mma_kd<L::kSub, 16384, 16384>(t_s, dQ + g * kSlot, dK + st * kSlot, kIdS, 0u);
+          mma_commit(bar(L::B_SF + 2 * g));
+          ++n_s[g];
+        }
+        mma_commit(bar(L::B_KE + st));
+        mma_commit(bar(L::B_VE + before));
+        ++ns;
+        return true;
+      };
+      const auto item_steps = [&](int n0, int n1) -> bool {
+        const int total = max(n0, n1), both = min(n0, n1);
+        for (int n = 0; n < total; ++n) {
+          if (!step(n, n0, n1)) return false;
+          if (n == 1)
+            for (; n + 2 < both; ++n)
+              if (!inner()) return false;
+        }
+        return true;
+      };
+      const auto finish = [&]() -> bool {
+        if (!waiting[0] && !waiting[1]) return true;
+        const int before = (ns - 1) % R;
+        if (!wait(L::B_VF + before, (ns - 1) / R)) return false;
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          if (waiting[g] && !pv(g)) return false;
+        mma_commit(bar(L::B_VE + before));
+        return true;
+      };
+      run(item_steps, finish);
+    } else {
+      // S goes to the three buffers in turn; one is free again when the P V that read its P is issued, so that
+      // S of a group's next step is issued before its P is there (8,192 tokens, 32 + 8 heads: 859 -> 728 us).
+      // What is known of an open P V, 8 bits each, the oldest first
+      constexpr uint32_t kGroup = 1, kFirst = 2, kLast = 4, kNewV = 8, kEndV = 16;
+      uint32_t queue = 0, s_at = 0, p_at = 0;        // ... the buffers of the next S and of the oldest P
+      int open = 0, n_k = 0, n_v = 0;                // steps whose S, whose P V are all issued
+      int s0 = 0, s1 = 0, p0 = 0, p1 = 0, q0 = 0, q1 = 0;  // S, P V and items of the two groups
+      const auto next = [](uint32_t i) { return i + 1 == L::kScores ? 0u : i + 1; };
+      // P V of group g, its P the oldest; the step's V is in slot n_v % R
+      const auto pv = [&](int g, bool first) -> bool {
+        const int j = g ? p1++ : p0++;
+        if (!wait(L::B_PF + L::barrier(g, j), L::phase(j))) return false;
+        tc_fence_after();
+        const uint64_t b = dV + ((uint32_t)n_v % R) * kSlot;
+        const uint32_t o_at = tmem + L::T_O + g * D, p = tmem + L::T_S + 128 * p_at;
+        mma_ts_k64_mn(o_at, p, b, kIdO, first ? 0u : 1u);
+        mma_ts_k64_mn(o_at, p + 32, b + (8192 >> 4), kIdO, 1u);
+        mma_commit(bar(L::B_PV + g));
+        p_at = next(p_at);
+        return true;
+      };
+      const auto wait_v = [&] { return wait(L::B_VF + n_v % R, n_v / R); };
+      const auto end_v = [&] { mma_commit(bar(L::B_VE + n_v % R)), ++n_v; };
+      // S of group g's next step, K in slot n_k % R
+      const auto scores = [&](int g) {
+        const int j = g ? s1++ : s0++;
+        mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S + 128 * s_at, dQ + g * kSlot, dK + ((uint32_t)n_k % R) * kSlot, kIdS, 0u);
+        mma_commit(bar(L::B_SF + L::barrier(g, j)));
+        s_at = next(s_at);
+      };
+      const auto end_k = [&] { mma_commit(bar(L::B_KE + n_k % R)), ++n_k; };
+      // the oldest open P V
+      const auto close = [&]() -> bool {
+        const uint32_t info = queue & 255u;
+        queue >>= 8, --open;
+        if ((info & kNewV) && !wait_v()) return false;
+        if (!pv((info & kGroup) != 0, (info & kFirst) != 0)) return false;
+        if (info & kLast) mma_commit(bar(L::B_OF + (info & kGroup)));
+        if (info & kEndV) end_v();
+        return true;
+      };
+      // The next K is loaded behind the last V, and that one when the V of kRing steps before is free: more steps
+      // than that may not be open when it is waited for (three, where one group alone takes every S).
+      const auto within_ring = [&]() -> bool {
+        while (n_k - n_v > R)
+          if (!close()) return false;
+        return true;
+      };
+      const auto item_steps = [&](int n0, int n1) -> bool {
+        const int total = max(n0, n1), both = min(n0, n1);
+        for (int n = 0; n < total; ++n) {
+          if (!within_ring() || !wait(L::B_KF + n_k % R, n_k / R)) return false;
+          tc_fence_after();
+          if (n >= L::kScores && n + 1 < both) {
+            // neither group's first or last step, nor are the open ones first steps: the same as below, and the
+            // queue stays what it is
+            if (!pv(1, false)) return false;
+            end_v();
+            scores(0);
+            if (!wait_v() || !pv(0, false)) return false;
+            scores(1);
+            end_k();
+            continue;
+          }
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const int mine = g ? n1 : n0, other = g ? n0 : n1;
+            if (n >= mine) continue;
+            const bool alone = n >= other;
+            if (n == 0) {
+              if (!wait(L::B_QF + g, g ? q1 : q0)) return false;
+              tc_fence_after();
+            }
+            if (open == L::kScores && !close()) return false;
+            scores(g);
+            const bool last = n + 1 == mine;
+            if (last) mma_commit(bar(L::B_QE + g)), g ? ++q1 : ++q0;
+            queue |= ((uint32_t)g | (n == 0 ? kFirst : 0) | (last ? kLast : 0) | (g == 0 || alone ? kNewV : 0) |
+                      (g == 1 || alone ? kEndV : 0)) << (8 * open);
+            ++open;
+            if (g == 1 || alone) end_k();
+          }
+        }
+        return within_ring();
+      };
+      const auto finish = [&]() -> bool {
+        while (open > 0)
+          if (!close()) return false;
+        return true;
+      };
+      run(item_steps, finish);
     }
-    if (ok) flush();
     // every product is done before TMEM is released
     if (lane == 0) {
       mma_commit(bar(L::B_DRAIN));
@@ -714,9 +834,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int g = warp >> 2;
     const int r = (warp & 3) * 32 + lane;  // row of the tile == TMEM lane
     const int t_of_row = over_group(r, group_inverse(hd.group)), head_of_row = r - t_of_row * hd.group;
-    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * 256;
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_o = t_lane + L::T_O + g * D;
     const int heads = hd.keys * hd.group;
     int n_s = 0, n_o = 0;
+    uint32_t before = 0;  // steps of both groups in the items before
     bool ok = true;
     while (ok && next_item(at, items, sm + L::ITEMS, ring, abort_flag, lane, kErrFwdSoftmax)) {
       if (at.kind != kTile) {
@@ -728,7 +849,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         continue;
       }
       const FwdSteps w(at, n_tok, causal, grid.parts);
-      const int n_steps = g ? w.n[1] : w.n[0], last = g ? w.last[1] : w.last[0];
+      const int n_steps = g ? w.n[1] : w.n[0], of_other = g ? w.n[0] : w.n[1], last = g ? w.last[1] : w.last[0];
       const int tok = w.tok0 + g * n_tok + t_of_row;
       const bool valid = r < rows && tok < at.nq;
       // keys that this row sees; rows without a token go along with the last one
@@ -739,14 +860,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int lim0 = seen - (w.from + n) * kRows, lim1 = lim0 - 64;
         const bool all0 = __all_sync(0xffffffffu, lim0 >= 64), all1 = __all_sync(0xffffffffu, lim1 >= 64);
         const bool none0 = __all_sync(0xffffffffu, lim0 <= 0), none1 = __all_sync(0xffffffffu, lim1 <= 0);
-        if (!wait_warp(bar(L::B_SF + g), n_s & 1, abort_flag, kErrFwdSoftmax)) {
+        if (!wait_warp(bar(L::B_SF + L::barrier(g, n_s)), L::phase(n_s), abort_flag, kErrFwdSoftmax)) {
           ok = false;
           break;
         }
         ++n_s;
         tc_fence_after();
+        // its S: the group's, or, of three, the steps of both groups take them in turn
+        const uint32_t t_s =
+            t_lane + L::T_S + 128 * (L::kScores == 2 ? (uint32_t)g : (before + n + min(n + g, of_other)) % 3);
+        // before O is touched, the group's P V before is done: with two S, the step's own S was issued after it
+        const auto o_settled = [&] {
+          if (L::kScores > 2 && n > 0) ok = wait_warp(bar(L::B_PV + g), n_s & 1, abort_flag, kErrFwdSoftmax);
+        };
         const auto scores = [&](int u, float(&s)[64]) {
-          tmem_load<2>(t_lane + L::T_S + u * 64, s);
+          tmem_load<2>(t_s + u * 64, s);
           if (!(u ? all1 : all0)) mask_from(s, u ? lim1 : lim0);
         };
         float sum0 = 0.f, sum1 = 0.f;
@@ -789,8 +917,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool o_live = __any_sync(0xffffffffu, need && m != -INFINITY);
             l *= alpha;
             m = m_new;
-            // every earlier P V of the group is done: S was issued after them
-            if (n > 0 && o_live) scale_tmem_rows<D / 32>(t_lane + L::T_O, alpha);
+            if (n > 0 && o_live) {
+              o_settled();
+              scale_tmem_rows<D / 32>(t_o, alpha);
+            }
           }
           const float mb = (m == -INFINITY) ? 0.0f : m;
 #pragma unroll
@@ -805,10 +935,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float t = exp_pairs<T>(s, qk_scale, mb, pk);
               if (u) sum1 = t; else sum0 = t;
             }
-            tmem_st32(t_lane + L::T_S + u * 32, pk);  // over scores of the first half, which are read
+            tmem_st32(t_s + u * 32, pk);  // over scores of the first half, which are read
           }
         } else {
-          tmem_st32(t_lane + L::T_S, pk0);
+          tmem_st32(t_s, pk0);
           uint32_t pk1[32];
           if (none1) {
 #pragma unroll
@@ -824,30 +954,33 @@ __global__ void __launch_bounds__(kThreads, 1)
             scores(1, s);
             const float m_new = need ? fmaxf(m, tile_max(s) * qk_scale - H::kShift) : m;
             const float alpha = ex2(m - m_new);
-            if (n > 0) scale_tmem_rows<D / 32>(t_lane + L::T_O, alpha);
+            o_settled();
+            if (n > 0) scale_tmem_rows<D / 32>(t_o, alpha);
             tmem_wait_st();
             uint32_t raw[32];
-            tmem_ld32(t_lane + L::T_S, raw);
+            tmem_ld32(t_s, raw);
             tmem_wait_ld_dep(raw);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
               const float2 p = H::unpack(raw[i]);
               raw[i] = H::pack(p.x * alpha, p.y * alpha);
             }
-            tmem_st32(t_lane + L::T_S, raw);
+            tmem_st32(t_s, raw);
             l = (l + sum0) * alpha;
             sum0 = 0.f;
             m = m_new;
             sum1 = exp_pairs<T>(s, qk_scale, m, pk1);
           }
-          tmem_st32(t_lane + L::T_S + 32, pk1);
+          tmem_st32(t_s + 32, pk1);
         }
         l += sum0 + sum1;
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(L::B_PF + g));
+        if (lane == 0) mbar_arrive(bar(L::B_PF + L::barrier(g, n_s - 1)));
+        if (!ok) break;
       }
+      before += w.n[0] + w.n[1];
       if (!ok) break;
       // epilogue
       const bool empty = m == -INFINITY;  // no key
@@ -867,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t raw[32];
-          tmem_ld32(t_lane + L::T_O + c * 32, raw);
+          tmem_ld32(t_o + c * 32, raw);
           tmem_wait_ld_dep(raw);
           if constexpr (kMode == kPart) {
             float* dst = parts.o + ((int64_t)at.part * seqs.q_rows * heads + out_row) * D + c * 32;
@@ -1250,8 +1383,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kMmaWarp) {
     // ---------------------------------------------------------- MMA issuer
     // Steps of all items in one stream: S^T(n) | dK(n-1) | dP^T(n) | dV(n), or, with two S^T, within an item
-    // dK(n-1) | S^T(n+1) | dP^T(n) | dV(n).  The softmax computes P^T(n) while
-    // dK(n-1) and dP^T(n) run, dS^T(n) while dV(n) and S^T(n+1) do.  S^T(n) overwrites P^T(n-1), read by
+    // dK(n-1) | S^T(n+1) | dP^T(n) | dV(n).  The softmax computes P^T(n) while dK(n-1) and dP^T(n) run, dS^T(n)
+    // while dV(n) and S^T(n+1) do.  S^T(n) overwrites P^T(n-1), read by
     // dV(n-1), dP^T(n) overwrites dS^T(n-1), read by dK(n-1): issued earlier, and one thread's products run in
     // issue order.  An item's first dV and dK overwrite sums that the epilogue of the item before has read: the
     // P^T and dS^T that they wait for are written after it.
