@@ -804,7 +804,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!wait(L::B_QF + g, g ? q1 : q0)) return false;
               tc_fence_after();
             }
-            if (open == L::kScores && !close()) return false;
+            // a buffer, and no third step of one group: it has two barriers
+            while (open == L::kScores || (g ? s1 - p1 : s0 - p0) == 2)
+              if (!close()) return false;
             scores(g);
             const bool last = n + 1 == mine;
             if (last) mma_commit(bar(L::B_QE + g)), g ? ++q1 : ++q0;
