@@ -481,9 +481,10 @@ enum Mode : int { kInfer, kTrain, kPart };
 __device__ __forceinline__ uint32_t rest_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0051), __byte_perm(c, d, 0x0051), 0x5410);
 }
-// ... and a value again, from its bf16 and byte i of `left`, to 2^-9 of bf16's last place.
+// ... and a value again, from its bf16 and byte i of `left`, to 2^-8 of bf16's last place; one that is a bf16
+// comes back as it was.
 __device__ __forceinline__ float with_rest(uint32_t high, uint32_t left, int i) {
-  return __uint_as_float(high + (uint32_t)((int)(int8_t)(left >> (8 * i)) * 256 + 128));
+  return __uint_as_float(high + (uint32_t)((int)(int8_t)(left >> (8 * i)) * 256));
 }
 
 // What the parts of a row leave: sums [part][row][head][D] and (maximum, sum) [part][row][head].
@@ -1193,7 +1194,9 @@ struct DkdvLayout {
   static constexpr int B_KV = 0, B_KVE = 1,   // an item's keys; its last S^T and dP^T done
                        B_QF = 2, B_QE = B_QF + kRing,
                        B_SF = B_QE + kRing,   // [buffer]
-                       B_DPF = B_SF + kScores, B_PF = B_DPF + 1, B_DSF = B_PF + 1, B_FIN = B_DSF + 1, B_DRAIN = B_FIN + 1, NBAR = B_DRAIN + 1;
+                       B_DPF = B_SF + kScores,
+                       B_PF = B_DPF + 1,      // [buffer]: a warp may be at P^T of the next S^T before all are at this one
+                       B_DSF = B_PF + kScores, B_FIN = B_DSF + 1, B_DRAIN = B_FIN + 1, NBAR = B_DRAIN + 1;
   static constexpr int TMEM_SLOT = BAR + NBAR * 8;
   static constexpr int ABORT = TMEM_SLOT + 4;
   static constexpr int SCRATCH = ABORT + 4;
@@ -1310,9 +1313,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(bar(L::B_QF + i), 1);
       mbar_init(bar(L::B_QE + i), 1);
     }
-    for (int i = 0; i < L::kScores; ++i) mbar_init(bar(L::B_SF + i), 1);
+    for (int i = 0; i < L::kScores; ++i) {
+      mbar_init(bar(L::B_SF + i), 1);
+      mbar_init(bar(L::B_PF + i), 8);
+    }
     mbar_init(bar(L::B_DPF), 1);
-    mbar_init(bar(L::B_PF), 8);
     mbar_init(bar(L::B_DSF), 8);
     mbar_init(bar(L::B_FIN), 1);
     mbar_init(bar(L::B_DRAIN), 1);
@@ -1428,9 +1433,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       mma_commit(bar(L::B_DPF));
       first = n == 0, last = n + 1 == steps;
       if (last) mma_commit(bar(L::B_KVE)), ++n_kv;
-      if (!wait(L::B_PF, ns)) return false;
+      const uint32_t buffer = (uint32_t)ns % L::kScores, p = tmem + L::T_S + 128 * buffer;
+      if (!wait(L::B_PF + buffer, ns / L::kScores)) return false;
       tc_fence_after();
-      const uint32_t p = tmem + L::T_S + 128 * ((uint32_t)ns % L::kScores);
       mma_ts_k64_mn(tmem + L::T_DV, p, dDOmn + st * kSlot, kIdG, first ? 0u : 1u);
       mma_ts_k64_mn(tmem + L::T_DV, p + 64, dDOmn + st * kSlot + 512, kIdG, 1u);
       ++ns;
@@ -1520,7 +1525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(L::B_PF));
+        if (lane == 0) mbar_arrive(bar(L::B_PF + ns % L::kScores));
         if (!wait_warp(bar(L::B_DPF), ns & 1, abort_flag, kErrDkdvSoftmax)) {
           ok = false;
           break;
