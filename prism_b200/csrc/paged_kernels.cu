@@ -446,9 +446,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     at.b = blockIdx.x / units, at.unit = blockIdx.x - at.b * units;
     at.length = length_of(c, at.b), at.tiles = tiles_of<kTile>(at.length);
     steps = at.tiles;
-    if (steps == 0) {
+    if (steps == 0) {  // no keys, or no table for them
+      const float x = c.lengths[at.b] > 0 ? __int_as_float(0x7fc00000) : 0.0f;
+      const uint32_t w = M::pack(x, x);
       for (int i = threadIdx.x; i < rows_of(s, at.unit) * (D / 8); i += kThreads)
-        reinterpret_cast<uint4*>(o + out_row(s, at.b, at.unit, i / (D / 8)) * D)[i % (D / 8)] = make_uint4(0, 0, 0, 0);
+        reinterpret_cast<uint4*>(o + out_row(s, at.b, at.unit, i / (D / 8)) * D)[i % (D / 8)] = make_uint4(w, w, w, w);
       return;
     }
   } else {

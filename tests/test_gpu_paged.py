@@ -264,6 +264,20 @@ def test_wrong_pages_and_lengths_give_nan(page, cuda):
     assert all(bool(got[b].isnan().all()) for b in (1, 2, 3))
 
 
+def test_no_table_and_no_cache(cuda):
+    """A table without columns, a cache without pages: 0 without a token, NaN with one."""
+    q = torch.randn(2, 2, 64, device="cuda").bfloat16()
+    lengths = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    for pages, width in ((4, 0), (0, 1), (0, 0)):
+        cache = [torch.zeros(pages, 16, 1, 64, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+        table = torch.zeros(2, width, dtype=torch.int32, device="cuda")
+        o = paged_attention(q, *cache, table, lengths)
+        assert not o[0].any() and bool(o[1].isnan().all())
+        new = torch.ones(2, 1, 64, device="cuda", dtype=torch.bfloat16)
+        out = append_paged(new, new, *cache, table, lengths, q=q)
+        assert not out[0].any() and bool(out[1].isnan().all()) and not cache[0].any()
+
+
 def test_strided_queries(cuda):
     c = Cache([600, 40], 16, 2, 64, torch.bfloat16)
     qkv = torch.randn(2, 12, 64, device="cuda").bfloat16()
