@@ -1425,7 +1425,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // step n of `steps`; early: S^T of it is issued; next: S^T of the one behind it may be
     const auto step = [&](int n, int steps, bool early, bool next) -> bool {
       const uint32_t st = (uint32_t)ns % R;
-      if (n == 0 && !wait(L::B_KV, n_kv)) return false;
+      if (n == 0) {  // keys that are not there yet are not waited for with a product to issue
+        if (waiting && !mbar_try(bar(L::B_KV), n_kv & 1) && !dk_step()) return false;
+        if (!wait(L::B_KV, n_kv)) return false;
+      }
       if (!early && !scores(ns)) return false;
       if (waiting && !dk_step()) return false;
       if (next && !scores(ns + 1)) return false;
@@ -1772,7 +1775,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     const auto step = [&](int n, int steps) -> bool {
       const int sk = ns % RK, sv = ns % RV;
-      if (n == 0 && !wait(L::B_QD, n_q)) return false;
+      if (n == 0) {  // rows that are not there yet are not waited for with a product to issue
+        if (waiting && !mbar_try(bar(L::B_QD), n_q & 1)) {
+          if (!dq_step(ns - 1, first, last)) return false;
+          waiting = false;
+        }
+        if (!wait(L::B_QD, n_q)) return false;
+      }
       if (!wait(L::B_KF + sk, ns / RK) || (ns > 0 && !wait(L::B_DPE, ns - 1))) return false;
       tc_fence_after();
       mma_kd<L::kSub, 16384, 16384>(tmem + L::T_S, dQ, dKk + sk * kSlot, kIdS, 0u);
