@@ -417,6 +417,10 @@ __device__ __forceinline__ float exp_pairs(const float (&s)[64], float scale, fl
 // An item: two tiles of 128 rows (groups 0 and 1) of one key head, which share the stream of K and V steps, so
 // that the tensor core works on one group's products while the other group's softmax runs.  Where there are
 // few tiles and long keys, an item is a part of the steps, and join_kernel adds the parts up.
+//
+// 8,192 causal tokens of 32 + 8 heads: 500 us at 128 columns (1,100 TFLOP/s, the tensor pipe 53 % busy), 425 at 64
+// (650 TFLOP/s, 30 %).  Bound by the softmax warps between the products: 2^x of every score alone takes 240 us at
+// 16 a clock and SM, and the multiplications, conversions and TMEM traffic around it have the same issue slots.
 template <int D>
 struct FwdLayout {
   // 64 columns leave room in TMEM for a third S: that of a group's next step is issued before its P is there
@@ -1123,7 +1127,8 @@ __device__ void find_place(const Sequences& s, int my, int per, Place* place, in
 // ===================================================================== delta
 // delta = dO . O of every row of every tile, 0 for rows without a token, in the forward's tile order: D / 8
 // threads a row.  O with the 8 bits that the forward kept of what its rounding left: delta enters ds next to
-// do . v, and o's rounding alone would be as large an error as that of ds.  Bound by memory.
+// do . v, and o's rounding alone would be as large an error as that of ds.  Bound by memory: 75,600 tokens of 40
+// heads of 128 take 291 us (6.6 TB/s).
 constexpr int kDeltaThreads = 256;
 
 template <typename T, int D>
@@ -1173,6 +1178,10 @@ __global__ void __launch_bounds__(kDeltaThreads)
 // The softmax reads the 16x256b TMEM layout: a thread holds, in each 16-lane half, key lanes a and a + 8
 // (a = lane / 4) at columns 8 j + 2 (lane % 4) + {0, 1}, so that it needs 16 of a half tile's 64 lse and
 // delta values instead of all of them.
+//
+// 8,192 causal tokens of 32 + 8 heads: 920 us at 128 columns (8 D operations a score: 1,195 TFLOP/s, the tensor pipe
+// 56 % busy), 704 at 64 (780 TFLOP/s, 36 %).  Bound by the chain S, P, dP, dS of a step through the softmax warps
+// (two TMEM reads, two writes and a 2^x a score), which the four products of the step before cover only in part.
 template <int D>
 struct DkdvLayout {
   // 64 columns leave room in TMEM for a second S^T: that of step n + 1 is issued before P^T of step n is there
@@ -1586,7 +1595,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// dK and dV from the sums of their parts, in order.  Bound by memory.
+// dK and dV from the sums of their parts, in order.  Bound by memory: 42 us for 12 parts of 512 keys of 40 heads of
+// 128 (252 MB, L2 holding some of it).
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads)
     add_parts_kernel(const float* __restrict__ sums, int parts, int64_t count, float scale, T* __restrict__ dk,
@@ -1609,6 +1619,9 @@ __global__ void __launch_bounds__(kJoinThreads)
 // An item: one tile of 128 query rows; a step is 128 keys: S = Q K^T and dP = dO V^T in TMEM, the softmax
 // warpgroups (64 keys each) write dS = P (dP - delta) into columns of its own, dQ += dS K reads them from
 // there.  S and dP of step n + 1 are issued as soon as those of step n are read.
+//
+// 8,192 causal tokens of 32 + 8 heads: 690 us at 128 columns (6 D operations a score: 1,195 TFLOP/s, the tensor pipe
+// 55 % busy), 585 at 64 (705 TFLOP/s, 32 %).  Bound as dK and dV are.
 template <int D>
 struct DqLayout {
   static constexpr int kRingK = 3, kRingV = 2;  // K serves two products
@@ -2017,15 +2030,16 @@ struct Shape {
   // Values of lse, or of delta: of all rows of all tiles.
   int64_t stats() const { return pair_bound(q_rows, count, q_heads / k_heads) * 2 * kRows * k_heads; }
   // Parts that the steps of `items` items are divided into: those for which the SMs' rounds of them take the
-  // fewest steps, an item's own costs counted as 2.5 and the addition of the parts as 4.  Not divided where the
-  // items fill a round (16 sequences of 16 queries on 4,096 keys: 66 us, 87 in seven parts), divided where they
-  // do not (128 queries on 32,768 keys, 8 items: 402 us, 71 in 16 parts) or leave much of the last one idle.
+  // fewest steps, with 2.5 a round for an item's own costs and, where the parts are added up, 1.3 for reading
+  // their sums and 4 for the launch.  Not divided where the items fill a round (16 sequences of 16 queries on
+  // 4,096 keys: 66 us, 87 in seven parts), divided where they do not (128 queries on 32,768 keys, 8 items: 402 us,
+  // 71 in 16 parts) or leave much of the last one idle, up to 16 rounds (310 MB of sums).
   static int parts(int64_t items, int64_t steps) {
     int best = 1;
     double least = 0.0;
-    for (int p = 1; p <= 16 && (p == 1 || steps >= 4 * p); ++p) {
+    for (int p = 1; p <= 16 && (p == 1 || (steps >= 4 * p && items * p <= 16 * kSms)); ++p) {
       const double rounds = (double)((items * p + kSms - 1) / kSms);
-      const double cost = rounds * ((double)steps / p + 2.5) + (p > 1 ? 4.0 : 0.0);
+      const double cost = rounds * ((double)steps / p + (p > 1 ? 3.8 : 2.5)) + (p > 1 ? 4.0 : 0.0);
       if (p == 1 || cost < least) best = p, least = cost;
     }
     return best;

@@ -38,6 +38,9 @@ struct Cache {
 // computed meanwhile.  A CTA takes a few tokens; their places and factors are found once and kept in
 // shared memory, and each thread keeps one unit (16 bytes of a head, or the two vectors that a rotation
 // of halves needs) and runs along the tokens' heads of q, k and v.
+//
+// 23,442 tokens of 24 + 8 heads of 128, 96 columns rotated as adjacent pairs: 86 us (5.6 TB/s); one token each
+// of 16 sequences: 3.2 us.
 struct Append {
   const void* in[3];          // q, k, v
   int64_t in_t[3], in_h[3];   // strides of token and head
@@ -237,6 +240,8 @@ static cudaError_t dispatch_append(const Append& a, const Cache& c, const double
 //   * Where no sequence can have more than kWhole keys (the table's width), a CTA takes one unit and there
 //     is no second launch.
 //   * Keys behind a sequence's end are not read (zero-filled), so what lies there does not matter.
+// 131,001 keys of 8 heads of 128, 32 query heads: 82 us (6.5 TB/s) and 6.5 for the join; 4 sequences of up to 100
+// keys in one launch: 4.6 us.
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kRows = 16, kCtas = 2 * kSms;
 constexpr int kWhole = 512;
 

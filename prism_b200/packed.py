@@ -31,7 +31,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
     Any row and head strides (copied where they are not multiples of 16 bytes).  Differentiable in q, k
     and v, once: a gradient of a gradient is an error.  What is not finite in one sequence, or behind the last
-    one, changes nothing in another; within a sequence it reaches every query of the sequence, as in a product
+    one, changes nothing in another; within a sequence it may reach every query of the sequence, as in a product
     with a zero probability."""
     return _lib.torch_ops().packed_attention(q, k, v, offsets, k_offsets, causal, scale)
 
