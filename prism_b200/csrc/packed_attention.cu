@@ -397,8 +397,11 @@ __device__ __forceinline__ void mask_from(float (&s)[64], int lim) {
     if (c >= lim) s[c] = -INFINITY;
 }
 
-// p = exp2(s * scale - m) of 64 scores as 32 pairs of T; returns their fp32 sum.
-template <typename T>
+// p = exp2(s * scale - m) of 64 scores as 32 pairs of T; returns their fp32 sum, kRounded: of the rounded values.
+// m is a maximum of earlier scores, so a row's largest p is no power of two and its rounding is off by half a
+// step; where that p is nearly all of its row, o = sum p v / sum p is right only if both sums have the same p.  o
+// itself is rounded as coarsely, but delta = dO . o is subtracted from a nearly equal dO . v.
+template <typename T, bool kRounded>
 __device__ __forceinline__ float exp_pairs(const float (&s)[64], float scale, float m, uint32_t (&pk)[32]) {
   const float2 sc = make_float2(scale, scale), nm = make_float2(-m, -m);
   float2 even = make_float2(0.f, 0.f), odd = even;
@@ -406,9 +409,10 @@ __device__ __forceinline__ float exp_pairs(const float (&s)[64], float scale, fl
   for (int c = 0; c < 32; ++c) {
     const float2 x = __ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sc, nm);
     const float2 p = make_float2(ex2(x.x), ex2(x.y));
-    if (c & 1) odd = __fadd2_rn(odd, p);
-    else even = __fadd2_rn(even, p);
     pk[c] = Half<T>::pack(p.x, p.y);
+    const float2 add = kRounded ? make_float2(__uint_as_float(pk[c] << 16), __uint_as_float(pk[c] & 0xffff0000u)) : p;
+    if (c & 1) odd = __fadd2_rn(odd, add);
+    else even = __fadd2_rn(even, add);
   }
   return (even.x + even.y) + (odd.x + odd.y);
 }
@@ -902,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (m == -INFINITY) l = 1.0f;
             two_pass = __any_sync(0xffffffffu, m == -INFINITY);
           }
-          sum0 = exp_pairs<T>(s, qk_scale, m, pk0);
+          sum0 = exp_pairs<T, kMode == kTrain>(s, qk_scale, m, pk0);
           two_pass = two_pass || __any_sync(0xffffffffu, !(sum0 <= H::kSum));
         }
         if (two_pass) {
@@ -938,7 +942,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
               float s[64];
               scores(u, s);
-              const float t = exp_pairs<T>(s, qk_scale, mb, pk);
+              const float t = exp_pairs<T, kMode == kTrain>(s, qk_scale, mb, pk);
               if (u) sum1 = t; else sum0 = t;
             }
             tmem_st32(t_s + u * 32, pk);  // over scores of the first half, which are read
@@ -952,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             float s[64];
             scores(1, s);
-            sum1 = exp_pairs<T>(s, qk_scale, m, pk1);
+            sum1 = exp_pairs<T, kMode == kTrain>(s, qk_scale, m, pk1);
           }
           const bool need = !(sum1 <= H::kSum);
           if (__any_sync(0xffffffffu, need)) {  // rare
@@ -975,7 +979,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             l = (l + sum0) * alpha;
             sum0 = 0.f;
             m = m_new;
-            sum1 = exp_pairs<T>(s, qk_scale, m, pk1);
+            sum1 = exp_pairs<T, kMode == kTrain>(s, qk_scale, m, pk1);
           }
           tmem_st32(t_s + 32, pk1);
         }
