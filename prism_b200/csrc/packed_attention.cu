@@ -400,7 +400,8 @@ __device__ __forceinline__ void mask_from(float (&s)[64], int lim) {
 // p = exp2(s * scale - m) of 64 scores as 32 pairs of T; returns their fp32 sum, kRounded: of the rounded values.
 // m is a maximum of earlier scores, so a row's largest p is no power of two and its rounding is off by half a
 // step; where that p is nearly all of its row, o = sum p v / sum p is right only if both sums have the same p.  o
-// itself is rounded as coarsely, but delta = dO . o is subtracted from a nearly equal dO . v.
+// itself is rounded as coarsely, but delta = dO . o is subtracted from a nearly equal dO . v: for training only
+// (8,192 causal tokens at 128 columns: 473 us, 497 so).
 template <typename T, bool kRounded>
 __device__ __forceinline__ float exp_pairs(const float (&s)[64], float scale, float m, uint32_t (&pk)[32]) {
   const float2 sc = make_float2(scale, scale), nm = make_float2(-m, -m);
@@ -422,8 +423,8 @@ __device__ __forceinline__ float exp_pairs(const float (&s)[64], float scale, fl
 // that the tensor core works on one group's products while the other group's softmax runs.  Where there are
 // few tiles and long keys, an item is a part of the steps, and join_kernel adds the parts up.
 //
-// 8,192 causal tokens of 32 + 8 heads: 500 us at 128 columns (1,100 TFLOP/s, the tensor pipe 53 % busy), 425 at 64
-// (650 TFLOP/s, 30 %).  Bound by the softmax warps between the products: 2^x of every score alone takes 240 us at
+// 8,192 causal tokens of 32 + 8 heads: 473 us at 128 columns (1,160 TFLOP/s, the tensor pipe 53 % busy), 395 at 64
+// (700 TFLOP/s, 30 %).  Bound by the softmax warps between the products: 2^x of every score alone takes 240 us at
 // 16 a clock and SM, and the multiplications, conversions and TMEM traffic around it have the same issue slots.
 template <int D>
 struct FwdLayout {
