@@ -223,3 +223,33 @@ def test_same_bits_many_times(D, group, cuda):
             got = [o.detach(), *torch.autograd.grad(o, leaves, do)]
             first = first or got
             assert all(torch.equal(a, b) and not bool(a.isnan().any()) for a, b in zip(got, first))
+
+
+@pytest.mark.parametrize("D,group", [(64, 1), (64, 4), (128, 1), (128, 8)])
+def test_gradients_of_rows_with_one_dominant_key(D, group, cuda):
+    """One query a sequence with most of its weight on one key: ds = p (do . v - delta) is a small difference.
+    Element by element: half steps of 2^-8 (bf16) of o's weights, which move delta by 2^-8 of the sum of |ds|
+    and once more in their sum; of ds and of p by as much of |ds|; of dq itself.  o is kept to 2^-15, and the fp32
+    sums of up to 451 products to 451 2^-24 of their terms' magnitudes (in s: times the exponent's slope, |ds|)."""
+    u, count, keys, scale = 2.0 ** -8, 48, 451, D ** -0.5
+    q, k, v, do, qa, ka = _inputs([1] * count, [keys] * count, 2 * group, 2, D, torch.bfloat16, seed=D + group)
+    q *= 6
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    o = packed_attention(*leaves, *_offsets(qa, ka))
+    dq, dk = torch.autograd.grad(o, leaves[:2], do)
+    rows, cols = slice(qa[0], qa[-1]), slice(ka[0], ka[-1])
+    Q, DO = (t[rows].detach().double().unflatten(1, (2, group)) for t in (q, do))          # [count, 2, group, D]
+    K, V = (t[cols].detach().double().unflatten(0, (count, keys)).transpose(1, 2) for t in (k, v))  # [count, 2, keys, D]
+    p = (Q @ K.transpose(2, 3) * scale).softmax(-1)
+    dp, delta = DO @ V.transpose(2, 3), (DO * (p @ V)).sum(-1, keepdim=True)
+    ds = p * (dp - delta)
+    sums = keys * 2.0 ** -24
+    off_s = sums * (Q.abs() @ K.abs().transpose(2, 3)) * scale
+    terms = DO.abs() @ V.abs().transpose(2, 3)
+    off = (2 * u + 2 * off_s.amax(-1, keepdim=True)) * ds.abs() + sums * p * terms
+    off += p * (2 * u * ds.abs().sum(-1, keepdim=True) + 2.0 ** -15 * (DO * (p @ V)).abs().sum(-1, keepdim=True)
+                + sums * (p * terms).sum(-1, keepdim=True))
+    for got, ref, bound in ((dq[rows].double().unflatten(1, (2, group)), ds @ K * scale, off @ K.abs() * scale),
+                            (dk[cols].double().unflatten(0, (count, keys)).transpose(1, 2), ds.transpose(2, 3) @ Q * scale,
+                             off.transpose(2, 3) @ Q.abs() * scale)):
+        assert bool(((got - ref).abs() <= bound + u * (ref.abs() + bound) + 1e-30).all())
