@@ -460,11 +460,11 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
   } else {
     // sequences without keys
-    const int chunks = s.tokens * s.heads * s.group * (D / 8);
+    const int64_t chunks = (int64_t)s.tokens * s.heads * s.group * (D / 8);
     for (int b = blockIdx.x; b < s.batch; b += kCtas)
       if (c.lengths[b] <= 0)
-        for (int i = threadIdx.x; i < chunks; i += kThreads)
-          reinterpret_cast<uint4*>(o + (int64_t)b * chunks * 8)[i] = make_uint4(0, 0, 0, 0);
+        for (int64_t i = threadIdx.x; i < chunks; i += kThreads)
+          reinterpret_cast<uint4*>(o + b * chunks * 8)[i] = make_uint4(0, 0, 0, 0);
     const Share share = share_of<kTile>(c, s.batch, units, scratch);
     steps = share.steps;
     if (steps == 0) return;
@@ -877,9 +877,9 @@ prism_status_t prism_paged_attention(const void* q, const int64_t* q_strides, in
   PRISM_CHECK_ARG(q && q_strides && o && (workspace || prism_paged_attention_workspace_bytes(D, page_size, table_width) == 0) && aligned16(o) && aligned16(workspace), "%s: null pointer, or a buffer off 16 bytes", what);
   c.k_page = k_cache_strides[0], c.k_place = k_cache_strides[1], c.k_head = k_cache_strides[2];
   c.v_page = v_cache_strides[0], c.v_place = v_cache_strides[1], c.v_head = v_cache_strides[2];
-  PRISM_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache) &&
-                      ((c.k_page | c.k_place | c.k_head | c.v_page | c.v_place | c.v_head) & 7) == 0,
-                  "%s: the caches' rows must start on 16 bytes", what);
+  const int64_t all_strides = c.k_page | c.k_place | c.k_head | c.v_page | c.v_place | c.v_head;
+  PRISM_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache) && all_strides >= 0 && (all_strides & 7) == 0,
+                  "%s: the caches' rows must start on 16 bytes, with strides that are not negative", what);
   constexpr int64_t kMost = (int64_t)1 << 35;  // elements: 2^32 units of 16 bytes
   PRISM_CHECK_ARG((pages - 1) * c.k_page + (page_size - 1) * c.k_place + k_heads * c.k_head < kMost &&
                       (pages - 1) * c.v_page + (page_size - 1) * c.v_place + k_heads * c.v_head < kMost,
