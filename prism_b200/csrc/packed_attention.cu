@@ -397,25 +397,44 @@ __device__ __forceinline__ void mask_from(float (&s)[64], int lim) {
     if (c >= lim) s[c] = -INFINITY;
 }
 
-// p = exp2(s * scale - m) of 64 scores as 32 pairs of T; returns their fp32 sum, kRounded: of the rounded values.
+// Sums of a row's p: before their rounding, and after it where kRounded.
+template <bool kRounded>
+struct RowSum {
+  float exact, rounded;
+  __device__ __forceinline__ void scale(float by) {
+    exact *= by;
+    if constexpr (kRounded) rounded *= by;
+  }
+  __device__ __forceinline__ void add(const RowSum& x) {
+    exact += x.exact;
+    if constexpr (kRounded) rounded += x.rounded;
+  }
+  __device__ __forceinline__ float of_products() const { return kRounded ? rounded : exact; }
+};
+
+// p = exp2(s * scale - m) of 64 scores as 32 pairs of T; returns their fp32 sums.
 // m is a maximum of earlier scores, so a row's largest p is no power of two and its rounding is off by half a
 // step; where that p is nearly all of its row, o = sum p v / sum p is right only if both sums have the same p.  o
 // itself is rounded as coarsely, but delta = dO . o is subtracted from a nearly equal dO . v: for training only
-// (8,192 causal tokens at 128 columns: 473 us, 497 so).
+// (8,192 causal tokens at 128 columns: 484 us, 512 so).  lse is that of the p before rounding.
 template <typename T, bool kRounded>
-__device__ __forceinline__ float exp_pairs(const float (&s)[64], float scale, float m, uint32_t (&pk)[32]) {
-  const float2 sc = make_float2(scale, scale), nm = make_float2(-m, -m);
-  float2 even = make_float2(0.f, 0.f), odd = even;
+__device__ __forceinline__ RowSum<kRounded> exp_pairs(const float (&s)[64], float scale, float m, uint32_t (&pk)[32]) {
+  const float2 sc = make_float2(scale, scale), nm = make_float2(-m, -m), zero = make_float2(0.f, 0.f);
+  float2 even = zero, odd = zero, even_r = zero, odd_r = zero;
 #pragma unroll
   for (int c = 0; c < 32; ++c) {
     const float2 x = __ffma2_rn(make_float2(s[2 * c], s[2 * c + 1]), sc, nm);
     const float2 p = make_float2(ex2(x.x), ex2(x.y));
+    if (c & 1) odd = __fadd2_rn(odd, p);
+    else even = __fadd2_rn(even, p);
     pk[c] = Half<T>::pack(p.x, p.y);
-    const float2 add = kRounded ? make_float2(__uint_as_float(pk[c] << 16), __uint_as_float(pk[c] & 0xffff0000u)) : p;
-    if (c & 1) odd = __fadd2_rn(odd, add);
-    else even = __fadd2_rn(even, add);
+    if constexpr (kRounded) {
+      const float2 r = Half<T>::unpack(pk[c]);
+      if (c & 1) odd_r = __fadd2_rn(odd_r, r);
+      else even_r = __fadd2_rn(even_r, r);
+    }
   }
-  return (even.x + even.y) + (odd.x + odd.y);
+  return {(even.x + even.y) + (odd.x + odd.y), (even_r.x + even_r.y) + (odd_r.x + odd_r.y)};
 }
 
 // ===================================================================== forward
@@ -865,7 +884,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool valid = r < rows && tok < at.nq;
       // keys that this row sees; rows without a token go along with the last one
       const int seen = causal ? min(max(min(tok, last) + w.shift + 1, 0), at.nk) : at.nk;
-      float m = -INFINITY, l = 1.0f;
+      using Sum = RowSum<kMode == kTrain>;
+      float m = -INFINITY;
+      Sum l = {1.0f, 1.0f};
       for (int n = 0; n < n_steps; ++n) {
         // keys of the two halves of the step that the row sees; all / none of them for every row of the warp
         const int lim0 = seen - (w.from + n) * kRows, lim1 = lim0 - 64;
@@ -888,7 +909,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_load<2>(t_s + u * 64, s);
           if (!(u ? all1 : all0)) mask_from(s, u ? lim1 : lim0);
         };
-        float sum0 = 0.f, sum1 = 0.f;
+        Sum sum0 = {0.f, 0.f}, sum1 = {0.f, 0.f};
         // Exponentials against the running maximum in one pass over S; a row's first maximum is that of its
         // first half step.  A first half whose exponentials sum past kSum, and a row that has seen no key yet,
         // take two passes (maximum, then exponentials; S is intact).  If only the second half passes the limit,
@@ -903,15 +924,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           float s[64];
           scores(0, s);
           if (__any_sync(0xffffffffu, m == -INFINITY)) {
-            if (m == -INFINITY) m = tile_max(s) * qk_scale - H::kShift, l = 0.0f;
-            if (m == -INFINITY) l = 1.0f;
+            if (m == -INFINITY) m = tile_max(s) * qk_scale - H::kShift, l = {0.0f, 0.0f};
+            if (m == -INFINITY) l = {1.0f, 1.0f};
             two_pass = __any_sync(0xffffffffu, m == -INFINITY);
           }
           sum0 = exp_pairs<T, kMode == kTrain>(s, qk_scale, m, pk0);
-          two_pass = two_pass || __any_sync(0xffffffffu, !(sum0 <= H::kSum));
+          two_pass = two_pass || __any_sync(0xffffffffu, !(sum0.exact <= H::kSum));
         }
         if (two_pass) {
-          sum0 = 0.f;
+          sum0 = {0.f, 0.f};
           float mx = -INFINITY;
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
@@ -926,7 +947,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float m_new = need ? mx : m;
             const float alpha = need ? ex2(m - m_new) : 1.0f;  // m = -inf -> 0
             const bool o_live = __any_sync(0xffffffffu, need && m != -INFINITY);
-            l *= alpha;
+            l.scale(alpha);
             m = m_new;
             if (n > 0 && o_live) {
               o_settled();
@@ -943,7 +964,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
               float s[64];
               scores(u, s);
-              const float t = exp_pairs<T, kMode == kTrain>(s, qk_scale, mb, pk);
+              const Sum t = exp_pairs<T, kMode == kTrain>(s, qk_scale, mb, pk);
               if (u) sum1 = t; else sum0 = t;
             }
             tmem_st32(t_s + u * 32, pk);  // over scores of the first half, which are read
@@ -959,7 +980,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             scores(1, s);
             sum1 = exp_pairs<T, kMode == kTrain>(s, qk_scale, m, pk1);
           }
-          const bool need = !(sum1 <= H::kSum);
+          const bool need = !(sum1.exact <= H::kSum);
           if (__any_sync(0xffffffffu, need)) {  // rare
             float s[64];
             scores(1, s);
@@ -969,22 +990,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (n > 0) scale_tmem_rows<D / 32>(t_o, alpha);
             tmem_wait_st();
             uint32_t raw[32];
+            float again = 0.f;
             tmem_ld32(t_s, raw);
             tmem_wait_ld_dep(raw);
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-              const float2 p = H::unpack(raw[i]);
+              float2 p = H::unpack(raw[i]);
               raw[i] = H::pack(p.x * alpha, p.y * alpha);
+              if (kMode == kTrain) {  // rounded a second time
+                p = H::unpack(raw[i]);
+                again += p.x + p.y;
+              }
             }
             tmem_st32(t_s, raw);
-            l = (l + sum0) * alpha;
-            sum0 = 0.f;
+            l.scale(alpha);
+            l.add({sum0.exact * alpha, again});
+            sum0 = {0.f, 0.f};
             m = m_new;
             sum1 = exp_pairs<T, kMode == kTrain>(s, qk_scale, m, pk1);
           }
           tmem_st32(t_s + 32, pk1);
         }
-        l += sum0 + sum1;
+        sum0.add(sum1), l.add(sum0);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -997,9 +1024,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool empty = m == -INFINITY;  // no key
       const int64_t out_row = (int64_t)(at.q0 + tok) * heads + at.h * hd.group + head_of_row;
       if constexpr (kMode == kTrain)
-        lse[(((int64_t)at.h * hd.pairs + at.index) * 2 + g) * kRows + r] = valid && !empty ? m + __log2f(l) : INFINITY;
+        lse[(((int64_t)at.h * hd.pairs + at.index) * 2 + g) * kRows + r] = valid && !empty ? m + __log2f(l.exact) : INFINITY;
       if (kMode == kPart && valid)
-        parts.ml[(int64_t)at.part * seqs.q_rows * heads + out_row] = make_float2(m, empty ? 0.0f : l);
+        parts.ml[(int64_t)at.part * seqs.q_rows * heads + out_row] = make_float2(m, empty ? 0.0f : l.of_products());
       if (n_steps > 0) {
         if (!wait_warp(bar(L::B_OF + g), n_o & 1, abort_flag, kErrFwdSoftmax)) {
           ok = false;
@@ -1007,7 +1034,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++n_o;
         tc_fence_after();
-        const float inv = 1.0f / l;
+        const float inv = 1.0f / l.of_products();
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t raw[32];
