@@ -913,23 +913,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Exponentials against the running maximum in one pass over S; a row's first maximum is that of its
         // first half step.  A first half whose exponentials sum past kSum, and a row that has seen no key yet,
         // take two passes (maximum, then exponentials; S is intact).  If only the second half passes the limit,
-        // P of the first half, l and O are scaled to the new maximum.
+        // P of the first half, l and O are scaled to the new maximum.  The two ways raise a maximum at different
+        // scores, so only the sequence's own rows have a vote: what lies behind it in the tile must not choose the
+        // rounding of its P.
         bool two_pass = false;
         uint32_t pk0[32];
         if (none0) {
-          two_pass = __any_sync(0xffffffffu, m == -INFINITY);
+          two_pass = __any_sync(0xffffffffu, valid && m == -INFINITY);
 #pragma unroll
           for (int i = 0; i < 32; ++i) pk0[i] = 0u;
         } else {
           float s[64];
           scores(0, s);
-          if (__any_sync(0xffffffffu, m == -INFINITY)) {
+          if (__any_sync(0xffffffffu, valid && m == -INFINITY)) {
             if (m == -INFINITY) m = tile_max(s) * qk_scale - H::kShift, l = {0.0f, 0.0f};
             if (m == -INFINITY) l = {1.0f, 1.0f};
-            two_pass = __any_sync(0xffffffffu, m == -INFINITY);
+            two_pass = __any_sync(0xffffffffu, valid && m == -INFINITY);
           }
           sum0 = exp_pairs<T, kMode == kTrain>(s, qk_scale, m, pk0);
-          two_pass = two_pass || __any_sync(0xffffffffu, !(sum0.exact <= H::kSum));
+          two_pass = two_pass || __any_sync(0xffffffffu, valid && !(sum0.exact <= H::kSum));
         }
         if (two_pass) {
           sum0 = {0.f, 0.f};
@@ -942,7 +944,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mx = fmaxf(mx, tile_max(s));
           }
           mx = mx * qk_scale - H::kShift;
-          const bool need = mx > m + H::kLag;  // m = -inf: any key
+          const bool need = valid && mx > m + H::kLag;  // m = -inf: any key
           if (__any_sync(0xffffffffu, need)) {
             const float m_new = need ? mx : m;
             const float alpha = need ? ex2(m - m_new) : 1.0f;  // m = -inf -> 0
@@ -980,7 +982,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             scores(1, s);
             sum1 = exp_pairs<T, kMode == kTrain>(s, qk_scale, m, pk1);
           }
-          const bool need = !(sum1.exact <= H::kSum);
+          const bool need = valid && !(sum1.exact <= H::kSum);
           if (__any_sync(0xffffffffu, need)) {  // rare
             float s[64];
             scores(1, s);
