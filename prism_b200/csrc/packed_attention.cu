@@ -503,10 +503,13 @@ struct FwdSteps {
 enum Mode : int { kInfer, kTrain, kPart };
 
 // What rounding an fp32 value to bf16 leaves, in 8 bits: the second byte of its bit pattern, signed.  The
-// lower half of the pattern is what was rounded off, up where its first bit is set (but for a value in the very
-// middle that went down, one in 2^17, which comes back a place too low).  The bytes of four values:
+// lower half of the pattern is what was rounded off, up where its first bit is set.  A value in the very middle
+// goes to the even side, and +128 is no signed byte: one that went down leaves +127.  Such values are common:
+// of means of two bf16 values a tenth.  The bytes of four values:
+__device__ __forceinline__ uint32_t below_middle(uint32_t x) { return x - ((x & 0x1ffffu) == 0x8000u ? 1u : 0u); }
 __device__ __forceinline__ uint32_t rest_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __byte_perm(__byte_perm(a, b, 0x0051), __byte_perm(c, d, 0x0051), 0x5410);
+  return __byte_perm(__byte_perm(below_middle(a), below_middle(b), 0x0051),
+                     __byte_perm(below_middle(c), below_middle(d), 0x0051), 0x5410);
 }
 // ... and a value again, from its bf16 and byte i of `left`, to 2^-8 of bf16's last place; one that is a bf16
 // comes back as it was.
