@@ -1026,12 +1026,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       before += w.n[0] + w.n[1];
       if (!ok) break;
       // epilogue
-      const bool empty = m == -INFINITY;  // no key
+      // No key here, which gives 0, is told by the mask: a row all of whose scores are -inf or NaN has no maximum
+      // either, and its softmax is undefined.
+      const bool empty = n_steps == 0 || seen <= w.from * kRows, undefined = !empty && m == -INFINITY;
+      const float nan = __uint_as_float(0x7fc00000u);
       const int64_t out_row = (int64_t)(at.q0 + tok) * heads + at.h * hd.group + head_of_row;
       if constexpr (kMode == kTrain)
-        lse[(((int64_t)at.h * hd.pairs + at.index) * 2 + g) * kRows + r] = valid && !empty ? m + __log2f(l.exact) : INFINITY;
-      if (kMode == kPart && valid)
-        parts.ml[(int64_t)at.part * seqs.q_rows * heads + out_row] = make_float2(m, empty ? 0.0f : l.of_products());
+        lse[(((int64_t)at.h * hd.pairs + at.index) * 2 + g) * kRows + r] =
+            !valid || empty ? INFINITY : undefined ? nan : m + __log2f(l.exact);
+      if (kMode == kPart && valid)  // undefined: the sum is 1, or NaN with a NaN among the scores
+        parts.ml[(int64_t)at.part * seqs.q_rows * heads + out_row] = make_float2(empty ? -INFINITY : m, empty ? 0.0f : l.of_products());
       if (n_steps > 0) {
         if (!wait_warp(bar(L::B_OF + g), n_o & 1, abort_flag, kErrFwdSoftmax)) {
           ok = false;
@@ -1039,7 +1043,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ++n_o;
         tc_fence_after();
-        const float inv = 1.0f / l.of_products();
+        const float inv = undefined ? nan : 1.0f / l.of_products();
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t raw[32];
@@ -1106,8 +1110,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Parts parts, int cou
 #pragma unroll 4
   for (int p = 0; p < count; ++p) {
     const float2 x = parts.ml[p * rows + row];
-    if (x.x == -INFINITY) {  // no key; its sums were not written
-      sum += x.y;            // 0, or NaN for wrong offsets
+    if (x.x == -INFINITY) {
+      // no key (0; its sums were not written), scores of -inf only (1: undefined if the others have none either),
+      // or NaN for a NaN among them and for wrong offsets
+      if (!(x.y == 0.0f) && (top == -INFINITY || x.y != x.y)) sum = __uint_as_float(0x7fc00000u);
       continue;
     }
     const float f = ex2(x.x - top);
