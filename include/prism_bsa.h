@@ -618,7 +618,7 @@ prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_stride
  * each sequence; D = 64 or 128) -> o alike, contiguous: query i of sequence b attends the keys
  * j <= lengths[b] - tokens + i, softmax(scale q k) v, scale > 0; 0 without a key, NaN for a sequence whose
  * length or one of whose pages is outside the table or the cache.  What lies in the cache behind a sequence's end is
- * not read.  Rows of the caches start on 16 bytes, of q on 4.  workspace:
+ * not read; a value that is not finite may reach every query of its sequence that has a key.  Rows of the caches start on 16 bytes, of q on 4.  workspace:
  * prism_paged_attention_workspace_bytes (NULL where that is 0).  Both read lengths and the table on the device. */
 prism_status_t prism_append_paged(const void* q, const int64_t* q_strides, int q_heads, const void* k,
                                   const int64_t* k_strides, const void* v, const int64_t* v_strides,

@@ -427,6 +427,19 @@ __device__ __forceinline__ int64_t out_row(const Queries& s, int b, int unit, in
 __device__ __forceinline__ int rows_of(const Queries& s, int unit) {
   return min(kRows, s.tokens * s.group - unit % s.row_tiles * kRows);
 }
+// Whether a row of a unit sees no key of its sequence's `length`.
+__device__ __forceinline__ bool sees_none(const Queries& s, int unit, int row, int length) {
+  return length - s.tokens + (unit % s.row_tiles * kRows + row) / s.group < 0;
+}
+// A row's result from its sums: 0 without a key, whatever is in the values that its zeros were multiplied with
+// (a sum that is NaN says that a page is wrong), and 0 / 0 where all of its scores are -inf.
+template <typename M>
+__device__ __forceinline__ uint2 row_result(const float4& acc, float sum, bool none) {
+  const float inv = 1.0f / sum;
+  uint2 out = make_uint2(M::pack(acc.x * inv, acc.y * inv), M::pack(acc.z * inv, acc.w * inv));
+  if (none && sum == 0.0f) out = make_uint2(0u, 0u);
+  return out;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2)
@@ -683,9 +696,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           all.x = fmaf(v.x, f, all.x), all.y = fmaf(v.y, f, all.y), all.z = fmaf(v.z, f, all.z), all.w = fmaf(v.w, f, all.w);
         }
         if (whole) {
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row without keys
           *reinterpret_cast<uint2*>(o + out_row(s, done.b, done.unit, 8 * half + r) * D + col) =
-              make_uint2(M::pack(all.x * inv, all.y * inv), M::pack(all.z * inv, all.w * inv));
+              row_result<M>(all, sum, sees_none(s, done.unit, 8 * half + r, done.length));
         } else {
           const int64_t slot = ((int64_t)blockIdx.x * 2 + (at_start ? 0 : 1)) * kRows + 8 * half + r;
           *reinterpret_cast<float4*>(part_o + slot * D + col) = all;
@@ -714,7 +726,7 @@ __global__ void __launch_bounds__(kThreads)
   __shared__ float4 of_groups[kThreads];
   constexpr int kTile = Layout<D>::kTile;
   const int units = s.heads * s.row_tiles, b = blockIdx.x / units, unit = blockIdx.x - b * units, r = blockIdx.y;
-  const int tiles = tiles_of<kTile>(length_of(c, b));
+  const int length = length_of(c, b), tiles = tiles_of<kTile>(length);
   const Deal deal(tiles_before<kTile>(c, s.batch, units, scratch));
   const int64_t first = tiles_before<kTile>(c, b, units, scratch) + (int64_t)unit * tiles;
   cudaGridDependencySynchronize();  // in every CTA: what follows in the stream waits for the attention too
@@ -762,9 +774,7 @@ __global__ void __launch_bounds__(kThreads)
     const float4 v = of_groups[g * kCols + threadIdx.x];
     acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  *reinterpret_cast<uint2*>(o + out_row(s, b, unit, r) * D + col * 4) =
-      make_uint2(Mma<T>::pack(acc.x * inv, acc.y * inv), Mma<T>::pack(acc.z * inv, acc.w * inv));
+  *reinterpret_cast<uint2*>(o + out_row(s, b, unit, r) * D + col * 4) = row_result<Mma<T>>(acc, sum, sees_none(s, unit, r, length));
 }
 
 template <typename T, int D>

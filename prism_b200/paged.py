@@ -48,8 +48,10 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     lengths[b] - n + i.  D is 64 or 128; Hq a multiple of Hk.  scale: 1 / sqrt(D) if not given.
 
     Meant for few tokens: 16 rows (query, head of a group) at a time read the sequence's keys.  A query without a
-    key (lengths[b] = 0) gives 0; a sequence that is longer than its table, or whose table names a page that is
-    not in the cache, gives NaN.  Cache places behind a sequence's end are not read.  Inference only."""
+    key (lengths[b] < n: the first ones) gives 0; a sequence that is longer than its table, or whose table names a
+    page that is not in the cache, gives NaN.  Cache places behind a sequence's end are not read.  A value that is not finite may
+    reach every query of its sequence that has a key, one that does not see it too, as in a product with a zero
+    probability.  Inference only."""
     return _lib.torch_ops().paged_attention(q, k_cache, v_cache, page_table, lengths, scale)
 
 
