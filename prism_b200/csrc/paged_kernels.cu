@@ -811,6 +811,12 @@ static prism_status_t check_cache(const Cache& c, const int64_t* k_strides, cons
   return PRISM_OK;
 }
 
+// Strides of dimensions of one are never used, and may be anything: 0 then.
+static void take_strides(Cache& c, const int64_t* k, const int64_t* v, int heads) {
+  c.k_page = c.pages > 1 ? k[0] : 0, c.k_place = c.page_size > 1 ? k[1] : 0, c.k_head = heads > 1 ? k[2] : 0;
+  c.v_page = c.pages > 1 ? v[0] : 0, c.v_place = c.page_size > 1 ? v[1] : 0, c.v_head = heads > 1 ? v[2] : 0;
+}
+
 }  // namespace paged
 }  // namespace prism
 
@@ -842,8 +848,7 @@ prism_status_t prism_append_paged(const void* q, const int64_t* q_strides, int q
   PRISM_CHECK_ARG(k && v && k_strides && v_strides && (q_heads == 0 || (q && q_strides && q_out)) && (rot == 0 || freqs) &&
                       batch >= 1,
                   "%s: null pointer, or tokens without a sequence", what);
-  c.k_page = k_cache_strides[0], c.k_place = k_cache_strides[1], c.k_head = k_cache_strides[2];
-  c.v_page = v_cache_strides[0], c.v_place = v_cache_strides[1], c.v_head = v_cache_strides[2];
+  paged::take_strides(c, k_cache_strides, v_cache_strides, k_heads);
   paged::Append a = {};
   const void* in[3] = {q, k, v};
   const int64_t* strides[3] = {q_strides, k_strides, v_strides};
@@ -885,14 +890,15 @@ prism_status_t prism_paged_attention(const void* q, const int64_t* q_strides, in
   if (st != PRISM_OK) return st;
   if ((int64_t)batch * tokens == 0) return PRISM_OK;
   PRISM_CHECK_ARG(q && q_strides && o && (workspace || prism_paged_attention_workspace_bytes(D, page_size, table_width) == 0) && aligned16(o) && aligned16(workspace), "%s: null pointer, or a buffer off 16 bytes", what);
-  c.k_page = k_cache_strides[0], c.k_place = k_cache_strides[1], c.k_head = k_cache_strides[2];
-  c.v_page = v_cache_strides[0], c.v_place = v_cache_strides[1], c.v_head = v_cache_strides[2];
+  paged::take_strides(c, k_cache_strides, v_cache_strides, k_heads);
   const int64_t all_strides = c.k_page | c.k_place | c.k_head | c.v_page | c.v_place | c.v_head;
   PRISM_CHECK_ARG(aligned16(k_cache) && aligned16(v_cache) && all_strides >= 0 && (all_strides & 7) == 0,
                   "%s: the caches' rows must start on 16 bytes, with strides that are not negative", what);
-  constexpr int64_t kMost = (int64_t)1 << 35;  // elements: 2^32 units of 16 bytes
-  PRISM_CHECK_ARG((pages - 1) * c.k_page + (page_size - 1) * c.k_place + k_heads * c.k_head < kMost &&
-                      (pages - 1) * c.v_page + (page_size - 1) * c.v_place + k_heads * c.v_head < kMost,
+  constexpr double kMost = 34359738368.0;  // elements: 2^32 units of 16 bytes
+  const auto extent = [&](int64_t page, int64_t place, int64_t head) {
+    return (double)(pages - 1) * page + (double)(page_size - 1) * place + (double)(k_heads - 1) * head + D;
+  };
+  PRISM_CHECK_ARG(extent(c.k_page, c.k_place, c.k_head) <= kMost && extent(c.v_page, c.v_place, c.v_head) <= kMost,
                   "%s: caches of 64 GiB and more", what);
   PRISM_CHECK_ARG(aligned_to(q, 4) && ((q_strides[0] | q_strides[1] | q_strides[2]) & 1) == 0, "%s: q's rows must start on 4 bytes", what);
   paged::Queries s = {q, q_strides[0], q_strides[1], q_strides[2], batch, tokens, k_heads, q_heads / k_heads, 0, 0};

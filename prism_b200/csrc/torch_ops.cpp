@@ -636,7 +636,8 @@ Tensor paged_attention(const Tensor& q_in, const Tensor& k_cache, const Tensor& 
   refuse_tangents({q_in, k_cache, v_cache}, what);
   TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({q_in, k_cache, v_cache}), what, " is inference only");
   const auto fits = [](const Tensor& t) {
-    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.stride(0) | t.stride(1) | t.stride(2)) % 8 == 0;
+    const auto whole = [&](int64_t d) { return t.size(d) <= 1 || t.stride(d) % 8 == 0; };
+    return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && whole(0) && whole(1) && whole(2);
   };
   const Launch launch(device_of({q_in, k_cache, v_cache, table_in, lengths_in}));
   TORCH_CHECK_VALUE(fits(k_cache) && fits(v_cache), what, ": the caches' rows must start on 16 bytes");
