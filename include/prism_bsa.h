@@ -612,7 +612,7 @@ prism_status_t prism_packed_attention_bwd(const void* q, const int64_t* q_stride
  * is multiplied by scale * exp(i p freqs[j]), p the token's number; the other columns are copied.  dim <= 256.  A
  * token of no sequence, or with a negative number (lengths[b] below its new tokens: an empty slot of a padded
  * batch), writes nothing and its q_out is 0; one whose page lies outside the table or the cache writes
- * nothing and its q_out is NaN.  Places must differ: two tokens of one call on one place race.
+ * nothing and its q_out is NaN.  Places must differ, and not share memory: two tokens of one call on one place race.
  *
  * prism_paged_attention: q [batch, tokens, q_heads, D] (strides {sequence, token, head}; the last `tokens` of
  * each sequence; D = 64 or 128) -> o alike, contiguous: query i of sequence b attends the keys

@@ -9,11 +9,13 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <array>
 #include <cmath>
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "prism_bsa.h"
@@ -561,6 +563,20 @@ PagedCache check_cache(const Tensor& k, const Tensor& v, const Tensor& table, co
   c.pages = (int)k.size(0), c.page_size = (int)k.size(1);
   return c;
 }
+// Whether elements of t share memory: by growing strides, a dimension has to step over all that lies within.
+bool overlaps(const Tensor& t) {
+  if (t.numel() == 0) return false;
+  std::vector<std::pair<int64_t, int64_t>> dims;  // stride, size
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1) dims.emplace_back(t.stride(d), t.size(d));
+  std::sort(dims.begin(), dims.end());
+  int64_t extent = 1;
+  for (const auto& [stride, size] : dims) {
+    if (stride < extent) return true;
+    extent += (size - 1) * stride;
+  }
+  return false;
+}
 Tensor unit_columns(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
 
 // t [B, H, D] (one token a sequence) or [B, n, H, D] as rows [tokens, H, D], or [T, H, D] with offsets.
@@ -573,6 +589,8 @@ Optional append_paged(const Tensor& k_in, const Tensor& v_in, const Tensor& k_ca
   const Tensor q_given = or_undefined(q_in), offsets = or_undefined(offsets_in), freqs = or_undefined(freqs_in);
   TORCH_CHECK_VALUE(layout == "interleaved" || layout == "half", "layout must be 'interleaved' or 'half', got '", layout, "'");
   const PagedCache c = check_cache(k_cache, v_cache, table_in, lengths_in, what);
+  TORCH_CHECK_VALUE(!overlaps(k_cache) && !overlaps(v_cache) && (k_cache.numel() == 0 || k_cache.data_ptr() != v_cache.data_ptr()),
+                    what, ": places of the caches share memory");
   const int64_t dims = k_in.dim(), batch = lengths_in.size(0), D = k_cache.size(3);
   TORCH_CHECK_VALUE((dims == 3 || (dims == 4 && !offsets.defined())) && v_in.sizes() == k_in.sizes() && k_in.size(-1) == D &&
                         k_in.size(-2) == k_cache.size(2),

@@ -29,8 +29,9 @@ def append_paged(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     k, v [B, Hk, D] (one new token a sequence), [B, n, Hk, D] (n each), or [T, Hk, D] with offsets, int32 or int64
     [B + 1]: the new tokens of sequence b are the rows offsets[b] .. offsets[b + 1] - 1.  q alike, with its own
     heads.  bf16 or fp16, any strides of token and head; D up to 256.
-    k_cache, v_cache [pages, page_size, Hk, D], any strides with contiguous columns; page_table int32
-    [B, pages of a sequence]: token j is at place j % page_size of page page_table[b, j // page_size].
+    k_cache, v_cache [pages, page_size, Hk, D], any strides with contiguous columns, no two places on the same
+    memory; page_table int32 [B, pages of a sequence]: token j is at place j % page_size of page
+    page_table[b, j // page_size].
     lengths int32 [B]: each sequence's tokens, the new ones counted.
     freqs float64, layout, scale: as for ``apply_rotary``; the position is the token's number in its
     sequence.  Without freqs nothing is rotated.
