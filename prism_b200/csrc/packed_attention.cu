@@ -22,7 +22,9 @@
 //     a product sums over (V; K in dQ; Q and dO in dK / dV) are set to zero in shared memory first:
 //     a NaN in one sequence stays there, 0 * NaN being NaN.
 //   * Scores in log2 units; fp32 statistics and accumulators; P and dS rounded to the inputs' 16 bits
-//     for the second products, as the matrix instruction takes them.
+//     for the second products, as the matrix instruction takes them (a second part of P, for what that leaves,
+//     would be half as many products again): o is off by 0.0021 of its norm in bf16, 0.00029 in fp16, where one
+//     rounding of the result gives 0.0016 and 0.00021.
 //   * The tiles of a grid are its CTAs' work items; a grid has the upper bound of tiles that the row counts
 //     allow, and its spare items clear the rows that no sequence holds.  Offsets that decrease or leave the
 //     tensors give NaN.  The lengths are read on the device only: no host copy, no plan kernel.
@@ -416,7 +418,8 @@ struct RowSum {
 // m is a maximum of earlier scores, so a row's largest p is no power of two and its rounding is off by half a
 // step; where that p is nearly all of its row, o = sum p v / sum p is right only if both sums have the same p.  o
 // itself is rounded as coarsely, but delta = dO . o is subtracted from a nearly equal dO . v: for training only
-// (8,192 causal tokens at 128 columns: 484 us, 512 so).  lse is that of the p before rounding.
+// (8,192 causal tokens of 32 + 8 heads at 128 columns: 475 us, 515 so and with o's remainder written).  lse is that of
+// the p before rounding.
 template <typename T, bool kRounded>
 __device__ __forceinline__ RowSum<kRounded> exp_pairs(const float (&s)[64], float scale, float m, uint32_t (&pk)[32]) {
   const float2 sc = make_float2(scale, scale), nm = make_float2(-m, -m), zero = make_float2(0.f, 0.f);
@@ -442,8 +445,8 @@ __device__ __forceinline__ RowSum<kRounded> exp_pairs(const float (&s)[64], floa
 // that the tensor core works on one group's products while the other group's softmax runs.  Where there are
 // few tiles and long keys, an item is a part of the steps, and join_kernel adds the parts up.
 //
-// 8,192 causal tokens of 32 + 8 heads: 473 us at 128 columns (1,160 TFLOP/s, the tensor pipe 53 % busy), 395 at 64
-// (700 TFLOP/s, 30 %).  Bound by the softmax warps between the products: 2^x of every score alone takes 240 us at
+// 8,192 causal tokens of 32 + 8 heads: 475 us at 128 columns (1,155 TFLOP/s, the tensor pipe 53 % busy), 390 at 64
+// (705 TFLOP/s, 30 %).  Bound by the softmax warps between the products: 2^x of every score alone takes 240 us at
 // 16 a clock and SM, and the multiplications, conversions and TMEM traffic around it have the same issue slots.
 template <int D>
 struct FwdLayout {
@@ -1224,8 +1227,8 @@ __global__ void __launch_bounds__(kDeltaThreads)
 // (a = lane / 4) at columns 8 j + 2 (lane % 4) + {0, 1}, so that it needs 16 of a half tile's 64 lse and
 // delta values instead of all of them.
 //
-// 8,192 causal tokens of 32 + 8 heads: 920 us at 128 columns (8 D operations a score: 1,195 TFLOP/s, the tensor pipe
-// 56 % busy), 704 at 64 (780 TFLOP/s, 36 %).  Bound by the chain S, P, dP, dS of a step through the softmax warps
+// 8,192 causal tokens of 32 + 8 heads: 945 us at 128 columns (8 D operations a score: 1,165 TFLOP/s, the tensor pipe
+// 56 % busy), 720 at 64 (765 TFLOP/s, 36 %).  Bound by the chain S, P, dP, dS of a step through the softmax warps
 // (two TMEM reads, two writes and a 2^x a score), which the four products of the step before cover only in part.
 template <int D>
 struct DkdvLayout {
@@ -1665,7 +1668,7 @@ __global__ void __launch_bounds__(kJoinThreads)
 // warpgroups (64 keys each) write dS = P (dP - delta) into columns of its own, dQ += dS K reads them from
 // there.  S and dP of step n + 1 are issued as soon as those of step n are read.
 //
-// 8,192 causal tokens of 32 + 8 heads: 690 us at 128 columns (6 D operations a score: 1,195 TFLOP/s, the tensor pipe
+// 8,192 causal tokens of 32 + 8 heads: 690 to 700 us at 128 columns (6 D operations a score: 1,190 TFLOP/s, the tensor pipe
 // 55 % busy), 585 at 64 (705 TFLOP/s, 32 %).  Bound as dK and dV are.
 template <int D>
 struct DqLayout {

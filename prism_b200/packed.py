@@ -32,7 +32,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     Any row and head strides (copied where they are not multiples of 16 bytes).  Differentiable in q, k
     and v, once: a gradient of a gradient is an error.  What is not finite in one sequence, or behind the last
     one, changes nothing in another; within a sequence it may reach every query of the sequence, as in a product
-    with a zero probability."""
+    with a zero probability.
+
+    The probabilities are rounded to the inputs' type for the product with v.  With a gradient to take, the result is
+    divided by the sum of those rounded ones and its keys are not divided among SMs, without one (inference,
+    ``no_grad``) it is the exact sum and they may be: the two differ by roundings, so a block that is recomputed
+    for its backward pass does not repeat the bits of its first pass under ``no_grad``."""
     return _lib.torch_ops().packed_attention(q, k, v, offsets, k_offsets, causal, scale)
 
 

@@ -46,13 +46,14 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                     lengths: torch.Tensor, *, scale: Optional[float] = None) -> torch.Tensor:
     """q [B, Hq, D], or [B, n, Hq, D] for the last n tokens of each sequence, over the caches of
     ``append_paged`` -> the same shape: softmax(scale q k^T) v, query i over the keys up to its own place,
-    lengths[b] - n + i.  D is 64 or 128; Hq a multiple of Hk.  scale: 1 / sqrt(D) if not given.
+    lengths[b] - n + i.  D is 64 or 128; Hq a multiple of Hk.  scale: 1 / sqrt(D) if not given.  The caches' rows start
+    on 16 bytes; caches of 64 GiB and more are refused.
 
     Meant for few tokens: 16 rows (query, head of a group) at a time read the sequence's keys.  A query without a
     key (lengths[b] < n: the first ones) gives 0; a sequence that is longer than its table, or whose table names a
-    page that is not in the cache, gives NaN.  Cache places behind a sequence's end are not read.  A value that is not finite may
-    reach every query of its sequence that has a key, one that does not see it too, as in a product with a zero
-    probability.  Inference only."""
+    page that is not in the cache, gives NaN.  Cache places behind a sequence's end are not read.  A value that is
+    not finite may reach every query of its sequence that has a key, one that does not see it too, as in a product
+    with a zero probability.  Inference only."""
     return _lib.torch_ops().paged_attention(q, k_cache, v_cache, page_table, lengths, scale)
 
 
