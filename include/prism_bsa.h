@@ -566,7 +566,8 @@ prism_status_t prism_linear_fp8(const void* x8, int64_t ldx, const float* x_scal
  * [q_offsets[b], q_offsets[b + 1]) and [k_offsets[b], k_offsets[b + 1]) (device arrays of count + 1 int32, or
  * int64 with offsets_64; non-decreasing, within the rows: else every output is NaN).  Of a sequence's n
  * queries and m keys, query i attends all keys, or with causal != 0 the keys j <= i + m - n:
- *   o_i = sum_j p_ij v_j,  p_ij = softmax_j(scale q_i . k_j), scale > 0;  o_i = 0 without a key.
+ *   o_i = sum_j p_ij v_j,  p_ij = softmax_j(scale q_i . k_j), scale > 0;  o_i = 0 without a key, NaN where all
+ * scores are -inf or NaN.
  * o [q_rows, q_heads, D] contiguous, 0 in rows that no sequence holds.  Strides {row, head} in elements, whole
  * 16 bytes; columns contiguous.  Outputs and workspaces start on 32 bytes.  A NaN or an infinity in one
  * sequence reaches no other.  workspace:

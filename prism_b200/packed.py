@@ -27,7 +27,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
     causal: with n queries and m keys, query i attends keys 0 .. i + m - n, so the last query attends all of
     them (a prompt has m = n; its next part n < m).  A query without a key gives 0, and so do rows behind the
-    last sequence.  scale: 1 / sqrt(D) if not given.
+    last sequence; one all of whose scores are -inf or NaN gives NaN.  scale: 1 / sqrt(D) if not given.
 
     Any row and head strides (copied where they are not multiples of 16 bytes).  Differentiable in q, k
     and v, once: a gradient of a gradient is an error.  What is not finite in one sequence, or behind the last
