@@ -1668,8 +1668,8 @@ __global__ void __launch_bounds__(kJoinThreads)
 // warpgroups (64 keys each) write dS = P (dP - delta) into columns of its own, dQ += dS K reads them from
 // there.  S and dP of step n + 1 are issued as soon as those of step n are read.
 //
-// 8,192 causal tokens of 32 + 8 heads: 690 to 700 us at 128 columns (6 D operations a score: 1,190 TFLOP/s, the tensor pipe
-// 55 % busy), 585 at 64 (705 TFLOP/s, 32 %).  Bound as dK and dV are.
+// 8,192 causal tokens of 32 + 8 heads: 690 to 700 us at 128 columns (6 D operations a score: 1,190 TFLOP/s, the tensor
+// pipe 55 % busy), 585 at 64 (705 TFLOP/s, 32 %).  Bound as dK and dV are.
 template <int D>
 struct DqLayout {
   static constexpr int kRingK = 3, kRingV = 2;  // K serves two products
